@@ -7,7 +7,7 @@ CSRC  := snickery_amd/csrc
 HIPFLAGS := --offload-arch=$(ARCH) -O3 -fPIC -std=c++17 -ffp-contract=off -Wno-unused-value -Iinclude \
             -Xclang -target-feature -Xclang -packed-fp32-ops
 LIB   := snickery_amd/libsnkhip.so
-OBJS  := $(CSRC)/knn_kernels.o $(CSRC)/knn16_kernels.o $(CSRC)/viterbi_kernels.o $(CSRC)/joinfast_kernels.o $(CSRC)/joinlb2_kernels.o $(CSRC)/greedy_kernels.o $(CSRC)/greedy32_kernels.o $(CSRC)/greedy_hoist_kernels.o $(CSRC)/greedy_res_kernels.o $(CSRC)/concat_kernels.o $(CSRC)/kmeans_kernels.o $(CSRC)/api_core.o $(CSRC)/api_knn.o $(CSRC)/api_viterbi.o $(CSRC)/api_greedy.o $(CSRC)/api_shard.o $(CSRC)/api_options.o
+OBJS  := $(CSRC)/knn_kernels.o $(CSRC)/knn16_kernels.o $(CSRC)/viterbi_kernels.o $(CSRC)/joinfast_kernels.o $(CSRC)/joinlb2_kernels.o $(CSRC)/greedy_kernels.o $(CSRC)/greedy32_kernels.o $(CSRC)/greedy_hoist_kernels.o $(CSRC)/greedy_res_kernels.o $(CSRC)/concat_kernels.o $(CSRC)/kmeans_kernels.o $(CSRC)/sample_kernels.o $(CSRC)/trellis_kernels.o $(CSRC)/api_core.o $(CSRC)/api_knn.o $(CSRC)/api_viterbi.o $(CSRC)/api_greedy.o $(CSRC)/api_shard.o $(CSRC)/api_sample.o $(CSRC)/api_options.o
 
 all: $(LIB) oracle
 
@@ -18,7 +18,7 @@ $(CSRC)/knn16_kernels.o: HIPFLAGS += -mllvm -amdgpu-mfma-vgpr-form
 # (MI355X_MICROARCH.md, 'price of one filler beside MFMAs'; measured on the B* step: 4.09 -> 4.23 M frames/s)
 $(CSRC)/joinlb2_kernels.o $(CSRC)/joinfast_kernels.o $(CSRC)/knn16_kernels.o: HIPFLAGS += -fno-slp-vectorize
 
-$(CSRC)/%.o: $(CSRC)/%.hip $(CSRC)/snk_internal.h $(CSRC)/snk_engine.h $(CSRC)/greedy_common.h $(CSRC)/greedy32_device.h include/snk.h
+$(CSRC)/%.o: $(CSRC)/%.hip $(CSRC)/snk_internal.h $(CSRC)/snk_engine.h $(CSRC)/greedy_common.h $(CSRC)/greedy32_device.h $(CSRC)/sample_device.h include/snk.h
 	$(HIPCC) $(HIPFLAGS) -c $< -o $@
 
 $(LIB): $(OBJS) $(CSRC)/libsnkhip.map
@@ -36,7 +36,7 @@ ASAN_FLAGS := --cuda-host-only -O1 -g -fPIC -std=c++17 -ffp-contract=off -Wno-un
               -fsanitize=address,undefined -fno-sanitize-recover=undefined -fno-omit-frame-pointer -shared-libasan
 ASAN_OBJS  := $(patsubst $(CSRC)/%.o,$(ASAN_DIR)/%.o,$(OBJS)) $(ASAN_DIR)/fake_hip.o
 asan-host: $(ASAN_DIR)/libsnkhip_host_asan.so
-$(ASAN_DIR)/%.o: $(CSRC)/%.hip $(CSRC)/snk_internal.h $(CSRC)/snk_engine.h $(CSRC)/greedy_common.h $(CSRC)/greedy32_device.h include/snk.h
+$(ASAN_DIR)/%.o: $(CSRC)/%.hip $(CSRC)/snk_internal.h $(CSRC)/snk_engine.h $(CSRC)/greedy_common.h $(CSRC)/greedy32_device.h $(CSRC)/sample_device.h include/snk.h
 	@mkdir -p $(ASAN_DIR)
 	$(HIPCC) $(ASAN_FLAGS) -c $< -o $@
 $(ASAN_DIR)/fake_hip.o: tools/fakehip/fake_hip.cpp

@@ -304,6 +304,71 @@ int snk_sharded_greedy(snk_handle h, const double *Q, int64_t T, int D, int64_t 
 int snk_copy_to_host(void *dst_host, const void *src_dev, int64_t bytes);
 int snk_copy_to_device(void *dst_dev, const void *src_host, int64_t bytes);
 
+/* ---- draws and probabilities over the candidates of a preselection ------------------------------
+ * No counterpart in the reference: its searches return the cheapest sequence and nothing else, and its settings
+ * forbid_repetition / forbid_regression (synth_halfphone.py:3215-3216) are read without an effect (:3282-3287).
+ *
+ * snk_sample_rows: n_draws draws from every row of scores (R, V), row r starting row_stride * r scores on.  dtype: 0 float64,
+ * 1 float32, 2 float16, 3 bfloat16.  With m the row's largest score, a score x has the weight exp((x - m) / temperature); of the
+ * scores in descending order (equal ones by ascending index) the first top_k are kept, of those the shortest prefix that holds
+ * top_p of their weight, of those the ones of weight min_p and more; u (R, n_draws), numbers in [0, 1) from the caller, picks the
+ * first kept index whose cumulative weight exceeds u times the kept weight.  temperature 0: the lowest index of the largest
+ * score.  top_k 0, top_p 1, min_p 0: off.  -inf and NaN take no part; a row without any other score gives index -1, log
+ * probability -inf; +inf shares the row among its holders.
+ *   row_rules (R, 4) float64, or NULL: temperature, top_k, top_p, min_p of each row instead of the call's
+ *   index_out (R, n_draws) int64; logp_out (R, n_draws) float64, or NULL: log of the drawn weight over the kept weight
+ * Draws are reproducible: sums of weights are whole numbers, the same in any order.  V is at most 2^24.
+ * The _dev form takes device memory throughout and puts its kernels on `stream` (a hipStream_t; NULL: the default stream)
+ * without waiting; it uses nothing of the engine and can be captured into a graph.  It cannot look at device memory first: a number
+ * u below 0 or NaN draws the first kept index, one of 1 or more the last; a row rule without meaning counts as off (a temperature
+ * as 0). */
+int snk_sample_rows(snk_handle h, const void *scores, int dtype, int64_t R, int64_t V, int64_t row_stride, const double *u, int n_draws,
+                    double temperature, int64_t top_k, double top_p, double min_p, const double *row_rules,
+                    int64_t *index_out, double *logp_out);
+int snk_sample_rows_dev(snk_handle h, const void *scores_dev, int dtype, int64_t R, int64_t V, int64_t row_stride, const double *u_dev,
+                        int n_draws, double temperature, int64_t top_k, double top_p, double min_p, const double *row_rules_dev,
+                        int64_t *index_dev_out, double *logp_dev_out, void *stream);
+
+/* A bias on the relative position of consecutive units of a path, by buckets: joining unit i to unit j adds
+ * bias[class, bucket(j - i)] to the join cost, bucket(d) = number of edges <= d, class = the join's own (join_class below).
+ *   bias (n_classes, n_buckets) float64, finite or +inf (the join is forbidden); edges (n_buckets - 1) int64, ascending;
+ *   n_classes up to 65535, n_buckets up to 64.  n_classes 0 clears it.
+ * It applies to snk_sample_paths and snk_path_posterior (the searches above keep the reference's costs) and stays until it is
+ * set again. */
+int snk_set_position_bias(snk_handle h, const double *bias, int n_classes, int n_buckets, const int64_t *edges);
+
+/* Draws of whole paths: p(path) ~ exp(-cost / temperature), cost = target costs + join costs + position bias, over the
+ * candidates cand / tdist (row_offsets[n_utts], K) of n_utts utterances (as snk_viterbi_batch; candidates of a unit that cannot
+ * join or without a finite target cost take no part).  Each path is drawn from its end: the last candidate from its marginal,
+ * every one before from its probability given the one behind it, each of these distributions truncated by top_k, top_p and
+ * min_p as in snk_sample_rows.  temperature 0: the cheapest path (ties as in snk_viterbi).
+ *   join_class (rows) int32, or NULL (class 0): class of the join from row r to row r + 1; outside 0 .. n_classes - 1: no bias
+ *   u (n_draws, rows) float64 in [0, 1)
+ *   path_out (n_draws, rows) int64 unit ids, -1 throughout an utterance without a complete path
+ *   cost_out (n_draws, n_utts) float64 (+inf there); logp_out likewise, or NULL: log of the product of the truncated
+ *   probabilities (-inf there)
+ * K up to 208; an utterance of a single row is a draw from its target costs.
+ * The _dev form takes device memory (row_offsets excepted), waits for what `stream` holds and makes `stream` wait for the
+ * results, without a host wait; it refuses a stream that is being captured. */
+int snk_sample_paths(snk_handle h, const int64_t *cand, const double *tdist, const int64_t *row_offsets, int n_utts, int K,
+                     const int32_t *join_class, const double *u, int n_draws, double temperature, int64_t top_k, double top_p,
+                     double min_p, int64_t *path_out, double *cost_out, double *logp_out);
+int snk_sample_paths_dev(snk_handle h, const int64_t *cand_dev, const double *tdist_dev, const int64_t *row_offsets, int n_utts, int K,
+                         const int32_t *join_class_dev, const double *u_dev, int n_draws, double temperature, int64_t top_k,
+                         double top_p, double min_p, int64_t *path_dev_out, double *cost_dev_out, double *logp_dev_out, void *stream);
+
+/* The same model's log partition function and what its gradients need (arguments as snk_sample_paths, temperature > 0):
+ *   logz_out (n_utts)        log of the sum of exp(-cost / temperature) over all paths; -inf: there is none
+ *   posterior_out (rows, K)  probability of every candidate:  d logZ / d tdist = -posterior / temperature
+ *   uses_out (n_classes, n_buckets), or NULL: expected uses of every entry of the position bias, summed over the utterances:
+ *                            d logZ / d bias = -uses / temperature
+ * An utterance without a complete path has posteriors 0 and adds no uses. */
+int snk_path_posterior(snk_handle h, const int64_t *cand, const double *tdist, const int64_t *row_offsets, int n_utts, int K,
+                       const int32_t *join_class, double temperature, double *logz_out, double *posterior_out, double *uses_out);
+int snk_path_posterior_dev(snk_handle h, const int64_t *cand_dev, const double *tdist_dev, const int64_t *row_offsets, int n_utts, int K,
+                           const int32_t *join_class_dev, double temperature, double *logz_dev_out, double *posterior_dev_out,
+                           double *uses_dev_out, void *stream);
+
 /* Waveform side (the step after the search).  Replaces retrieve_magphase_frag
  * (synth_simple.py:538-652) and the overlap-add loop of concatenateMagPhaseEpoch_sep_files
  * (:677-747) up to the call of the external vocoder.

@@ -70,7 +70,8 @@ int snk_concat_fragments(snk_handle h, const int64_t *first_row, const int64_t *
 const char *kTimerNames[TM_COUNT] = {
     "h2d_queries", "prepare_queries", "knn_minima", "knn_threshold", "knn_filter", "knn_bucket", "knn_finalize",
     "join_costs", "viterbi_dp", "d2h_results", "greedy_target_gemm", "greedy_steps", "set_weights",
-    "merge_topk", "join_lower_bounds", "viterbi_lower_bound", "join_exact_sparse", "viterbi_sparse", "knn_ball_bound"};
+    "merge_topk", "join_lower_bounds", "viterbi_lower_bound", "join_exact_sparse", "viterbi_sparse", "knn_ball_bound",
+    "sample_rows", "trellis_sums", "trellis_draws", "trellis_posteriors"};
 
 int snk_timer_count(void) { return TM_COUNT; }
 const char *snk_timer_name(int i) { return (i >= 0 && i < TM_COUNT) ? kTimerNames[i] : ""; }

@@ -1,0 +1,367 @@
+// C ABI of libsnkhip.so, part 6: draws and probabilities over the candidates of a preselection (include/snk.h snk_sample_rows,
+// snk_set_position_bias, snk_sample_paths, snk_path_posterior).
+//
+// Streams.  snk_sample_rows_dev touches nothing of the engine: its kernels go straight to the caller's stream.  The trellis calls
+// use the engine's workspaces, so their kernels run on the engine's main stream, in the order of the calls; a _dev call makes that
+// stream wait for what the caller's stream holds and the caller's stream for the results, without a host wait in between.
+#include "snk_engine.h"
+
+// the caller's device again when a _dev call returns
+struct DeviceGuard {
+    int before = -1;
+    ~DeviceGuard() { if (before >= 0) (void)hipSetDevice(before); }
+    int enter(int device)
+    {
+        int now = 0;
+        HIPCHK(hipGetDevice(&now));
+        if (now != device) { HIPCHK(hipSetDevice(device)); before = now; }
+        return 0;
+    }
+};
+
+static const size_t kScoreBytes[4] = {8, 4, 2, 2};
+
+static int check_rule(const char *who, double temperature, int64_t top_k, double top_p, double min_p)
+{
+    if (!(temperature >= 0.0) || !(temperature - temperature == 0.0)) return fail("%s: temperature %g is not a finite number >= 0", who, temperature);
+    if (top_k < 0) return fail("%s: top_k %lld < 0 (0: off)", who, (long long)top_k);
+    if (!(top_p > 0.0 && top_p <= 1.0)) return fail("%s: top_p %g outside (0, 1]", who, top_p);
+    if (!(min_p >= 0.0 && min_p <= 1.0)) return fail("%s: min_p %g outside [0, 1]", who, min_p);
+    return 0;
+}
+
+static int check_randoms(const char *who, const double *u, int64_t n)
+{
+    for (int64_t i = 0; i < n; ++i)
+        if (!(u[i] >= 0.0 && u[i] < 1.0)) return fail("%s: random number %lld is %g, outside [0, 1)", who, (long long)i, u[i]);
+    return 0;
+}
+
+static int check_rows(const char *who, int dtype, int64_t R, int64_t V, int64_t stride, int n_draws)
+{
+    if (dtype < 0 || dtype > 3) return fail("%s: unknown score type %d", who, dtype);
+    if (R < 0 || R > 0x7fffffff) return fail("%s: %lld rows", who, (long long)R);
+    if (V < 1 || V > sample_rows_max()) return fail("%s: rows of %lld scores (1 .. %lld)", who, (long long)V, (long long)sample_rows_max());
+    if (stride < V && R > 1) return fail("%s: row stride %lld < %lld scores", who, (long long)stride, (long long)V);
+    if (n_draws < 1) return fail("%s: %d draws per row", who, n_draws);
+    return 0;
+}
+
+int snk_sample_rows(snk_handle h, const void *scores, int dtype, int64_t R, int64_t V, int64_t row_stride, const double *u, int n_draws,
+                    double temperature, int64_t top_k, double top_p, double min_p, const double *row_rules, int64_t *index_out,
+                    double *logp_out)
+{
+    const char *who = "snk_sample_rows";
+    if (!h) return fail("null handle");
+    CHK(no_batch_in_flight(h, who));
+    CHK(check_rows(who, dtype, R, V, row_stride, n_draws));
+    if (R == 0) return 0;
+    if (!scores || !u || !index_out) return fail("%s: null argument", who);
+    if (row_rules) {
+        for (int64_t r = 0; r < R; ++r) {
+            const double *q = row_rules + 4 * r;
+            if (!(q[1] >= 0.0 && q[1] < 9.0e15) || q[1] != floor(q[1])) return fail("%s: top_k %g of row %lld is not a whole number >= 0", who, q[1], (long long)r);
+            CHK(check_rule(who, q[0], (int64_t)q[1], q[2], q[3]));
+        }
+    } else CHK(check_rule(who, temperature, top_k, top_p, min_p));
+    CHK(check_randoms(who, u, R * n_draws));
+    HIPCHK(hipSetDevice(h->device));
+    const size_t width = kScoreBytes[dtype], n = (size_t)R * n_draws;
+    CHK(h->sr_scores.ensure((size_t)R * V * width));
+    CHK(h->sr_u.ensure(n * sizeof(double)));
+    CHK(h->sr_index.ensure(n * sizeof(int64_t)));
+    CHK(h->sr_logp.ensure(n * sizeof(double)));
+    CHK(h2d_rows(h, h->sr_scores.p, (size_t)V * width, scores, (size_t)(R > 1 ? row_stride : V) * width, (size_t)V * width, (size_t)R, h->stream));
+    CHK(h2d(h, h->sr_u.p, u, n * sizeof(double), h->stream));
+    if (row_rules) {
+        CHK(h->sr_rules.ensure((size_t)R * 4 * sizeof(double)));
+        CHK(h2d(h, h->sr_rules.p, row_rules, (size_t)R * 4 * sizeof(double), h->stream));
+    }
+    {
+        StageTimer t(h, h->stream, TM_SAMPLE_ROWS);
+        const SampleRuleHost rule = {temperature, top_k, top_p, min_p};
+        launch_sample_rows(h->sr_scores.p, dtype, V, R, V, h->sr_u.as<double>(), n_draws, rule, row_rules ? h->sr_rules.as<double>() : nullptr,
+                           h->sr_index.as<int64_t>(), logp_out ? h->sr_logp.as<double>() : nullptr, h->stream);
+    }
+    HIPCHK(hipGetLastError());
+    D2HPart parts[2] = {{index_out, h->sr_index.p, n * sizeof(int64_t)}, {logp_out, h->sr_logp.p, logp_out ? n * sizeof(double) : 0}};
+    CHK(staged_d2h(h, h->stream, parts, 2));
+    collect_timers(h);
+    return 0;
+}
+
+int snk_sample_rows_dev(snk_handle h, const void *scores_dev, int dtype, int64_t R, int64_t V, int64_t row_stride, const double *u_dev,
+                        int n_draws, double temperature, int64_t top_k, double top_p, double min_p, const double *row_rules_dev,
+                        int64_t *index_dev_out, double *logp_dev_out, void *stream)
+{
+    const char *who = "snk_sample_rows_dev";
+    if (!h) return fail("null handle");
+    CHK(check_rows(who, dtype, R, V, row_stride, n_draws));
+    if (R == 0) return 0;
+    if (!scores_dev || !u_dev || !index_dev_out) return fail("%s: null argument", who);
+    if (!row_rules_dev) CHK(check_rule(who, temperature, top_k, top_p, min_p));
+    DeviceGuard device;
+    CHK(device.enter(h->device));
+    const SampleRuleHost rule = {temperature, top_k, top_p, min_p};
+    launch_sample_rows(scores_dev, dtype, row_stride, R, V, u_dev, n_draws, rule, row_rules_dev, index_dev_out, logp_dev_out, (hipStream_t)stream);
+    HIPCHK(hipGetLastError());
+    return 0;
+}
+
+int snk_set_position_bias(snk_handle h, const double *bias, int n_classes, int n_buckets, const int64_t *edges)
+{
+    const char *who = "snk_set_position_bias";
+    if (!h) return fail("null handle");
+    CHK(no_batch_in_flight(h, who));
+    if (n_classes == 0) { h->pb_classes = 0; h->pb_buckets = 0; return 0; }
+    if (n_classes < 0 || n_classes > 65535) return fail("%s: %d classes (0 .. 65535)", who, n_classes);
+    if (n_buckets < 1 || n_buckets > 64) return fail("%s: %d buckets (1 .. 64)", who, n_buckets);
+    if (!bias || (n_buckets > 1 && !edges)) return fail("%s: null argument", who);
+    for (int i = 1; i < n_buckets - 1; ++i)
+        if (edges[i] <= edges[i - 1]) return fail("%s: edges have to ascend (edge %d is %lld after %lld)", who, i, (long long)edges[i], (long long)edges[i - 1]);
+    const int64_t n = (int64_t)n_classes * n_buckets;
+    for (int64_t i = 0; i < n; ++i)
+        if (!(bias[i] > -INFINITY)) return fail("%s: bias %lld is %g (finite, or +inf to forbid)", who, (long long)i, bias[i]);
+    HIPCHK(hipSetDevice(h->device));
+    h->pb_classes = 0;
+    CHK(h->pb_bias.ensure((size_t)n * sizeof(double)));
+    CHK(h->pb_edges.ensure(64 * sizeof(int64_t)));
+    CHK(h2d_sync(h, h->pb_bias.p, bias, (size_t)n * sizeof(double)));
+    if (n_buckets > 1) CHK(h2d_sync(h, h->pb_edges.p, edges, (size_t)(n_buckets - 1) * sizeof(int64_t)));
+    h->pb_classes = n_classes;
+    h->pb_buckets = n_buckets;
+    return 0;
+}
+
+// ---- the trellis ------------------------------------------------------------------------------------------------------------------
+static int check_trellis(const char *who, snk_engine *h, const void *cand, const void *tdist, const int64_t *row_offsets, int n_utts, int K)
+{
+    CHK(check_ready(h, false, true));
+    CHK(no_batch_in_flight(h, who));
+    if (!cand || !tdist || !row_offsets || n_utts < 1) return fail("%s: null/empty argument", who);
+    if (K < 1 || K > 208) return fail("%s: n_candidates=%d outside 1..208", who, K);
+    if (row_offsets[0] != 0) return fail("%s: row_offsets[0] must be 0 (got %lld)", who, (long long)row_offsets[0]);
+    for (int v = 0; v < n_utts; ++v)
+        if (row_offsets[v + 1] <= row_offsets[v]) return fail("%s: utterance %d has no rows", who, v);
+    if (row_offsets[n_utts] > 0x7fffffff) return fail("%s: %lld rows", who, (long long)row_offsets[n_utts]);
+    return 0;
+}
+
+// Costs of the rows of as many utterances as fit the workspace, then `use` on them; group after group on the engine's stream.
+// 4 GB hold 53 000 rows of 100 candidates: larger groups would not fill the chip better, smaller ones would (a sentence alone
+// keeps a handful of compute units busy in the recursions).  An utterance that is longer than that is a group by itself.
+static const size_t kTrellisGroupBytes = (size_t)4 << 30;
+
+template <typename Use>
+static int trellis_groups(snk_engine *h, bool timed, const int64_t *cand, const double *tdist, const int32_t *join_class, const int64_t *off_dev,
+                          const int64_t *row_offsets, int n_utts, int K, double inv_tau, Use use)
+{
+    const size_t row_bytes = (size_t)K * K * sizeof(double);
+    for (int v0 = 0; v0 < n_utts;) {
+        int v1 = v0 + 1;
+        while (v1 < n_utts && (size_t)(row_offsets[v1 + 1] - row_offsets[v0]) * row_bytes <= kTrellisGroupBytes) ++v1;
+        TrellisView view;
+        view.cand = cand; view.tdist = tdist; view.off = off_dev;
+        view.first = v0; view.n_utts = v1 - v0; view.K = K;
+        view.c0 = row_offsets[v0]; view.rows = row_offsets[v1] - row_offsets[v0];
+        view.n_units = h->Njc - 1;
+        view.inv_tau = inv_tau;
+        CHK(h->tr_C.ensure((size_t)view.rows * row_bytes));
+        view.C = h->tr_C.as<double>();
+        {
+            StageTimer t(h, h->stream, timed ? TM_JOIN : -1);
+            launch_join_costs(h->JCw.as<double>(), h->Djpad, h->Dj, view.n_units, cand + view.c0 * K, view.rows, K, h->tr_C.as<double>(), h->stream);
+            if (h->pb_classes > 0)
+                launch_position_bias(cand + view.c0 * K, join_class ? join_class + view.c0 : nullptr, h->pb_bias.as<double>(), h->pb_edges.as<int64_t>(),
+                                     h->pb_classes, h->pb_buckets, view.rows, K, h->tr_C.as<double>(), h->stream);
+        }
+        CHK(use(view));
+        v0 = v1;
+    }
+    HIPCHK(hipGetLastError());
+    return 0;
+}
+
+static int trellis_offsets(snk_engine *h, const int64_t *row_offsets, int n_utts)
+{
+    CHK(h->tr_off.ensure((size_t)(n_utts + 1) * sizeof(int64_t)));
+    return h2d(h, h->tr_off.p, row_offsets, (size_t)(n_utts + 1) * sizeof(int64_t), h->stream);
+}
+
+static int sample_paths_device(snk_engine *h, bool timed, const int64_t *cand, const double *tdist, const int64_t *row_offsets, int n_utts,
+                               int K, const int32_t *join_class, const double *u, int n_draws, const SampleRuleHost &rule,
+                               int64_t *path, double *cost, double *logp)
+{
+    const int64_t rows = row_offsets[n_utts];
+    const bool sum = rule.temperature > 0.0;
+    CHK(trellis_offsets(h, row_offsets, n_utts));
+    CHK(h->tr_alpha.ensure((size_t)rows * K * sizeof(double)));
+    return trellis_groups(h, timed, cand, tdist, join_class, h->tr_off.as<int64_t>(), row_offsets, n_utts, K, sum ? 1.0 / rule.temperature : 1.0,
+                          [&](const TrellisView &view) -> int {
+        {
+            StageTimer t(h, h->stream, timed ? TM_TRELLIS_SUM : -1);
+            launch_trellis_forward(view, sum, h->tr_alpha.as<double>(), nullptr, h->stream);
+        }
+        StageTimer t(h, h->stream, timed ? TM_TRELLIS_DRAW : -1);
+        launch_trellis_draw(view, rule, h->tr_alpha.as<double>(), u, n_draws, rows, n_utts, path, cost, logp, h->stream);
+        return 0;
+    });
+}
+
+static int path_posterior_device(snk_engine *h, bool timed, const int64_t *cand, const double *tdist, const int64_t *row_offsets, int n_utts,
+                                 int K, const int32_t *join_class, double temperature, double *logz, double *posterior, double *uses)
+{
+    const int64_t rows = row_offsets[n_utts];
+    CHK(trellis_offsets(h, row_offsets, n_utts));
+    CHK(h->tr_alpha.ensure((size_t)rows * K * sizeof(double)));
+    CHK(h->tr_beta.ensure((size_t)rows * K * sizeof(double)));
+    if (uses) CHK(h->tr_row_uses.ensure((size_t)rows * h->pb_buckets * sizeof(double)));
+    CHK(trellis_groups(h, timed, cand, tdist, join_class, h->tr_off.as<int64_t>(), row_offsets, n_utts, K, 1.0 / temperature,
+                       [&](const TrellisView &view) -> int {
+        {
+            StageTimer t(h, h->stream, timed ? TM_TRELLIS_SUM : -1);
+            launch_trellis_forward(view, true, h->tr_alpha.as<double>(), logz, h->stream);
+            launch_trellis_backward(view, h->tr_beta.as<double>(), h->stream);
+        }
+        StageTimer t(h, h->stream, timed ? TM_TRELLIS_POST : -1);
+        launch_trellis_posterior(view, h->tr_alpha.as<double>(), h->tr_beta.as<double>(), logz, h->pb_edges.as<int64_t>(), h->pb_buckets,
+                                 posterior, uses ? h->tr_row_uses.as<double>() : nullptr, h->stream);
+        return 0;
+    }));
+    if (uses) launch_trellis_uses(h->tr_row_uses.as<double>(), join_class, rows, h->pb_classes, h->pb_buckets, uses, h->stream);
+    HIPCHK(hipGetLastError());
+    return 0;
+}
+
+// host arrays of a trellis call -> the engine's workspaces
+static int upload_trellis(snk_engine *h, const int64_t *cand, const double *tdist, int64_t rows, int K, const int32_t *join_class)
+{
+    StageTimer t(h, h->stream, TM_H2D);
+    const size_t n = (size_t)rows * K;
+    CHK(h->tr_cand.ensure(n * sizeof(int64_t)));
+    CHK(h->tr_tdist.ensure(n * sizeof(double)));
+    CHK(h2d(h, h->tr_cand.p, cand, n * sizeof(int64_t), h->stream));
+    CHK(h2d(h, h->tr_tdist.p, tdist, n * sizeof(double), h->stream));
+    if (join_class) {
+        CHK(h->tr_class.ensure((size_t)rows * sizeof(int32_t)));
+        CHK(h2d(h, h->tr_class.p, join_class, (size_t)rows * sizeof(int32_t), h->stream));
+    }
+    return 0;
+}
+
+// the engine's stream behind what the caller's stream holds; refused while that stream is being captured: a captured call would
+// share the engine's workspaces with every later one
+static int trellis_enter(snk_engine *h, const char *who, hipStream_t caller)
+{
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(caller, &st) != hipSuccess || st != hipStreamCaptureStatusNone) {
+        (void)hipGetLastError();
+        return fail("%s: the stream is being captured (this call uses the engine's workspaces)", who);
+    }
+    if (!h->tr_in) {
+        HIPCHK(hipEventCreateWithFlags(&h->tr_in, hipEventDisableTiming));
+        HIPCHK(hipEventCreateWithFlags(&h->tr_done, hipEventDisableTiming));
+    }
+    HIPCHK(hipEventRecord(h->tr_in, caller));
+    HIPCHK(hipStreamWaitEvent(h->stream, h->tr_in, 0));
+    return 0;
+}
+static int trellis_leave(snk_engine *h, hipStream_t caller)
+{
+    HIPCHK(hipEventRecord(h->tr_done, h->stream));
+    HIPCHK(hipStreamWaitEvent(caller, h->tr_done, 0));
+    return 0;
+}
+
+static int check_draws(const char *who, const void *u, int n_draws, const SampleRuleHost &rule, const void *path, const void *cost)
+{
+    if (!u || !path || !cost) return fail("%s: null argument", who);
+    if (n_draws < 1 || n_draws > 65535) return fail("%s: %d draws (1 .. 65535)", who, n_draws);
+    return check_rule(who, rule.temperature, rule.top_k, rule.top_p, rule.min_p);
+}
+
+int snk_sample_paths(snk_handle h, const int64_t *cand, const double *tdist, const int64_t *row_offsets, int n_utts, int K,
+                     const int32_t *join_class, const double *u, int n_draws, double temperature, int64_t top_k, double top_p, double min_p,
+                     int64_t *path_out, double *cost_out, double *logp_out)
+{
+    const char *who = "snk_sample_paths";
+    const SampleRuleHost rule = {temperature, top_k, top_p, min_p};
+    CHK(check_trellis(who, h, cand, tdist, row_offsets, n_utts, K));
+    CHK(check_draws(who, u, n_draws, rule, path_out, cost_out));
+    const int64_t rows = row_offsets[n_utts];
+    CHK(check_randoms(who, u, rows * n_draws));
+    HIPCHK(hipSetDevice(h->device));
+    const size_t np = (size_t)n_draws * rows * 8, nc = (size_t)n_draws * n_utts * 8;
+    CHK(h->tr_u.ensure(np));
+    CHK(h->tr_out.ensure(np + 2 * nc));
+    CHK(upload_trellis(h, cand, tdist, rows, K, join_class));
+    CHK(h2d(h, h->tr_u.p, u, np, h->stream));
+    char *out = h->tr_out.as<char>();
+    CHK(sample_paths_device(h, true, h->tr_cand.as<int64_t>(), h->tr_tdist.as<double>(), row_offsets, n_utts, K,
+                            join_class ? h->tr_class.as<int32_t>() : nullptr, h->tr_u.as<double>(), n_draws, rule, (int64_t *)out,
+                            (double *)(out + np), logp_out ? (double *)(out + np + nc) : nullptr));
+    D2HPart parts[3] = {{path_out, out, np}, {cost_out, out + np, nc}, {logp_out, out + np + nc, logp_out ? nc : 0}};
+    CHK(staged_d2h(h, h->stream, parts, 3));
+    collect_timers(h);
+    return 0;
+}
+
+int snk_sample_paths_dev(snk_handle h, const int64_t *cand_dev, const double *tdist_dev, const int64_t *row_offsets, int n_utts, int K,
+                         const int32_t *join_class_dev, const double *u_dev, int n_draws, double temperature, int64_t top_k, double top_p,
+                         double min_p, int64_t *path_dev_out, double *cost_dev_out, double *logp_dev_out, void *stream)
+{
+    const char *who = "snk_sample_paths_dev";
+    const SampleRuleHost rule = {temperature, top_k, top_p, min_p};
+    CHK(check_trellis(who, h, cand_dev, tdist_dev, row_offsets, n_utts, K));
+    CHK(check_draws(who, u_dev, n_draws, rule, path_dev_out, cost_dev_out));
+    DeviceGuard device;
+    CHK(device.enter(h->device));
+    CHK(trellis_enter(h, who, (hipStream_t)stream));
+    CHK(sample_paths_device(h, false, cand_dev, tdist_dev, row_offsets, n_utts, K, join_class_dev, u_dev, n_draws, rule, path_dev_out, cost_dev_out,
+                            logp_dev_out));
+    return trellis_leave(h, (hipStream_t)stream);
+}
+
+static int check_posterior(const char *who, snk_engine *h, double temperature, const void *logz, const void *posterior, const void *uses)
+{
+    if (!logz || !posterior) return fail("%s: null argument", who);
+    if (!(temperature > 0.0) || !(temperature - temperature == 0.0)) return fail("%s: temperature %g is not a finite number > 0", who, temperature);
+    if (uses && h->pb_classes == 0) return fail("%s: no position bias set (snk_set_position_bias)", who);
+    return 0;
+}
+
+int snk_path_posterior(snk_handle h, const int64_t *cand, const double *tdist, const int64_t *row_offsets, int n_utts, int K,
+                       const int32_t *join_class, double temperature, double *logz_out, double *posterior_out, double *uses_out)
+{
+    const char *who = "snk_path_posterior";
+    CHK(check_trellis(who, h, cand, tdist, row_offsets, n_utts, K));
+    CHK(check_posterior(who, h, temperature, logz_out, posterior_out, uses_out));
+    HIPCHK(hipSetDevice(h->device));
+    const int64_t rows = row_offsets[n_utts];
+    const size_t nz = (size_t)n_utts * 8, np = (size_t)rows * K * 8, nu = uses_out ? (size_t)h->pb_classes * h->pb_buckets * 8 : 0;
+    CHK(h->tr_out.ensure(nz + np + nu));
+    CHK(upload_trellis(h, cand, tdist, rows, K, join_class));
+    char *out = h->tr_out.as<char>();
+    CHK(path_posterior_device(h, true, h->tr_cand.as<int64_t>(), h->tr_tdist.as<double>(), row_offsets, n_utts, K,
+                              join_class ? h->tr_class.as<int32_t>() : nullptr, temperature, (double *)out, (double *)(out + nz),
+                              uses_out ? (double *)(out + nz + np) : nullptr));
+    D2HPart parts[3] = {{logz_out, out, nz}, {posterior_out, out + nz, np}, {uses_out, out + nz + np, nu}};
+    CHK(staged_d2h(h, h->stream, parts, 3));
+    collect_timers(h);
+    return 0;
+}
+
+int snk_path_posterior_dev(snk_handle h, const int64_t *cand_dev, const double *tdist_dev, const int64_t *row_offsets, int n_utts, int K,
+                           const int32_t *join_class_dev, double temperature, double *logz_dev_out, double *posterior_dev_out,
+                           double *uses_dev_out, void *stream)
+{
+    const char *who = "snk_path_posterior_dev";
+    CHK(check_trellis(who, h, cand_dev, tdist_dev, row_offsets, n_utts, K));
+    CHK(check_posterior(who, h, temperature, logz_dev_out, posterior_dev_out, uses_dev_out));
+    DeviceGuard device;
+    CHK(device.enter(h->device));
+    CHK(trellis_enter(h, who, (hipStream_t)stream));
+    CHK(path_posterior_device(h, false, cand_dev, tdist_dev, row_offsets, n_utts, K, join_class_dev, temperature, logz_dev_out, posterior_dev_out,
+                              uses_dev_out));
+    return trellis_leave(h, (hipStream_t)stream);
+}

@@ -38,7 +38,7 @@ const std::string &last_error_string();
 enum TimerId {
     TM_H2D = 0, TM_PREP, TM_KNN_MINIMA, TM_KNN_THRESHOLD, TM_KNN_FILTER, TM_KNN_BUCKET, TM_KNN_FINALIZE,
     TM_JOIN, TM_VITERBI_DP, TM_D2H, TM_GREEDY_TARGET, TM_GREEDY_STEPS, TM_WEIGHTS, TM_MERGE, TM_JOIN_LB, TM_DP_LB,
-    TM_JOIN_SPARSE, TM_DP_SPARSE, TM_KNN_BALLMIN, TM_COUNT
+    TM_JOIN_SPARSE, TM_DP_SPARSE, TM_KNN_BALLMIN, TM_SAMPLE_ROWS, TM_TRELLIS_SUM, TM_TRELLIS_DRAW, TM_TRELLIS_POST, TM_COUNT
 };
 
 extern const char *kTimerNames[TM_COUNT];
@@ -445,6 +445,12 @@ struct snk_engine {
     int lb_warm_eff = 0;       // 0: lb_warm
     int lb_warm_long = 48;
     int64_t lb_warm_raises = 0;
+    // draws and posteriors (api_sample.hip): everything on the engine's main stream
+    DevBuf pb_bias, pb_edges;              // position bias (classes, buckets) and the buckets' edges
+    int pb_classes = 0, pb_buckets = 0;    // 0: none set
+    DevBuf sr_scores, sr_u, sr_rules, sr_index, sr_logp;
+    DevBuf tr_off, tr_cand, tr_tdist, tr_class, tr_u, tr_C, tr_alpha, tr_beta, tr_row_uses, tr_out;
+    hipEvent_t tr_in = nullptr, tr_done = nullptr;      // hand-over between a caller's stream and the engine's
     DevBuf vstats;             // [0] cells refined, [1] steps with a refinement, [2] exact costs computed there
     // pass 1 of the sparse path, second form (joinfast_kernels.hip: join_lb2_kernel): float32 copy of the weighted join rows,
     // built at the first sparse recursion after snk_set_weights; [0] of jw_umax: bits of the largest row norm

@@ -357,6 +357,29 @@ void launch_concat_fragments(const float *spec, int W, const double *fzv, const 
                              const int64_t *utt_lo, const int64_t *utt_hi, int64_t n, int me, int ov,
                              const double *in_taper, double *out_spec, double *out_fz, hipStream_t s);
 
+// ---- draws (sample_kernels.hip, trellis_kernels.hip) ----------------------------
+struct SampleRuleHost { double temperature; int64_t top_k; double top_p, min_p; };
+int64_t sample_rows_max();            // longest row of scores
+void launch_sample_rows(const void *scores, int dtype, int64_t stride, int64_t R, int64_t V, const double *u, int n_draws,
+                        const SampleRuleHost &rule, const double *rules, int64_t *index, double *logp, hipStream_t s);
+// utterances first .. first + n_utts - 1 of a batch, `rows` rows from row c0 on; C holds the costs of those rows only, the other
+// pointers are the whole batch's
+struct TrellisView {
+    const int64_t *cand; const double *tdist; const double *C; const int64_t *off;
+    int first, n_utts, K;
+    int64_t c0, rows, n_units;
+    double inv_tau;
+};
+void launch_position_bias(const int64_t *cand, const int32_t *join_class, const double *bias, const int64_t *edges, int n_classes,
+                          int n_buckets, int64_t rows, int K, double *C, hipStream_t s);
+void launch_trellis_forward(const TrellisView &v, bool sum, double *alpha, double *logz, hipStream_t s);
+void launch_trellis_backward(const TrellisView &v, double *beta, hipStream_t s);
+void launch_trellis_posterior(const TrellisView &v, const double *alpha, const double *beta, const double *logz, const int64_t *edges,
+                              int n_buckets, double *posterior, double *row_uses, hipStream_t s);
+void launch_trellis_uses(const double *row_uses, const int32_t *join_class, int64_t rows, int n_classes, int n_buckets, double *uses, hipStream_t s);
+void launch_trellis_draw(const TrellisView &v, const SampleRuleHost &rule, const double *alpha, const double *u, int n_draws, int64_t all_rows,
+                         int all_utts, int64_t *path, double *cost, double *logp, hipStream_t s);
+
 // ---- self test --------------------------------------------------------------
 void launch_mfma_selftest(const double *A, const double *B, double *C, hipStream_t s);
 

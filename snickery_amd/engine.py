@@ -39,6 +39,23 @@ _SIGNATURES = {
     'snk_set_weights': (ctypes.c_int, [ctypes.c_void_p, _c_f64p, ctypes.c_int, _c_f64p, ctypes.c_int]),
     'snk_knn': (ctypes.c_int, [ctypes.c_void_p, _c_f64p, ctypes.c_int64, ctypes.c_int, ctypes.c_int,
                                _c_i64p, _c_f64p]),
+    'snk_sample_rows': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
+                                       ctypes.c_int, ctypes.c_double, ctypes.c_int64, ctypes.c_double, ctypes.c_double, ctypes.c_void_p,
+                                       ctypes.c_void_p, ctypes.c_void_p]),
+    'snk_sample_rows_dev': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
+                                           ctypes.c_int, ctypes.c_double, ctypes.c_int64, ctypes.c_double, ctypes.c_double, ctypes.c_void_p,
+                                           ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    'snk_set_position_bias': (ctypes.c_int, [ctypes.c_void_p, _c_f64p, ctypes.c_int, ctypes.c_int, _c_i64p]),
+    'snk_sample_paths': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, _c_i64p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+                                        ctypes.c_void_p, ctypes.c_int, ctypes.c_double, ctypes.c_int64, ctypes.c_double, ctypes.c_double,
+                                        ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    'snk_sample_paths_dev': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, _c_i64p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+                                            ctypes.c_void_p, ctypes.c_int, ctypes.c_double, ctypes.c_int64, ctypes.c_double, ctypes.c_double,
+                                            ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    'snk_path_posterior': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, _c_i64p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+                                          ctypes.c_double, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+    'snk_path_posterior_dev': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, _c_i64p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
+                                              ctypes.c_double, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
     'snk_set_unit_classes': (ctypes.c_int, [ctypes.c_void_p, _c_i32p, ctypes.c_int64]),
     'snk_knn_by_class': (ctypes.c_int, [ctypes.c_void_p, _c_f64p, ctypes.c_int64, ctypes.c_int,
                                         ctypes.c_int, _c_i32p, _c_i64p, _c_f64p]),
@@ -159,6 +176,14 @@ def _f64(a):
 
 def _ptr(a, typ):
     return a.ctypes.data_as(typ)
+
+
+def _is_device(a):
+    """A torch tensor in GPU memory (everything else is taken as a numpy array)."""
+    return getattr(a, 'is_cuda', False) is True
+
+
+_SCORE_TYPES = {'float64': 0, 'float32': 1, 'float16': 2, 'bfloat16': 3}
 
 
 class QueryBatch(object):
@@ -490,6 +515,167 @@ class HipSearchEngine(object):
         self._check(self._lib.snk_path_scores(self._h, _ptr(Q, _c_f64p), _ptr(p, _c_i64p), L, int(mode),
                                               _ptr(tsq, _c_f64p), _ptr(jsq, _c_f64p)))
         return tsq, jsq
+
+    # -- draws and probabilities over the candidates ---------------------------
+    # Every method takes numpy arrays (and returns them: the results are there when it returns) or torch tensors on the engine's
+    # GPU (and returns tensors; the work is queued on torch's current stream).
+    def _tensor(self, a, dtype, shape, what):
+        import torch
+        if not _is_device(a):
+            raise SnkError('%s: expected a tensor on the GPU, like the other arguments' % what)
+        if a.device.index != self.device:
+            raise SnkError('%s is on %s, the engine on device %d' % (what, a.device, self.device))
+        if tuple(a.shape) != tuple(shape):
+            raise SnkError('%s has the shape %s, expected %s' % (what, tuple(a.shape), tuple(shape)))
+        if a.dtype != getattr(torch, dtype):
+            raise SnkError('%s has the type %s, expected %s' % (what, a.dtype, dtype))
+        return a.contiguous()
+
+    def _stream(self):
+        import torch
+        return ctypes.c_void_p(torch.cuda.current_stream(self.device).cuda_stream)
+
+    @staticmethod
+    def _rule(temperature, top_k, top_p, min_p):
+        if int(top_k) != top_k:
+            raise SnkError('top_k %s is not a whole number' % (top_k,))
+        return (float(temperature), int(top_k), float(top_p), float(min_p))
+
+    def sample_rows(self, scores, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """snk_sample_rows: draws from every row of scores (R, V) (float64, float32, float16, bfloat16) with the random numbers
+        u (R,) or (R, draws): (index int64, log probability float64), both shaped like u.  temperature, top_k, top_p and min_p
+        are numbers, or arrays of R for a rule per row."""
+        rules = (temperature, top_k, top_p, min_p)
+        per_row = any(np.ndim(r) > 0 for r in rules)
+        if getattr(scores, 'ndim', 0) != 2 or getattr(u, 'ndim', 0) not in (1, 2) or u.shape[0] != scores.shape[0]:
+            raise SnkError('sample_rows: scores (R, V) and random numbers (R,) or (R, draws) expected')
+        R, V = int(scores.shape[0]), int(scores.shape[1])
+        draws = 1 if u.ndim == 1 else int(u.shape[1])
+        if _is_device(scores):
+            import torch
+            name = str(scores.dtype).replace('torch.', '')
+            if name not in _SCORE_TYPES:
+                raise SnkError('sample_rows: scores of type %s' % scores.dtype)
+            if scores.device.index != self.device:
+                raise SnkError('scores are on %s, the engine on device %d' % (scores.device, self.device))
+            if V > 1 and scores.stride(1) != 1 or R > 1 and scores.stride(0) < V:
+                scores = scores.contiguous()
+            u = self._tensor(u, 'float64', u.shape, 'u')
+            table = None
+            if per_row:
+                cols = [r.to(dtype=torch.float64, device=scores.device) if torch.is_tensor(r) else
+                        torch.as_tensor(np.asarray(r, dtype=np.float64)).to(scores.device) for r in rules]
+                if any(c.ndim and tuple(c.shape) != (R,) for c in cols):
+                    raise SnkError('sample_rows: a rule per row needs %d entries' % R)
+                table = torch.stack([c.expand(R) for c in cols], 1).contiguous()
+            index = torch.empty(u.shape, dtype=torch.int64, device=scores.device)
+            logp = torch.empty(u.shape, dtype=torch.float64, device=scores.device)
+            rule = (1.0, 0, 1.0, 0.0) if per_row else self._rule(*rules)
+            self._check(self._lib.snk_sample_rows_dev(
+                self._h, scores.data_ptr(), _SCORE_TYPES[name], R, V, scores.stride(0) if R > 1 else V, u.data_ptr(), draws, *rule,
+                table.data_ptr() if per_row else None, index.data_ptr(), logp.data_ptr(), self._stream()))
+            return index, logp
+        scores = np.asarray(scores)
+        if str(scores.dtype) not in _SCORE_TYPES:
+            raise SnkError('sample_rows: scores of type %s' % scores.dtype)
+        size = scores.dtype.itemsize
+        if V > 1 and scores.strides[1] != size or R > 1 and (scores.strides[0] < V * size or scores.strides[0] % size):
+            scores = np.ascontiguousarray(scores)
+        u = _f64(u)
+        table = None
+        if per_row:
+            cols = [np.asarray(r, dtype=np.float64) for r in rules]
+            if any(c.ndim and c.shape != (R,) for c in cols):
+                raise SnkError('sample_rows: a rule per row needs %d entries' % R)
+            table = np.ascontiguousarray(np.stack([np.broadcast_to(c, (R,)) for c in cols], axis=1))
+        index = np.empty(u.shape, dtype=np.int64)
+        logp = np.empty(u.shape, dtype=np.float64)
+        rule = (1.0, 0, 1.0, 0.0) if per_row else self._rule(*rules)
+        self._check(self._lib.snk_sample_rows(
+            self._h, scores.ctypes.data, _SCORE_TYPES[str(scores.dtype)], R, V, scores.strides[0] // size if R > 1 else V, u.ctypes.data, draws,
+            *rule, table.ctypes.data if per_row else None, index.ctypes.data, logp.ctypes.data))
+        return index, logp
+
+    def set_position_bias(self, bias, edges=()):
+        """snk_set_position_bias: bias (classes, buckets) on joining unit i to unit j, bucket = number of edges <= j - i; None
+        clears it.  Applies to sample_paths and path_posterior."""
+        if bias is None:
+            self._check(self._lib.snk_set_position_bias(self._h, None, 0, 0, None))
+            self._bias_shape = None
+            return
+        b = _f64(bias)
+        e = np.ascontiguousarray(edges, dtype=np.int64)
+        if b.ndim != 2 or b.size == 0 or e.shape != (b.shape[1] - 1,):
+            raise SnkError('set_position_bias: bias (classes, buckets) and buckets - 1 edges expected')
+        self._bias_shape = None
+        self._check(self._lib.snk_set_position_bias(self._h, _ptr(b, _c_f64p), b.shape[0], b.shape[1], _ptr(e, _c_i64p)))
+        self._bias_shape = b.shape
+
+    def _trellis(self, candidates, distances, row_offsets, join_class):
+        """(on device, candidates, distances, offsets, classes or None, pointers of the three)"""
+        if getattr(candidates, 'ndim', 0) != 2:
+            raise SnkError('candidates (rows, K) expected')
+        rows, K = int(candidates.shape[0]), int(candidates.shape[1])
+        offs = np.array([0, rows] if row_offsets is None else row_offsets, dtype=np.int64)
+        if offs.ndim != 1 or offs.size < 2 or int(offs[-1]) != rows:
+            raise SnkError('row_offsets have to end at the %d rows of the candidates' % rows)
+        if _is_device(candidates):
+            c = self._tensor(candidates, 'int64', (rows, K), 'candidates')
+            d = self._tensor(distances, 'float64', (rows, K), 'distances')
+            k = None if join_class is None else self._tensor(join_class, 'int32', (rows,), 'join_class')
+            return True, c, d, offs, k, (c.data_ptr(), d.data_ptr(), None if k is None else k.data_ptr())
+        c = np.ascontiguousarray(candidates, dtype=np.int64)
+        d = _f64(distances)
+        k = None if join_class is None else np.ascontiguousarray(join_class, dtype=np.int32)
+        if d.shape != c.shape or (k is not None and k.shape != (rows,)):
+            raise SnkError('distances (rows, K) and join_class (rows,) have to fit the candidates')
+        return False, c, d, offs, k, (c.ctypes.data, d.ctypes.data, None if k is None else k.ctypes.data)
+
+    def sample_paths(self, candidates, distances, u, row_offsets=None, join_class=None, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
+        """snk_sample_paths: paths drawn from exp(-cost / temperature) over the candidates (rows, K) of the utterances that
+        row_offsets separates (default: one), a draw per row of random numbers u (draws, rows); join_class (rows,) int32 picks the
+        row of the position bias for the join from row r to r + 1.
+        Returns (unit ids (draws, rows) int64, costs (draws, utterances), log probabilities (draws, utterances))."""
+        dev, c, d, offs, k, ptr = self._trellis(candidates, distances, row_offsets, join_class)
+        rows, n = int(c.shape[0]), offs.size - 1
+        if getattr(u, 'ndim', 0) != 2 or int(u.shape[1]) != rows:
+            raise SnkError('sample_paths: random numbers (draws, rows) expected')
+        S = int(u.shape[0])
+        rule = self._rule(temperature, top_k, top_p, min_p)
+        if dev:
+            import torch
+            u = self._tensor(u, 'float64', (S, rows), 'u')
+            path = torch.empty((S, rows), dtype=torch.int64, device=c.device)
+            out = torch.empty((2, S, n), dtype=torch.float64, device=c.device)
+            self._check(self._lib.snk_sample_paths_dev(self._h, ptr[0], ptr[1], _ptr(offs, _c_i64p), n, int(c.shape[1]), ptr[2], u.data_ptr(), S, *rule,
+                                                       path.data_ptr(), out[0].data_ptr(), out[1].data_ptr(), self._stream()))
+            return path, out[0], out[1]
+        u = _f64(u)
+        path = np.empty((S, rows), dtype=np.int64)
+        cost, logp = np.empty((S, n)), np.empty((S, n))
+        self._check(self._lib.snk_sample_paths(self._h, ptr[0], ptr[1], _ptr(offs, _c_i64p), n, int(c.shape[1]), ptr[2], u.ctypes.data, S, *rule,
+                                               path.ctypes.data, cost.ctypes.data, logp.ctypes.data))
+        return path, cost, logp
+
+    def path_posterior(self, candidates, distances, row_offsets=None, join_class=None, temperature=1.0):
+        """snk_path_posterior: (logZ (utterances,), posterior of every candidate (rows, K), expected uses of every entry of the
+        position bias (classes, buckets) -- None while no bias is set).  d logZ / d distances = -posterior / temperature,
+        d sum(logZ) / d bias = -uses / temperature."""
+        dev, c, d, offs, k, ptr = self._trellis(candidates, distances, row_offsets, join_class)
+        n, shape = offs.size - 1, getattr(self, '_bias_shape', None)
+        if dev:
+            import torch
+            logz = torch.empty((n,), dtype=torch.float64, device=c.device)
+            post = torch.empty(tuple(c.shape), dtype=torch.float64, device=c.device)
+            uses = None if shape is None else torch.empty(shape, dtype=torch.float64, device=c.device)
+            self._check(self._lib.snk_path_posterior_dev(self._h, ptr[0], ptr[1], _ptr(offs, _c_i64p), n, int(c.shape[1]), ptr[2], float(temperature),
+                                                         logz.data_ptr(), post.data_ptr(), None if uses is None else uses.data_ptr(), self._stream()))
+            return logz, post, uses
+        logz, post = np.empty((n,)), np.empty(c.shape)
+        uses = None if shape is None else np.empty(shape)
+        self._check(self._lib.snk_path_posterior(self._h, ptr[0], ptr[1], _ptr(offs, _c_i64p), n, int(c.shape[1]), ptr[2], float(temperature),
+                                                 logz.ctypes.data, post.ctypes.data, None if uses is None else uses.ctypes.data))
+        return logz, post, uses
 
     # -- multi-GPU (device pointers) ------------------------------------------
     def knn_local_dev(self, unit_features, n_candidates, d2_dev_ptr, id_dev_ptr):
