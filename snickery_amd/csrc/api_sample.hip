@@ -125,9 +125,14 @@ int snk_set_position_bias(snk_handle h, const double *bias, int n_classes, int n
     HIPCHK(hipSetDevice(h->device));
     h->pb_classes = 0;
     CHK(h->pb_bias.ensure((size_t)n * sizeof(double)));
-    CHK(h->pb_edges.ensure(64 * sizeof(int64_t)));
+    CHK(h->pb_edges.ensure(64 * sizeof(int)));
     CHK(h2d_sync(h, h->pb_bias.p, bias, (size_t)n * sizeof(double)));
-    if (n_buckets > 1) CHK(h2d_sync(h, h->pb_edges.p, edges, (size_t)(n_buckets - 1) * sizeof(int64_t)));
+    // unit ids have 31 bits: distances and edges fit 32, edges beyond them are never / always reached
+    int e32[64] = {0};
+    for (int i = 0; i < n_buckets - 1; ++i) e32[i] = (int)std::min<int64_t>(std::max<int64_t>(edges[i], -0x7fffffff - 1LL), 0x7fffffff);
+    CHK(h2d_sync(h, h->pb_edges.p, e32, sizeof(e32)));
+    h->pb_min = 0.0;
+    for (int64_t i = 0; i < n; ++i) h->pb_min = std::min(h->pb_min, bias[i]);
     h->pb_classes = n_classes;
     h->pb_buckets = n_buckets;
     return 0;
@@ -152,83 +157,108 @@ static int check_trellis(const char *who, snk_engine *h, const void *cand, const
 // keeps a handful of compute units busy in the recursions).  An utterance that is longer than that is a group by itself.
 static const size_t kTrellisGroupBytes = (size_t)4 << 30;
 
+struct TrellisCall {
+    const char *who; bool timed;                    // stage timers (calls that wait for their results)
+    const int64_t *cand; const double *tdist; const int64_t *row_offsets; const int32_t *join_class;
+    int n_utts, K;
+    double temperature;
+};
+
+// `use` gets the group's view (cells not made yet), the costs' parts
 template <typename Use>
-static int trellis_groups(snk_engine *h, bool timed, const int64_t *cand, const double *tdist, const int32_t *join_class, const int64_t *off_dev,
-                          const int64_t *row_offsets, int n_utts, int K, double inv_tau, Use use)
+static int trellis_groups(snk_engine *h, const TrellisCall &q, Use use)
 {
-    const size_t row_bytes = (size_t)K * K * sizeof(double);
-    for (int v0 = 0; v0 < n_utts;) {
+    const int64_t rows = q.row_offsets[q.n_utts];
+    const int Kp = roundup(q.K, 8);
+    const size_t row_bytes = (size_t)q.K * Kp * sizeof(double);
+    CHK(h->tr_off.ensure((size_t)(q.n_utts + 1) * sizeof(int64_t)));
+    CHK(h2d(h, h->tr_off.p, q.row_offsets, (size_t)(q.n_utts + 1) * sizeof(int64_t), h->stream));
+    CHK(h->tr_V.ensure((size_t)rows * Kp * sizeof(double)));
+    CHK(h->tr_local.ensure((size_t)rows * Kp * sizeof(double)));
+    CHK(h->tr_least.ensure((size_t)rows * sizeof(double)));
+    CHK(h->tr_flag.ensure((size_t)q.n_utts * sizeof(int)));
+    // temperature 0: every utterance goes through the launches that keep the largest term
+    HIPCHK(hipMemsetAsync(h->tr_flag.p, q.temperature > 0.0 ? 0 : 1, (size_t)q.n_utts * sizeof(int), h->stream));
+    TrellisCosts c;
+    c.JC = h->JC_unw.as<float>(); c.Jp = h->Jp; c.Dj = h->Dj; c.wj = h->wj.as<double>();
+    c.join_class = q.join_class; c.bias = h->pb_bias.as<double>(); c.edges = h->pb_edges.as<int>();
+    c.n_classes = h->pb_classes; c.n_buckets = h->pb_buckets;
+    c.bias_min = h->pb_classes > 0 ? h->pb_min : 0.0;
+    for (int v0 = 0; v0 < q.n_utts;) {
         int v1 = v0 + 1;
-        while (v1 < n_utts && (size_t)(row_offsets[v1 + 1] - row_offsets[v0]) * row_bytes <= kTrellisGroupBytes) ++v1;
-        TrellisView view;
-        view.cand = cand; view.tdist = tdist; view.off = off_dev;
-        view.first = v0; view.n_utts = v1 - v0; view.K = K;
-        view.c0 = row_offsets[v0]; view.rows = row_offsets[v1] - row_offsets[v0];
-        view.n_units = h->Njc - 1;
-        view.inv_tau = inv_tau;
-        CHK(h->tr_C.ensure((size_t)view.rows * row_bytes));
-        view.C = h->tr_C.as<double>();
-        {
-            StageTimer t(h, h->stream, timed ? TM_JOIN : -1);
-            launch_join_costs(h->JCw.as<double>(), h->Djpad, h->Dj, view.n_units, cand + view.c0 * K, view.rows, K, h->tr_C.as<double>(), h->stream);
-            if (h->pb_classes > 0)
-                launch_position_bias(cand + view.c0 * K, join_class ? join_class + view.c0 : nullptr, h->pb_bias.as<double>(), h->pb_edges.as<int64_t>(),
-                                     h->pb_classes, h->pb_buckets, view.rows, K, h->tr_C.as<double>(), h->stream);
-        }
-        CHK(use(view));
+        while (v1 < q.n_utts && (size_t)(q.row_offsets[v1 + 1] - q.row_offsets[v0]) * row_bytes <= kTrellisGroupBytes) ++v1;
+        TrellisView v;
+        v.cand = q.cand; v.tdist = q.tdist; v.off = h->tr_off.as<int64_t>();
+        v.first = v0; v.n_utts = v1 - v0; v.K = q.K; v.Kp = Kp;
+        v.c0 = q.row_offsets[v0]; v.rows = q.row_offsets[v1] - q.row_offsets[v0];
+        v.n_units = h->Njc - 1;
+        v.inv_tau = q.temperature > 0.0 ? 1.0 / q.temperature : 1.0;
+        CHK(h->tr_C.ensure((size_t)v.rows * row_bytes));
+        v.C = h->tr_C.as<double>();
+        CHK(use(v, c));
         v0 = v1;
     }
     HIPCHK(hipGetLastError());
     return 0;
 }
 
-static int trellis_offsets(snk_engine *h, const int64_t *row_offsets, int n_utts)
+static int sample_paths_device(snk_engine *h, const TrellisCall &q, const double *u, int n_draws, const SampleRuleHost &rule, int64_t *path,
+                               double *cost, double *logp)
 {
-    CHK(h->tr_off.ensure((size_t)(n_utts + 1) * sizeof(int64_t)));
-    return h2d(h, h->tr_off.p, row_offsets, (size_t)(n_utts + 1) * sizeof(int64_t), h->stream);
-}
-
-static int sample_paths_device(snk_engine *h, bool timed, const int64_t *cand, const double *tdist, const int64_t *row_offsets, int n_utts,
-                               int K, const int32_t *join_class, const double *u, int n_draws, const SampleRuleHost &rule,
-                               int64_t *path, double *cost, double *logp)
-{
-    const int64_t rows = row_offsets[n_utts];
-    const bool sum = rule.temperature > 0.0;
-    CHK(trellis_offsets(h, row_offsets, n_utts));
-    CHK(h->tr_alpha.ensure((size_t)rows * K * sizeof(double)));
-    return trellis_groups(h, timed, cand, tdist, join_class, h->tr_off.as<int64_t>(), row_offsets, n_utts, K, sum ? 1.0 / rule.temperature : 1.0,
-                          [&](const TrellisView &view) -> int {
-        {
-            StageTimer t(h, h->stream, timed ? TM_TRELLIS_SUM : -1);
-            launch_trellis_forward(view, sum, h->tr_alpha.as<double>(), nullptr, h->stream);
+    const int64_t rows = q.row_offsets[q.n_utts];
+    size_t at[5];
+    CHK(h->tr_draw.ensure(trellis_draw_bytes(rows, q.n_utts, q.K, n_draws, at)));
+    return trellis_groups(h, q, [&](const TrellisView &v, const TrellisCosts &c) -> int {
+        const bool sum = q.temperature > 0.0;
+        int *flag = h->tr_flag.as<int>();
+        double *V = h->tr_V.as<double>(), *X = h->tr_C.as<double>();
+        if (sum) {
+            {
+                StageTimer t(h, h->stream, q.timed ? TM_JOIN : -1);
+                launch_trellis_local(v, h->tr_local.as<double>(), h->tr_least.as<double>(), flag, h->stream);
+                launch_trellis_costs(v, c, false, flag, X, h->stream);
+            }
+            StageTimer t(h, h->stream, q.timed ? TM_TRELLIS_SUM : -1);
+            launch_trellis_forward(v, h->tr_local.as<double>(), h->tr_least.as<double>(), c.bias_min, flag, V, nullptr, h->stream);
         }
-        StageTimer t(h, h->stream, timed ? TM_TRELLIS_DRAW : -1);
-        launch_trellis_draw(view, rule, h->tr_alpha.as<double>(), u, n_draws, rows, n_utts, path, cost, logp, h->stream);
+        {
+            StageTimer t(h, h->stream, q.timed ? TM_TRELLIS_SUM : -1);
+            launch_trellis_costs(v, c, true, flag, X, h->stream);
+            launch_trellis_forward_log(v, sum, flag, V, nullptr, h->stream);
+        }
+        StageTimer t(h, h->stream, q.timed ? TM_TRELLIS_DRAW : -1);
+        launch_trellis_draw(v, c, rule, flag, V, u, n_draws, rows, q.n_utts, h->tr_draw.as<char>(), path, cost, logp, h->stream);
         return 0;
     });
 }
 
-static int path_posterior_device(snk_engine *h, bool timed, const int64_t *cand, const double *tdist, const int64_t *row_offsets, int n_utts,
-                                 int K, const int32_t *join_class, double temperature, double *logz, double *posterior, double *uses)
+static int path_posterior_device(snk_engine *h, const TrellisCall &q, double *logz, double *posterior, double *uses)
 {
-    const int64_t rows = row_offsets[n_utts];
-    CHK(trellis_offsets(h, row_offsets, n_utts));
-    CHK(h->tr_alpha.ensure((size_t)rows * K * sizeof(double)));
-    CHK(h->tr_beta.ensure((size_t)rows * K * sizeof(double)));
+    const int64_t rows = q.row_offsets[q.n_utts];
+    CHK(h->tr_W.ensure((size_t)rows * roundup(q.K, 8) * sizeof(double)));
     if (uses) CHK(h->tr_row_uses.ensure((size_t)rows * h->pb_buckets * sizeof(double)));
-    CHK(trellis_groups(h, timed, cand, tdist, join_class, h->tr_off.as<int64_t>(), row_offsets, n_utts, K, 1.0 / temperature,
-                       [&](const TrellisView &view) -> int {
+    CHK(trellis_groups(h, q, [&](const TrellisView &v, const TrellisCosts &c) -> int {
+        int *flag = h->tr_flag.as<int>();
+        double *V = h->tr_V.as<double>(), *W = h->tr_W.as<double>(), *X = h->tr_C.as<double>(), *local = h->tr_local.as<double>();
         {
-            StageTimer t(h, h->stream, timed ? TM_TRELLIS_SUM : -1);
-            launch_trellis_forward(view, true, h->tr_alpha.as<double>(), logz, h->stream);
-            launch_trellis_backward(view, h->tr_beta.as<double>(), h->stream);
+            StageTimer t(h, h->stream, q.timed ? TM_JOIN : -1);
+            launch_trellis_local(v, local, h->tr_least.as<double>(), flag, h->stream);
+            launch_trellis_costs(v, c, false, flag, X, h->stream);
         }
-        StageTimer t(h, h->stream, timed ? TM_TRELLIS_POST : -1);
-        launch_trellis_posterior(view, h->tr_alpha.as<double>(), h->tr_beta.as<double>(), logz, h->pb_edges.as<int64_t>(), h->pb_buckets,
-                                 posterior, uses ? h->tr_row_uses.as<double>() : nullptr, h->stream);
+        {
+            StageTimer t(h, h->stream, q.timed ? TM_TRELLIS_SUM : -1);
+            launch_trellis_forward(v, local, h->tr_least.as<double>(), c.bias_min, flag, V, logz, h->stream);
+            launch_trellis_backward(v, local, flag, W, h->stream);
+            launch_trellis_costs(v, c, true, flag, X, h->stream);
+            launch_trellis_forward_log(v, true, flag, V, logz, h->stream);
+            launch_trellis_backward_log(v, flag, W, h->stream);
+        }
+        StageTimer t(h, h->stream, q.timed ? TM_TRELLIS_POST : -1);
+        launch_trellis_posterior(v, flag, V, W, local, logz, h->pb_edges.as<int>(), h->pb_buckets, posterior,
+                                 uses ? h->tr_row_uses.as<double>() : nullptr, h->stream);
         return 0;
     }));
-    if (uses) launch_trellis_uses(h->tr_row_uses.as<double>(), join_class, rows, h->pb_classes, h->pb_buckets, uses, h->stream);
+    if (uses) launch_trellis_uses(h->tr_row_uses.as<double>(), q.join_class, rows, h->pb_classes, h->pb_buckets, uses, h->stream);
     HIPCHK(hipGetLastError());
     return 0;
 }
@@ -297,9 +327,10 @@ int snk_sample_paths(snk_handle h, const int64_t *cand, const double *tdist, con
     CHK(upload_trellis(h, cand, tdist, rows, K, join_class));
     CHK(h2d(h, h->tr_u.p, u, np, h->stream));
     char *out = h->tr_out.as<char>();
-    CHK(sample_paths_device(h, true, h->tr_cand.as<int64_t>(), h->tr_tdist.as<double>(), row_offsets, n_utts, K,
-                            join_class ? h->tr_class.as<int32_t>() : nullptr, h->tr_u.as<double>(), n_draws, rule, (int64_t *)out,
-                            (double *)(out + np), logp_out ? (double *)(out + np + nc) : nullptr));
+    const TrellisCall q = {who, true, h->tr_cand.as<int64_t>(), h->tr_tdist.as<double>(), row_offsets, join_class ? h->tr_class.as<int32_t>() : nullptr,
+                           n_utts, K, temperature};
+    CHK(sample_paths_device(h, q, h->tr_u.as<double>(), n_draws, rule, (int64_t *)out, (double *)(out + np),
+                            logp_out ? (double *)(out + np + nc) : nullptr));
     D2HPart parts[3] = {{path_out, out, np}, {cost_out, out + np, nc}, {logp_out, out + np + nc, logp_out ? nc : 0}};
     CHK(staged_d2h(h, h->stream, parts, 3));
     collect_timers(h);
@@ -317,8 +348,8 @@ int snk_sample_paths_dev(snk_handle h, const int64_t *cand_dev, const double *td
     DeviceGuard device;
     CHK(device.enter(h->device));
     CHK(trellis_enter(h, who, (hipStream_t)stream));
-    CHK(sample_paths_device(h, false, cand_dev, tdist_dev, row_offsets, n_utts, K, join_class_dev, u_dev, n_draws, rule, path_dev_out, cost_dev_out,
-                            logp_dev_out));
+    const TrellisCall q = {who, false, cand_dev, tdist_dev, row_offsets, join_class_dev, n_utts, K, temperature};
+    CHK(sample_paths_device(h, q, u_dev, n_draws, rule, path_dev_out, cost_dev_out, logp_dev_out));
     return trellis_leave(h, (hipStream_t)stream);
 }
 
@@ -342,9 +373,9 @@ int snk_path_posterior(snk_handle h, const int64_t *cand, const double *tdist, c
     CHK(h->tr_out.ensure(nz + np + nu));
     CHK(upload_trellis(h, cand, tdist, rows, K, join_class));
     char *out = h->tr_out.as<char>();
-    CHK(path_posterior_device(h, true, h->tr_cand.as<int64_t>(), h->tr_tdist.as<double>(), row_offsets, n_utts, K,
-                              join_class ? h->tr_class.as<int32_t>() : nullptr, temperature, (double *)out, (double *)(out + nz),
-                              uses_out ? (double *)(out + nz + np) : nullptr));
+    const TrellisCall q = {who, true, h->tr_cand.as<int64_t>(), h->tr_tdist.as<double>(), row_offsets, join_class ? h->tr_class.as<int32_t>() : nullptr,
+                           n_utts, K, temperature};
+    CHK(path_posterior_device(h, q, (double *)out, (double *)(out + nz), uses_out ? (double *)(out + nz + np) : nullptr));
     D2HPart parts[3] = {{logz_out, out, nz}, {posterior_out, out + nz, np}, {uses_out, out + nz + np, nu}};
     CHK(staged_d2h(h, h->stream, parts, 3));
     collect_timers(h);
@@ -361,7 +392,7 @@ int snk_path_posterior_dev(snk_handle h, const int64_t *cand_dev, const double *
     DeviceGuard device;
     CHK(device.enter(h->device));
     CHK(trellis_enter(h, who, (hipStream_t)stream));
-    CHK(path_posterior_device(h, false, cand_dev, tdist_dev, row_offsets, n_utts, K, join_class_dev, temperature, logz_dev_out, posterior_dev_out,
-                              uses_dev_out));
+    const TrellisCall q = {who, false, cand_dev, tdist_dev, row_offsets, join_class_dev, n_utts, K, temperature};
+    CHK(path_posterior_device(h, q, logz_dev_out, posterior_dev_out, uses_dev_out));
     return trellis_leave(h, (hipStream_t)stream);
 }

@@ -45,6 +45,7 @@ __device__ __forceinline__ double sample_exponent(double x, double m, double inv
 }
 
 // w in units of 2^-s; unit = 2^s, s <= 51.  2^52 + w 2^s < 2^53: the sum's last place is 1, its mantissa is the rounded weight
+#define SNK_SAMPLE_UNIT 2251799813685248.0       // 2^51
 __device__ __forceinline__ u64 sample_fix(double w, double unit)
 {
     const double t = __fma_rn(w, unit, 4503599627370496.0);
@@ -73,34 +74,64 @@ __device__ __forceinline__ u64 sample_exceed(double u, u64 total)
     return t >= (double)total ? total - 1 : (u64)t;
 }
 
-// ---- one wavefront, one row of up to 64 E scores: lane l holds the elements l E .. l E + E - 1 --------------------------------
+// ---- wavefront sums and maxima on the data-parallel moves: a step costs two moves and one operation, where a shuffle through
+// the LDS pipe waits ~ 100 cycles -- the six steps of a reduction are most of what a short row costs -------------------------------
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 dpp_move(u64 old, u64 v)
+{
+    const int lo = __builtin_amdgcn_update_dpp((int)(unsigned int)old, (int)(unsigned int)v, CTRL, ROWS, 0xf, false);
+    const int hi = __builtin_amdgcn_update_dpp((int)(unsigned int)(old >> 32), (int)(unsigned int)(v >> 32), CTRL, ROWS, 0xf, false);
+    return ((u64)(unsigned int)hi << 32) | (unsigned int)lo;
+}
+// (every lane of the wavefront has to be active in these)
+__device__ __forceinline__ u64 wave_scan_add(u64 v)        // inclusive: within rows of 16 lanes, then the rows below
+{
+    v += dpp_move<0x111, 0xf>(0, v);
+    v += dpp_move<0x112, 0xf>(0, v);
+    v += dpp_move<0x114, 0xf>(0, v);
+    v += dpp_move<0x118, 0xf>(0, v);
+    v += dpp_move<0x142, 0xa>(0, v);
+    v += dpp_move<0x143, 0xc>(0, v);
+    return v;
+}
+__device__ __forceinline__ u64 wave_lane(u64 v, int lane)    // uniform lane
+{
+    const unsigned int lo = (unsigned int)__builtin_amdgcn_readlane((int)(unsigned int)v, lane);
+    const unsigned int hi = (unsigned int)__builtin_amdgcn_readlane((int)(unsigned int)(v >> 32), lane);
+    return ((u64)hi << 32) | lo;
+}
+__device__ __forceinline__ double wave_lane(double v, int lane)
+{
+    return __longlong_as_double((long long)wave_lane((u64)__double_as_longlong(v), lane));
+}
+__device__ __forceinline__ u64 wave_add(u64 v) { return wave_lane(wave_scan_add(v), 63); }
+__device__ __forceinline__ double dpp_max(double v, u64 moved) { return fmax(v, __longlong_as_double((long long)moved)); }
 __device__ __forceinline__ double wave_max(double v)
 {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v = fmax(v, __shfl_xor(v, o, 64));
-    return v;
+#define SNK_BITS(x_) ((u64)__double_as_longlong(x_))
+    v = dpp_max(v, dpp_move<0x111, 0xf>(SNK_BITS(v), SNK_BITS(v)));
+    v = dpp_max(v, dpp_move<0x112, 0xf>(SNK_BITS(v), SNK_BITS(v)));
+    v = dpp_max(v, dpp_move<0x114, 0xf>(SNK_BITS(v), SNK_BITS(v)));
+    v = dpp_max(v, dpp_move<0x118, 0xf>(SNK_BITS(v), SNK_BITS(v)));
+    v = dpp_max(v, dpp_move<0x142, 0xa>(SNK_BITS(v), SNK_BITS(v)));
+    v = dpp_max(v, dpp_move<0x143, 0xc>(SNK_BITS(v), SNK_BITS(v)));
+    return wave_lane(v, 63);
 }
-__device__ __forceinline__ u64 wave_add(u64 v)
+__device__ __forceinline__ double wave_sum(double v)
 {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o, 64);
-    return v;
-}
-__device__ __forceinline__ u64 wave_scan_add(u64 v)        // inclusive
-{
-    const int lane = threadIdx.x & 63;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const u64 b = __shfl_up(v, o, 64);
-        if (lane >= o) v += b;
-    }
-    return v;
+    v += __longlong_as_double((long long)dpp_move<0x111, 0xf>(0, SNK_BITS(v)));
+    v += __longlong_as_double((long long)dpp_move<0x112, 0xf>(0, SNK_BITS(v)));
+    v += __longlong_as_double((long long)dpp_move<0x114, 0xf>(0, SNK_BITS(v)));
+    v += __longlong_as_double((long long)dpp_move<0x118, 0xf>(0, SNK_BITS(v)));
+    v += __longlong_as_double((long long)dpp_move<0x142, 0xa>(0, SNK_BITS(v)));
+    v += __longlong_as_double((long long)dpp_move<0x143, 0xc>(0, SNK_BITS(v)));
+#undef SNK_BITS
+    return wave_lane(v, 63);
 }
 
+// ---- one wavefront, one row of up to 64 E scores: lane l holds the elements l E .. l E + E - 1 --------------------------------
 template <int E>
 struct WaveRow {
-    double m;                   // the row's maximum; -inf: empty
-    double log_total;           // log of the kept mass
     u64 total;                  // the kept mass
     u64 before;                 // kept mass in the lanes below
     u64 w[E];                   // kept weights (0: not kept)
@@ -113,28 +144,17 @@ __device__ __forceinline__ int nth_bit(u64 mask, int n)
     return __ffsll((long long)mask) - 1;
 }
 
+// The truncations.  x: the order's values (-inf: takes no part), row.w: their weights in units of 1 / unit (equal values, equal
+// weights; the largest weighs `unit`).  On return row.w is what is kept, row.before / row.total its sums.
 template <int E>
-__device__ __forceinline__ void wave_row_weights(const double (&x)[E], const SampleRule &rule, double unit, WaveRow<E> &row)
+__device__ __forceinline__ void wave_row_keep(const double (&x)[E], const SampleRule &rule, double unit, WaveRow<E> &row)
 {
     const double ninf = -__builtin_inf();
-    double m = ninf;
-#pragma unroll
-    for (int e = 0; e < E; ++e) m = fmax(m, x[e]);
-    m = wave_max(m);
-    row.m = m;
-    if (m == ninf) { row.total = 0; return; }
-    u64 mass = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-        row.w[e] = x[e] == ninf ? 0 : sample_weight(sample_exponent(x[e], m, rule.inv_tau), unit);
-        mass += row.w[e];
-    }
-
-    // The order's prefix: found by bisection on the scores themselves.  `live` are the elements whose side is not known yet; a
-    // pivot among them splits them, one ballot per element slot counts a side.  The middle live element is the pivot: a sorted
-    // list is halved, an unsorted one takes ~ 2 ln V rounds.
+    // The order's prefix, by bisection on the values: `live` are the elements whose side is not known yet, a pivot among them splits
+    // them, one ballot per element slot counts a side.  The middle live element is the pivot: a sorted list is halved, an
+    // unsorted one takes ~ 2 ln V rounds.
     double cut = ninf;          // kept: x > cut, and the first n_tie of the elements equal to it
-    int n_tie = 64 * E;
+    int n_tie = 0, ties = 0;
     auto search = [&](bool by_mass, u64 want) {
         u64 above = 0;                                          // count / mass of everything above the live elements
         unsigned live = 0;
@@ -146,48 +166,59 @@ __device__ __forceinline__ void wave_row_weights(const double (&x)[E], const Sam
 #pragma unroll
             for (int e = 0; e < E; ++e) { b[e] = __ballot((live >> e) & 1u); n += __popcll(b[e]); }
             if (n == 0) return;                                 // (the prefix is the whole row)
-            // the middle one
-            int left = n >> 1;
+            int left = n >> 1;                                  // the middle one
             double pivot = 0.0;
+            u64 weight = 0;
             bool found = false;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const int c = __popcll(b[e]);
-                if (!found && left < c) { pivot = __shfl(x[e], nth_bit(b[e], left), 64); found = true; }
+                if (!found && left < c) {
+                    const int l = nth_bit(b[e], left);
+                    pivot = wave_lane(x[e], l);
+                    weight = wave_lane(row.w[e], l);
+                    found = true;
+                }
                 if (!found) left -= c;
             }
-            u64 gt = 0, eq = 0;
+            u64 gt = 0;
+            int eq = 0;
             unsigned mgt = 0, meq = 0;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const bool l = (live >> e) & 1u, g = l && x[e] > pivot, q = l && x[e] == pivot;
                 mgt |= g ? 1u << e : 0u;
                 meq |= q ? 1u << e : 0u;
-                if (by_mass) { gt += g ? row.w[e] : 0; eq += q ? row.w[e] : 0; }
-                else { gt += __popcll(__ballot(g)); eq += __popcll(__ballot(q)); }
+                if (by_mass) gt += g ? row.w[e] : 0;
+                else gt += __popcll(__ballot(g));
+                eq += __popcll(__ballot(q));
             }
-            if (by_mass) { gt = wave_add(gt); eq = wave_add(eq); }
+            if (by_mass) gt = wave_add(gt);
             if (above + gt >= want) { live = mgt; continue; }
-            if (above + gt + eq >= want) {
+            const u64 each = by_mass ? weight : 1;               // (equal values: equal weights)
+            if (above + gt + each * (u64)eq >= want) {
                 cut = pivot;
-                if (by_mass) {
-                    int c = 0;
-#pragma unroll
-                    for (int e = 0; e < E; ++e) c += __popcll(__ballot((meq >> e) & 1u));
-                    const u64 each = eq / (u64)c;               // (equal scores: equal weights)
-                    n_tie = (int)((want - above - gt + each - 1) / each);
-                } else n_tie = (int)(want - above - gt);
+                ties = eq;
+                u64 need = want - above - gt;
+                n_tie = 0;
+                if (each == 1) n_tie = (int)need;
+                else while (need) { ++n_tie; need = need > each ? need - each : 0; }
                 return;
             }
-            above += gt + eq;
+            above += gt + each * (u64)eq;
             live &= ~(mgt | meq);
         }
     };
     auto apply = [&]() {        // weights outside the prefix -> 0
-        int ties = 0;
+        if (ties == n_tie) {
 #pragma unroll
-        for (int e = 0; e < E; ++e) ties += (x[e] == cut) ? 1 : 0;
-        int rank = (int)(wave_scan_add((u64)ties)) - ties;       // equal elements in the lanes below
+            for (int e = 0; e < E; ++e) row.w[e] = x[e] >= cut ? row.w[e] : 0;
+            return;
+        }
+        int mine = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) mine += (x[e] == cut) ? 1 : 0;
+        int rank = (int)wave_scan_add((u64)mine) - mine;         // equal elements in the lanes below
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const bool tie = x[e] == cut;
@@ -195,36 +226,33 @@ __device__ __forceinline__ void wave_row_weights(const double (&x)[E], const Sam
             rank += tie ? 1 : 0;
         }
     };
+    auto sum = [&]() {
+        u64 mass = 0;
+#pragma unroll
+        for (int e = 0; e < E; ++e) mass += row.w[e];
+        return mass;
+    };
     if (rule.top_k > 0 && rule.top_k < 64 * E) {
         search(false, (u64)rule.top_k);
-        if (cut > ninf) {
-            apply();
-            mass = 0;
-#pragma unroll
-            for (int e = 0; e < E; ++e) mass += row.w[e];
-        }
+        if (cut > ninf) apply();
     }
     if (rule.top_p < 1.0) {
-        const u64 total = wave_add(mass);
-        cut = ninf; n_tie = 64 * E;
+        const u64 total = wave_add(sum());
+        cut = ninf;
         search(true, sample_reach(rule.top_p, total));
         if (cut > ninf) apply();
     }
     if (rule.min_p > 0.0) {
+        const double least = rule.min_p * unit;
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if (row.w[e] && exp(sample_exponent(x[e], m, rule.inv_tau)) < rule.min_p) row.w[e] = 0;
+        for (int e = 0; e < E; ++e) row.w[e] = (double)row.w[e] < least ? 0 : row.w[e];
     }
-    mass = 0;
-#pragma unroll
-    for (int e = 0; e < E; ++e) mass += row.w[e];
-    const u64 upto = wave_scan_add(mass);
+    const u64 mass = sum(), upto = wave_scan_add(mass);
     row.before = upto - mass;
-    row.total = __shfl(upto, 63, 64);
-    row.log_total = log((double)row.total / unit);
+    row.total = wave_lane(upto, 63);
 }
 
-// element that u picks (uniform), the lane that holds it and its slot
+// element that u picks, the lane that holds it and its slot (uniform)
 template <int E>
 __device__ __forceinline__ int wave_row_pick(const WaveRow<E> &row, double u, int &lane_out, int &slot_out)
 {
@@ -238,17 +266,17 @@ __device__ __forceinline__ int wave_row_pick(const WaveRow<E> &row, double u, in
     }
     const int lane = __ffsll((long long)__ballot(slot >= 0)) - 1;
     lane_out = lane;
-    slot_out = __shfl(slot, lane, 64);
+    slot_out = __builtin_amdgcn_readlane(slot, lane);
     return lane * E + slot_out;
 }
 
-template <int E>
-__device__ __forceinline__ double wave_row_value(const double (&x)[E], int lane, int slot)
+template <int E, typename V>
+__device__ __forceinline__ V wave_row_value(const V (&x)[E], int lane, int slot)
 {
-    double v = x[0];
+    V v = x[0];
 #pragma unroll
     for (int e = 1; e < E; ++e) v = slot == e ? x[e] : v;
-    return __shfl(v, lane, 64);
+    return wave_lane(v, lane);
 }
 
 }  // namespace snk

@@ -52,16 +52,27 @@ sample_rows_wave_kernel(const T *__restrict__ scores, int64_t stride, int64_t R,
         const int i = lane * E + e;
         x[e] = i < V ? score_load(p + i) : -__builtin_inf();
     }
-    WaveRow<E> row;
-    wave_row_weights<E>(x, rule, unit, row);
-    for (int d = 0; d < n_draws; ++d) {
-        int64_t pick = -1;
-        double lp = -__builtin_inf();
-        if (row.m > -__builtin_inf()) {
-            int l, s;
-            pick = wave_row_pick<E>(row, u[r * n_draws + d], l, s);
-            lp = sample_exponent(wave_row_value<E>(x, l, s), row.m, rule.inv_tau) - row.log_total;
+    const double ninf = -__builtin_inf();
+    double m = ninf;
+#pragma unroll
+    for (int e = 0; e < E; ++e) m = fmax(m, x[e]);
+    m = wave_max(m);
+    if (m == ninf) {
+        for (int d = lane; d < n_draws; d += 64) {
+            index[r * n_draws + d] = -1;
+            if (logp) logp[r * n_draws + d] = ninf;
         }
+        return;
+    }
+    WaveRow<E> row;
+#pragma unroll
+    for (int e = 0; e < E; ++e) row.w[e] = x[e] == ninf ? 0 : sample_weight(sample_exponent(x[e], m, rule.inv_tau), unit);
+    wave_row_keep<E>(x, rule, unit, row);
+    const double log_total = log((double)row.total / unit);
+    for (int d = 0; d < n_draws; ++d) {
+        int l, s;
+        const int pick = wave_row_pick<E>(row, u[r * n_draws + d], l, s);
+        const double lp = sample_exponent(wave_row_value<E>(x, l, s), m, rule.inv_tau) - log_total;
         if (lane == 0) {
             index[r * n_draws + d] = pick;
             if (logp) logp[r * n_draws + d] = lp;

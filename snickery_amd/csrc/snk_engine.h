@@ -449,7 +449,8 @@ struct snk_engine {
     DevBuf pb_bias, pb_edges;              // position bias (classes, buckets) and the buckets' edges
     int pb_classes = 0, pb_buckets = 0;    // 0: none set
     DevBuf sr_scores, sr_u, sr_rules, sr_index, sr_logp;
-    DevBuf tr_off, tr_cand, tr_tdist, tr_class, tr_u, tr_C, tr_alpha, tr_beta, tr_row_uses, tr_out;
+    double pb_min = 0.0;                   // the smallest finite bias, at most 0
+    DevBuf tr_off, tr_cand, tr_tdist, tr_class, tr_u, tr_C, tr_V, tr_W, tr_local, tr_least, tr_flag, tr_draw, tr_row_uses, tr_out;
     hipEvent_t tr_in = nullptr, tr_done = nullptr;      // hand-over between a caller's stream and the engine's
     DevBuf vstats;             // [0] cells refined, [1] steps with a refinement, [2] exact costs computed there
     // pass 1 of the sparse path, second form (joinfast_kernels.hip: join_lb2_kernel): float32 copy of the weighted join rows,

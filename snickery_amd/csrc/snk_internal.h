@@ -362,23 +362,32 @@ struct SampleRuleHost { double temperature; int64_t top_k; double top_p, min_p; 
 int64_t sample_rows_max();            // longest row of scores
 void launch_sample_rows(const void *scores, int dtype, int64_t stride, int64_t R, int64_t V, const double *u, int n_draws,
                         const SampleRuleHost &rule, const double *rules, int64_t *index, double *logp, hipStream_t s);
-// utterances first .. first + n_utts - 1 of a batch, `rows` rows from row c0 on; C holds the costs of those rows only, the other
-// pointers are the whole batch's
+// utterances first .. first + n_utts - 1 of a batch, `rows` rows from row c0 on; C holds the cells of those rows only (K x Kp a row,
+// Kp = K rounded up to a multiple of eight), the other pointers are the whole batch's
 struct TrellisView {
     const int64_t *cand; const double *tdist; const double *C; const int64_t *off;
-    int first, n_utts, K;
+    int first, n_utts, K, Kp;
     int64_t c0, rows, n_units;
     double inv_tau;
 };
-void launch_position_bias(const int64_t *cand, const int32_t *join_class, const double *bias, const int64_t *edges, int n_classes,
-                          int n_buckets, int64_t rows, int K, double *C, hipStream_t s);
-void launch_trellis_forward(const TrellisView &v, bool sum, double *alpha, double *logz, hipStream_t s);
-void launch_trellis_backward(const TrellisView &v, double *beta, hipStream_t s);
-void launch_trellis_posterior(const TrellisView &v, const double *alpha, const double *beta, const double *logz, const int64_t *edges,
-                              int n_buckets, double *posterior, double *row_uses, hipStream_t s);
+struct TrellisCosts {         // what the cost of a join is made of
+    const float *JC; int Jp, Dj; const double *wj;
+    const int32_t *join_class; const double *bias; const int *edges; int n_classes, n_buckets;
+    double bias_min;          // the smallest finite bias, at most 0
+};
+void launch_trellis_local(const TrellisView &v, double *local, double *least, int *flag, hipStream_t s);
+void launch_trellis_costs(const TrellisView &v, const TrellisCosts &c, bool logs, int *flag, double *X, hipStream_t s);
+void launch_trellis_forward(const TrellisView &v, const double *local, const double *least, double bias_min, int *flag, double *V, double *logz,
+                            hipStream_t s);
+void launch_trellis_backward(const TrellisView &v, const double *local, int *flag, double *Wt, hipStream_t s);
+void launch_trellis_forward_log(const TrellisView &v, bool sum, const int *flag, double *alpha, double *logz, hipStream_t s);
+void launch_trellis_backward_log(const TrellisView &v, const int *flag, double *beta, hipStream_t s);
+void launch_trellis_posterior(const TrellisView &v, const int *flag, const double *V, const double *Wt, const double *local, const double *logz,
+                              const int *edges, int n_buckets, double *posterior, double *row_uses, hipStream_t s);
 void launch_trellis_uses(const double *row_uses, const int32_t *join_class, int64_t rows, int n_classes, int n_buckets, double *uses, hipStream_t s);
-void launch_trellis_draw(const TrellisView &v, const SampleRuleHost &rule, const double *alpha, const double *u, int n_draws, int64_t all_rows,
-                         int all_utts, int64_t *path, double *cost, double *logp, hipStream_t s);
+size_t trellis_draw_bytes(int64_t rows, int n_utts, int K, int n_draws, size_t (&at)[5]);
+void launch_trellis_draw(const TrellisView &v, const TrellisCosts &c, const SampleRuleHost &rule, const int *flag, const double *V, const double *u,
+                         int n_draws, int64_t all_rows, int all_utts, char *work, int64_t *path, double *cost, double *logp, hipStream_t s);
 
 // ---- self test --------------------------------------------------------------
 void launch_mfma_selftest(const double *A, const double *B, double *C, hipStream_t s);

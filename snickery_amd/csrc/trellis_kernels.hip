@@ -4,72 +4,471 @@
 //     C[t,a,b] = J[t,a,b] + B[class_t, bucket(cand[t+1,b] - cand[t,a])]        (join cost + bias by relative position)
 //     p(path)  ~ exp(-(sum_t d[t,a_t] + sum_t C[t,a_t,a_t+1]) / tau)
 // a candidate takes part if its unit can join (1 <= id < N - 1, as in the Viterbi search) and its target cost is finite.
-//     alpha_0[b]   = -d[0,b] / tau          alpha_t+1[b] = -d[t+1,b] / tau + log sum_a exp(alpha_t[a] - C[t,a,b] / tau)
-//     beta_T-1[a]  = 0                      beta_t[a]    = log sum_b exp(-C[t,a,b] / tau - d[t+1,b] / tau + beta_t+1[b])
-//     log Z        = log sum_a exp(alpha_T-1[a])
-//     draw: a_T-1 from alpha_T-1, then a_t from alpha_t[.] - C[t,.,a_t+1] / tau, every row of scores truncated like those of
-//           sample_kernels.hip; temperature 0 keeps the largest term of every sum instead (tau = 1), and the draws follow it
+// With  l[t,a] = exp((min d[t,.] - d[t,a]) / tau)  and  E[t,a,b] = exp((min B - C[t,a,b]) / tau), both at most 1,
+//     v_0 = l_0              v_t+1[b] = l_t+1[b] * sum_a v_t[a] E[t,a,b]        up to a factor per row: p(a_t | rows <= t)
+//     x_T-1 = l_T-1          w_t[a]   = sum_b E[t,a,b] x_t+1[b],  x_t = l_t w_t                      p(rows > t | a_t)
+//     log Z = log sum v_T-1 + what was scaled out
+//     draw: a_T-1 from v_T-1, then a_t from v_t[.] E[t,.,a_t+1]: rows of weights, truncated like those of sample_kernels.hip
+//
+// The exponentials are taken once per cell, where the costs are made; the recursions are products and sums.  Every row is scaled by
+// a power of two, and an utterance whose weights span more than float64's exponents carry -- a tau far below the costs, or a
+// candidate that only a forbidden join leaves -- is recognised (a cost beyond SNK_COST_RANGE tau, a target cost beyond
+// SNK_LOCAL_RANGE tau, a weight below SNK_WEIGHT_LEAST) and done again in logarithms: the launches named _log work on the flagged
+// utterances only.  Within those limits no product underflows: weight, cell and local weight 2^-490 e^-230 e^-100 > 2^-967, the
+// weights of the two directions 2^-490 2^-490.
 #include "sample_device.h"
+
+#define SNK_COST_RANGE 230.0
+#define SNK_LOCAL_RANGE 100.0
+#define SNK_WEIGHT_LEAST 0x1p-490
+#define SNK_USES_UNIT 1125899906842624.0      // 2^50
 
 namespace snk {
 
+typedef double f64x2 __attribute__((ext_vector_type(2)));
+
 __device__ __forceinline__ bool trellis_usable(int64_t id, int64_t n_units) { return id >= 1 && id < n_units - 1; }
+__device__ __forceinline__ bool trellis_takes_part(int64_t id, double d, int64_t n_units) { return trellis_usable(id, n_units) && d - d == 0.0; }
 
 // -d / tau of a candidate that takes part
 __device__ __forceinline__ double trellis_local(int64_t id, double d, int64_t n_units, double inv_tau)
 {
-    return trellis_usable(id, n_units) && d - d == 0.0 ? -d * inv_tau : -__builtin_inf();
+    return trellis_takes_part(id, d, n_units) ? -d * inv_tau : -__builtin_inf();
 }
 
-// ---- position bias, in place on the join costs: a workgroup per pair of rows ----------------------------------------------------
-__global__ void __launch_bounds__(256)
-position_bias_kernel(const int64_t *__restrict__ cand, const int32_t *__restrict__ join_class, const double *__restrict__ bias,
-                     const int64_t *__restrict__ edges, int n_classes, int n_buckets, int K, double *__restrict__ C)
+// utterance of a row (first .. first + n - 1): off[u] <= t < off[u + 1]
+__device__ __forceinline__ int trellis_utterance(const int64_t *__restrict__ off, int first, int n, int64_t t)
 {
-    __shared__ int64_t e[64];
-    __shared__ double b[64];
-    const int64_t t = blockIdx.x;
-    const int c = join_class ? join_class[t] : 0;
-    if (c < 0 || c >= n_classes) return;                        // a join without a class carries no bias
-    const int tid = threadIdx.x;
-    if (tid < n_buckets - 1) e[tid] = edges[tid];
-    if (tid < n_buckets) b[tid] = bias[(int64_t)c * n_buckets + tid];
-    __syncthreads();
-    for (int i = blockIdx.y * 256 + tid; i < K * K; i += gridDim.y * 256) {
-        const int64_t apart = cand[(t + 1) * K + i % K] - cand[t * K + i / K];
-        int k = 0;
-        for (int j = 0; j < n_buckets - 1; ++j) k += apart >= e[j] ? 1 : 0;
-        C[t * K * K + i] += b[k];
+    int u = first, hi = first + n;
+    while (hi - u > 1) { const int mid = (u + hi) >> 1; if (off[mid] <= t) u = mid; else hi = mid; }
+    return u;
+}
+
+// bucket of a distance: most joins are far ones, the two outermost buckets are decided first
+__device__ __forceinline__ int trellis_bucket(int apart, const int *edges, int n_buckets)
+{
+    const int n = n_buckets - 1;
+    if (n == 0 || apart < edges[0]) return 0;
+    if (apart >= edges[n - 1]) return n;
+    int lo = 0, hi = n - 1;                                    // edges[lo] <= apart < edges[hi]
+    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (apart >= edges[mid]) lo = mid; else hi = mid; }
+    return lo + 1;
+}
+
+__device__ __forceinline__ double trellis_pow2(int e)           // 2^e, -1022 <= e <= 1023
+{
+    return __longlong_as_double((long long)(e + 1023) << 52);
+}
+// exponent of the power of two that scales a row whose largest weight is m to [1, 2): 0 for an empty row
+__device__ __forceinline__ int trellis_exponent(double m)
+{
+    return m > 0.0 ? (int)(((u64)__double_as_longlong(m) >> 52) & 0x7ff) - 1023 : 0;
+}
+
+// ---- local weights: a wavefront per row ---------------------------------------------------------------------------------------------
+__global__ void __launch_bounds__(256)
+trellis_local_kernel(const TrellisView v, double *__restrict__ local, double *__restrict__ least, int *__restrict__ flag)
+{
+    const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (i >= v.rows) return;
+    const int64_t t = v.c0 + i;
+    const int lane = threadIdx.x & 63;
+    const double inf = __builtin_inf();
+    double d[4], lo = inf, hi = -inf;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int a = lane + 64 * j;
+        d[j] = inf;
+        if (a < v.K) {
+            const double c = v.tdist[t * v.K + a];
+            if (trellis_takes_part(v.cand[t * v.K + a], c, v.n_units)) { d[j] = c; hi = fmax(hi, c); }
+        }
+        lo = fmin(lo, d[j]);
+    }
+    lo = -wave_max(-lo);
+    hi = wave_max(hi);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        const int a = lane + 64 * j;
+        if (a < v.Kp) local[t * v.Kp + a] = d[j] < inf ? exp((lo - d[j]) * v.inv_tau) : 0.0;
+    }
+    if (lane == 0) {
+        least[t] = lo < inf ? lo : 0.0;
+        if ((hi - lo) * v.inv_tau > SNK_LOCAL_RANGE) flag[trellis_utterance(v.off, v.first, v.n_utts, t)] = 1;
     }
 }
 
-// ---- forward: a workgroup per utterance -------------------------------------------------------------------------------------------
+// ---- costs: a workgroup per pair of rows and tile of 16 RT x 16 RT cells ------------------------------------------------------------
+// Distances in difference form (a unit and its natural successor join at exactly 0), one subtraction and one fused multiply-add per
+// column: the float64 vector pipe is what bounds it, 2 Dj instructions a cell.  A thread keeps RT x RT cells; 16 columns of the two
+// sets of rows go through LDS at a time, weighted and widened on the way, the next 16 are in flight meanwhile.
+template <int RT, bool LOG>
+__global__ void __launch_bounds__(256, 2)
+trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__ flag, double *__restrict__ X)
+{
+    constexpr int N = 16 * RT, DC = 16, LD = N + 4, PASS = (N + 63) / 64;
+    __shared__ double Es[DC * LD], Ss[DC * LD];
+    __shared__ int idE[N], idS[N];                              // unit id, -1: cannot join
+    __shared__ int edges[64];
+    __shared__ double bias[64];
+    const int64_t t = v.c0 + blockIdx.x;
+    const int u = trellis_utterance(v.off, v.first, v.n_utts, t);
+    if (t + 1 == v.off[u + 1]) return;
+    if (LOG && !flag[u]) return;
+    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const int a0 = blockIdx.y * N, b0 = blockIdx.z * N;
+    for (int i = tid; i < 2 * N; i += 256) {
+        const bool second = i >= N;
+        const int k = second ? b0 + i - N : a0 + i;
+        const int64_t id = k < v.K ? v.cand[(t + (second ? 1 : 0)) * v.K + k] : -1;
+        (second ? idS[i - N] : idE[i]) = trellis_usable(id, v.n_units) ? (int)id : -1;
+    }
+    int cls = -1;
+    if (c.n_classes) {
+        cls = c.join_class ? c.join_class[t] : 0;
+        if (cls >= c.n_classes) cls = -1;
+        if (tid < c.n_buckets - 1) edges[tid] = c.edges[tid];
+        if (cls >= 0 && tid < c.n_buckets) bias[tid] = c.bias[(int64_t)cls * c.n_buckets + tid];
+    }
+    __syncthreads();
+
+    const int q = tid & 3, r0 = tid >> 2;
+    const float *pe[PASS], *ps[PASS];
+    float4 fe[PASS], fs[PASS];
+    double w[4];
+#pragma unroll
+    for (int p = 0; p < PASS; ++p) {
+        const int r = r0 + 64 * p < N ? r0 + 64 * p : 0;
+        pe[p] = c.JC + (int64_t)(idE[r] >= 0 ? idE[r] + 1 : 0) * c.Jp + 4 * q;
+        ps[p] = c.JC + (int64_t)(idS[r] >= 0 ? idS[r] : 0) * c.Jp + 4 * q;
+    }
+    auto fetch = [&](int col) {
+        const bool in = col + 4 * q < c.Jp;                     // (rows are padded to multiples of four columns)
+#pragma unroll
+        for (int p = 0; p < PASS; ++p) {
+            fe[p] = in ? *reinterpret_cast<const float4 *>(pe[p] + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+            fs[p] = in ? *reinterpret_cast<const float4 *>(ps[p] + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) w[e] = col + 4 * q + e < c.Dj ? c.wj[col + 4 * q + e] : 0.0;
+    };
+    double acc[RT][RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < RT; ++j) acc[i][j] = 0.0;
+    fetch(0);
+    for (int col = 0; col < c.Dj; col += DC) {
+#pragma unroll
+        for (int p = 0; p < PASS; ++p) {
+            const int r = r0 + 64 * p;
+            if (r < N) {
+                const float e4[4] = {fe[p].x, fe[p].y, fe[p].z, fe[p].w}, s4[4] = {fs[p].x, fs[p].y, fs[p].z, fs[p].w};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    Es[(4 * q + e) * LD + r] = (double)e4[e] * w[e];
+                    Ss[(4 * q + e) * LD + r] = (double)s4[e] * w[e];
+                }
+            }
+        }
+        __syncthreads();
+        if (col + DC < c.Dj) fetch(col + DC);
+#pragma unroll 2
+        for (int k = 0; k < DC; ++k) {
+            double ev[RT], sv[RT];
+#pragma unroll
+            for (int i = 0; i < RT; ++i) ev[i] = Es[k * LD + ty + 16 * i];
+#pragma unroll
+            for (int j = 0; j < RT; ++j) sv[j] = Ss[k * LD + tx + 16 * j];
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int j = 0; j < RT; ++j) {
+                    const double d = ev[i] - sv[j];
+                    acc[i][j] = __fma_rn(d, d, acc[i][j]);
+                }
+        }
+        __syncthreads();
+    }
+    bool wide = false;
+    double *__restrict__ out = X + (t - v.c0) * v.K * v.Kp;
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < RT; ++j) {
+            const int al = ty + 16 * i, bl = tx + 16 * j, a = a0 + al, b = b0 + bl;
+            if (a < v.K && b < v.Kp) {
+                const int ie = idE[al], is = idS[bl];
+                double cost = __builtin_inf();
+                if (ie >= 0 && is >= 0) {
+                    cost = sqrt(acc[i][j]);
+                    if (cls >= 0) cost += bias[trellis_bucket(is - ie, edges, c.n_buckets)];
+                }
+                if (LOG) out[(int64_t)a * v.Kp + b] = -cost * v.inv_tau;
+                else {
+                    const double x = (c.bias_min - cost) * v.inv_tau;
+                    wide |= x < -SNK_COST_RANGE && cost < __builtin_inf();
+                    out[(int64_t)a * v.Kp + b] = exp(x);
+                }
+            }
+        }
+    if (!LOG && wide) flag[u] = 1;
+}
+
+// ---- forward: a workgroup per utterance, a step per row ------------------------------------------------------------------------------
+// A wavefront owns 32 columns (two a lane); its four rows of 16 lanes split the predecessors, so a step's sums end inside the
+// wavefront and a step costs one barrier.  The cells of the next steps are in flight in registers: a slab is K x Kp x 8 bytes
+// through one compute unit, and that (64 bytes a cycle) is what a step takes.  A thread's R = 4 CH KPM / 4 predecessors come in CH
+// pieces of KPM.
+template <int KPM, int CH, int NB, int NTH>
+__global__ void __launch_bounds__(NTH)
+trellis_forward_kernel(const TrellisView v, const double *__restrict__ local, const double *__restrict__ least, double bias_min,
+                       int *__restrict__ flag, double *__restrict__ V, double *__restrict__ logz)
+{
+    constexpr int W = NTH / 64, R = KPM * CH;
+    static_assert(NB % CH == 0 || CH % NB == 0, "a step's pieces go round the buffers");
+    __shared__ double cur[2][4 * R];
+    __shared__ double top[2][W];
+    __shared__ double part[NTH];
+    __shared__ int bad;
+    const int u = v.first + blockIdx.x;
+    if (flag[u]) return;
+    const int64_t r0 = v.off[u], T = v.off[u + 1] - r0;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int b = wave * 32 + (lane & 15) * 2, rows = lane >> 4;
+    const int K = v.K, Kp = v.Kp;
+    const bool lead = rows == 0 && b < Kp;
+    const int slab_bytes = K * Kp * 8;
+    const int voff = b < Kp ? (rows * R * Kp + b) * 8 : 0x7ff00000;
+    for (int i = tid; i < 8 * R; i += NTH) (&cur[0][0])[i] = 0.0;
+    if (tid == 0) bad = 0;
+    __syncthreads();
+
+    f64x2 cell[NB][KPM];
+    const int64_t pieces = (T - 1) * CH;
+    auto load = [&](int64_t piece, f64x2 (&dst)[KPM]) {
+        piece = piece < pieces ? piece : pieces - 1;
+        const double *base = v.C + (r0 - v.c0 + piece / CH) * ((int64_t)K * Kp);
+        const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc(const_cast<double *>(base), 0, slab_bytes, 0x00020000);
+        const int row = (int)(piece % CH) * KPM;
+#pragma unroll
+        for (int i = 0; i < KPM; ++i)                          // (rows beyond K lie beyond the slab: they read as 0)
+            dst[i] = __builtin_bit_cast(f64x2, __builtin_amdgcn_raw_buffer_load_b128(res, voff + (row + i) * Kp * 8, 0, 0));
+    };
+    auto load_local = [&](int64_t t) -> f64x2 {
+        f64x2 x = {0.0, 0.0};
+        if (lead) x = *reinterpret_cast<const f64x2 *>(local + (r0 + (t < T ? t : T - 1)) * Kp + b);
+        return x;
+    };
+    // new weights of the lead lanes: LDS, memory, their maximum; small ones are remembered
+    bool small = false;
+    auto publish = [&](int64_t t, f64x2 x, int at) {
+        double m = 0.0;
+        if (lead) {
+            cur[at][b] = x[0];
+            if (b + 1 < 4 * R) cur[at][b + 1] = x[1];
+            *reinterpret_cast<f64x2 *>(V + (r0 + t) * Kp + b) = x;
+            m = fmax(x[0], x[1]);
+            small |= (x[0] > 0.0 && x[0] < SNK_WEIGHT_LEAST) || (x[1] > 0.0 && x[1] < SNK_WEIGHT_LEAST);
+        }
+        m = wave_max(m);
+        if (lane == 0) top[at][wave] = m;
+    };
+    if (pieces > 0) {
+#pragma unroll
+        for (int s = 0; s < NB; ++s) load(s, cell[s]);
+    }
+    f64x2 l1 = load_local(1), l2 = load_local(2);
+    publish(0, load_local(0), 0);
+    __syncthreads();
+    int64_t scaled = 0;                                         // sum of the exponents taken out
+    constexpr int TRIP = NB / CH > 0 ? NB / CH : 1;             // steps a trip, so that buffer indexes are constants
+    for (int64_t t = 1; t < T; t += TRIP) {
+#pragma unroll
+        for (int s = 0; s < TRIP; ++s) {
+            const int64_t now = t + s;
+            const bool valid = now < T;
+            const int from = (int)(now - 1) & 1;
+            double m = top[from][0];
+#pragma unroll
+            for (int i = 1; i < W; ++i) m = fmax(m, top[from][i]);
+            const int e = trellis_exponent(m);
+            f64x2 sum = {0.0, 0.0};
+#pragma unroll
+            for (int ch = 0; ch < CH; ++ch) {
+                f64x2(&c)[KPM] = cell[(s * CH + ch) % NB];
+                const double *p = &cur[from][rows * R + ch * KPM];
+#pragma unroll
+                for (int i = 0; i < KPM; ++i) {
+                    sum[0] = __fma_rn(p[i], c[i][0], sum[0]);
+                    sum[1] = __fma_rn(p[i], c[i][1], sum[1]);
+                }
+                load((now - 1) * CH + ch + NB, c);
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                double x = sum[k];
+                x += __shfl_xor(x, 16, 64);
+                x += __shfl_xor(x, 32, 64);
+                sum[k] = x;
+            }
+            const double f = trellis_pow2(-e);
+            if (valid) {
+                scaled += e;
+                const f64x2 x = {l1[0] * (sum[0] * f), l1[1] * (sum[1] * f)};
+                publish(now, x, 1 - from);
+            }
+            l1 = l2;
+            l2 = load_local(now + 2);
+            __syncthreads();
+        }
+    }
+    if (small) bad = 1;
+    __syncthreads();
+    if (bad) { if (tid == 0) flag[u] = 1; return; }
+    if (!logz) return;
+    double s = 0.0;
+    for (int64_t t = tid; t < T; t += NTH) s += least[r0 + t];
+    part[tid] = s;
+    __syncthreads();
+    if (tid == 0) {
+        s = 0.0;
+        for (int i = 0; i < NTH; ++i) s += part[i];
+        double z = 0.0;
+        for (int a = 0; a < K; ++a) z += cur[(T - 1) & 1][a];
+        logz[u] = z > 0.0 ? log(z) + (double)scaled * 0.69314718055994530942 - (s + (double)(T - 1) * bias_min) * v.inv_tau : -__builtin_inf();
+    }
+}
+
+// ---- backward: as forward; a wavefront owns CH x 16 predecessors, four lanes share each one's successors -----------------------------
+template <int KC, int CH, int NB, int NTH>
+__global__ void __launch_bounds__(NTH)
+trellis_backward_kernel(const TrellisView v, const double *__restrict__ local, int *__restrict__ flag, double *__restrict__ Wt)
+{
+    constexpr int W = NTH / 64;
+    static_assert(NB % CH == 0, "a step's pieces go round the buffers");
+    __shared__ double cur[2][8 * KC];
+    __shared__ double top[2][W];
+    __shared__ int bad;
+    const int u = v.first + blockIdx.x;
+    if (flag[u]) return;
+    const int64_t r0 = v.off[u], T = v.off[u + 1] - r0;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int q = lane & 3, K = v.K, Kp = v.Kp;
+    const int slab_bytes = K * Kp * 8;
+    int a[CH], voff[CH];
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch) {
+        a[ch] = (ch * W + wave) * 16 + (lane >> 2);
+        voff[ch] = a[ch] < K ? (a[ch] * Kp + 2 * q) * 8 : 0x7ff00000;
+    }
+    for (int i = tid; i < 16 * KC; i += NTH) (&cur[0][0])[i] = 0.0;
+    if (tid == 0) bad = 0;
+    __syncthreads();
+    f64x2 cell[NB][KC];
+    const int64_t pieces = (T - 1) * CH;                        // from the last slab down
+    auto load = [&](int64_t piece, f64x2 (&dst)[KC], int off) {
+        piece = piece < pieces ? piece : pieces - 1;
+        const double *base = v.C + (r0 - v.c0 + (T - 2 - piece / CH)) * ((int64_t)K * Kp);
+        const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc(const_cast<double *>(base), 0, slab_bytes, 0x00020000);
+#pragma unroll
+        for (int i = 0; i < KC; ++i)                           // (columns beyond Kp are the next row's or nothing: their weights are 0)
+            dst[i] = __builtin_bit_cast(f64x2, __builtin_amdgcn_raw_buffer_load_b128(res, off + i * 64, 0, 0));
+    };
+    auto load_local = [&](int64_t t, int ch) -> double {
+        return a[ch] < K && q == 0 ? local[(r0 + (t > 0 ? t : 0)) * Kp + a[ch]] : 0.0;
+    };
+    if (pieces > 0) {
+#pragma unroll
+        for (int s = 0; s < NB; ++s) load(s, cell[s], voff[s % CH]);
+    }
+    double l1[CH], l2[CH];
+    double m0 = 0.0;
+#pragma unroll
+    for (int ch = 0; ch < CH; ++ch) {
+        const double x = load_local(T - 1, ch);
+        if (a[ch] < K && q == 0) { cur[(T - 1) & 1][a[ch]] = x; Wt[(r0 + T - 1) * Kp + a[ch]] = 1.0; m0 = fmax(m0, x); }
+        l1[ch] = load_local(T - 2, ch);
+        l2[ch] = load_local(T - 3, ch);
+    }
+    m0 = wave_max(m0);
+    if (lane == 0) top[(T - 1) & 1][wave] = m0;
+    __syncthreads();
+    bool small = false;
+    constexpr int TRIP = NB / CH;
+    for (int64_t k = 0; k + 1 < T; k += TRIP) {
+#pragma unroll
+        for (int s = 0; s < TRIP; ++s) {
+            const int64_t t = T - 2 - (k + s);                  // the row of this step; < 0: beyond the first
+            const bool valid = t >= 0;
+            const int from = (int)(t + 1) & 1, to = 1 - from;
+            double m = top[from][0];
+#pragma unroll
+            for (int i = 1; i < W; ++i) m = fmax(m, top[from][i]);
+            const double f = trellis_pow2(-trellis_exponent(m));
+            m = 0.0;
+#pragma unroll
+            for (int ch = 0; ch < CH; ++ch) {
+                f64x2(&c)[KC] = cell[(s * CH + ch) % NB];
+                f64x2 sum = {0.0, 0.0};
+#pragma unroll
+                for (int i = 0; i < KC; ++i) {
+                    const f64x2 x = *reinterpret_cast<const f64x2 *>(&cur[from][8 * i + 2 * q]);
+                    sum[0] = __fma_rn(x[0], c[i][0], sum[0]);
+                    sum[1] = __fma_rn(x[1], c[i][1], sum[1]);
+                }
+                load((k + s) * CH + ch + NB, c, voff[ch]);
+                double y = sum[0] + sum[1];
+                y += __shfl_xor(y, 1, 64);
+                y += __shfl_xor(y, 2, 64);
+                y *= f;
+                if (valid && a[ch] < K && q == 0) {
+                    const double x = l1[ch] * y;
+                    cur[to][a[ch]] = x;
+                    Wt[(r0 + t) * Kp + a[ch]] = y;
+                    small |= x > 0.0 && x < SNK_WEIGHT_LEAST;
+                    m = fmax(m, x);
+                }
+                l1[ch] = l2[ch];
+                l2[ch] = load_local(t - 2, ch);
+            }
+            m = wave_max(m);
+            if (valid && lane == 0) top[to][wave] = m;
+            __syncthreads();
+        }
+    }
+    if (small) bad = 1;
+    __syncthreads();
+    if (bad && tid == 0) flag[u] = 1;
+}
+
+// ---- the flagged utterances in logarithms (SUM false: temperature 0, the largest term of every sum) ----------------------------------
 template <bool SUM>
 __global__ void __launch_bounds__(1024)
-trellis_forward_kernel(const int64_t *__restrict__ cand, const double *__restrict__ tdist, const double *__restrict__ C,
-                       const int64_t *__restrict__ off, int first, int64_t c0, int K, int64_t n_units, double inv_tau,
-                       double *__restrict__ alpha, double *__restrict__ logz)
+trellis_forward_log_kernel(const TrellisView v, const int *__restrict__ flag, double *__restrict__ alpha, double *__restrict__ logz)
 {
     __shared__ double cur[256], part_max[1024], part_sum[1024];
-    const int tid = threadIdx.x;
+    const int u = v.first + blockIdx.x;
+    if (!flag[u]) return;
+    const int K = v.K, Kp = v.Kp, tid = threadIdx.x;
     const int KB = (K + 63) & ~63, P = 1024 / KB;
     const int b = tid % KB, part = tid / KB;
-    const int64_t r0 = off[first + blockIdx.x], T = off[first + blockIdx.x + 1] - r0;
+    const int64_t r0 = v.off[u], T = v.off[u + 1] - r0;
     const double ninf = -__builtin_inf();
     const bool mine = b < K && part < P;
     if (tid < K) {
-        const double v = trellis_local(cand[r0 * K + tid], tdist[r0 * K + tid], n_units, inv_tau);
-        cur[tid] = v;
-        alpha[r0 * K + tid] = v;
+        const double x = trellis_local(v.cand[r0 * K + tid], v.tdist[r0 * K + tid], v.n_units, v.inv_tau);
+        cur[tid] = x;
+        alpha[r0 * Kp + tid] = x;
     }
     __syncthreads();
     for (int64_t t = 0; t + 1 < T; ++t) {
-        const double *__restrict__ c = C + (r0 + t - c0) * K * K + b;
+        const double *__restrict__ c = v.C + (r0 + t - v.c0) * K * Kp + b;
         double top = ninf, sum = 0.0;
         if (mine) {
-            for (int a = part; a < K; a += P) top = fmax(top, cur[a] - c[(int64_t)a * K] * inv_tau);
+            for (int a = part; a < K; a += P) top = fmax(top, cur[a] + c[(int64_t)a * Kp]);
             if (SUM && top > ninf)
-                for (int a = part; a < K; a += P) sum += exp(cur[a] - c[(int64_t)a * K] * inv_tau - top);
+                for (int a = part; a < K; a += P) sum += exp(cur[a] + c[(int64_t)a * Kp] - top);
         }
         part_max[tid] = top;
         part_sum[tid] = sum;
@@ -77,17 +476,17 @@ trellis_forward_kernel(const int64_t *__restrict__ cand, const double *__restric
         if (tid < K) {
             double all = ninf;
             for (int q = 0; q < P; ++q) all = fmax(all, part_max[q * KB + tid]);
-            double v = all;
+            double x = all;
             if (SUM && all > ninf) {
                 double s = 0.0;
                 for (int q = 0; q < P; ++q)
                     if (part_max[q * KB + tid] > ninf) s += part_sum[q * KB + tid] * exp(part_max[q * KB + tid] - all);
-                v = all + log(s);
+                x = all + log(s);
             }
             const int64_t at = (r0 + t + 1) * K + tid;
-            v += trellis_local(cand[at], tdist[at], n_units, inv_tau);
-            cur[tid] = v;
-            alpha[at] = v;
+            x += trellis_local(v.cand[at], v.tdist[at], v.n_units, v.inv_tau);
+            cur[tid] = x;
+            alpha[(r0 + t + 1) * Kp + tid] = x;
         }
         __syncthreads();
     }
@@ -97,34 +496,34 @@ trellis_forward_kernel(const int64_t *__restrict__ cand, const double *__restric
         double s = 0.0;
         if (all > ninf)
             for (int a = 0; a < K; ++a) s += exp(cur[a] - all);
-        logz[first + blockIdx.x] = all > ninf ? all + log(s) : ninf;
+        logz[u] = all > ninf ? all + log(s) : ninf;
     }
 }
 
-// ---- backward: a workgroup per utterance, a wavefront per predecessor ----------------------------------------------------------
 __global__ void __launch_bounds__(1024)
-trellis_backward_kernel(const int64_t *__restrict__ cand, const double *__restrict__ tdist, const double *__restrict__ C,
-                        const int64_t *__restrict__ off, int first, int64_t c0, int K, int64_t n_units, double inv_tau, double *__restrict__ beta)
+trellis_backward_log_kernel(const TrellisView v, const int *__restrict__ flag, double *__restrict__ beta)
 {
     __shared__ double into[2][256];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t r0 = off[first + blockIdx.x], T = off[first + blockIdx.x + 1] - r0;
+    const int u = v.first + blockIdx.x;
+    if (!flag[u]) return;
+    const int K = v.K, Kp = v.Kp, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t r0 = v.off[u], T = v.off[u + 1] - r0;
     const double ninf = -__builtin_inf();
     if (tid < K) {
         const int64_t at = (r0 + T - 1) * K + tid;
-        beta[at] = 0.0;
-        into[(T - 1) & 1][tid] = trellis_local(cand[at], tdist[at], n_units, inv_tau);
+        beta[(r0 + T - 1) * Kp + tid] = 0.0;
+        into[(T - 1) & 1][tid] = trellis_local(v.cand[at], v.tdist[at], v.n_units, v.inv_tau);
     }
     __syncthreads();
     for (int64_t t = T - 2; t >= 0; --t) {
         const double *next = into[(t + 1) & 1];
         for (int a = wave; a < K; a += 16) {
-            const double *__restrict__ c = C + (r0 + t - c0) * K * K + (int64_t)a * K;
+            const double *__restrict__ c = v.C + (r0 + t - v.c0) * K * Kp + (int64_t)a * Kp;
             double x[4], top = ninf;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const int b = lane + 64 * j;
-                x[j] = b < K ? next[b] - c[b] * inv_tau : ninf;
+                x[j] = b < K ? next[b] + c[b] : ninf;
                 top = fmax(top, x[j]);
             }
             top = wave_max(top);
@@ -132,70 +531,97 @@ trellis_backward_kernel(const int64_t *__restrict__ cand, const double *__restri
             if (top > ninf) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j) s += exp(x[j] - top);
-#pragma unroll
-                for (int o = 32; o; o >>= 1) s += __shfl_xor(s, o, 64);
+                s = wave_sum(s);
             }
             if (lane == 0) {
-                const double v = top > ninf ? top + log(s) : ninf;
+                const double y = top > ninf ? top + log(s) : ninf;
                 const int64_t at = (r0 + t) * K + a;
-                beta[at] = v;
-                into[t & 1][a] = v + trellis_local(cand[at], tdist[at], n_units, inv_tau);
+                beta[(r0 + t) * Kp + a] = y;
+                into[t & 1][a] = y + trellis_local(v.cand[at], v.tdist[at], v.n_units, v.inv_tau);
             }
         }
         __syncthreads();
     }
 }
 
-// ---- posteriors: a workgroup per row; the row's bucket uses as integers in units of 2^-50 (sums in any order are the same) --------
+// ---- posteriors: a workgroup per row ---------------------------------------------------------------------------------------------------
+// The row's bucket uses are integers in units of 2^-50: their sums are the same in any order.  The two outermost buckets take most
+// cells and are summed in registers; the others go to LDS.
 __global__ void __launch_bounds__(256)
-trellis_posterior_kernel(const int64_t *__restrict__ cand, const double *__restrict__ tdist, const double *__restrict__ C,
-                         const double *__restrict__ alpha, const double *__restrict__ beta, const double *__restrict__ logz,
-                         const int64_t *__restrict__ off, int first, int n_utts, int64_t c0, int K, int64_t n_units, double inv_tau,
-                         const int64_t *__restrict__ edges, int n_buckets, double *__restrict__ posterior, double *__restrict__ row_uses)
+trellis_posterior_kernel(const TrellisView v, const int *__restrict__ flag, const double *__restrict__ V, const double *__restrict__ Wt,
+                         const double *__restrict__ local, const double *__restrict__ logz, const int *__restrict__ bucket_edges, int n_buckets,
+                         double *__restrict__ posterior, double *__restrict__ row_uses)
 {
-    __shared__ double in[256];
-    __shared__ double out[256];
-    __shared__ int64_t e[64], id0[256], id1[256];
+    __shared__ double in[256], out[256], red[8];
+    __shared__ int edges[64], id0[256], id1[256];
     __shared__ u64 uses[64];
-    const int64_t t = c0 + blockIdx.x;
-    const int tid = threadIdx.x;
-    int u = first, hi = first + n_utts;                         // off[u] <= t < off[u + 1]
-    while (hi - u > 1) { const int mid = (u + hi) >> 1; if (off[mid] <= t) u = mid; else hi = mid; }
-    const double z = logz[u];
-    const bool dead = !(z > -__builtin_inf());
-    const bool last = t + 1 == off[u + 1];
-    if (tid < K) {
-        const double a = alpha[t * K + tid];
-        posterior[t * K + tid] = dead ? 0.0 : exp(a + beta[t * K + tid] - z);
-        in[tid] = a - z;
-        id0[tid] = cand[t * K + tid];
-        if (!last) {
-            const int64_t at = (t + 1) * K + tid;
-            id1[tid] = cand[at];
-            out[tid] = trellis_local(cand[at], tdist[at], n_units, inv_tau) + beta[at];
+    const int64_t t = v.c0 + blockIdx.x;
+    const int K = v.K, Kp = v.Kp, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int u = trellis_utterance(v.off, v.first, v.n_utts, t);
+    const bool logs = flag[u] != 0, last = t + 1 == v.off[u + 1];
+    const double ninf = -__builtin_inf(), z = logz[u];
+    const bool dead = !(z > ninf);
+    if (logs) {
+        if (tid < K) {
+            const double a = V[t * Kp + tid];
+            posterior[t * K + tid] = dead ? 0.0 : exp(a + Wt[t * Kp + tid] - z);
+            in[tid] = a - z;
+        }
+    } else {
+        // sum_a v w of the row, and the power of two that the backward step into this row took out
+        const double a = tid < K ? V[t * Kp + tid] : 0.0, w = tid < K ? Wt[t * Kp + tid] : 0.0;
+        const double p = a * w, s = wave_sum(p);
+        const double x = !last && tid < K ? local[(t + 1) * Kp + tid] * Wt[(t + 1) * Kp + tid] : 0.0;
+        const double m = wave_max(x);
+        if (lane == 0) { red[wave] = s; red[4 + wave] = m; }
+        __syncthreads();
+        const double total = (red[0] + red[1]) + (red[2] + red[3]);
+        const double most = fmax(fmax(red[4], red[5]), fmax(red[6], red[7]));
+        if (tid < K) {
+            posterior[t * K + tid] = dead ? 0.0 : p / total;
+            // (a / total <= 1 / w <= 2^490; a candidate that leads nowhere has no share)
+            in[tid] = w > 0.0 ? a / total * trellis_pow2(-trellis_exponent(most)) : 0.0;
+            out[tid] = x;
         }
     }
     if (!row_uses) return;
-    if (tid < 64) uses[tid] = 0;
-    if (tid < n_buckets - 1) e[tid] = edges[tid];
-    __syncthreads();
-    if (!last && !dead) {
-        for (int i = tid; i < K * K; i += 256) {
-            const int a = i / K, b = i - a * K;
-            const double x = in[a] - C[(t - c0) * K * K + i] * inv_tau + out[b];
-            const u64 w = x < -36.0 ? 0ull : (u64)__double2ll_rn(exp(x) * 1125899906842624.0);
-            if (!w) continue;
-            const int64_t apart = id1[b] - id0[a];
-            int k = 0;
-            for (int j = 0; j < n_buckets - 1; ++j) k += apart >= e[j] ? 1 : 0;
-            atomicAdd(&uses[k], w);
+    if (tid < K) {
+        id0[tid] = (int)v.cand[t * K + tid];
+        if (!last) {
+            const int64_t at = (t + 1) * K + tid;
+            id1[tid] = (int)v.cand[at];
+            if (logs) out[tid] = trellis_local(v.cand[at], v.tdist[at], v.n_units, v.inv_tau) + Wt[(t + 1) * Kp + tid];
         }
     }
+    if (tid < 64) uses[tid] = 0;
+    if (tid < n_buckets - 1) edges[tid] = bucket_edges[tid];
     __syncthreads();
-    if (tid < n_buckets) row_uses[t * n_buckets + tid] = (double)uses[tid] * (1.0 / 1125899906842624.0);
+    if (!last && !dead) {
+        const double *__restrict__ c = v.C + (t - v.c0) * K * Kp;
+        u64 first = 0, far = 0;
+        for (int a = wave; a < K; a += 4) {
+            const double va = in[a];
+            for (int b = lane; b < K; b += 64) {
+                const double x = c[a * Kp + b];
+                double p;
+                if (logs) p = exp(va + x + out[b]);
+                else p = va * x * out[b];
+                const u64 w = sample_fix(p, SNK_USES_UNIT);
+                if (!w) continue;
+                const int k = trellis_bucket(id1[b] - id0[a], edges, n_buckets);
+                if (k == 0) first += w;
+                else if (k == n_buckets - 1) far += w;
+                else atomicAdd(&uses[k], w);
+            }
+        }
+        if (first) atomicAdd(&uses[0], first);
+        if (far) atomicAdd(&uses[n_buckets - 1], far);
+    }
+    __syncthreads();
+    if (tid < n_buckets) row_uses[t * n_buckets + tid] = (double)uses[tid] * (1.0 / SNK_USES_UNIT);
 }
 
-// uses[class, bucket] = sum over the rows of the class: a workgroup per class, the rows in a fixed order
+// uses[class, bucket] = sum over the rows of the class: a workgroup per class and bucket, the rows in a fixed order
 __global__ void __launch_bounds__(256)
 trellis_uses_kernel(const double *__restrict__ row_uses, const int32_t *__restrict__ join_class, int64_t rows, int n_buckets,
                     double *__restrict__ uses)
@@ -214,68 +640,271 @@ trellis_uses_kernel(const double *__restrict__ row_uses, const int32_t *__restri
     if (tid == 0) uses[(int64_t)blockIdx.x * n_buckets + k] = part[0];
 }
 
-// ---- draws: a wavefront per (utterance, draw) walks the trellis from its end ------------------------------------------------------
+// ---- draws -----------------------------------------------------------------------------------------------------------------------------
+// The random number of a row does not depend on the candidate behind it, so the predecessor of EVERY candidate is drawn at once,
+// all rows side by side (the weights and their truncation once per candidate, whatever the number of draws); what is left of the
+// chain is following those pointers.
+//
+// Weights of the row of scores V[t,.] (E[t,.,after]) / alpha + X: x in the order of the scores, -inf: takes no part.
 template <int E>
-__global__ void __launch_bounds__(64)
-trellis_draw_kernel(const int64_t *__restrict__ cand, const double *__restrict__ tdist, const double *__restrict__ C,
-                    const double *__restrict__ alpha, const int64_t *__restrict__ off, int first, int64_t c0, int K, int64_t n_units, double inv_tau,
-                    SampleRule rule, bool greedy, const double *__restrict__ u, int64_t rows, int n_utts, int64_t *__restrict__ path,
-                    double *__restrict__ cost, double *__restrict__ logp)
+__device__ __forceinline__ bool trellis_row(const double (&p)[E], bool logs, const SampleRule &rule, double (&x)[E], WaveRow<E> &row, double &m)
 {
-    const int v = first + blockIdx.x, s = blockIdx.y, lane = threadIdx.x;
-    const int64_t r0 = off[v], T = off[v + 1] - r0;
     const double ninf = -__builtin_inf();
-    double spent = 0.0, lp = 0.0;
-    int after = 0;
-    for (int64_t t = T - 1; t >= 0; --t) {
-        double x[E], c[E];
+    m = ninf;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        x[e] = logs || p[e] > 0.0 ? p[e] : ninf;
+        m = fmax(m, x[e]);
+    }
+    m = wave_max(m);
+    if (m == ninf) return false;
+    const double inv = logs ? 0.0 : 1.0 / m;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        if (logs) row.w[e] = x[e] == ninf ? 0 : sample_weight(sample_exponent(x[e], m, 1.0), SNK_SAMPLE_UNIT);
+        else row.w[e] = x[e] == m ? (u64)SNK_SAMPLE_UNIT : x[e] == ninf ? 0 : sample_fix(x[e] * inv, SNK_SAMPLE_UNIT);
+    }
+    wave_row_keep<E>(x, rule, SNK_SAMPLE_UNIT, row);
+    return true;
+}
+
+#define SNK_POINTER_COLUMNS 32
+template <int E>
+__global__ void __launch_bounds__(256)
+trellis_pointer_kernel(const TrellisView v, const int *__restrict__ flag, const double *__restrict__ V, SampleRule rule, bool greedy,
+                       const double *__restrict__ u, int n_draws, int64_t all_rows, int all_utts, unsigned char *__restrict__ pointer,
+                       int *__restrict__ root)
+{
+    extern __shared__ double cells[];                           // [SNK_POINTER_COLUMNS][LDA], LDA = K | 1
+    const int64_t t = v.c0 + blockIdx.x;
+    const int K = v.K, Kp = v.Kp, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int utt = trellis_utterance(v.off, v.first, v.n_utts, t);
+    const bool logs = flag[utt] != 0, last = t + 1 == v.off[utt + 1];
+    double vt[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) vt[e] = lane * E + e < K ? V[t * Kp + lane * E + e] : (logs ? -__builtin_inf() : 0.0);
+    double x[E], m;
+    WaveRow<E> row;
+    if (last) {                                                 // the path's end
+        if (blockIdx.y || wave) return;
+        const bool any = trellis_row<E>(vt, logs, rule, x, row, m);
+        for (int s = 0; s < n_draws; ++s) {
+            int l, slot, k = -1;
+            if (any) k = wave_row_pick<E>(row, greedy ? 0.0 : u[(int64_t)s * all_rows + t], l, slot);
+            if (lane == 0) root[(int64_t)s * all_utts + utt] = k;
+        }
+        return;
+    }
+    const int LDA = K | 1, b0 = blockIdx.y * SNK_POINTER_COLUMNS;
+    const double *__restrict__ c = v.C + (t - v.c0) * K * Kp;
+    for (int i = tid; i < K * SNK_POINTER_COLUMNS; i += 256) {
+        const int a = i >> 5, b = i & 31;
+        cells[b * LDA + a] = b0 + b < K ? c[a * Kp + b0 + b] : 0.0;
+    }
+    __syncthreads();
+    for (int b = wave; b < SNK_POINTER_COLUMNS && b0 + b < K; b += 4) {
+        double p[E];
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const int a = lane * E + e;
-            c[e] = (t + 1 < T && a < K) ? C[(r0 + t - c0) * K * K + (int64_t)a * K + after] : 0.0;
-            x[e] = a < K ? alpha[(r0 + t) * K + a] - c[e] * inv_tau : ninf;
+            const double cell = a < K ? cells[b * LDA + a] : 0.0;
+            p[e] = logs ? vt[e] + cell : vt[e] * cell;
         }
-        WaveRow<E> row;
-        wave_row_weights<E>(x, rule, 2251799813685248.0, row);
-        if (!(row.m > ninf)) {                                  // no complete path (only the last row can be empty)
-            for (int64_t i = lane; i < T; i += 64) path[s * rows + r0 + i] = -1;
-            if (lane == 0) { cost[(int64_t)s * n_utts + v] = -ninf; if (logp) logp[(int64_t)s * n_utts + v] = ninf; }
-            return;
+        const bool any = trellis_row<E>(p, logs, rule, x, row, m);
+        for (int s = 0; s < n_draws; ++s) {
+            int l, slot, k = 0;                                 // (a candidate nothing leads to is on no path)
+            if (any) k = wave_row_pick<E>(row, greedy ? 0.0 : u[(int64_t)s * all_rows + t], l, slot);
+            if (lane == 0) pointer[((int64_t)s * all_rows + t) * K + b0 + b] = (unsigned char)k;
         }
-        int l, slot;
-        const int k = wave_row_pick<E>(row, greedy ? 0.0 : u[(int64_t)s * rows + r0 + t], l, slot);
-        lp += sample_exponent(wave_row_value<E>(x, l, slot), row.m, rule.inv_tau) - row.log_total;
-        spent += wave_row_value<E>(c, l, slot) + tdist[(r0 + t) * K + k];
-        after = k;
-        if (lane == 0) path[s * rows + r0 + t] = cand[(r0 + t) * K + k];
     }
-    if (lane == 0) { cost[(int64_t)s * n_utts + v] = spent; if (logp) logp[(int64_t)s * n_utts + v] = lp; }
 }
 
-void launch_position_bias(const int64_t *cand, const int32_t *join_class, const double *bias, const int64_t *edges, int n_classes,
-                          int n_buckets, int64_t rows, int K, double *C, hipStream_t s)
+// Follows the pointers of an utterance and draw: a workgroup each, as many rows at a time as LDS holds.  The rows are cut into
+// pieces of 32: all K ways through every piece side by side, then the pieces' ends one after the other, then the pieces side by side.
+#define SNK_CHASE_BYTES (128 * 1024)
+#define SNK_CHASE_PIECE 32
+__global__ void __launch_bounds__(512)
+trellis_chase_kernel(const TrellisView v, const unsigned char *__restrict__ pointer, const int *__restrict__ root, int64_t all_rows, int all_utts,
+                     unsigned char *__restrict__ slots)
 {
-    if (rows < 2) return;
-    hipLaunchKernelGGL(position_bias_kernel, dim3((unsigned)(rows - 1), (unsigned)((K * K + 4095) / 4096)), dim3(256), 0, s, cand, join_class, bias, edges,
-                       n_classes, n_buckets, K, C);
+    extern __shared__ unsigned char lds[];
+    const int utt = v.first + blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
+    const int K = v.K;
+    const int64_t r0 = v.off[utt], T = v.off[utt + 1] - r0;
+    const int at_end = root[(int64_t)s * all_utts + utt];
+    if (at_end < 0) return;
+    const int64_t fit = SNK_CHASE_BYTES / (K + (K + SNK_CHASE_PIECE - 1) / SNK_CHASE_PIECE + 1) - SNK_CHASE_PIECE;
+    unsigned char *__restrict__ out = slots + (int64_t)s * all_rows + r0;
+    int after = at_end;                                         // slot of row `hi`
+    if (tid == 0) out[T - 1] = (unsigned char)at_end;
+    for (int64_t hi = T - 1; hi > 0;) {
+        const int n = (int)(hi < fit ? hi : fit);               // rows hi - n .. hi - 1
+        const int64_t lo = hi - n;
+        const int pieces = (n + SNK_CHASE_PIECE - 1) / SNK_CHASE_PIECE;
+        unsigned char *ptr = lds, *way = lds + (size_t)n * K, *start = way + (size_t)pieces * K;
+        const unsigned char *__restrict__ src = pointer + ((int64_t)s * all_rows + r0 + lo) * K;
+        __syncthreads();
+        for (int i = tid; i < n * K; i += 512) ptr[i] = src[i];
+        __syncthreads();
+        for (int i = tid; i < pieces * K; i += 512) {           // piece p: rows p 32 .. from its end to its first row
+            const int p = i / K, from = p * SNK_CHASE_PIECE, to = from + SNK_CHASE_PIECE < n ? from + SNK_CHASE_PIECE : n;
+            int k = i - p * K;
+            for (int r = to - 1; r >= from; --r) k = ptr[r * K + k];
+            way[i] = (unsigned char)k;
+        }
+        __syncthreads();
+        if (tid == 0) {
+            int k = after;
+            for (int p = pieces - 1; p >= 0; --p) { start[p] = (unsigned char)k; k = way[p * K + k]; }
+        }
+        __syncthreads();
+        for (int p = tid; p < pieces; p += 512) {
+            const int from = p * SNK_CHASE_PIECE, to = from + SNK_CHASE_PIECE < n ? from + SNK_CHASE_PIECE : n;
+            int k = start[p];
+            for (int r = to - 1; r >= from; --r) { k = ptr[r * K + k]; out[lo + r] = (unsigned char)k; }
+        }
+        if (pieces) after = way[start[0]];
+        hi = lo;
+    }
 }
 
-void launch_trellis_forward(const TrellisView &v, bool sum, double *alpha, double *logz, hipStream_t s)
+// Unit, cost and log probability of every row of a path: a wavefront per row and draw.  The join cost is taken from the units
+// themselves, in differences: the cells only hold its exponential.
+template <int E>
+__global__ void __launch_bounds__(256)
+trellis_path_kernel(const TrellisView v, const TrellisCosts c, const int *__restrict__ flag, const double *__restrict__ V, SampleRule rule,
+                    const int *__restrict__ root, const unsigned char *__restrict__ slots, int64_t all_rows, int all_utts,
+                    int64_t *__restrict__ path, double *__restrict__ row_cost, double *__restrict__ row_logp)
 {
-    if (sum) hipLaunchKernelGGL((trellis_forward_kernel<true>), dim3(v.n_utts), dim3(1024), 0, s, v.cand, v.tdist, v.C, v.off, v.first, v.c0, v.K, v.n_units, v.inv_tau, alpha, logz);
-    else hipLaunchKernelGGL((trellis_forward_kernel<false>), dim3(v.n_utts), dim3(1024), 0, s, v.cand, v.tdist, v.C, v.off, v.first, v.c0, v.K, v.n_units, v.inv_tau, alpha, logz);
+    const int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (i >= v.rows) return;
+    const int64_t t = v.c0 + i;
+    const int s = blockIdx.y, lane = threadIdx.x & 63, K = v.K, Kp = v.Kp;
+    const int utt = trellis_utterance(v.off, v.first, v.n_utts, t);
+    const int64_t at = (int64_t)s * all_rows + t;
+    if (root[(int64_t)s * all_utts + utt] < 0) {
+        if (lane == 0) path[at] = -1;
+        return;
+    }
+    const bool logs = flag[utt] != 0, last = t + 1 == v.off[utt + 1];
+    const int k = slots[at], after = last ? 0 : slots[at + 1];
+    double p[E], x[E], m;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int a = lane * E + e;
+        p[e] = a < K ? V[t * Kp + a] : (logs ? -__builtin_inf() : 0.0);
+        if (!last && a < K) {
+            const double cell = v.C[((t - v.c0) * K + a) * Kp + after];
+            p[e] = logs ? p[e] + cell : p[e] * cell;
+        }
+    }
+    WaveRow<E> row;
+    trellis_row<E>(p, logs, rule, x, row, m);
+    const double mine = wave_row_value<E>(x, k / E, k % E);
+    const double lp = (logs ? sample_exponent(mine, m, 1.0) : mine == m ? 0.0 : log(mine * (1.0 / m))) - log((double)row.total / SNK_SAMPLE_UNIT);
+    double cost = v.tdist[t * K + k];
+    const int64_t id = v.cand[t * K + k];
+    if (!last) {
+        const int64_t next = v.cand[(t + 1) * K + after];
+        const float *__restrict__ pe = c.JC + (id + 1) * c.Jp, *__restrict__ ps = c.JC + next * c.Jp;
+        double d2 = 0.0;
+        for (int j = lane; j < c.Dj; j += 64) {
+            const double d = (double)pe[j] * c.wj[j] - (double)ps[j] * c.wj[j];
+            d2 = __fma_rn(d, d, d2);
+        }
+        cost += sqrt(wave_sum(d2));
+        int cls = c.n_classes ? (c.join_class ? c.join_class[t] : 0) : -1;
+        if (cls >= 0 && cls < c.n_classes) cost += c.bias[(int64_t)cls * c.n_buckets + trellis_bucket((int)(next - id), c.edges, c.n_buckets)];
+    }
+    if (lane == 0) { path[at] = id; row_cost[at] = cost; row_logp[at] = lp; }
 }
 
-void launch_trellis_backward(const TrellisView &v, double *beta, hipStream_t s)
+// sums over an utterance's rows, in a fixed order
+__global__ void __launch_bounds__(256)
+trellis_total_kernel(const TrellisView v, const int *__restrict__ root, const double *__restrict__ row_cost, const double *__restrict__ row_logp,
+                     int64_t all_rows, int all_utts, double *__restrict__ cost, double *__restrict__ logp)
 {
-    hipLaunchKernelGGL(trellis_backward_kernel, dim3(v.n_utts), dim3(1024), 0, s, v.cand, v.tdist, v.C, v.off, v.first, v.c0, v.K, v.n_units, v.inv_tau, beta);
+    __shared__ double pc[256], pl[256];
+    const int utt = v.first + blockIdx.x, s = blockIdx.y, tid = threadIdx.x;
+    const int64_t r0 = v.off[utt], T = v.off[utt + 1] - r0, at = (int64_t)s * all_utts + utt;
+    const bool dead = root[at] < 0;
+    double c = 0.0, l = 0.0;
+    if (!dead)
+        for (int64_t t = tid; t < T; t += 256) { c += row_cost[(int64_t)s * all_rows + r0 + t]; l += row_logp[(int64_t)s * all_rows + r0 + t]; }
+    pc[tid] = c; pl[tid] = l;
+    __syncthreads();
+    for (int o = 128; o; o >>= 1) {
+        if (tid < o) { pc[tid] += pc[tid + o]; pl[tid] += pl[tid + o]; }
+        __syncthreads();
+    }
+    if (tid == 0) {
+        cost[at] = dead ? __builtin_inf() : pc[0];
+        if (logp) logp[at] = dead ? -__builtin_inf() : pl[0];
+    }
 }
 
-void launch_trellis_posterior(const TrellisView &v, const double *alpha, const double *beta, const double *logz, const int64_t *edges,
-                              int n_buckets, double *posterior, double *row_uses, hipStream_t s)
+// ---- launches ---------------------------------------------------------------------------------------------------------------------------
+void launch_trellis_local(const TrellisView &v, double *local, double *least, int *flag, hipStream_t s)
 {
-    hipLaunchKernelGGL(trellis_posterior_kernel, dim3((unsigned)v.rows), dim3(256), 0, s, v.cand, v.tdist, v.C, alpha, beta, logz, v.off, v.first,
-                       v.n_utts, v.c0, v.K, v.n_units, v.inv_tau, edges, n_buckets, posterior, row_uses);
+    hipLaunchKernelGGL(trellis_local_kernel, dim3((unsigned)((v.rows + 3) / 4)), dim3(256), 0, s, v, local, least, flag);
+}
+
+// The widest tile a thread's registers hold is 7 x 7 cells (two workgroups a compute unit): K is cut into as few equal tiles.
+void launch_trellis_costs(const TrellisView &v, const TrellisCosts &c, bool logs, int *flag, double *X, hipStream_t s)
+{
+    if (v.rows < 2) return;
+    const int n = (v.K + 111) / 112, rt = ((v.K + n - 1) / n + 15) / 16;
+    const dim3 grid((unsigned)(v.rows - 1), n, n);
+#define SNK_COST(RT_)                                                                                                        \
+    do {                                                                                                                     \
+        if (logs) hipLaunchKernelGGL((trellis_cost_kernel<RT_, true>), grid, dim3(256), 0, s, v, c, flag, X);                \
+        else hipLaunchKernelGGL((trellis_cost_kernel<RT_, false>), grid, dim3(256), 0, s, v, c, flag, X);                    \
+    } while (0)
+    if (rt <= 2) SNK_COST(2);
+    else if (rt <= 4) SNK_COST(4);
+    else if (rt == 5) SNK_COST(5);
+    else if (rt == 6) SNK_COST(6);
+    else SNK_COST(7);
+#undef SNK_COST
+}
+
+void launch_trellis_forward(const TrellisView &v, const double *local, const double *least, double bias_min, int *flag, double *V,
+                            double *logz, hipStream_t s)
+{
+#define SNK_FWD(KPM_, CH_, NB_, NTH_) hipLaunchKernelGGL((trellis_forward_kernel<KPM_, CH_, NB_, NTH_>), dim3(v.n_utts), dim3(NTH_), 0, s, v, local, least, bias_min, flag, V, logz)
+    if (v.K <= 32) SNK_FWD(8, 1, 4, 64);
+    else if (v.K <= 64) SNK_FWD(16, 1, 4, 128);
+    else if (v.K <= 104) SNK_FWD(26, 1, 2, 256);
+    else if (v.K <= 128) SNK_FWD(16, 2, 4, 256);
+    else SNK_FWD(26, 2, 2, 448);
+#undef SNK_FWD
+}
+
+void launch_trellis_backward(const TrellisView &v, const double *local, int *flag, double *Wt, hipStream_t s)
+{
+#define SNK_BWD(KC_, CH_, NB_, NTH_) hipLaunchKernelGGL((trellis_backward_kernel<KC_, CH_, NB_, NTH_>), dim3(v.n_utts), dim3(NTH_), 0, s, v, local, flag, Wt)
+    if (v.K <= 32) SNK_BWD(4, 1, 4, 128);
+    else if (v.K <= 64) SNK_BWD(8, 1, 4, 256);
+    else if (v.K <= 112) SNK_BWD(14, 1, 3, 448);
+    else SNK_BWD(26, 2, 2, 448);
+#undef SNK_BWD
+}
+
+void launch_trellis_forward_log(const TrellisView &v, bool sum, const int *flag, double *alpha, double *logz, hipStream_t s)
+{
+    if (sum) hipLaunchKernelGGL((trellis_forward_log_kernel<true>), dim3(v.n_utts), dim3(1024), 0, s, v, flag, alpha, logz);
+    else hipLaunchKernelGGL((trellis_forward_log_kernel<false>), dim3(v.n_utts), dim3(1024), 0, s, v, flag, alpha, logz);
+}
+
+void launch_trellis_backward_log(const TrellisView &v, const int *flag, double *beta, hipStream_t s)
+{
+    hipLaunchKernelGGL(trellis_backward_log_kernel, dim3(v.n_utts), dim3(1024), 0, s, v, flag, beta);
+}
+
+void launch_trellis_posterior(const TrellisView &v, const int *flag, const double *V, const double *Wt, const double *local, const double *logz,
+                              const int *edges, int n_buckets, double *posterior, double *row_uses, hipStream_t s)
+{
+    hipLaunchKernelGGL(trellis_posterior_kernel, dim3((unsigned)v.rows), dim3(256), 0, s, v, flag, V, Wt, local, logz, edges, n_buckets, posterior, row_uses);
 }
 
 void launch_trellis_uses(const double *row_uses, const int32_t *join_class, int64_t rows, int n_classes, int n_buckets, double *uses, hipStream_t s)
@@ -283,19 +912,46 @@ void launch_trellis_uses(const double *row_uses, const int32_t *join_class, int6
     hipLaunchKernelGGL(trellis_uses_kernel, dim3(n_classes, n_buckets), dim3(256), 0, s, row_uses, join_class, rows, n_buckets, uses);
 }
 
-void launch_trellis_draw(const TrellisView &v, const SampleRuleHost &rule, const double *alpha, const double *u, int n_draws, int64_t all_rows,
-                         int all_utts, int64_t *path, double *cost, double *logp, hipStream_t s)
+size_t trellis_draw_bytes(int64_t rows, int n_utts, int K, int n_draws, size_t (&at)[5])
 {
-    // the scores of a row carry the temperature already
+    // pointers | slots | roots | row costs | row log probabilities
+    const size_t n = (size_t)n_draws * rows;
+    const size_t part[5] = {n * K, n, (size_t)n_draws * n_utts * sizeof(int), n * sizeof(double), n * sizeof(double)};
+    size_t total = 0;
+    for (int i = 0; i < 5; ++i) { at[i] = total; total += (part[i] + 255) & ~(size_t)255; }
+    return total;
+}
+
+void launch_trellis_draw(const TrellisView &v, const TrellisCosts &c, const SampleRuleHost &rule, const int *flag, const double *V, const double *u,
+                         int n_draws, int64_t all_rows, int all_utts, char *work, int64_t *path, double *cost, double *logp, hipStream_t s)
+{
+    // the weights carry the temperature already
     SampleRule k;
     const bool greedy = !(rule.temperature > 0.0);
     k.inv_tau = 1.0; k.top_k = greedy ? 1 : rule.top_k; k.top_p = rule.top_p; k.min_p = rule.min_p;
-#define SNK_DRAW(E_) hipLaunchKernelGGL((trellis_draw_kernel<E_>), dim3(v.n_utts, n_draws), dim3(64), 0, s, v.cand, v.tdist, v.C, alpha, v.off, v.first, v.c0, \
-                                        v.K, v.n_units, v.inv_tau, k, greedy, u, all_rows, all_utts, path, cost, logp)
+    size_t at[5];
+    trellis_draw_bytes(all_rows, all_utts, v.K, n_draws, at);
+    unsigned char *pointer = (unsigned char *)work + at[0], *slots = (unsigned char *)work + at[1];
+    int *root = (int *)(work + at[2]);
+    double *row_cost = (double *)(work + at[3]), *row_logp = (double *)(work + at[4]);
+    const dim3 grid((unsigned)v.rows, (v.K + SNK_POINTER_COLUMNS - 1) / SNK_POINTER_COLUMNS);
+    const size_t lds = (size_t)SNK_POINTER_COLUMNS * (v.K | 1) * sizeof(double);
+#define SNK_DRAW(E_) hipLaunchKernelGGL((trellis_pointer_kernel<E_>), grid, dim3(256), lds, s, v, flag, V, k, greedy, u, n_draws, all_rows, all_utts, pointer, root)
     if (v.K <= 64) SNK_DRAW(1);
     else if (v.K <= 128) SNK_DRAW(2);
     else SNK_DRAW(4);
 #undef SNK_DRAW
+    static size_t attr_set[32] = {0};
+    lds_attr_ensure(attr_set, SNK_CHASE_BYTES, [] {
+        (void)hipFuncSetAttribute(reinterpret_cast<const void *>(&trellis_chase_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, SNK_CHASE_BYTES); });
+    hipLaunchKernelGGL(trellis_chase_kernel, dim3(v.n_utts, n_draws), dim3(512), SNK_CHASE_BYTES, s, v, pointer, root, all_rows, all_utts, slots);
+    const dim3 rows((unsigned)((v.rows + 3) / 4), n_draws);
+#define SNK_PATH(E_) hipLaunchKernelGGL((trellis_path_kernel<E_>), rows, dim3(256), 0, s, v, c, flag, V, k, root, slots, all_rows, all_utts, path, row_cost, row_logp)
+    if (v.K <= 64) SNK_PATH(1);
+    else if (v.K <= 128) SNK_PATH(2);
+    else SNK_PATH(4);
+#undef SNK_PATH
+    hipLaunchKernelGGL(trellis_total_kernel, dim3(v.n_utts, n_draws), dim3(256), 0, s, v, root, row_cost, row_logp, all_rows, all_utts, cost, logp);
 }
 
 }  // namespace snk
