@@ -500,3 +500,20 @@ def load_full_spectra(full_magphase_dir, names, fft_half_len=FFTHALFLEN):
         spans[name] = (row, row + n)
         row += n
     return np.vstack(specs), np.vstack(fzvs), spans
+
+
+def position_bucket_edges(n_buckets, max_distance):
+    """Edges of n_buckets buckets of the distance between consecutive units (engine.set_position_bias): the steps 0 (the same
+    unit again) and 1 (its natural successor) in buckets of their own, growing distances up to max_distance either side."""
+    if n_buckets < 4:
+        raise ValueError('position_bucket_edges: at least 4 buckets')
+    behind, ahead = (n_buckets - 4) // 2, (n_buckets - 4) - (n_buckets - 4) // 2
+
+    def far(n):
+        # n distances from 2 to max_distance, growing by a constant factor where that is more than one step
+        out = []
+        for i in range(n):
+            d = int(round(2.0 * (max_distance / 2.0) ** ((i + 1.0) / n)))
+            out.append(max(d, out[-1] + 1 if out else 3))
+        return out
+    return [-d + 1 for d in reversed(far(behind))] + [0, 1, 2] + far(ahead)

@@ -16,6 +16,7 @@ import glob
 import re
 import os
 import timeit
+import zlib
 
 import numpy as np
 
@@ -28,6 +29,7 @@ VERY_BIG_WEIGHT_VALUE = 1000000000000000.0
 
 
 class Synthesiser(object):
+    _position_bias = None
 
     def __init__(self, config_file, holdout_percent=0.0, flavour=None, device=0, verbose=True):
         self.mode_of_operation = 'normal'
@@ -119,6 +121,9 @@ class Synthesiser(object):
             self.get_tree_for_greedy_search()
         elif self.config.get('preselection_method') == 'monophone_then_acoustic':
             self._setup_monophone_classes()
+
+        if self.config.get('position_bias'):
+            self.set_position_bias(**self.config['position_bias'])
 
         self.test_data_target_dirs = hp.locate_stream_directories(self.config['test_data_dirs'], self.stream_list_target)
         if self.config.get('tune_data_dirs', ''):
@@ -371,6 +376,91 @@ class Synthesiser(object):
         self.report(best_path)
         return best_path
 
+    # ------------------------------------------------------------------ draws
+    # Settings (no counterpart in the reference), for configurations that preselect candidates:
+    #   unit_sampling = {'temperature': 0.5, 'top_k': 20, 'top_p': 0.9, 'min_p': 0.0, 'seed': 0, 'joins': True}
+    #       synth_utt draws its path from exp(-cost / temperature) instead of taking the cheapest; joins False: every row from
+    #       its target costs alone.  The draws of an utterance follow from the seed and its name.
+    #   position_bias = {'bias': [[...], ...], 'edges': [...], 'classes': {phone: row of the bias}}
+    #       added to the join costs by the distance between the units joined (train_position_bias.py learns one); the class of
+    #       a join is its left unit's phone where 'classes' is given, row 0 otherwise.
+    def set_position_bias(self, bias, edges=(), classes=None):
+        """Position bias of the searches below (engine.set_position_bias); None removes it."""
+        self.engine.set_position_bias(bias, edges)
+        self._position_bias = None if bias is None else {'bias': np.array(bias, dtype=np.float64), 'edges': [int(e) for e in edges], 'classes': classes}
+
+    def join_classes(self, unit_names, rows):
+        """Row of the position bias for the join behind every unit: int32 (rows,), or None (row 0 throughout)."""
+        classes = self._position_bias['classes'] if self._position_bias else None
+        if classes is None or unit_names is None:
+            return None
+        assert len(unit_names) == rows, (len(unit_names), rows)
+        return np.array([classes.get(name.split(LABEL_DELIMITER)[2], -1) for name in unit_names], dtype=np.int32)
+
+    def _random_numbers(self, base, shape):
+        seed = (self.config.get('unit_sampling') or {}).get('seed', 0)
+        return np.random.RandomState([int(seed) & 0xffffffff, zlib.crc32(base.encode())]).random_sample(shape)
+
+    def _sampling_rule(self):
+        """Truncations of a draw; without unit_sampling: temperature 0, the cheapest path under the position bias."""
+        how = self.config.get('unit_sampling')
+        if not how:
+            return dict(temperature=0.0)
+        unknown = set(how) - set(['temperature', 'top_k', 'top_p', 'min_p', 'seed', 'joins'])
+        if unknown:
+            raise ValueError('unit_sampling: unknown settings %s' % sorted(unknown))
+        return dict(temperature=how.get('temperature', 1.0), top_k=how.get('top_k', 0), top_p=how.get('top_p', 1.0), min_p=how.get('min_p', 0.0))
+
+    def draws_paths(self):
+        """Whether synth_utt draws (or biases) its path instead of taking that of viterbi_search."""
+        return bool(self.config.get('unit_sampling')) or self._position_bias is not None
+
+    def sample_units(self, candidates, distances, u):
+        """A unit per row, drawn from its target costs alone: unit ids (draws, rows) with -1 where a row has no candidate.
+        u (draws, rows)."""
+        candidates = np.asarray(candidates, dtype=np.int64)
+        usable = (candidates >= 1) & (candidates < self.join_contexts_unweighted.shape[0] - 2)
+        scores = np.where(usable, -np.asarray(distances, dtype=np.float64), -np.inf)
+        index, _ = self.engine.sample_rows(scores, np.ascontiguousarray(np.asarray(u).T), **self._sampling_rule())
+        units = np.take_along_axis(candidates, np.maximum(index, 0), axis=1)
+        return np.where(index >= 0, units, -1).T
+
+    def sample_search(self, candidates, distances, u, row_offsets=None, join_class=None):
+        """Paths drawn from the candidates of one or several utterances (engine.sample_paths under unit_sampling and
+        position_bias): unit ids (draws, rows), costs and log probabilities (draws, utterances)."""
+        t = self.start_clock('Draw paths')
+        out = self.engine.sample_paths(candidates, distances, u, row_offsets=row_offsets, join_class=join_class, **self._sampling_rule())
+        self.stop_clock(t)
+        return out
+
+    def draw_paths(self, names, candidates, distances, unit_names):
+        """One path per utterance, as viterbi_search returns them: an empty one where there is none."""
+        how = self.config.get('unit_sampling') or {}
+        lengths = [len(c) for c in candidates]
+        offs = np.concatenate([[0], np.cumsum(lengths)]).astype(np.int64)
+        cand, dist = np.vstack(candidates), np.vstack(distances)
+        u = np.concatenate([self._random_numbers(n, (1, k)) for n, k in zip(names, lengths)], axis=1)
+        if not how.get('joins', True):
+            path = self.sample_units(cand, dist, u)
+        else:
+            classes = [self.join_classes(w, k) for w, k in zip(unit_names, lengths)]
+            join_class = None if classes[0] is None else np.concatenate(classes)
+            path, cost, _ = self.sample_search(cand, dist, u, row_offsets=offs, join_class=join_class)
+            self.last_path_cost = float(cost[0, -1])
+        paths = [path[0, a:b] for a, b in zip(offs[:-1], offs[1:])]
+        return [[] if (p < 0).any() else [int(k) for k in p] for p in paths]
+
+    def preselect_units(self, unit_features, unit_names):
+        """Candidates and target costs by the configured method."""
+        method = self.config['preselection_method']
+        if method == 'acoustic':
+            return self.preselect_units_acoustic(unit_features)
+        if method == 'quinphone':
+            return self.preselect_units_quinphone(unit_features, unit_names)
+        if method == 'monophone_then_acoustic':
+            return self.preselect_units_monophone_then_acoustic(unit_features, unit_names)
+        raise SystemExit('preselection_method unknown')
+
     # ------------------------------------------------------------------ drivers
     def get_sentence_set(self, set_name):
         """synth_simple.py:287-339."""
@@ -442,7 +532,7 @@ class Synthesiser(object):
         """What set_*_weights / truncate_* / reconfigure_settings changed since the config file was read."""
         return {'config': dict(self.config), 'target_weight_vector': self.target_weight_vector.copy(),
                 'join_weight_vector': self.join_weight_vector.copy(), 'target_trunc': self._target_trunc,
-                'join_trunc': self._join_trunc, 'mode_of_operation': self.mode_of_operation}
+                'join_trunc': self._join_trunc, 'mode_of_operation': self.mode_of_operation, 'position_bias': self._position_bias}
 
     def _restore_runtime_state(self, state):
         self.config = dict(state['config'])
@@ -452,6 +542,7 @@ class Synthesiser(object):
         if self._target_trunc is not None:
             self.target_truncation_vector = self._target_trunc
         self.mode_of_operation = state['mode_of_operation']
+        self.set_position_bias(**(state['position_bias'] or {'bias': None}))
         self._apply_weights()
 
     def _weight_targets(self, unit_features):
@@ -522,6 +613,19 @@ class Synthesiser(object):
                         for U, p in zip(feats, paths)]
             return paths
         method = self.config.get('preselection_method')
+        if plain and fnames and self.draws_paths() and not self.config.get('greedy_search', False):
+            # candidates per utterance as in synth_utt, then ONE call for the draws of all of them
+            t = self.start_clock('Get speech + preselection (bulk)')
+            feats, names, cands, dists = [], [], [], []
+            for f in fnames:
+                U, w = self.prepare_targets(f, synth_type, return_names=True)
+                c, d = self.preselect_units(U, w)
+                feats.append(U); names.append(w); cands.append(c); dists.append(d)
+            self.stop_clock(t)
+            paths = self.draw_paths(fnames, cands, dists, names)
+            if self.mode_of_operation == 'stream_weight_balancing':
+                return [(self.get_target_scores_per_stream(U, p), self.get_join_scores_per_stream(p)) for U, p in zip(feats, paths)]
+            return paths
         if (plain and len(fnames) > 1 and not self.config.get('greedy_search', False)
                 and method in ('quinphone', 'monophone_then_acoustic')):
             # label-driven preselection (the reference's own configs use 'quinphone'): candidates per utterance as in
@@ -586,18 +690,13 @@ class Synthesiser(object):
             assert self.config.get('target_representation') == 'epoch'
             best_path = self.greedy_joint_search(unit_features)
         else:
-            method = self.config['preselection_method']
-            if method == 'acoustic':
-                candidates, distances = self.preselect_units_acoustic(unit_features)
-            elif method == 'quinphone':
-                candidates, distances = self.preselect_units_quinphone(unit_features, unit_names)
-            elif method == 'monophone_then_acoustic':
-                candidates, distances = self.preselect_units_monophone_then_acoustic(unit_features, unit_names)
-            else:
-                raise SystemExit('preselection_method unknown')
+            candidates, distances = self.preselect_units(unit_features, unit_names)
             if self.mode_of_operation == 'find_join_candidates':
                 return candidates
-            best_path = self.viterbi_search(candidates, distances)
+            if self.draws_paths():
+                best_path = self.draw_paths([base], [candidates], [distances], [unit_names])[0]
+            else:
+                best_path = self.viterbi_search(candidates, distances)
         if self.mode_of_operation == 'stream_weight_balancing':
             return (self.get_target_scores_per_stream(unit_features, best_path),
                     self.get_join_scores_per_stream(best_path))
