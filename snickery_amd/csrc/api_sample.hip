@@ -193,6 +193,15 @@ static int trellis_groups(snk_engine *h, const TrellisCall &q, Use use)
         v.c0 = q.row_offsets[v0]; v.rows = q.row_offsets[v1] - q.row_offsets[v0];
         v.n_units = h->Njc - 1;
         v.inv_tau = q.temperature > 0.0 ? 1.0 / q.temperature : 1.0;
+        v.pieces = trellis_most_pieces(q.row_offsets + v0, v.n_utts);
+        if (v.pieces > 1) {
+            const size_t n = trellis_piece_places(v);
+            CHK(h->tr_M.ensure(n * row_bytes));
+            CHK(h->tr_exps.ensure(n * q.K * sizeof(int)));
+            CHK(h->tr_ends_v.ensure(n * Kp * sizeof(double)));
+            CHK(h->tr_ends_w.ensure(n * Kp * sizeof(double)));
+            CHK(h->tr_scaled.ensure((size_t)q.n_utts * sizeof(int64_t)));
+        }
         CHK(h->tr_C.ensure((size_t)v.rows * row_bytes));
         v.C = h->tr_C.as<double>();
         CHK(use(v, c));
@@ -219,7 +228,10 @@ static int sample_paths_device(snk_engine *h, const TrellisCall &q, const double
                 launch_trellis_costs(v, c, false, flag, X, h->stream);
             }
             StageTimer t(h, h->stream, q.timed ? TM_TRELLIS_SUM : -1);
-            launch_trellis_forward(v, h->tr_local.as<double>(), h->tr_least.as<double>(), c.bias_min, flag, V, nullptr, h->stream);
+            launch_trellis_ends(v, h->tr_local.as<double>(), false, flag, h->tr_M.as<double>(), h->tr_exps.as<int>(), h->tr_ends_v.as<double>(),
+                                h->tr_ends_w.as<double>(), h->tr_scaled.as<int64_t>(), h->stream);
+            launch_trellis_forward(v, h->tr_local.as<double>(), h->tr_least.as<double>(), c.bias_min, h->tr_ends_v.as<double>(), h->tr_scaled.as<int64_t>(),
+                                   flag, V, nullptr, h->stream);
         }
         {
             StageTimer t(h, h->stream, q.timed ? TM_TRELLIS_SUM : -1);
@@ -247,14 +259,17 @@ static int path_posterior_device(snk_engine *h, const TrellisCall &q, double *lo
         }
         {
             StageTimer t(h, h->stream, q.timed ? TM_TRELLIS_SUM : -1);
-            launch_trellis_forward(v, local, h->tr_least.as<double>(), c.bias_min, flag, V, logz, h->stream);
-            launch_trellis_backward(v, local, flag, W, h->stream);
+            launch_trellis_ends(v, local, true, flag, h->tr_M.as<double>(), h->tr_exps.as<int>(), h->tr_ends_v.as<double>(), h->tr_ends_w.as<double>(),
+                                h->tr_scaled.as<int64_t>(), h->stream);
+            launch_trellis_forward(v, local, h->tr_least.as<double>(), c.bias_min, h->tr_ends_v.as<double>(), h->tr_scaled.as<int64_t>(), flag, V, logz,
+                                   h->stream);
+            launch_trellis_backward(v, local, h->tr_ends_w.as<double>(), flag, W, h->stream);
             launch_trellis_costs(v, c, true, flag, X, h->stream);
             launch_trellis_forward_log(v, true, flag, V, logz, h->stream);
             launch_trellis_backward_log(v, flag, W, h->stream);
         }
         StageTimer t(h, h->stream, q.timed ? TM_TRELLIS_POST : -1);
-        launch_trellis_posterior(v, flag, V, W, local, logz, h->pb_edges.as<int>(), h->pb_buckets, posterior,
+        launch_trellis_posterior(v, flag, V, W, h->tr_ends_w.as<double>(), local, logz, h->pb_edges.as<int>(), h->pb_buckets, posterior,
                                  uses ? h->tr_row_uses.as<double>() : nullptr, h->stream);
         return 0;
     }));

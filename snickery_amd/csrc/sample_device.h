@@ -117,6 +117,26 @@ __device__ __forceinline__ double wave_max(double v)
     v = dpp_max(v, dpp_move<0x143, 0xc>(SNK_BITS(v), SNK_BITS(v)));
     return wave_lane(v, 63);
 }
+__device__ __forceinline__ double row16_max(double v)      // of each row of 16 lanes, in its last lane
+{
+    v = dpp_max(v, dpp_move<0x111, 0xf>(SNK_BITS(v), SNK_BITS(v)));
+    v = dpp_max(v, dpp_move<0x112, 0xf>(SNK_BITS(v), SNK_BITS(v)));
+    v = dpp_max(v, dpp_move<0x114, 0xf>(SNK_BITS(v), SNK_BITS(v)));
+    v = dpp_max(v, dpp_move<0x118, 0xf>(SNK_BITS(v), SNK_BITS(v)));
+    return v;
+}
+__device__ __forceinline__ double quad_sum(double v)       // of each four lanes, in all of them
+{
+    v += __longlong_as_double((long long)dpp_move<0xb1, 0xf>(0, SNK_BITS(v)));
+    v += __longlong_as_double((long long)dpp_move<0x4e, 0xf>(0, SNK_BITS(v)));
+    return v;
+}
+__device__ __forceinline__ double rows4_sum(double v)      // of the same lane of the four rows of 16, in all of them
+{
+    v += __shfl_xor(v, 16, 64);
+    v += __shfl_xor(v, 32, 64);
+    return v;
+}
 __device__ __forceinline__ double wave_sum(double v)
 {
     v += __longlong_as_double((long long)dpp_move<0x111, 0xf>(0, SNK_BITS(v)));

@@ -451,6 +451,7 @@ struct snk_engine {
     DevBuf sr_scores, sr_u, sr_rules, sr_index, sr_logp;
     double pb_min = 0.0;                   // the smallest finite bias, at most 0
     DevBuf tr_off, tr_cand, tr_tdist, tr_class, tr_u, tr_C, tr_V, tr_W, tr_local, tr_least, tr_flag, tr_draw, tr_row_uses, tr_out;
+    DevBuf tr_M, tr_exps, tr_ends_v, tr_ends_w, tr_scaled;      // the pieces of the recursions
     hipEvent_t tr_in = nullptr, tr_done = nullptr;      // hand-over between a caller's stream and the engine's
     DevBuf vstats;             // [0] cells refined, [1] steps with a refinement, [2] exact costs computed there
     // pass 1 of the sparse path, second form (joinfast_kernels.hip: join_lb2_kernel): float32 copy of the weighted join rows,

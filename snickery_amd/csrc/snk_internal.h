@@ -369,6 +369,7 @@ struct TrellisView {
     int first, n_utts, K, Kp;
     int64_t c0, rows, n_units;
     double inv_tau;
+    int pieces;               // most pieces an utterance's recursions are cut into
 };
 struct TrellisCosts {         // what the cost of a join is made of
     const float *JC; int Jp, Dj; const double *wj;
@@ -377,12 +378,16 @@ struct TrellisCosts {         // what the cost of a join is made of
 };
 void launch_trellis_local(const TrellisView &v, double *local, double *least, int *flag, hipStream_t s);
 void launch_trellis_costs(const TrellisView &v, const TrellisCosts &c, bool logs, int *flag, double *X, hipStream_t s);
-void launch_trellis_forward(const TrellisView &v, const double *local, const double *least, double bias_min, int *flag, double *V, double *logz,
-                            hipStream_t s);
-void launch_trellis_backward(const TrellisView &v, const double *local, int *flag, double *Wt, hipStream_t s);
+int trellis_most_pieces(const int64_t *off, int n_utts);
+size_t trellis_piece_places(const TrellisView &v);    // entries of the pieces' tables: products (K x Kp), exponents (K), ends (Kp)
+void launch_trellis_ends(const TrellisView &v, const double *local, bool both, int *flag, double *M, int *exps, double *ends_v, double *ends_w,
+                         int64_t *scaled, hipStream_t s);
+void launch_trellis_forward(const TrellisView &v, const double *local, const double *least, double bias_min, const double *ends,
+                            const int64_t *ends_scaled, int *flag, double *V, double *logz, hipStream_t s);
+void launch_trellis_backward(const TrellisView &v, const double *local, const double *ends, int *flag, double *Wt, hipStream_t s);
 void launch_trellis_forward_log(const TrellisView &v, bool sum, const int *flag, double *alpha, double *logz, hipStream_t s);
 void launch_trellis_backward_log(const TrellisView &v, const int *flag, double *beta, hipStream_t s);
-void launch_trellis_posterior(const TrellisView &v, const int *flag, const double *V, const double *Wt, const double *local, const double *logz,
+void launch_trellis_posterior(const TrellisView &v, const int *flag, const double *V, const double *Wt, const double *ends, const double *local, const double *logz,
                               const int *edges, int n_buckets, double *posterior, double *row_uses, hipStream_t s);
 void launch_trellis_uses(const double *row_uses, const int32_t *join_class, int64_t rows, int n_classes, int n_buckets, double *uses, hipStream_t s);
 size_t trellis_draw_bytes(int64_t rows, int n_utts, int K, int n_draws, size_t (&at)[5]);

@@ -215,108 +215,382 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
     if (!LOG && wide) flag[u] = 1;
 }
 
-// ---- forward: a workgroup per utterance, a step per row ------------------------------------------------------------------------------
-// A wavefront owns 32 columns (two a lane); its four rows of 16 lanes split the predecessors, so a step's sums end inside the
-// wavefront and a step costs one barrier.  The cells of the next steps are in flight in registers: a slab is K x Kp x 8 bytes
-// through one compute unit, and that (64 bytes a cycle) is what a step takes.  A thread's R = 4 CH KPM / 4 predecessors come in CH
-// pieces of KPM.
+// ---- the recursions, cut into pieces ---------------------------------------------------------------------------------------------------
+// A step of a recursion is one K x K slab of cells through one compute unit: a chain of T of them takes T times 1 - 5 us and keeps
+// one unit of 256 busy.  So an utterance's T - 1 slabs are cut into pieces of L, and
+//     1. every piece's product  M = prod E[t] diag(l_t+1)  is formed, sixteen of its rows a workgroup, on the float64 matrix pipe
+//     2. the weights at the pieces' ends follow from the products, one vector-matrix product a piece (both directions)
+//     3. every piece runs its own recursion from there, all pieces side by side
+// Pieces of L take  L (product + step) + T / L ends  where the chain takes T steps, and a product, a step and an end cost about the
+// same on their own: L = sqrt(T).  Below 24 slabs the chain is as fast, the third launch alone.  Only an utterance's own length decides:
+// its results are the same in any batch.  A piece is found without a table: no piece has less than 8 slabs, so those of utterance u
+// begin at  floor((off[u] - c0) / 8) + u - first.
+#define SNK_PIECE_LEAST 8
+__host__ __device__ __forceinline__ int64_t trellis_piece_length(int64_t slabs)
+{
+    if (slabs < 24) return slabs > 0 ? slabs : 1;
+    const int64_t L = (int64_t)ceil(sqrt((double)slabs));
+    return L < SNK_PIECE_LEAST ? SNK_PIECE_LEAST : L;
+}
+
+struct TrellisPiece { int64_t r0, T, L; int u, k, n, P; int64_t at; };   // rows of the utterance; piece k of P, n of L slabs, its place in the tables
+
+__device__ __forceinline__ TrellisPiece trellis_piece(const TrellisView &v, int utt, int k)
+{
+    TrellisPiece p;
+    p.u = v.first + utt;
+    p.r0 = v.off[p.u];
+    p.T = v.off[p.u + 1] - p.r0;
+    const int64_t S = p.T - 1;
+    p.L = trellis_piece_length(S);
+    p.P = S > p.L ? (int)((S + p.L - 1) / p.L) : 1;
+    p.k = k;
+    const int64_t left = S - (int64_t)k * p.L;
+    p.n = k < p.P ? (int)(left < p.L ? left : p.L) : 0;
+    p.at = (p.r0 - v.c0) / SNK_PIECE_LEAST + utt + k;
+    return p;
+}
+
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+
+// 1. products: workgroup = sixteen start candidates of one piece, wavefront = CT tiles of sixteen end candidates; v_mfma_f64_16x16x4
+// over KH CH steps of four.  The weights X (16 x K) alternate between two LDS buffers; the slab's fragments live in registers and
+// each is reloaded with the next slab's (or the next half's) right after its use.  The row blocks of a piece are dealt to one XCD,
+// so that a slab comes from memory once and from that XCD's L2 for the others.
+template <int CT, int KH, int CH, int NTH>
+__global__ void __launch_bounds__(NTH)
+trellis_product_kernel(const TrellisView v, const double *__restrict__ local, int max_pieces, int row_blocks, bool skip_last, int *__restrict__ flag,
+                       double *__restrict__ M, int *__restrict__ exps)
+{
+    constexpr int W = NTH / 64, COLS = 4 * KH * CH, LDX = COLS + 4;
+    __shared__ double X[2][16 * LDX];
+    __shared__ double top[2][W][16];
+    __shared__ int bad;
+    const int j = blockIdx.x >> 3;
+    const int i0 = (j % row_blocks) * 16, flat = (j / row_blocks) * 8 + (blockIdx.x & 7);
+    if (flat >= max_pieces * v.n_utts) return;
+    const TrellisPiece p = trellis_piece(v, flat / max_pieces, flat % max_pieces);
+    if (p.k >= p.P || p.P == 1 || (skip_last && p.k == p.P - 1) || flag[p.u]) return;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c16 = lane & 15, g = lane >> 4;
+    const int K = v.K, Kp = v.Kp, slab_bytes = K * Kp * 8;
+    const int64_t first_row = p.r0 + (int64_t)p.k * p.L;
+    const double *__restrict__ slab0 = v.C + (first_row - v.c0) * ((int64_t)K * Kp);
+    int col[CT], voff[CT];
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        col[c] = (wave * CT + c) * 16 + c16;
+        voff[c] = col[c] < Kp ? (g * Kp + col[c]) * 8 : 0x7ff00000;
+    }
+    double frag[KH][CT];
+    auto load = [&](int slab, int half, int ks, int c) {        // (rows beyond K lie beyond the slab: they read as 0)
+        slab = slab < p.n ? slab : p.n - 1;
+        const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc(const_cast<double *>(slab0 + slab * ((int64_t)K * Kp)), 0, slab_bytes, 0x00020000);
+        const int row = min((half * KH + ks) * 4 * Kp * 8, slab_bytes);
+        frag[ks][c] = __builtin_bit_cast(double, __builtin_amdgcn_raw_buffer_load_b64(res, voff[c], row, 0));
+    };
+    if (p.n > 1) {
+#pragma unroll
+        for (int ks = 0; ks < KH; ++ks)
+#pragma unroll
+            for (int c = 0; c < CT; ++c) load(1, 0, ks, c);
+    }
+    for (int i = tid; i < 2 * 16 * LDX; i += NTH) (&X[0][0])[i] = 0.0;
+    if (tid == 0) bad = 0;
+    if (tid < W * 16) top[0][tid >> 4][tid & 15] = 0.0;
+    __syncthreads();
+    // the first slab: the start candidate's own cells
+    bool small = false;
+    double m4[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+    for (int c = 0; c < CT; ++c) {
+        if (col[c] >= Kp) continue;
+        const double l = local[(first_row + 1) * Kp + col[c]];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int row = g + 4 * r;
+            const double x = i0 + row < K ? slab0[(int64_t)(i0 + row) * Kp + col[c]] * l : 0.0;
+            X[0][row * LDX + col[c]] = x;
+            m4[r] = fmax(m4[r], x);
+            small |= x > 0.0 && x < SNK_WEIGHT_LEAST;
+        }
+    }
+    auto row_max = [&](int at) {                                // largest weight of every row, per wavefront (lane 15 of each row of lanes has it)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const double m = row16_max(m4[r]);
+            if (c16 == 15) top[at][wave][g + 4 * r] = m;
+        }
+    };
+    row_max(0);
+    __syncthreads();
+    int e4[4] = {0, 0, 0, 0};
+    for (int s = 1; s < p.n; ++s) {
+        const int from = (s - 1) & 1, to = s & 1;
+        f64x4 acc[CT];
+#pragma unroll
+        for (int c = 0; c < CT; ++c) acc[c] = f64x4{0.0, 0.0, 0.0, 0.0};
+        double lw[CT];
+#pragma unroll
+        for (int c = 0; c < CT; ++c) lw[c] = col[c] < Kp ? local[(first_row + s + 1) * Kp + col[c]] : 0.0;
+#pragma unroll
+        for (int half = 0; half < CH; ++half) {
+            const int nslab = half + 1 < CH ? s : s + 1, nhalf = half + 1 < CH ? half + 1 : 0;
+#pragma unroll
+            for (int ks = 0; ks < KH; ++ks) {
+                const double x = X[from][c16 * LDX + (half * KH + ks) * 4 + g];
+#pragma unroll
+                for (int c = 0; c < CT; ++c) {
+                    acc[c] = __builtin_amdgcn_mfma_f64_16x16x4f64(x, frag[ks][c], acc[c], 0, 0, 0);
+                    load(nslab, nhalf, ks, c);
+                }
+            }
+        }
+        double f[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            double m = top[from][0][g + 4 * r];
+#pragma unroll
+            for (int w = 1; w < W; ++w) m = fmax(m, top[from][w][g + 4 * r]);
+            const int e = trellis_exponent(m);
+            e4[r] += e;
+            f[r] = trellis_pow2(-e);
+            m4[r] = 0.0;
+        }
+#pragma unroll
+        for (int c = 0; c < CT; ++c)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const double x = (acc[c][r] * f[r]) * lw[c];
+                if (col[c] < Kp) X[to][(g + 4 * r) * LDX + col[c]] = x;
+                m4[r] = fmax(m4[r], x);
+                small |= x > 0.0 && x < SNK_WEIGHT_LEAST;
+            }
+        row_max(to);
+        __syncthreads();
+    }
+    if (small) bad = 1;
+    __syncthreads();
+    if (bad) { if (tid == 0) flag[p.u] = 1; return; }
+    // out: rows scaled to [1, 2), their exponents beside them
+    const int at = (p.n - 1) & 1;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        const int row = g + 4 * r, i = i0 + row;
+        double m = top[at][0][row];
+#pragma unroll
+        for (int w = 1; w < W; ++w) m = fmax(m, top[at][w][row]);
+        const int e = trellis_exponent(m);
+        const double f = trellis_pow2(-e);
+        if (i < K) {
+#pragma unroll
+            for (int c = 0; c < CT; ++c)
+                if (col[c] < Kp) M[(p.at * K + i) * Kp + col[c]] = X[at][row * LDX + col[c]] * f;
+            if (wave == 0 && c16 == 0) exps[p.at * K + i] = e4[r] + e;
+        }
+    }
+}
+
+// 2. the weights at the pieces' ends: a workgroup per utterance.  Forward: thread = (pair of columns, every PARTS-th row), backward:
+// Q threads a row, (row, every Q-th pair of columns).  A thread's cells come in H parts of R; each is reloaded with the next part's
+// right after its use.
+template <int R, int H, int Q>
+__global__ void __launch_bounds__(1024)
+trellis_ends_kernel(const TrellisView v, const double *__restrict__ local, const double *__restrict__ M, const int *__restrict__ exps,
+                    int *__restrict__ flag, double *__restrict__ ends_out, int64_t *__restrict__ scaled_out)
+{
+    constexpr bool BACK = Q > 0;
+    __shared__ double vec[256], part[2048], red[16];
+    __shared__ int bad;
+    const TrellisPiece p = trellis_piece(v, blockIdx.x, 0);
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, K = v.K, Kp = v.Kp;
+    if (flag[p.u]) return;
+    const int bytes = K * Kp * 8;
+    const double *__restrict__ m0 = M + p.at * K * Kp;
+    const int *__restrict__ e0 = exps + p.at * K;
+    double *__restrict__ ends = ends_out + p.at * Kp;
+    if (tid == 0) bad = 0;
+    const int pairs = Kp >> 1, parts = 1024 / pairs;
+    const int b = BACK ? 2 * (tid % (BACK ? Q : 1)) : 2 * (tid % pairs), a = BACK ? tid / (BACK ? Q : 1) : tid / pairs;
+    const bool on = BACK ? a < K : a < parts;
+    const int steps = p.P - 1, pieces = steps * H;
+    f64x2 m[R];
+    auto load = [&](int piece, int i) {                         // (rows beyond K and columns beyond Kp read as 0 or meet a weight of 0)
+        piece = piece < pieces ? piece : pieces - 1;
+        const int k = BACK ? p.P - 1 - piece / H : piece / H, n = (piece % H) * R + i;
+        const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc(const_cast<double *>(m0 + (int64_t)k * K * Kp), 0, bytes, 0x00020000);
+        const int off = on ? (a * Kp + b) * 8 : 0x7ff00000;
+        const int more = min(BACK ? n * Q * 16 : n * parts * Kp * 8, bytes);
+        m[i] = __builtin_bit_cast(f64x2, __builtin_amdgcn_raw_buffer_load_b128(res, off, more, 0));
+    };
+    double x = 0.0;                                             // weight of candidate tid
+    if (tid < Kp) {
+        x = BACK ? (tid < K ? 1.0 : 0.0) : local[p.r0 * Kp + tid];
+        ends[(int64_t)(BACK ? p.P - 1 : 0) * Kp + tid] = x;
+    }
+    if (tid < 256) vec[tid] = 0.0;
+    if (pieces > 0) {
+#pragma unroll
+        for (int i = 0; i < R; ++i) load(0, i);
+    }
+    int64_t scaled = 0;
+    bool small = false;
+    // scales the candidates' weights y 2^e to at most 2: forward the exponents belong to what goes into a product, backward to what comes out
+    auto scale = [&](double y, int e) -> double {
+        const double t = wave_max(y > 0.0 ? (double)(e + trellis_exponent(y)) : -1e30);
+        if (lane == 0) red[wave] = t;
+        __syncthreads();
+        double most = red[0];
+        for (int i = 1; i < (Kp + 63) >> 6; ++i) most = fmax(most, red[i]);
+        if (!(most > -1e29)) return 0.0;
+        scaled += (int64_t)most;
+        if (!(y > 0.0)) return 0.0;
+        const int have = trellis_exponent(y), d = have + e - (int)most;
+        if (d < -489) { small = true; return 0.0; }
+        return y * trellis_pow2(-have) * trellis_pow2(d);       // (y in [1, 2), then scaled down)
+    };
+    for (int s = 0; s < steps; ++s) {
+        const int k = BACK ? p.P - 1 - s : s;
+        const int e = tid < K ? e0[(int64_t)k * K + tid] : 0;
+        if (!BACK) x = scale(x, e);
+        if (tid < Kp) vec[tid] = x;
+        __syncthreads();
+        f64x2 sum = {0.0, 0.0};
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int i = 0; i < R; ++i) {
+                const int n = h * R + i;
+                if (BACK) {
+                    const int c = min(b + n * 2 * Q, 254);
+                    sum[0] = __fma_rn(vec[c], m[i][0], sum[0]);
+                    sum[1] = __fma_rn(vec[c + 1], m[i][1], sum[1]);
+                } else {
+                    const double w = vec[min(a + n * parts, 255)];
+                    sum[0] = __fma_rn(w, m[i][0], sum[0]);
+                    sum[1] = __fma_rn(w, m[i][1], sum[1]);
+                }
+                load(s * H + h + 1, i);
+            }
+        if (BACK) {
+            double y = sum[0] + sum[1];
+#pragma unroll
+            for (int o = 1; o < Q; o <<= 1) y += __shfl_xor(y, o, 64);
+            if (on && b == 0) part[a] = y;
+        } else if (on) { part[a * Kp + b] = sum[0]; part[a * Kp + b + 1] = sum[1]; }
+        __syncthreads();
+        if (BACK) x = scale(tid < K ? part[tid] : 0.0, e);
+        else if (tid < Kp) {
+            x = 0.0;
+            for (int i = 0; i < parts; ++i) x += part[i * Kp + tid];
+        }
+        if (tid < Kp) ends[(int64_t)(BACK ? k - 1 : k + 1) * Kp + tid] = x;
+    }
+    if (small) bad = 1;
+    __syncthreads();
+    if (tid == 0) {
+        if (bad) flag[p.u] = 1;
+        if (!BACK) scaled_out[p.u] = scaled;
+    }
+}
+
+// 3. forward.  A wavefront owns 32 columns (two a lane); its four rows of 16 lanes split the predecessors, so a step's sums end inside
+// the wavefront and a step costs one barrier.  A thread's KPM CH predecessors come in CH parts; every cell's register is reloaded
+// with a later slab's right after its use (NB parts ahead).
 template <int KPM, int CH, int NB, int NTH>
 __global__ void __launch_bounds__(NTH)
 trellis_forward_kernel(const TrellisView v, const double *__restrict__ local, const double *__restrict__ least, double bias_min,
-                       int *__restrict__ flag, double *__restrict__ V, double *__restrict__ logz)
+                       const double *__restrict__ ends, const int64_t *__restrict__ ends_scaled, int *__restrict__ flag, double *__restrict__ V,
+                       double *__restrict__ logz)
 {
     constexpr int W = NTH / 64, R = KPM * CH;
-    static_assert(NB % CH == 0 || CH % NB == 0, "a step's pieces go round the buffers");
-    __shared__ double cur[2][4 * R];
+    static_assert(NB % CH == 0 || CH % NB == 0, "a step's parts go round the buffers");
+    __shared__ __align__(16) double cur[2][4 * R];
     __shared__ double top[2][W];
     __shared__ double part[NTH];
     __shared__ int bad;
-    const int u = v.first + blockIdx.x;
-    if (flag[u]) return;
-    const int64_t r0 = v.off[u], T = v.off[u + 1] - r0;
+    const TrellisPiece p = trellis_piece(v, blockIdx.y, blockIdx.x);
+    if (p.k >= p.P || flag[p.u]) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int b = wave * 32 + (lane & 15) * 2, rows = lane >> 4;
-    const int K = v.K, Kp = v.Kp;
+    const int K = v.K, Kp = v.Kp, n = p.n;
     const bool lead = rows == 0 && b < Kp;
     const int slab_bytes = K * Kp * 8;
     const int voff = b < Kp ? (rows * R * Kp + b) * 8 : 0x7ff00000;
+    const int64_t first_row = p.r0 + (int64_t)p.k * p.L;
     for (int i = tid; i < 8 * R; i += NTH) (&cur[0][0])[i] = 0.0;
     if (tid == 0) bad = 0;
     __syncthreads();
 
     f64x2 cell[NB][KPM];
-    const int64_t pieces = (T - 1) * CH;
-    auto load = [&](int64_t piece, f64x2 (&dst)[KPM]) {
+    const int pieces = n * CH;
+    const double *__restrict__ slab0 = v.C + (first_row - v.c0) * ((int64_t)K * Kp);
+    auto load = [&](int piece, int i, f64x2 &dst) {             // (rows beyond K lie beyond the slab: they read as 0)
         piece = piece < pieces ? piece : pieces - 1;
-        const double *base = v.C + (r0 - v.c0 + piece / CH) * ((int64_t)K * Kp);
-        const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc(const_cast<double *>(base), 0, slab_bytes, 0x00020000);
-        const int row = (int)(piece % CH) * KPM;
-#pragma unroll
-        for (int i = 0; i < KPM; ++i)                          // (rows beyond K lie beyond the slab: they read as 0)
-            dst[i] = __builtin_bit_cast(f64x2, __builtin_amdgcn_raw_buffer_load_b128(res, voff + (row + i) * Kp * 8, 0, 0));
+        const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc(const_cast<double *>(slab0 + (piece / CH) * ((int64_t)K * Kp)), 0, slab_bytes, 0x00020000);
+        const int row = min(((piece % CH) * KPM + i) * Kp * 8, slab_bytes);
+        dst = __builtin_bit_cast(f64x2, __builtin_amdgcn_raw_buffer_load_b128(res, voff, row, 0));
     };
-    auto load_local = [&](int64_t t) -> f64x2 {
+    auto load_local = [&](int t) -> f64x2 {
         f64x2 x = {0.0, 0.0};
-        if (lead) x = *reinterpret_cast<const f64x2 *>(local + (r0 + (t < T ? t : T - 1)) * Kp + b);
+        if (lead) x = *reinterpret_cast<const f64x2 *>(local + (first_row + (t < n ? t : n)) * Kp + b);
         return x;
     };
     // new weights of the lead lanes: LDS, memory, their maximum; small ones are remembered
     bool small = false;
-    auto publish = [&](int64_t t, f64x2 x, int at) {
+    auto publish = [&](int t, f64x2 x, int at, bool store) {
         double m = 0.0;
         if (lead) {
-            cur[at][b] = x[0];
-            if (b + 1 < 4 * R) cur[at][b + 1] = x[1];
-            *reinterpret_cast<f64x2 *>(V + (r0 + t) * Kp + b) = x;
+            *reinterpret_cast<f64x2 *>(&cur[at][b]) = x;
+            if (store) *reinterpret_cast<f64x2 *>(V + (first_row + t) * Kp + b) = x;
             m = fmax(x[0], x[1]);
             small |= (x[0] > 0.0 && x[0] < SNK_WEIGHT_LEAST) || (x[1] > 0.0 && x[1] < SNK_WEIGHT_LEAST);
         }
-        m = wave_max(m);
-        if (lane == 0) top[at][wave] = m;
+        m = row16_max(m);
+        if (lane == 15) top[at][wave] = m;
     };
     if (pieces > 0) {
 #pragma unroll
-        for (int s = 0; s < NB; ++s) load(s, cell[s]);
+        for (int s = 0; s < NB; ++s)
+#pragma unroll
+            for (int i = 0; i < KPM; ++i) load(s, i, cell[s][i]);
     }
     f64x2 l1 = load_local(1), l2 = load_local(2);
-    publish(0, load_local(0), 0);
+    {
+        f64x2 x = {0.0, 0.0};
+        if (lead) x = p.k == 0 ? load_local(0) : *reinterpret_cast<const f64x2 *>(ends + p.at * Kp + b);
+        publish(0, x, 0, p.k == 0);
+    }
     __syncthreads();
     int64_t scaled = 0;                                         // sum of the exponents taken out
     constexpr int TRIP = NB / CH > 0 ? NB / CH : 1;             // steps a trip, so that buffer indexes are constants
-    for (int64_t t = 1; t < T; t += TRIP) {
+    for (int t = 1; t <= n; t += TRIP) {
 #pragma unroll
         for (int s = 0; s < TRIP; ++s) {
-            const int64_t now = t + s;
-            const bool valid = now < T;
-            const int from = (int)(now - 1) & 1;
-            double m = top[from][0];
-#pragma unroll
-            for (int i = 1; i < W; ++i) m = fmax(m, top[from][i]);
-            const int e = trellis_exponent(m);
+            const int now = t + s, from = (now - 1) & 1;
+            const bool valid = now <= n;
             f64x2 sum = {0.0, 0.0};
 #pragma unroll
             for (int ch = 0; ch < CH; ++ch) {
                 f64x2(&c)[KPM] = cell[(s * CH + ch) % NB];
-                const double *p = &cur[from][rows * R + ch * KPM];
+                const double *w = &cur[from][rows * R + ch * KPM];
 #pragma unroll
                 for (int i = 0; i < KPM; ++i) {
-                    sum[0] = __fma_rn(p[i], c[i][0], sum[0]);
-                    sum[1] = __fma_rn(p[i], c[i][1], sum[1]);
+                    sum[0] = __fma_rn(w[i], c[i][0], sum[0]);
+                    sum[1] = __fma_rn(w[i], c[i][1], sum[1]);
+                    load((now - 1) * CH + ch + NB, i, c[i]);
                 }
-                load((now - 1) * CH + ch + NB, c);
             }
+            sum[0] = rows4_sum(sum[0]);
+            sum[1] = rows4_sum(sum[1]);
+            double m = top[from][0];
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
-                double x = sum[k];
-                x += __shfl_xor(x, 16, 64);
-                x += __shfl_xor(x, 32, 64);
-                sum[k] = x;
-            }
+            for (int i = 1; i < W; ++i) m = fmax(m, top[from][i]);
+            const int e = trellis_exponent(m);
             const double f = trellis_pow2(-e);
             if (valid) {
                 scaled += e;
                 const f64x2 x = {l1[0] * (sum[0] * f), l1[1] * (sum[1] * f)};
-                publish(now, x, 1 - from);
+                publish(now, x, 1 - from, true);
             }
             l1 = l2;
             l2 = load_local(now + 2);
@@ -325,37 +599,39 @@ trellis_forward_kernel(const TrellisView v, const double *__restrict__ local, co
     }
     if (small) bad = 1;
     __syncthreads();
-    if (bad) { if (tid == 0) flag[u] = 1; return; }
-    if (!logz) return;
+    if (bad) { if (tid == 0) flag[p.u] = 1; return; }
+    if (!logz || p.k != p.P - 1) return;
     double s = 0.0;
-    for (int64_t t = tid; t < T; t += NTH) s += least[r0 + t];
+    for (int64_t t = tid; t < p.T; t += NTH) s += least[p.r0 + t];
     part[tid] = s;
     __syncthreads();
     if (tid == 0) {
         s = 0.0;
         for (int i = 0; i < NTH; ++i) s += part[i];
         double z = 0.0;
-        for (int a = 0; a < K; ++a) z += cur[(T - 1) & 1][a];
-        logz[u] = z > 0.0 ? log(z) + (double)scaled * 0.69314718055994530942 - (s + (double)(T - 1) * bias_min) * v.inv_tau : -__builtin_inf();
+        for (int a = 0; a < K; ++a) z += cur[n & 1][a];
+        if (p.P > 1) scaled += ends_scaled[p.u];
+        logz[p.u] = z > 0.0 ? log(z) + (double)scaled * 0.69314718055994530942 - (s + (double)(p.T - 1) * bias_min) * v.inv_tau : -__builtin_inf();
     }
 }
 
-// ---- backward: as forward; a wavefront owns CH x 16 predecessors, four lanes share each one's successors -----------------------------
+// 3. backward: a wavefront owns CH x 16 predecessors, four lanes share each one's successors
 template <int KC, int CH, int NB, int NTH>
 __global__ void __launch_bounds__(NTH)
-trellis_backward_kernel(const TrellisView v, const double *__restrict__ local, int *__restrict__ flag, double *__restrict__ Wt)
+trellis_backward_kernel(const TrellisView v, const double *__restrict__ local, const double *__restrict__ ends, int *__restrict__ flag,
+                        double *__restrict__ Wt)
 {
     constexpr int W = NTH / 64;
-    static_assert(NB % CH == 0, "a step's pieces go round the buffers");
-    __shared__ double cur[2][8 * KC];
+    static_assert(NB % CH == 0 || CH % NB == 0, "a step's parts go round the buffers");
+    __shared__ __align__(16) double cur[2][8 * KC];
     __shared__ double top[2][W];
     __shared__ int bad;
-    const int u = v.first + blockIdx.x;
-    if (flag[u]) return;
-    const int64_t r0 = v.off[u], T = v.off[u + 1] - r0;
+    const TrellisPiece p = trellis_piece(v, blockIdx.y, blockIdx.x);
+    if (p.k >= p.P || flag[p.u]) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int q = lane & 3, K = v.K, Kp = v.Kp;
+    const int q = lane & 3, K = v.K, Kp = v.Kp, n = p.n;
     const int slab_bytes = K * Kp * 8;
+    const int64_t first_row = p.r0 + (int64_t)p.k * p.L;
     int a[CH], voff[CH];
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
@@ -366,42 +642,47 @@ trellis_backward_kernel(const TrellisView v, const double *__restrict__ local, i
     if (tid == 0) bad = 0;
     __syncthreads();
     f64x2 cell[NB][KC];
-    const int64_t pieces = (T - 1) * CH;                        // from the last slab down
-    auto load = [&](int64_t piece, f64x2 (&dst)[KC], int off) {
+    const int pieces = n * CH;                                  // from the last slab down
+    const double *__restrict__ slab0 = v.C + (first_row - v.c0) * ((int64_t)K * Kp);
+    auto load = [&](int piece, int i, f64x2 &dst, int off) {    // (columns beyond Kp are the next row's or nothing: their weights are 0)
         piece = piece < pieces ? piece : pieces - 1;
-        const double *base = v.C + (r0 - v.c0 + (T - 2 - piece / CH)) * ((int64_t)K * Kp);
-        const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc(const_cast<double *>(base), 0, slab_bytes, 0x00020000);
-#pragma unroll
-        for (int i = 0; i < KC; ++i)                           // (columns beyond Kp are the next row's or nothing: their weights are 0)
-            dst[i] = __builtin_bit_cast(f64x2, __builtin_amdgcn_raw_buffer_load_b128(res, off + i * 64, 0, 0));
+        const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc(const_cast<double *>(slab0 + (n - 1 - piece / CH) * ((int64_t)K * Kp)), 0, slab_bytes, 0x00020000);
+        dst = __builtin_bit_cast(f64x2, __builtin_amdgcn_raw_buffer_load_b128(res, off + i * 64, 0, 0));
     };
-    auto load_local = [&](int64_t t, int ch) -> double {
-        return a[ch] < K && q == 0 ? local[(r0 + (t > 0 ? t : 0)) * Kp + a[ch]] : 0.0;
+    auto load_local = [&](int t, int ch) -> double {
+        return a[ch] < K && q == 0 ? local[(first_row + (t > 0 ? t : 0)) * Kp + a[ch]] : 0.0;
     };
     if (pieces > 0) {
 #pragma unroll
-        for (int s = 0; s < NB; ++s) load(s, cell[s], voff[s % CH]);
+        for (int s = 0; s < NB; ++s)
+#pragma unroll
+            for (int i = 0; i < KC; ++i) load(s, i, cell[s][i], voff[s % CH]);
     }
     double l1[CH], l2[CH];
     double m0 = 0.0;
+    bool small = false;
 #pragma unroll
     for (int ch = 0; ch < CH; ++ch) {
-        const double x = load_local(T - 1, ch);
-        if (a[ch] < K && q == 0) { cur[(T - 1) & 1][a[ch]] = x; Wt[(r0 + T - 1) * Kp + a[ch]] = 1.0; m0 = fmax(m0, x); }
-        l1[ch] = load_local(T - 2, ch);
-        l2[ch] = load_local(T - 3, ch);
+        if (a[ch] < K && q == 0) {
+            const double w = p.k == p.P - 1 ? 1.0 : ends[p.at * Kp + a[ch]], x = load_local(n, ch) * w;
+            cur[n & 1][a[ch]] = x;
+            if (p.k == p.P - 1) Wt[(first_row + n) * Kp + a[ch]] = w;
+            small |= x > 0.0 && x < SNK_WEIGHT_LEAST;
+            m0 = fmax(m0, x);
+        }
+        l1[ch] = load_local(n - 1, ch);
+        l2[ch] = load_local(n - 2, ch);
     }
     m0 = wave_max(m0);
-    if (lane == 0) top[(T - 1) & 1][wave] = m0;
+    if (lane == 0) top[n & 1][wave] = m0;
     __syncthreads();
-    bool small = false;
-    constexpr int TRIP = NB / CH;
-    for (int64_t k = 0; k + 1 < T; k += TRIP) {
+    constexpr int TRIP = NB / CH > 0 ? NB / CH : 1;
+    for (int k = 0; k < n; k += TRIP) {
 #pragma unroll
         for (int s = 0; s < TRIP; ++s) {
-            const int64_t t = T - 2 - (k + s);                  // the row of this step; < 0: beyond the first
+            const int t = n - 1 - (k + s);                      // the row of this step; < 0: beyond the piece
             const bool valid = t >= 0;
-            const int from = (int)(t + 1) & 1, to = 1 - from;
+            const int from = (t + 1) & 1, to = 1 - from;
             double m = top[from][0];
 #pragma unroll
             for (int i = 1; i < W; ++i) m = fmax(m, top[from][i]);
@@ -416,16 +697,14 @@ trellis_backward_kernel(const TrellisView v, const double *__restrict__ local, i
                     const f64x2 x = *reinterpret_cast<const f64x2 *>(&cur[from][8 * i + 2 * q]);
                     sum[0] = __fma_rn(x[0], c[i][0], sum[0]);
                     sum[1] = __fma_rn(x[1], c[i][1], sum[1]);
+                    load((k + s) * CH + ch + NB, i, c[i], voff[(ch + NB) % CH]);
                 }
-                load((k + s) * CH + ch + NB, c, voff[ch]);
                 double y = sum[0] + sum[1];
-                y += __shfl_xor(y, 1, 64);
-                y += __shfl_xor(y, 2, 64);
-                y *= f;
+                y = quad_sum(y) * f;
                 if (valid && a[ch] < K && q == 0) {
                     const double x = l1[ch] * y;
                     cur[to][a[ch]] = x;
-                    Wt[(r0 + t) * Kp + a[ch]] = y;
+                    Wt[(first_row + t) * Kp + a[ch]] = y;
                     small |= x > 0.0 && x < SNK_WEIGHT_LEAST;
                     m = fmax(m, x);
                 }
@@ -439,7 +718,7 @@ trellis_backward_kernel(const TrellisView v, const double *__restrict__ local, i
     }
     if (small) bad = 1;
     __syncthreads();
-    if (bad && tid == 0) flag[u] = 1;
+    if (bad && tid == 0) flag[p.u] = 1;
 }
 
 // ---- the flagged utterances in logarithms (SUM false: temperature 0, the largest term of every sum) ----------------------------------
@@ -549,7 +828,7 @@ trellis_backward_log_kernel(const TrellisView v, const int *__restrict__ flag, d
 // cells and are summed in registers; the others go to LDS.
 __global__ void __launch_bounds__(256)
 trellis_posterior_kernel(const TrellisView v, const int *__restrict__ flag, const double *__restrict__ V, const double *__restrict__ Wt,
-                         const double *__restrict__ local, const double *__restrict__ logz, const int *__restrict__ bucket_edges, int n_buckets,
+                         const double *__restrict__ ends, const double *__restrict__ local, const double *__restrict__ logz, const int *__restrict__ bucket_edges, int n_buckets,
                          double *__restrict__ posterior, double *__restrict__ row_uses)
 {
     __shared__ double in[256], out[256], red[8];
@@ -571,7 +850,12 @@ trellis_posterior_kernel(const TrellisView v, const int *__restrict__ flag, cons
         // sum_a v w of the row, and the power of two that the backward step into this row took out
         const double a = tid < K ? V[t * Kp + tid] : 0.0, w = tid < K ? Wt[t * Kp + tid] : 0.0;
         const double p = a * w, s = wave_sum(p);
-        const double x = !last && tid < K ? local[(t + 1) * Kp + tid] * Wt[(t + 1) * Kp + tid] : 0.0;
+        // (behind a piece's last row stand the weights that its recursion began with)
+        const int64_t L = trellis_piece_length(v.off[u + 1] - v.off[u] - 1);
+        const TrellisPiece piece = trellis_piece(v, u - v.first, (int)((t - v.off[u]) / L));
+        const bool edge = piece.k + 1 < piece.P && (t + 1 - piece.r0) % L == 0;
+        const double *__restrict__ next = edge ? ends + piece.at * Kp : Wt + (t + 1) * Kp;
+        const double x = !last && tid < K ? local[(t + 1) * Kp + tid] * next[tid] : 0.0;
         const double m = wave_max(x);
         if (lane == 0) { red[wave] = s; red[4 + wave] = m; }
         __syncthreads();
@@ -868,25 +1152,65 @@ void launch_trellis_costs(const TrellisView &v, const TrellisCosts &c, bool logs
 #undef SNK_COST
 }
 
-void launch_trellis_forward(const TrellisView &v, const double *local, const double *least, double bias_min, int *flag, double *V,
-                            double *logz, hipStream_t s)
+int trellis_most_pieces(const int64_t *off, int n_utts)
 {
-#define SNK_FWD(KPM_, CH_, NB_, NTH_) hipLaunchKernelGGL((trellis_forward_kernel<KPM_, CH_, NB_, NTH_>), dim3(v.n_utts), dim3(NTH_), 0, s, v, local, least, bias_min, flag, V, logz)
+    int64_t most = 1;
+    for (int i = 0; i < n_utts; ++i) {
+        const int64_t S = off[i + 1] - off[i] - 1, L = trellis_piece_length(S);
+        if (S > L && (S + L - 1) / L > most) most = (S + L - 1) / L;
+    }
+    return (int)most;
+}
+size_t trellis_piece_places(const TrellisView &v) { return (size_t)(v.rows / SNK_PIECE_LEAST + v.n_utts); }
+
+void launch_trellis_ends(const TrellisView &v, const double *local, bool both, int *flag, double *M, int *exps, double *ends_v, double *ends_w,
+                         int64_t *scaled, hipStream_t s)
+{
+    const int n = v.pieces;
+    if (n == 1) return;
+    const int row_blocks = (v.K + 15) / 16;
+    const dim3 grid((unsigned)((((int64_t)n * v.n_utts + 7) / 8) * 8 * row_blocks));
+#define SNK_PROD(CT_, KH_, CH_, NTH_) hipLaunchKernelGGL((trellis_product_kernel<CT_, KH_, CH_, NTH_>), grid, dim3(NTH_), 0, s, v, local, n, row_blocks, !both, flag, M, exps)
+    if (v.K <= 32) SNK_PROD(1, 8, 1, 128);
+    else if (v.K <= 64) SNK_PROD(1, 16, 1, 256);
+    else if (v.K <= 104) SNK_PROD(2, 26, 1, 256);
+    else if (v.K <= 128) SNK_PROD(2, 32, 1, 256);
+    else SNK_PROD(2, 26, 2, 448);
+#undef SNK_PROD
+#define SNK_ENDS(R_, H_, RB_, HB_, Q_)                                                                                                                    \
+    do {                                                                                                                                              \
+        hipLaunchKernelGGL((trellis_ends_kernel<R_, H_, 0>), dim3(v.n_utts), dim3(1024), 0, s, v, local, M, exps, flag, ends_v, scaled);              \
+        if (both) hipLaunchKernelGGL((trellis_ends_kernel<RB_, HB_, Q_>), dim3(v.n_utts), dim3(1024), 0, s, v, local, M, exps, flag, ends_w, scaled); \
+    } while (0)
+    if (v.K <= 32) SNK_ENDS(1, 1, 2, 1, 8);
+    else if (v.K <= 64) SNK_ENDS(2, 1, 4, 1, 8);
+    else if (v.K <= 104) SNK_ENDS(6, 1, 7, 1, 8);
+    else if (v.K <= 128) SNK_ENDS(8, 1, 8, 1, 8);
+    else SNK_ENDS(8, 3, 13, 2, 4);
+#undef SNK_ENDS
+}
+
+void launch_trellis_forward(const TrellisView &v, const double *local, const double *least, double bias_min, const double *ends,
+                            const int64_t *ends_scaled, int *flag, double *V, double *logz, hipStream_t s)
+{
+    const dim3 grid(v.pieces, v.n_utts);
+#define SNK_FWD(KPM_, CH_, NB_, NTH_) hipLaunchKernelGGL((trellis_forward_kernel<KPM_, CH_, NB_, NTH_>), grid, dim3(NTH_), 0, s, v, local, least, bias_min, ends, ends_scaled, flag, V, logz)
     if (v.K <= 32) SNK_FWD(8, 1, 4, 64);
-    else if (v.K <= 64) SNK_FWD(16, 1, 4, 128);
-    else if (v.K <= 104) SNK_FWD(26, 1, 2, 256);
-    else if (v.K <= 128) SNK_FWD(16, 2, 4, 256);
-    else SNK_FWD(26, 2, 2, 448);
+    else if (v.K <= 64) SNK_FWD(16, 1, 1, 128);
+    else if (v.K <= 104) SNK_FWD(26, 1, 1, 256);
+    else if (v.K <= 128) SNK_FWD(32, 1, 1, 256);
+    else SNK_FWD(26, 2, 1, 448);
 #undef SNK_FWD
 }
 
-void launch_trellis_backward(const TrellisView &v, const double *local, int *flag, double *Wt, hipStream_t s)
+void launch_trellis_backward(const TrellisView &v, const double *local, const double *ends, int *flag, double *Wt, hipStream_t s)
 {
-#define SNK_BWD(KC_, CH_, NB_, NTH_) hipLaunchKernelGGL((trellis_backward_kernel<KC_, CH_, NB_, NTH_>), dim3(v.n_utts), dim3(NTH_), 0, s, v, local, flag, Wt)
+    const dim3 grid(v.pieces, v.n_utts);
+#define SNK_BWD(KC_, CH_, NB_, NTH_) hipLaunchKernelGGL((trellis_backward_kernel<KC_, CH_, NB_, NTH_>), grid, dim3(NTH_), 0, s, v, local, ends, flag, Wt)
     if (v.K <= 32) SNK_BWD(4, 1, 4, 128);
-    else if (v.K <= 64) SNK_BWD(8, 1, 4, 256);
-    else if (v.K <= 112) SNK_BWD(14, 1, 3, 448);
-    else SNK_BWD(26, 2, 2, 448);
+    else if (v.K <= 64) SNK_BWD(8, 1, 2, 256);
+    else if (v.K <= 112) SNK_BWD(14, 1, 2, 448);
+    else SNK_BWD(26, 2, 1, 448);
 #undef SNK_BWD
 }
 
@@ -901,10 +1225,10 @@ void launch_trellis_backward_log(const TrellisView &v, const int *flag, double *
     hipLaunchKernelGGL(trellis_backward_log_kernel, dim3(v.n_utts), dim3(1024), 0, s, v, flag, beta);
 }
 
-void launch_trellis_posterior(const TrellisView &v, const int *flag, const double *V, const double *Wt, const double *local, const double *logz,
+void launch_trellis_posterior(const TrellisView &v, const int *flag, const double *V, const double *Wt, const double *ends, const double *local, const double *logz,
                               const int *edges, int n_buckets, double *posterior, double *row_uses, hipStream_t s)
 {
-    hipLaunchKernelGGL(trellis_posterior_kernel, dim3((unsigned)v.rows), dim3(256), 0, s, v, flag, V, Wt, local, logz, edges, n_buckets, posterior, row_uses);
+    hipLaunchKernelGGL(trellis_posterior_kernel, dim3((unsigned)v.rows), dim3(256), 0, s, v, flag, V, Wt, ends, local, logz, edges, n_buckets, posterior, row_uses);
 }
 
 void launch_trellis_uses(const double *row_uses, const int32_t *join_class, int64_t rows, int n_classes, int n_buckets, double *uses, hipStream_t s)

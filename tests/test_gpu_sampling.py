@@ -453,6 +453,20 @@ def test_gradients_against_differences(engine):
             assert abs((values[0] - values[1]) / (2.0 * h) + uses[c, b] / tau) <= tol + h * h / 6.0 * 22.0 ** 3 / tau ** 3
 
 
+@pytest.mark.parametrize('lengths,K', [([100], 5), ([64, 1, 9, 2, 150], 30), ([200, 33], 50), ([24, 25, 26, 65, 66], 20), ([120], 100), ([90, 91, 2], 104),
+                                       ([60], 120), ([70, 8, 40], 200), ([300], 64)])
+def test_recursions_in_pieces(engine, lengths, K):
+    """Utterances of 25 rows and more run their recursions in pieces, side by side."""
+    v = Voice(engine, Dj=9, n=300 + 5 * K)
+    v.set_bias(2, 8, forbid=True)
+    cand, dist, offs = v.candidates(lengths, K)
+    rng = np.random.RandomState(1)
+    cls, u = rng.randint(0, 2, cand.shape[0]).astype(np.int32), rng.rand(1, cand.shape[0])
+    for tau in (0.3, 2.0):
+        check_posterior(v, cand, dist, offs, cls, tau)
+        check_paths(v, cand, dist, offs, u, cls, temperature=tau, top_p=0.9)
+
+
 def test_trellis_results_do_not_depend_on_the_batch(engine):
     v = Voice(engine)
     v.set_bias(2, 8)
