@@ -276,10 +276,11 @@ int snk_destroy(snk_handle h)
         for (int i = 0; i < 2; ++i) if (t.side_done[i]) (void)hipEventDestroy(t.side_done[i]);
     }
     for (auto &b : h->bslot) { b.Qall.release(); b.cand.release(); b.dist.release(); b.path.release(); b.plen.release(); b.cost.release(); b.status.release(); b.stage.release(); b.qstage.release(); if (b.done) (void)hipEventDestroy(b.done); if (b.knn_end) (void)hipEventDestroy(b.knn_end); }
-    { DevBuf *db[] = {&h->pb_bias, &h->pb_edges, &h->sr_scores, &h->sr_u, &h->sr_rules, &h->sr_index, &h->sr_logp, &h->tr_off, &h->tr_cand, &h->tr_tdist,
+    { DevBuf *db[] = {&h->pb_bias, &h->pb_edges, &h->sr_scores, &h->sr_u, &h->sr_rules, &h->sr_index, &h->sr_logp, &h->sr_work, &h->tr_off, &h->tr_cand, &h->tr_tdist,
                       &h->tr_class, &h->tr_u, &h->tr_C, &h->tr_V, &h->tr_W, &h->tr_local, &h->tr_least, &h->tr_flag, &h->tr_draw,
                       &h->tr_row_uses, &h->tr_out, &h->tr_M, &h->tr_exps, &h->tr_ends_v, &h->tr_ends_w, &h->tr_scaled};
       for (auto *b : db) b->release(); }
+    if (h->sr_done) (void)hipEventDestroy(h->sr_done);
     if (h->tr_in) (void)hipEventDestroy(h->tr_in);
     if (h->tr_done) (void)hipEventDestroy(h->tr_done);
     if (h->stream) (void)hipStreamDestroy(h->stream);

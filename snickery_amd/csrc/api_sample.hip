@@ -1,7 +1,8 @@
 // C ABI of libsnkhip.so, part 6: draws and probabilities over the candidates of a preselection (include/snk.h snk_sample_rows,
 // snk_set_position_bias, snk_sample_paths, snk_path_posterior).
 //
-// Streams.  snk_sample_rows_dev touches nothing of the engine: its kernels go straight to the caller's stream.  The trellis calls
+// Streams.  snk_sample_rows_dev puts its kernels straight on the caller's stream; rows of more than 1024 scores use the engine's
+// row workspace, which a later call on another stream waits for.  The trellis calls
 // use the engine's workspaces, so their kernels run on the engine's main stream, in the order of the calls; a _dev call makes that
 // stream wait for what the caller's stream holds and the caller's stream for the results, without a host wait in between.
 #include "snk_engine.h"
@@ -47,6 +48,29 @@ static int check_rows(const char *who, int dtype, int64_t R, int64_t V, int64_t 
     return 0;
 }
 
+// the row workspace for a call on stream `s`, behind the stream that used it last; nullptr: none needed, or `s` is being captured (a
+// graph would share it with every later call)
+static int rows_workspace(snk_engine *h, const char *who, int64_t R, int64_t V, hipStream_t s, char **work)
+{
+    *work = nullptr;
+    const size_t bytes = sample_rows_work(sample_rows_together(R, V), V);
+    if (!bytes) return 0;
+    hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
+    if (hipStreamIsCapturing(s, &st) != hipSuccess) { (void)hipGetLastError(); return fail("%s: another stream's capture forbids work on this one", who); }
+    if (st != hipStreamCaptureStatusNone) return 0;
+    CHK(h->sr_work.ensure(bytes));
+    if (!h->sr_done) HIPCHK(hipEventCreateWithFlags(&h->sr_done, hipEventDisableTiming));
+    if (h->sr_used) HIPCHK(hipStreamWaitEvent(s, h->sr_done, 0));
+    *work = h->sr_work.as<char>();
+    return 0;
+}
+static int rows_workspace_used(snk_engine *h, hipStream_t s)
+{
+    HIPCHK(hipEventRecord(h->sr_done, s));
+    h->sr_used = true;
+    return 0;
+}
+
 int snk_sample_rows(snk_handle h, const void *scores, int dtype, int64_t R, int64_t V, int64_t row_stride, const double *u, int n_draws,
                     double temperature, int64_t top_k, double top_p, double min_p, const double *row_rules, int64_t *index_out,
                     double *logp_out)
@@ -77,13 +101,16 @@ int snk_sample_rows(snk_handle h, const void *scores, int dtype, int64_t R, int6
         CHK(h->sr_rules.ensure((size_t)R * 4 * sizeof(double)));
         CHK(h2d(h, h->sr_rules.p, row_rules, (size_t)R * 4 * sizeof(double), h->stream));
     }
+    char *work;
+    CHK(rows_workspace(h, who, R, V, h->stream, &work));
     {
         StageTimer t(h, h->stream, TM_SAMPLE_ROWS);
         const SampleRuleHost rule = {temperature, top_k, top_p, min_p};
-        launch_sample_rows(h->sr_scores.p, dtype, V, R, V, h->sr_u.as<double>(), n_draws, rule, row_rules ? h->sr_rules.as<double>() : nullptr,
+        launch_sample_rows(h->sr_scores.p, dtype, V, R, V, h->sr_u.as<double>(), n_draws, rule, row_rules ? h->sr_rules.as<double>() : nullptr, work,
                            h->sr_index.as<int64_t>(), logp_out ? h->sr_logp.as<double>() : nullptr, h->stream);
     }
     HIPCHK(hipGetLastError());
+    if (work) CHK(rows_workspace_used(h, h->stream));
     D2HPart parts[2] = {{index_out, h->sr_index.p, n * sizeof(int64_t)}, {logp_out, h->sr_logp.p, logp_out ? n * sizeof(double) : 0}};
     CHK(staged_d2h(h, h->stream, parts, 2));
     collect_timers(h);
@@ -103,8 +130,11 @@ int snk_sample_rows_dev(snk_handle h, const void *scores_dev, int dtype, int64_t
     DeviceGuard device;
     CHK(device.enter(h->device));
     const SampleRuleHost rule = {temperature, top_k, top_p, min_p};
-    launch_sample_rows(scores_dev, dtype, row_stride, R, V, u_dev, n_draws, rule, row_rules_dev, index_dev_out, logp_dev_out, (hipStream_t)stream);
+    char *work;
+    CHK(rows_workspace(h, who, R, V, (hipStream_t)stream, &work));
+    launch_sample_rows(scores_dev, dtype, row_stride, R, V, u_dev, n_draws, rule, row_rules_dev, work, index_dev_out, logp_dev_out, (hipStream_t)stream);
     HIPCHK(hipGetLastError());
+    if (work) CHK(rows_workspace_used(h, (hipStream_t)stream));
     return 0;
 }
 

@@ -1,5 +1,6 @@
 // Draws from rows of scores with temperature, top-k, top-p and min-p (snk_sample_rows; the mathematics: sample_device.h).
 #include "sample_device.h"
+#include <algorithm>
 #include <hip/hip_bf16.h>
 #include <hip/hip_fp16.h>
 
@@ -80,7 +81,7 @@ sample_rows_wave_kernel(const T *__restrict__ scores, int64_t stride, int64_t R,
     }
 }
 
-// ---- longer rows: a workgroup each, the row read once per pass ---------------------------------------------------------------------
+// ---- longer rows without a workspace: a workgroup each, the row read once per pass ---------------------------------------------------------------------
 #define SNK_SAMPLE_TILES 4096
 #define SNK_SAMPLE_VEC 4
 
@@ -124,9 +125,10 @@ __device__ __forceinline__ void block_scan2(u64 &a, u64 &b, u64 &ta, u64 &tb, Bl
 template <typename T, int NT>
 __global__ void __launch_bounds__(NT)
 sample_rows_block_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, const double *__restrict__ u, int n_draws,
-                         SampleRule call, const double *__restrict__ rules, double unit, int64_t *__restrict__ index,
+                         SampleRule call, const double *__restrict__ rules, double unit, const int *__restrict__ only, int64_t *__restrict__ index,
                          double *__restrict__ logp)
 {
+    if (only && !only[blockIdx.x]) return;                      // (rows that the kernels below left over)
     typedef typename ScoreKey<T>::type Key;
     constexpr int BITS = ScoreKey<T>::bits;
     constexpr int64_t TILE = (int64_t)NT * SNK_SAMPLE_VEC;
@@ -221,8 +223,8 @@ sample_rows_block_kernel(const T *__restrict__ scores, int64_t stride, int64_t V
         if (!all && k < cut) return;
         const double e = sample_exponent(x, m, rule.inv_tau);
         if (e < SNK_SAMPLE_FLOOR) return;
-        const double v = exp(e);
-        if (use_min && v < rule.min_p) return;
+        const double v = sample_exp(e);
+        if (use_min && (double)sample_fix(v, unit) < rule.min_p * unit) return;
         if (!all && k == cut) { tie = 1; return; }
         w = sample_fix(v, unit);
     };
@@ -314,9 +316,448 @@ sample_rows_block_kernel(const T *__restrict__ scores, int64_t stride, int64_t V
     }
 }
 
+// ---- longer rows, every pass over all of the chip ----------------------------------------------------------------------------------
+// A row is cut into chunks of SNK_CHUNK scores, a workgroup each:
+//   extremes   the chunks' largest and smallest score
+//   histogram  count and mass by bins of the exponent (m - x) / tau, as many bins as the row's own range needs
+//   boundary   the bin in which the order reaches its goal (a count, or a share of the mass); the bin's scores go to a list
+//   select     the goal's place in the list, by radix on the scores' keys: the cut, and how many equal to it are kept
+//   masses     what every chunk keeps
+//   draw       the chunk, then the score that a random number falls on
+// top_k and top_p take a boundary / select pair each.  Counts and masses are integers: neither the order of the atomics nor the cutting
+// shows in a result.  A boundary bin of equal scores needs no list; one of more than SNK_LIST different ones (or a workspace that a
+// captured graph would have to share) leaves the row to the kernel above.
+#define SNK_CHUNK 8192
+#define SNK_LIST 16384
+#define SNK_BINS_MOST 4096
+
+struct RowState {
+    double m, bin_scale;        // largest score, bins per unit of exponent
+    double cut;                 // kept: above the cut, and the first n_tie equal to it
+    u64 n_tie, total;           // total: mass of what the goals so far keep
+    u64 above, key_min, key_max;
+    unsigned int listed, want_bin;
+    int all, pad;
+    u64 want;
+};
+
+struct RowsWork {
+    RowState *state;
+    double *chunk_max, *chunk_min;          // [rows][chunks]
+    u64 *hist_mass; unsigned int *hist_count;   // [rows][bins]
+    double *list_x;                         // [rows][list]
+    u64 *chunk_mass; unsigned int *chunk_ties;
+    int *left;                              // rows for the kernel above
+    int bins, chunks;
+    unsigned int list;                      // entries of a row's list: SNK_LIST, or the row's length
+};
+
+template <typename T> __device__ __forceinline__ double score_bits(const T *v, int j) { return score_load(v + j); }
+
+// every score of [lo, hi) once: 16-byte loads from the first aligned one on
+template <typename T, int NT, typename F>
+__device__ __forceinline__ void chunk_scores(const T *__restrict__ p, int64_t lo, int64_t hi, F f)
+{
+    constexpr int VEC = 16 / (int)sizeof(T);
+    const int tid = threadIdx.x;
+    const int skip = (int)(((16 - ((uintptr_t)(p + lo) & 15)) & 15) / sizeof(T));
+    const int64_t a = lo + skip < hi ? lo + skip : hi, n = (hi - a) / VEC, b = a + n * VEC;
+    if (lo + tid < a) f(score_load(p + lo + tid), lo + tid);
+    for (int64_t i = tid; i < n; i += NT) {
+        union { uint4 q; T v[VEC]; } u;
+        u.q = *reinterpret_cast<const uint4 *>(p + a + i * VEC);
+#pragma unroll
+        for (int j = 0; j < VEC; ++j) f(score_bits(u.v, j), a + i * VEC + j);
+    }
+    if (b + tid < hi) f(score_load(p + b + tid), b + tid);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(256)
+rows_extremes_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, const RowsWork w)
+{
+    __shared__ double hi[4], lo[4];
+    const int64_t r = blockIdx.y, c = blockIdx.x;
+    const int tid = threadIdx.x;
+    const double inf = __builtin_inf();
+    if (c == 0) {
+        for (int i = tid; i < w.bins; i += 256) { w.hist_mass[r * w.bins + i] = 0; w.hist_count[r * w.bins + i] = 0; }
+        if (tid == 0) {
+            RowState s;
+            s.m = -inf; s.bin_scale = 0.0; s.cut = -inf; s.n_tie = 0; s.total = 0; s.above = 0; s.key_min = ~0ull; s.key_max = 0;
+            s.listed = 0; s.want_bin = 0; s.all = 1; s.pad = 0; s.want = 0;
+            w.state[r] = s;
+            w.left[r] = 0;
+        }
+    }
+    double m = -inf, n = inf;
+    chunk_scores<T, 256>(scores + r * stride, c * SNK_CHUNK, min((c + 1) * SNK_CHUNK, V), [&](double x, int64_t) {
+        m = fmax(m, x);
+        n = x > -inf ? fmin(n, x) : n;
+    });
+    m = wave_max(m);
+    n = -wave_max(-n);
+    if ((tid & 63) == 0) { hi[tid >> 6] = m; lo[tid >> 6] = n; }
+    __syncthreads();
+    if (tid == 0) {
+        w.chunk_max[r * w.chunks + c] = fmax(fmax(hi[0], hi[1]), fmax(hi[2], hi[3]));
+        w.chunk_min[r * w.chunks + c] = fmin(fmin(lo[0], lo[1]), fmin(lo[2], lo[3]));
+    }
+}
+
+__device__ __forceinline__ int score_bin(double e, double scale, int bins)
+{
+    const double b = -e * scale;
+    return b < (double)(bins - 1) ? (int)b : bins - 1;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(512)
+rows_histogram_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, SampleRule call, const double *__restrict__ rules, double unit, const RowsWork w)
+{
+    extern __shared__ __align__(16) unsigned char smem[];
+    __shared__ double hi[8], lo[8];
+    u64 *mass = reinterpret_cast<u64 *>(smem);
+    unsigned int *count = reinterpret_cast<unsigned int *>(mass + w.bins);
+    const int64_t r = blockIdx.y, c = blockIdx.x;
+    const int tid = threadIdx.x;
+    const double inf = __builtin_inf();
+    const SampleRule rule = sample_rule(call, rules, r);
+    double m = -inf, n = inf;
+    for (int i = tid; i < w.chunks; i += 512) { m = fmax(m, w.chunk_max[r * w.chunks + i]); n = fmin(n, w.chunk_min[r * w.chunks + i]); }
+    m = wave_max(m);
+    n = -wave_max(-n);
+    if ((tid & 63) == 0) { hi[tid >> 6] = m; lo[tid >> 6] = n; }
+    for (int i = tid; i < w.bins; i += 512) { mass[i] = 0; count[i] = 0; }
+    __syncthreads();
+    for (int i = 0; i < 8; ++i) { m = fmax(m, hi[i]); n = fmin(n, lo[i]); }
+    if (m == -inf) return;                                      // an empty row
+    const double range = fmin(-sample_exponent(n, m, rule.inv_tau), -SNK_SAMPLE_FLOOR);
+    const double scale = range > 0.0 ? fmin((double)w.bins / range, 1e300) : 0.0;
+    if (c == 0 && tid == 0) { w.state[r].m = m; w.state[r].bin_scale = scale; }
+    chunk_scores<T, 512>(scores + r * stride, c * SNK_CHUNK, min((c + 1) * SNK_CHUNK, V), [&](double x, int64_t) {
+        if (x == -inf) return;
+        const double e = sample_exponent(x, m, rule.inv_tau);
+        const u64 q = sample_weight(e, unit);
+        if (!q) return;
+        const int b = score_bin(e, scale, w.bins);
+        atomicAdd(&mass[b], q);
+        atomicAdd(&count[b], 1u);
+    });
+    __syncthreads();
+    for (int i = tid; i < w.bins; i += 512)
+        if (count[i]) { atomicAdd(&w.hist_mass[r * w.bins + i], mass[i]); atomicAdd(&w.hist_count[r * w.bins + i], count[i]); }
+}
+
+// by_mass 0: the top_k-th score; 1: where top_p of the mass kept so far is reached
+template <typename T>
+__global__ void __launch_bounds__(256)
+rows_boundary_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, SampleRule call, const double *__restrict__ rules, double unit, int by_mass,
+                     const RowsWork w)
+{
+    __shared__ u64 sums[256], counts[256];
+    __shared__ u64 above_s, total_s;
+    __shared__ int bin_s;
+    const int64_t r = blockIdx.y, c = blockIdx.x;
+    const int tid = threadIdx.x;
+    const SampleRule rule = sample_rule(call, rules, r);
+    RowState *st = w.state + r;
+    const double m = st->m, scale = st->bin_scale, ninf = -__builtin_inf();
+    if (m == ninf || w.left[r]) return;
+    if (by_mass ? !(rule.top_p < 1.0) : !(rule.top_k > 0 && rule.top_k < V)) return;
+    const u64 *__restrict__ mass = w.hist_mass + r * w.bins;
+    const unsigned int *__restrict__ count = w.hist_count + r * w.bins;
+    const int per = w.bins >> 8;
+    u64 sm = 0, sc = 0;
+    for (int i = 0; i < per; ++i) { sm += mass[tid * per + i]; sc += count[tid * per + i]; }
+    sums[tid] = sm; counts[tid] = sc;
+    __syncthreads();
+    if (tid == 0) {
+        u64 tm = 0;
+        for (int i = 0; i < 256; ++i) tm += sums[i];
+        const u64 total = st->all ? tm : st->total;
+        const u64 want = by_mass ? sample_reach(rule.top_p, total) : (u64)rule.top_k;
+        const u64 *v = by_mass ? sums : counts;
+        u64 a = 0;
+        int bin = -1;
+        for (int i = 0; i < 256 && bin < 0; ++i) {
+            if (a + v[i] < want) { a += v[i]; continue; }
+            for (int j = i * per;; ++j) {
+                const u64 n = by_mass ? mass[j] : (u64)count[j];
+                if (a + n >= want) { bin = j; break; }
+                a += n;
+            }
+        }
+        bin_s = bin; above_s = a; total_s = tm;
+        if (c == 0) { st->want = want; st->above = a; st->want_bin = (unsigned int)bin; if (bin < 0) st->total = tm; }
+    }
+    __syncthreads();
+    const int bin = bin_s;
+    if (bin < 0) return;                                        // fewer scores than the goal: all are kept
+    chunk_scores<T, 256>(scores + r * stride, c * SNK_CHUNK, min((c + 1) * SNK_CHUNK, V), [&](double x, int64_t i) {
+        if (x == ninf) return;
+        const double e = sample_exponent(x, m, rule.inv_tau);
+        if (e < SNK_SAMPLE_FLOOR || score_bin(e, scale, w.bins) != bin || !sample_weight(e, unit)) return;
+        // (a bin of thousands of equal scores: one count a wavefront, no further extremes)
+        const u64 key = score_key<double>(x);
+        if (key < *(volatile u64 *)&st->key_min) atomicMin(&st->key_min, key);
+        if (key > *(volatile u64 *)&st->key_max) atomicMax(&st->key_max, key);
+        const u64 here = __ballot(1);
+        const int lead = __ffsll((long long)here) - 1, lane = tid & 63;
+        unsigned int at = 0;
+        if (lane == lead) at = atomicAdd(&st->listed, (unsigned int)__popcll(here));
+        at = __shfl(at, lead, 64) + (unsigned int)__popcll(here & ((1ull << lane) - 1));
+        if (at < w.list) w.list_x[r * w.list + at] = x;
+    });
+}
+
+__global__ void __launch_bounds__(1024)
+rows_select_kernel(int64_t V, SampleRule call, const double *__restrict__ rules, double unit, int by_mass, const RowsWork w)
+{
+    __shared__ u64 hist_mass[256], hist_count[256];
+    __shared__ u64 sh_above;
+    __shared__ unsigned int sh_digit;
+    __shared__ u64 red[16];
+    const int64_t r = blockIdx.x;
+    const int tid = threadIdx.x;
+    const SampleRule rule = sample_rule(call, rules, r);
+    RowState *st = w.state + r;
+    const double m = st->m;
+    if (m == -__builtin_inf() || w.left[r]) return;
+    if (by_mass ? !(rule.top_p < 1.0) : !(rule.top_k > 0 && rule.top_k < V)) return;
+    if ((int)st->want_bin < 0) return;
+    const unsigned int n = st->listed;
+    const u64 want = st->want;
+    u64 above = st->above, key = st->key_min;
+    u64 ties = n, each = 0;                                     // of the cut's own scores
+    if (st->key_min != st->key_max) {
+        if (n > w.list) { if (tid == 0) w.left[r] = 1; return; }
+        u64 prefix = 0;
+        // (keys that differ share their leading bits: start at the first digit in which they do)
+        int top = 63 - __clzll((long long)(st->key_min ^ st->key_max));
+        top = (top >> 3) << 3;
+        prefix = top + 8 < 64 ? (key >> (top + 8)) << (top + 8) : 0;
+        for (int shift = top; shift >= 0; shift -= 8) {
+            if (tid < 256) { hist_mass[tid] = 0; hist_count[tid] = 0; }
+            __syncthreads();
+            for (unsigned int i = tid; i < n; i += 1024) {
+                const double x = w.list_x[r * w.list + i];
+                const u64 k = score_key<double>(x);
+                if (shift + 8 < 64 && (k >> (shift + 8)) != (prefix >> (shift + 8))) continue;
+                const int d = (int)((k >> shift) & 255);
+                atomicAdd(&hist_mass[d], sample_weight(sample_exponent(x, m, rule.inv_tau), unit));
+                atomicAdd(&hist_count[d], 1ull);
+            }
+            __syncthreads();
+            if (tid < 64) {
+                u64 v[4], sum = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) { const int d = 255 - (4 * tid + j); v[j] = by_mass ? hist_mass[d] : hist_count[d]; sum += v[j]; }
+                const u64 upto = wave_scan_add(sum), hit = __ballot(above + upto >= want);
+                if (hit && tid == __ffsll((long long)hit) - 1) {
+                    u64 a = above + upto - sum;
+                    for (int j = 0; j < 4; ++j) {
+                        if (a + v[j] >= want) { sh_digit = 255 - (4 * tid + j); sh_above = a; break; }
+                        a += v[j];
+                    }
+                }
+            }
+            __syncthreads();
+            above = sh_above;
+            prefix |= (u64)sh_digit << shift;
+            ties = hist_count[sh_digit];
+            __syncthreads();
+        }
+        key = prefix;
+    }
+    // the cut's value back from its key
+    const double cut = __longlong_as_double((long long)((key >> 63) ? key & 0x7fffffffffffffffull : ~key));
+    each = sample_weight(sample_exponent(cut, m, rule.inv_tau), unit);
+    const u64 n_tie = by_mass ? (want - above + each - 1) / each : want - above;
+    // the mass above the cut: whole bins, and the list's scores above it
+    u64 mass = 0;
+    const int bin = (int)st->want_bin;
+    for (int i = tid; i < bin; i += 1024) mass += w.hist_mass[r * w.bins + i];
+    if (st->key_min != st->key_max)
+        for (unsigned int i = tid; i < n; i += 1024) {
+            const double x = w.list_x[r * w.list + i];
+            if (x > cut) mass += sample_weight(sample_exponent(x, m, rule.inv_tau), unit);
+        }
+    mass = wave_add(mass);
+    if ((tid & 63) == 0) red[tid >> 6] = mass;
+    __syncthreads();
+    if (tid == 0) {
+        u64 t = 0;
+        for (int i = 0; i < 16; ++i) t += red[i];
+        st->cut = cut; st->n_tie = n_tie < ties ? n_tie : ties; st->all = 0;
+        st->total = t + each * st->n_tie;
+        st->listed = 0; st->key_min = ~0ull; st->key_max = 0;
+    }
+}
+
+// weight of a score that is kept for certain, or whether it is one of the cut's
+__device__ __forceinline__ void row_element(double x, const RowState &st, const SampleRule &rule, double unit, u64 &q, unsigned int &tie)
+{
+    q = 0; tie = 0;
+    if (x == -__builtin_inf() || (!st.all && x < st.cut)) return;
+    const u64 weight = sample_weight(sample_exponent(x, st.m, rule.inv_tau), unit);
+    if ((double)weight < rule.min_p * unit) return;
+    if (!st.all && x == st.cut) tie = weight ? 1 : 0;
+    else q = weight;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(512)
+rows_masses_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, SampleRule call, const double *__restrict__ rules, double unit, const RowsWork w)
+{
+    __shared__ u64 sm[8], sc[8];
+    const int64_t r = blockIdx.y, c = blockIdx.x;
+    const int tid = threadIdx.x;
+    const RowState st = w.state[r];
+    if (st.m == -__builtin_inf() || w.left[r]) return;
+    const SampleRule rule = sample_rule(call, rules, r);
+    u64 mass = 0, ties = 0;
+    chunk_scores<T, 512>(scores + r * stride, c * SNK_CHUNK, min((c + 1) * SNK_CHUNK, V), [&](double x, int64_t) {
+        u64 q; unsigned int t;
+        row_element(x, st, rule, unit, q, t);
+        mass += q; ties += t;
+    });
+    mass = wave_add(mass);
+    ties = wave_add(ties);
+    if ((tid & 63) == 0) { sm[tid >> 6] = mass; sc[tid >> 6] = ties; }
+    __syncthreads();
+    if (tid == 0) {
+        u64 a = 0, b = 0;
+        for (int i = 0; i < 8; ++i) { a += sm[i]; b += sc[i]; }
+        w.chunk_mass[r * w.chunks + c] = a;
+        w.chunk_ties[r * w.chunks + c] = (unsigned int)b;
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(1024)
+rows_draw_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, const double *__restrict__ u, int n_draws, SampleRule call,
+                 const double *__restrict__ rules, double unit, const RowsWork w, int64_t *__restrict__ index, double *__restrict__ logp)
+{
+    constexpr int EACH = SNK_CHUNK / 1024;
+    __shared__ BlockScratch<1024> scratch;
+    __shared__ u64 sh_mass, sh_ties;
+    __shared__ int sh_chunk;
+    const int64_t r = blockIdx.x, at = r * n_draws + blockIdx.y;
+    const int tid = threadIdx.x;
+    const RowState st = w.state[r];
+    if (w.left[r]) return;
+    if (st.m == -__builtin_inf()) {
+        if (tid == 0) { index[at] = -1; if (logp) logp[at] = st.m; }
+        return;
+    }
+    const SampleRule rule = sample_rule(call, rules, r);
+    const u64 each = st.all ? 0 : sample_weight(sample_exponent(st.cut, st.m, rule.inv_tau), unit);
+    const u64 n_tie = st.all || (double)each < rule.min_p * unit ? 0 : st.n_tie;
+    // chunks: a thread takes `per` neighbours
+    const int per = (w.chunks + 1023) / 1024;
+    u64 mass = 0, ties = 0, total_m, total_t;
+    for (int i = 0; i < per; ++i) {
+        const int c = tid * per + i;
+        if (c < w.chunks) { mass += w.chunk_mass[r * w.chunks + c]; ties += w.chunk_ties[r * w.chunks + c]; }
+    }
+    u64 cm = mass, ct = ties;
+    block_scan2<1024>(cm, ct, total_m, total_t, scratch);
+    const u64 total = total_m + each * (total_t < n_tie ? total_t : n_tie);
+    const u64 t = sample_exceed(u[at], total);
+    u64 am = cm - mass, an = ct - ties;
+    for (int i = 0; i < per; ++i) {
+        const int c = tid * per + i;
+        if (c >= w.chunks) break;
+        const u64 lo = am + each * (an < n_tie ? an : n_tie);
+        const u64 m0 = am, t0 = an;
+        am += w.chunk_mass[r * w.chunks + c]; an += w.chunk_ties[r * w.chunks + c];
+        const u64 hi = am + each * (an < n_tie ? an : n_tie);
+        if (lo <= t && t < hi) { sh_chunk = c; sh_mass = m0; sh_ties = t0; }
+    }
+    __syncthreads();
+    const T *__restrict__ p = scores + r * stride;
+    const int64_t base = (int64_t)sh_chunk * SNK_CHUNK + tid * EACH;
+    const u64 mass0 = sh_mass, ties0 = sh_ties;
+    double x[EACH];
+    u64 q[EACH]; unsigned int k[EACH];
+    mass = 0; ties = 0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        x[i] = base + i < V ? score_load(p + base + i) : -__builtin_inf();
+        row_element(x[i], st, rule, unit, q[i], k[i]);
+        mass += q[i]; ties += k[i];
+    }
+    cm = mass; ct = ties;
+    block_scan2<1024>(cm, ct, total_m, total_t, scratch);
+    am = mass0 + cm - mass; an = ties0 + ct - ties;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+        const u64 lo = am + each * (an < n_tie ? an : n_tie);
+        am += q[i]; an += k[i];
+        const u64 hi = am + each * (an < n_tie ? an : n_tie);
+        if (lo <= t && t < hi) {
+            index[at] = base + i;
+            if (logp) logp[at] = sample_exponent(x[i], st.m, rule.inv_tau) - log((double)total / unit);
+        }
+    }
+}
+
+static int rows_bins(int64_t V) { int b = 256; while (b < SNK_BINS_MOST && b * 256 < V) b <<= 1; return b; }
+static int64_t rows_chunks(int64_t V) { return (V + SNK_CHUNK - 1) / SNK_CHUNK; }
+static unsigned int rows_list(int64_t V) { return V < SNK_LIST ? (unsigned int)V : SNK_LIST; }
+#define SNK_ALIGNED(bytes_) (((size_t)(bytes_) + 255) & ~(size_t)255)
+
+// rows of more than 1024 scores: bytes of workspace a row takes, and how many rows go together at most (2 GB)
+size_t sample_rows_work_bytes(int64_t V)
+{
+    if (V <= 1024) return 0;
+    const size_t c = (size_t)rows_chunks(V), b = (size_t)rows_bins(V);
+    return sizeof(RowState) + c * (2 * sizeof(double) + sizeof(u64) + sizeof(unsigned int)) + b * 12 + rows_list(V) * sizeof(double) + sizeof(int);
+}
+int64_t sample_rows_together(int64_t R, int64_t V)
+{
+    const size_t each = sample_rows_work_bytes(V);
+    if (!each) return R;
+    const int64_t most = (int64_t)(((size_t)2 << 30) / each);
+    return std::min<int64_t>(R, std::max<int64_t>(1, std::min<int64_t>(most, 32768)));
+}
+size_t sample_rows_work(int64_t rows, int64_t V) { return V <= 1024 ? 0 : rows * sample_rows_work_bytes(V) + 16 * 256; }
+
+template <typename T>
+static void launch_rows_split(const T *scores, int64_t stride, int64_t R, int64_t V, const double *u, int n_draws, const SampleRule &rule,
+                              const double *rules, double unit, char *work, int64_t *index, double *logp, hipStream_t s)
+{
+    RowsWork w;
+    w.bins = rows_bins(V);
+    w.chunks = (int)rows_chunks(V);
+    size_t at = 0;
+    auto take = [&](size_t bytes) { char *p = work + at; at += SNK_ALIGNED(bytes); return p; };
+    const size_t n = (size_t)R * w.chunks;
+    w.state = (RowState *)take(R * sizeof(RowState));
+    w.chunk_max = (double *)take(n * 8); w.chunk_min = (double *)take(n * 8);
+    w.chunk_mass = (u64 *)take(n * 8); w.chunk_ties = (unsigned int *)take(n * 4);
+    w.hist_mass = (u64 *)take((size_t)R * w.bins * 8); w.hist_count = (unsigned int *)take((size_t)R * w.bins * 4);
+    w.list = rows_list(V);
+    w.list_x = (double *)take((size_t)R * w.list * 8);
+    w.left = (int *)take(R * 4);
+    const dim3 grid((unsigned)w.chunks, (unsigned)R);
+    hipLaunchKernelGGL((rows_extremes_kernel<T>), grid, dim3(256), 0, s, scores, stride, V, w);
+    hipLaunchKernelGGL((rows_histogram_kernel<T>), grid, dim3(512), (size_t)w.bins * 12, s, scores, stride, V, rule, rules, unit, w);
+    for (int by_mass = 0; by_mass < 2; ++by_mass) {
+        if (!rules && (by_mass ? !(rule.top_p < 1.0) : !(rule.top_k > 0 && rule.top_k < V))) continue;
+        hipLaunchKernelGGL((rows_boundary_kernel<T>), grid, dim3(256), 0, s, scores, stride, V, rule, rules, unit, by_mass, w);
+        hipLaunchKernelGGL(rows_select_kernel, dim3((unsigned)R), dim3(1024), 0, s, V, rule, rules, unit, by_mass, w);
+    }
+    hipLaunchKernelGGL((rows_masses_kernel<T>), grid, dim3(512), 0, s, scores, stride, V, rule, rules, unit, w);
+    hipLaunchKernelGGL((rows_draw_kernel<T>), dim3((unsigned)R, n_draws), dim3(1024), 0, s, scores, stride, V, u, n_draws, rule, rules, unit, w, index, logp);
+    hipLaunchKernelGGL((sample_rows_block_kernel<T, 1024>), dim3((unsigned)R), dim3(1024), 0, s, scores, stride, V, u, n_draws, rule, rules, unit, w.left,
+                       index, logp);
+}
+
 template <typename T>
 static void launch_sample_t(const T *scores, int64_t stride, int64_t R, int64_t V, const double *u, int n_draws, const SampleRule &rule,
-                            const double *rules, int64_t *index, double *logp, hipStream_t s)
+                            const double *rules, char *work, int64_t *index, double *logp, hipStream_t s)
 {
     int s_bits = 62;
     for (int64_t v = 1; v < V; v <<= 1) --s_bits;
@@ -328,26 +769,36 @@ static void launch_sample_t(const T *scores, int64_t stride, int64_t R, int64_t 
     else if (V <= 256) SNK_WAVE(4);
     else if (V <= 512) SNK_WAVE(8);
     else if (V <= 1024) SNK_WAVE(16);
+    else if (work) launch_rows_split(scores, stride, R, V, u, n_draws, rule, rules, unit, work, index, logp, s);
     else
         hipLaunchKernelGGL((sample_rows_block_kernel<T, 1024>), dim3((unsigned)R), dim3(1024), 0, s, scores, stride, V, u, n_draws, rule, rules, unit,
-                           index, logp);
+                           (const int *)nullptr, index, logp);
 #undef SNK_WAVE
 }
 
 int64_t sample_rows_max() { return (int64_t)SNK_SAMPLE_TILES * 1024 * SNK_SAMPLE_VEC; }
 
 void launch_sample_rows(const void *scores, int dtype, int64_t stride, int64_t R, int64_t V, const double *u, int n_draws,
-                        const SampleRuleHost &rule, const double *rules, int64_t *index, double *logp, hipStream_t s)
+                        const SampleRuleHost &rule, const double *rules, char *work, int64_t *index, double *logp, hipStream_t s)
 {
     SampleRule k;
     k.inv_tau = rule.temperature > 0.0 ? 1.0 / rule.temperature : __builtin_inf();
     k.top_k = rule.temperature > 0.0 ? rule.top_k : 1;
     k.top_p = rule.top_p;
     k.min_p = rule.min_p;
-    if (dtype == 0) launch_sample_t((const double *)scores, stride, R, V, u, n_draws, k, rules, index, logp, s);
-    else if (dtype == 1) launch_sample_t((const float *)scores, stride, R, V, u, n_draws, k, rules, index, logp, s);
-    else if (dtype == 2) launch_sample_t((const __half *)scores, stride, R, V, u, n_draws, k, rules, index, logp, s);
-    else launch_sample_t((const __hip_bfloat16 *)scores, stride, R, V, u, n_draws, k, rules, index, logp, s);
+    const int64_t step = work ? sample_rows_together(R, V) : R;
+    const size_t width = dtype == 0 ? 8 : dtype == 1 ? 4 : 2;
+    for (int64_t r = 0; r < R; r += step) {
+        const int64_t n = R - r < step ? R - r : step;
+        const void *p = (const char *)scores + (size_t)r * stride * width;
+        const double *ru = u + r * n_draws, *rr = rules ? rules + 4 * r : nullptr;
+        int64_t *ri = index + r * n_draws;
+        double *rl = logp ? logp + r * n_draws : nullptr;
+        if (dtype == 0) launch_sample_t((const double *)p, stride, n, V, ru, n_draws, k, rr, work, ri, rl, s);
+        else if (dtype == 1) launch_sample_t((const float *)p, stride, n, V, ru, n_draws, k, rr, work, ri, rl, s);
+        else if (dtype == 2) launch_sample_t((const __half *)p, stride, n, V, ru, n_draws, k, rr, work, ri, rl, s);
+        else launch_sample_t((const __hip_bfloat16 *)p, stride, n, V, ru, n_draws, k, rr, work, ri, rl, s);
+    }
 }
 
 }  // namespace snk

@@ -448,7 +448,8 @@ struct snk_engine {
     // draws and posteriors (api_sample.hip): everything on the engine's main stream
     DevBuf pb_bias, pb_edges;              // position bias (classes, buckets) and the buckets' edges
     int pb_classes = 0, pb_buckets = 0;    // 0: none set
-    DevBuf sr_scores, sr_u, sr_rules, sr_index, sr_logp;
+    DevBuf sr_scores, sr_u, sr_rules, sr_index, sr_logp, sr_work;
+    hipEvent_t sr_done = nullptr; bool sr_used = false;      // end of the last call that used sr_work
     double pb_min = 0.0;                   // the smallest finite bias, at most 0
     DevBuf tr_off, tr_cand, tr_tdist, tr_class, tr_u, tr_C, tr_V, tr_W, tr_local, tr_least, tr_flag, tr_draw, tr_row_uses, tr_out;
     DevBuf tr_M, tr_exps, tr_ends_v, tr_ends_w, tr_scaled;      // the pieces of the recursions

@@ -361,7 +361,10 @@ void launch_concat_fragments(const float *spec, int W, const double *fzv, const 
 struct SampleRuleHost { double temperature; int64_t top_k; double top_p, min_p; };
 int64_t sample_rows_max();            // longest row of scores
 void launch_sample_rows(const void *scores, int dtype, int64_t stride, int64_t R, int64_t V, const double *u, int n_draws,
-                        const SampleRuleHost &rule, const double *rules, int64_t *index, double *logp, hipStream_t s);
+                        const SampleRuleHost &rule, const double *rules, char *work, int64_t *index, double *logp, hipStream_t s);
+// workspace of the rows that launch_sample_rows takes together (0: none needed); without one a row is a workgroup's
+int64_t sample_rows_together(int64_t R, int64_t V);
+size_t sample_rows_work(int64_t rows, int64_t V);
 // utterances first .. first + n_utts - 1 of a batch, `rows` rows from row c0 on; C holds the cells of those rows only (K x Kp a row,
 // Kp = K rounded up to a multiple of eight), the other pointers are the whole batch's
 struct TrellisView {

@@ -80,6 +80,33 @@ def test_rows_long(engine, V, dtype):
         check_rows(engine, x, rng.rand(2, 2), **rule)
 
 
+@pytest.mark.parametrize('V', [1100, 9000, 20000, 70000])
+def test_rows_whose_scores_crowd(engine, V):
+    """Rows that leave a boundary bin full: equal scores by the thousand, different ones within a hair of each other, a few far ones."""
+    rng = np.random.RandomState(V)
+    crowd = 1.0 + 1e-9 * rng.rand(V)
+    spike = np.where(np.arange(V) % 1000 == 7, 3.0, crowd)
+    x = np.stack([np.full(V, -2.5), crowd, spike, np.where(rng.rand(V) < 0.5, 0.0, np.log(0.5)), -1e6 * rng.rand(V), np.round(rng.randn(V), 1)])
+    u = rng.rand(6, 2)
+    for rule in (dict(), dict(top_k=V // 2), dict(top_k=20), dict(top_p=0.5), dict(top_p=0.999), dict(top_k=V - 1, top_p=0.3), dict(temperature=1e-3, top_p=0.9),
+                 dict(temperature=50.0, top_k=700, top_p=0.9, min_p=0.5)):
+        check_rows(engine, x, u, **rule)
+
+
+def test_rows_share_a_workspace_in_turn(engine):
+    """Calls on two streams at once, of sizes that make the workspace grow in between: each finds its own results."""
+    import torch
+    rng = np.random.RandomState(9)
+    work, streams = [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for n, V in enumerate((3000, 40000, 2000, 90000, 5000, 60000)):
+        x, u = rng.randn(5, V).astype(np.float32), rng.rand(5, 2)
+        with torch.cuda.stream(streams[n % 2]):
+            work.append((engine.sample_rows(on_gpu(x), on_gpu(u), top_k=300, top_p=0.9)[0], o.sample_rows(x, u, top_k=300, top_p=0.9)[0]))
+    torch.cuda.synchronize()
+    for got, want in work:
+        assert np.array_equal(got.cpu().numpy(), want)
+
+
 @pytest.mark.parametrize('R', [1, 3, 4, 5, 257, 1000])
 def test_rows_counts(engine, R):
     rng = np.random.RandomState(R)
