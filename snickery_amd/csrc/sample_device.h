@@ -149,6 +149,14 @@ __device__ __forceinline__ double row16_max(double v)      // of each row of 16 
     v = dpp_max(v, dpp_move<0x118, 0xf>(SNK_BITS(v), SNK_BITS(v)));
     return v;
 }
+__device__ __forceinline__ double row16_sum(double v)      // of each row of 16 lanes, in all of them
+{
+    v += __longlong_as_double((long long)dpp_move<0x121, 0xf>(0, SNK_BITS(v)));     // rotations within the row
+    v += __longlong_as_double((long long)dpp_move<0x122, 0xf>(0, SNK_BITS(v)));
+    v += __longlong_as_double((long long)dpp_move<0x124, 0xf>(0, SNK_BITS(v)));
+    v += __longlong_as_double((long long)dpp_move<0x128, 0xf>(0, SNK_BITS(v)));
+    return v;
+}
 __device__ __forceinline__ double quad_sum(double v)       // of each four lanes, in all of them
 {
     v += __longlong_as_double((long long)dpp_move<0xb1, 0xf>(0, SNK_BITS(v)));
@@ -181,65 +189,54 @@ struct WaveRow {
     u64 w[E];                   // kept weights (0: not kept)
 };
 
-// n-th set bit of a mask that has more than n of them (uniform)
-__device__ __forceinline__ int nth_bit(u64 mask, int n)
-{
-    for (; n; --n) mask &= mask - 1;
-    return __ffsll((long long)mask) - 1;
-}
-
 // The truncations.  x: the order's values (-inf: takes no part), row.w: their weights in units of 1 / unit (equal values, equal
 // weights; the largest weighs `unit`).  On return row.w is what is kept, row.before / row.total its sums.
 template <int E>
 __device__ __forceinline__ void wave_row_keep(const double (&x)[E], const SampleRule &rule, double unit, WaveRow<E> &row)
 {
     const double ninf = -__builtin_inf();
-    // The order's prefix, by bisection on the values: `live` are the elements whose side is not known yet, a pivot among them splits
-    // them, one ballot per element slot counts a side.  The middle live element is the pivot: a sorted list is halved, an
-    // unsorted one takes ~ 2 ln V rounds.
+    // The order's prefix, by bisection on the values.  `live`: the lanes, per element slot, whose side is not known yet; one of them is
+    // the pivot, taken a third of the wavefront further on every round (about 2 ln V rounds, sorted rows or not).  A comparison with
+    // the pivot is a mask of lanes: masks, counts and the pivot's choice are scalar work beside the other wavefronts' vector work.
     double cut = ninf;          // kept: x > cut, and the first n_tie of the elements equal to it
     int n_tie = 0, ties = 0;
     auto search = [&](bool by_mass, u64 want) {
         u64 above = 0;                                          // count / mass of everything above the live elements
-        unsigned live = 0;
+        u64 live[E];
 #pragma unroll
-        for (int e = 0; e < E; ++e) live |= (by_mass ? row.w[e] != 0 : x[e] > ninf) ? 1u << e : 0u;
-        for (;;) {
-            u64 b[E];
-            int n = 0;
-#pragma unroll
-            for (int e = 0; e < E; ++e) { b[e] = __ballot((live >> e) & 1u); n += __popcll(b[e]); }
-            if (n == 0) return;                                 // (the prefix is the whole row)
-            int left = n >> 1;                                  // the middle one
+        for (int e = 0; e < E; ++e) live[e] = __ballot(by_mass ? row.w[e] != 0 : x[e] > ninf);
+        for (int turn = 21;; turn += 21) {
             double pivot = 0.0;
-            u64 weight = 0;
+            u64 each = 0;
             bool found = false;
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int c = __popcll(b[e]);
-                if (!found && left < c) {
-                    const int l = nth_bit(b[e], left);
+            for (int e = 0; e < E; ++e)
+                if (!found && live[e]) {
+                    const u64 later = live[e] & (~0ull << (turn & 63));
+                    const int l = __ffsll((long long)(later ? later : live[e])) - 1;
                     pivot = wave_lane(x[e], l);
-                    weight = wave_lane(row.w[e], l);
+                    if (by_mass) each = wave_lane(row.w[e], l);      // (equal values: equal weights)
                     found = true;
                 }
-                if (!found) left -= c;
-            }
-            u64 gt = 0;
+            if (!found) return;                                 // (the prefix is the whole row)
+            u64 g[E], q[E], gt = 0, part = 0;
             int eq = 0;
-            unsigned mgt = 0, meq = 0;
 #pragma unroll
             for (int e = 0; e < E; ++e) {
-                const bool l = (live >> e) & 1u, g = l && x[e] > pivot, q = l && x[e] == pivot;
-                mgt |= g ? 1u << e : 0u;
-                meq |= q ? 1u << e : 0u;
-                if (by_mass) gt += g ? row.w[e] : 0;
-                else gt += __popcll(__ballot(g));
-                eq += __popcll(__ballot(q));
+                const bool more = x[e] > pivot;
+                g[e] = __ballot(more) & live[e];
+                q[e] = __ballot(x[e] == pivot) & live[e];
+                eq += __popcll(q[e]);
+                if (by_mass) part += more && ((live[e] >> (threadIdx.x & 63)) & 1) ? row.w[e] : 0;
+                else gt += __popcll(g[e]);
             }
-            if (by_mass) gt = wave_add(gt);
-            if (above + gt >= want) { live = mgt; continue; }
-            const u64 each = by_mass ? weight : 1;               // (equal values: equal weights)
+            if (by_mass) gt = wave_add(part);
+            else each = 1;
+            if (above + gt >= want) {
+#pragma unroll
+                for (int e = 0; e < E; ++e) live[e] = g[e];
+                continue;
+            }
             if (above + gt + each * (u64)eq >= want) {
                 cut = pivot;
                 ties = eq;
@@ -250,7 +247,8 @@ __device__ __forceinline__ void wave_row_keep(const double (&x)[E], const Sample
                 return;
             }
             above += gt + each * (u64)eq;
-            live &= ~(mgt | meq);
+#pragma unroll
+            for (int e = 0; e < E; ++e) live[e] &= ~(g[e] | q[e]);
         }
     };
     auto apply = [&]() {        // weights outside the prefix -> 0

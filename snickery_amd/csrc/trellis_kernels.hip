@@ -44,15 +44,29 @@ __device__ __forceinline__ int trellis_utterance(const int64_t *__restrict__ off
     return u;
 }
 
-// bucket of a distance: most joins are far ones, the two outermost buckets are decided first
-__device__ __forceinline__ int trellis_bucket(int apart, const int *edges, int n_buckets)
+// Bucket of a distance: the number of edges up to it.  63 edges at most, in LDS behind INT_MAX padding: which eight of them it falls
+// among from every eighth (in registers), then those eight.  28 instructions and one LDS latency whatever the distance; a search by
+// halves waits for LDS five times.
+struct TrellisEdges { int head[7]; const int *all; };
+__device__ __forceinline__ TrellisEdges trellis_edges(const int *lds)
 {
-    const int n = n_buckets - 1;
-    if (n == 0 || apart < edges[0]) return 0;
-    if (apart >= edges[n - 1]) return n;
-    int lo = 0, hi = n - 1;                                    // edges[lo] <= apart < edges[hi]
-    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (apart >= edges[mid]) lo = mid; else hi = mid; }
-    return lo + 1;
+    TrellisEdges e;
+    e.all = lds;
+#pragma unroll
+    for (int i = 0; i < 7; ++i) e.head[i] = lds[8 * i + 7];
+    return e;
+}
+__device__ __forceinline__ int trellis_bucket(int apart, const TrellisEdges &e)
+{
+    int k = 0;
+#pragma unroll
+    for (int i = 0; i < 7; ++i) k += apart >= e.head[i] ? 8 : 0;
+    const int4 x = *reinterpret_cast<const int4 *>(e.all + k), y = *reinterpret_cast<const int4 *>(e.all + k + 4);
+    return k + (apart >= x.x) + (apart >= x.y) + (apart >= x.z) + (apart >= x.w) + (apart >= y.x) + (apart >= y.y) + (apart >= y.z) + (apart >= y.w);
+}
+__device__ __forceinline__ void trellis_load_edges(int *lds, const int *__restrict__ edges, int n_buckets)
+{
+    if (threadIdx.x < 64) lds[threadIdx.x] = (int)threadIdx.x < n_buckets - 1 ? edges[threadIdx.x] : 0x7fffffff;
 }
 
 __device__ __forceinline__ double trellis_pow2(int e)           // 2^e, -1022 <= e <= 1023
@@ -99,23 +113,52 @@ trellis_local_kernel(const TrellisView v, double *__restrict__ local, double *__
 }
 
 // ---- costs: a workgroup per pair of rows and tile of 16 RT x 16 RT cells ------------------------------------------------------------
-// Distances in difference form (a unit and its natural successor join at exactly 0), one subtraction and one fused multiply-add per
-// column: the float64 vector pipe is what bounds it, 2 Dj instructions a cell.  A thread keeps RT x RT cells; 16 columns of the two
-// sets of rows go through LDS at a time, weighted and widened on the way, the next 16 are in flight meanwhile.
-template <int RT, bool LOG>
+// |e - s|^2 = |e|^2 + |s|^2 - 2 e.s on the float64 matrix pipe: half the instructions of the difference form (one fused multiply-add
+// a column instead of a subtraction and one), which ran at two thirds of the vector pipe's rate.  Both sides are taken relative to
+// one of the tile's units, so that the norms are those of the candidates' spread and not of their distance from the origin.  Where
+// the difference is small against the norms -- a unit and its natural successor join at exactly 0 -- the product form cancels: a
+// cell below SNK_COST_NEAR of them is taken again in differences.  The others carry a relative error of at most Dj 2^-53 / SNK_COST_NEAR.
+// A wavefront owns RM x CM tiles of 16 x 16; 16 columns of the two sets of rows go through LDS at a time, weighted and widened on
+// the way, the next 16 are in flight meanwhile.
+#define SNK_COST_NEAR 0x1p-8
+typedef double f64x4 __attribute__((ext_vector_type(4)));
+
+// sum of squared differences of a pair of join rows by a row of sixteen lanes; in every one of them
+__device__ __forceinline__ double trellis_difference(const TrellisCosts &c, int end, int start)
+{
+    const float *__restrict__ pe = c.JC + (int64_t)(end + 1) * c.Jp, *__restrict__ ps = c.JC + (int64_t)start * c.Jp;
+    double d2 = 0.0;
+    for (int j = 4 * (threadIdx.x & 15); j < c.Dj; j += 64) {   // (rows are padded to multiples of four columns)
+        const float4 e = *reinterpret_cast<const float4 *>(pe + j), s = *reinterpret_cast<const float4 *>(ps + j);
+        const float e4[4] = {e.x, e.y, e.z, e.w}, s4[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const double w = j + k < c.Dj ? c.wj[j + k] : 0.0, d = (double)e4[k] * w - (double)s4[k] * w;
+            d2 = __fma_rn(d, d, d2);
+        }
+    }
+    return row16_sum(d2);
+}
+
+template <int RT, int RM, int CM, bool LOG>
 __global__ void __launch_bounds__(256, 2)
 trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__ flag, double *__restrict__ X)
 {
-    constexpr int N = 16 * RT, DC = 16, LD = N + 4, PASS = (N + 63) / 64;
-    __shared__ double Es[DC * LD], Ss[DC * LD];
+    constexpr int N = 16 * RT, DC = 16, LD = DC + 2, PASS = (N + 63) / 64, WC = (RT + CM - 1) / CM, NEAR = 2048;      // WC wavefronts side by side; cells to take again
+    __shared__ __align__(16) double Es[N * LD], Ss[N * LD];
+    __shared__ double nE[N], nS[N];
     __shared__ int idE[N], idS[N];                              // unit id, -1: cannot join
-    __shared__ int edges[64];
+    __shared__ __align__(16) int edges[64];
     __shared__ double bias[64];
+    __shared__ unsigned short near_cell[NEAR];
+    __shared__ unsigned int n_near;
     const int64_t t = v.c0 + blockIdx.x;
     const int u = trellis_utterance(v.off, v.first, v.n_utts, t);
     if (t + 1 == v.off[u + 1]) return;
     if (LOG && !flag[u]) return;
-    const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, g = lane >> 4;
+    const int wave = ((tid >> 6) + blockIdx.x) & 3;             // (the last wavefront has fewer tiles: not always on the same SIMD)
+    const int row0 = (wave / WC) * RM, col0 = (wave % WC) * CM;
     const int a0 = blockIdx.y * N, b0 = blockIdx.z * N;
     for (int i = tid; i < 2 * N; i += 256) {
         const bool second = i >= N;
@@ -127,91 +170,149 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
     if (c.n_classes) {
         cls = c.join_class ? c.join_class[t] : 0;
         if (cls >= c.n_classes) cls = -1;
-        if (tid < c.n_buckets - 1) edges[tid] = c.edges[tid];
+        trellis_load_edges(edges, c.edges, c.n_buckets);
         if (cls >= 0 && tid < c.n_buckets) bias[tid] = c.bias[(int64_t)cls * c.n_buckets + tid];
     }
+    if (tid == 0) n_near = 0;
     __syncthreads();
+    int about = 0;                                              // the row that both sides are taken relative to
+    for (int i = 0; i < N; ++i)
+        if (idS[i] >= 0) { about = idS[i]; break; }
 
     const int q = tid & 3, r0 = tid >> 2;
-    const float *pe[PASS], *ps[PASS];
-    float4 fe[PASS], fs[PASS];
-    double w[4];
+    const float *pe[PASS], *ps[PASS], *pc = c.JC + (int64_t)about * c.Jp + 4 * q;
+    float4 fe[PASS], fs[PASS], fc;
+    double w[4], ne[PASS], ns[PASS];
 #pragma unroll
     for (int p = 0; p < PASS; ++p) {
         const int r = r0 + 64 * p < N ? r0 + 64 * p : 0;
-        pe[p] = c.JC + (int64_t)(idE[r] >= 0 ? idE[r] + 1 : 0) * c.Jp + 4 * q;
-        ps[p] = c.JC + (int64_t)(idS[r] >= 0 ? idS[r] : 0) * c.Jp + 4 * q;
+        pe[p] = c.JC + (int64_t)(idE[r] >= 0 ? idE[r] + 1 : about) * c.Jp + 4 * q;
+        ps[p] = c.JC + (int64_t)(idS[r] >= 0 ? idS[r] : about) * c.Jp + 4 * q;
+        ne[p] = 0.0; ns[p] = 0.0;
     }
     auto fetch = [&](int col) {
-        const bool in = col + 4 * q < c.Jp;                     // (rows are padded to multiples of four columns)
+        const bool in = col + 4 * q < c.Jp;
+        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
+        fc = in ? *reinterpret_cast<const float4 *>(pc + col) : zero;
 #pragma unroll
         for (int p = 0; p < PASS; ++p) {
-            fe[p] = in ? *reinterpret_cast<const float4 *>(pe[p] + col) : make_float4(0.f, 0.f, 0.f, 0.f);
-            fs[p] = in ? *reinterpret_cast<const float4 *>(ps[p] + col) : make_float4(0.f, 0.f, 0.f, 0.f);
+            fe[p] = in ? *reinterpret_cast<const float4 *>(pe[p] + col) : zero;
+            fs[p] = in ? *reinterpret_cast<const float4 *>(ps[p] + col) : zero;
         }
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[e] = col + 4 * q + e < c.Dj ? c.wj[col + 4 * q + e] : 0.0;
     };
-    double acc[RT][RT];
+    f64x4 acc[RM][CM];
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
+    for (int i = 0; i < RM; ++i)
 #pragma unroll
-        for (int j = 0; j < RT; ++j) acc[i][j] = 0.0;
+        for (int j = 0; j < CM; ++j) acc[i][j] = f64x4{0.0, 0.0, 0.0, 0.0};
     fetch(0);
     for (int col = 0; col < c.Dj; col += DC) {
+        const float c4[4] = {fc.x, fc.y, fc.z, fc.w};
 #pragma unroll
         for (int p = 0; p < PASS; ++p) {
             const int r = r0 + 64 * p;
             if (r < N) {
                 const float e4[4] = {fe[p].x, fe[p].y, fe[p].z, fe[p].w}, s4[4] = {fs[p].x, fs[p].y, fs[p].z, fs[p].w};
+                double de[4], ds[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    Es[(4 * q + e) * LD + r] = (double)e4[e] * w[e];
-                    Ss[(4 * q + e) * LD + r] = (double)s4[e] * w[e];
+                    const double m = (double)c4[e] * w[e];
+                    de[e] = (double)e4[e] * w[e] - m;
+                    ds[e] = (double)s4[e] * w[e] - m;
+                    ne[p] = __fma_rn(de[e], de[e], ne[p]);
+                    ns[p] = __fma_rn(ds[e], ds[e], ns[p]);
                 }
+                f64x2 *te = reinterpret_cast<f64x2 *>(&Es[r * LD + 4 * q]), *ts = reinterpret_cast<f64x2 *>(&Ss[r * LD + 4 * q]);
+                te[0] = f64x2{de[0], de[1]}; te[1] = f64x2{de[2], de[3]};
+                ts[0] = f64x2{ds[0], ds[1]}; ts[1] = f64x2{ds[2], ds[3]};
             }
         }
         __syncthreads();
         if (col + DC < c.Dj) fetch(col + DC);
-#pragma unroll 2
-        for (int k = 0; k < DC; ++k) {
-            double ev[RT], sv[RT];
 #pragma unroll
-            for (int i = 0; i < RT; ++i) ev[i] = Es[k * LD + ty + 16 * i];
+        for (int ks = 0; ks < DC / 4; ++ks) {
+            double fa[RM], fb[CM];
 #pragma unroll
-            for (int j = 0; j < RT; ++j) sv[j] = Ss[k * LD + tx + 16 * j];
+            for (int i = 0; i < RM; ++i) fa[i] = row0 + i < RT ? Es[((row0 + i) * 16 + c16) * LD + 4 * ks + g] : 0.0;
 #pragma unroll
-            for (int i = 0; i < RT; ++i)
+            for (int j = 0; j < CM; ++j)
+                if (col0 + j < RT) {                            // (uniform)
+                    fb[j] = Ss[((col0 + j) * 16 + c16) * LD + 4 * ks + g];
 #pragma unroll
-                for (int j = 0; j < RT; ++j) {
-                    const double d = ev[i] - sv[j];
-                    acc[i][j] = __fma_rn(d, d, acc[i][j]);
+                    for (int i = 0; i < RM; ++i)
+                        if (row0 + i < RT) acc[i][j] = __builtin_amdgcn_mfma_f64_16x16x4f64(fa[i], fb[j], acc[i][j], 0, 0, 0);
                 }
         }
         __syncthreads();
     }
+#pragma unroll
+    for (int p = 0; p < PASS; ++p) {
+        const int r = r0 + 64 * p;
+        const double e = quad_sum(ne[p]), s = quad_sum(ns[p]);
+        if (r < N && q == 0) { nE[r] = e; nS[r] = s; }
+    }
+    __syncthreads();
     bool wide = false;
     double *__restrict__ out = X + (t - v.c0) * v.K * v.Kp;
+    const TrellisEdges look = trellis_edges(edges);
+    auto value = [&](double d2, int ie, int is) -> double {     // a cell from the squared distance; ie, is < 0: cannot join
+        const bool ok = (ie | is) >= 0;
+        double cost = sqrt(d2);
+        if (cls >= 0) cost += bias[trellis_bucket(is - ie, look)];
+        if (LOG) return ok ? -cost * v.inv_tau : -__builtin_inf();
+        const double x = (c.bias_min - cost) * v.inv_tau;
+        wide |= ok && x < -SNK_COST_RANGE && cost < __builtin_inf();
+        return ok && cost < __builtin_inf() ? sample_exp(fmax(x, -SNK_COST_RANGE)) : 0.0;
+    };
+    // (a loop over the tiles, not RM CM copies of its body; a wavefront's k-th tile is picked by uniform branches)
+#pragma unroll 1
+    for (int k = 0; k < RM * CM; ++k) {
+        f64x4 p = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
+        for (int i = 0; i < RM; ++i)
 #pragma unroll
-        for (int j = 0; j < RT; ++j) {
-            const int al = ty + 16 * i, bl = tx + 16 * j, a = a0 + al, b = b0 + bl;
-            if (a < v.K && b < v.Kp) {
-                const int ie = idE[al], is = idS[bl];
-                double cost = __builtin_inf();
-                if (ie >= 0 && is >= 0) {
-                    cost = sqrt(acc[i][j]);
-                    if (cls >= 0) cost += bias[trellis_bucket(is - ie, edges, c.n_buckets)];
-                }
-                if (LOG) out[(int64_t)a * v.Kp + b] = -cost * v.inv_tau;
-                else {
-                    const double x = (c.bias_min - cost) * v.inv_tau;
-                    wide |= x < -SNK_COST_RANGE && cost < __builtin_inf();
-                    out[(int64_t)a * v.Kp + b] = exp(x);
-                }
-            }
+            for (int j = 0; j < CM; ++j)
+                if (i * CM + j == k) p = acc[i][j];
+        const int ti = row0 + k / CM, tj = col0 + k % CM;
+        if (ti >= RT || tj >= RT) continue;
+        const int bl = tj * 16 + c16, is = idS[bl], b = b0 + bl;
+        const double sn = nS[bl];
+        bool again[4];
+        int any = 0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int al = ti * 16 + g + 4 * r, ie = idE[al], a = a0 + al;
+            const double both = nE[al] + sn, d2 = __fma_rn(-2.0, p[r], both);
+            again[r] = (ie | is) >= 0 && d2 < SNK_COST_NEAR * both;
+            any += again[r] ? 1 : 0;
+            const double x = value(fmax(d2, 0.0), ie, is);
+            if (a < v.K && b < v.Kp) out[(int64_t)a * v.Kp + b] = x;
         }
+        if (__ballot(any)) {
+            const unsigned int upto = (unsigned int)wave_scan_add((u64)any);
+            unsigned int at = 0;
+            if (lane == 63) at = atomicAdd(&n_near, upto);
+            at = (unsigned int)__builtin_amdgcn_readlane((int)at, 63) + upto - any;
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                if (again[r]) {
+                    if (at < NEAR) near_cell[at] = (unsigned short)((ti * 16 + g + 4 * r) * N + bl);
+                    ++at;
+                }
+        }
+    }
+    __syncthreads();
+    // the near cells in differences, sixteen lanes each (more of them than the list holds: every cell)
+    const bool every = n_near > NEAR;
+    const int todo = every ? N * N : (int)n_near;
+    for (int i = tid >> 4; i < todo; i += 16) {
+        const int cell = every ? i : near_cell[i], al = cell / N, bl = cell % N, ie = idE[al], is = idS[bl], a = a0 + al, b = b0 + bl;
+        if ((ie | is) < 0) continue;
+        const double x = value(trellis_difference(c, ie, is), ie, is);
+        if (c16 == 0 && a < v.K && b < v.Kp) out[(int64_t)a * v.Kp + b] = x;
+    }
     if (!LOG && wide) flag[u] = 1;
 }
 
@@ -251,8 +352,6 @@ __device__ __forceinline__ TrellisPiece trellis_piece(const TrellisView &v, int 
     return p;
 }
 
-typedef double f64x4 __attribute__((ext_vector_type(4)));
-
 // 1. products: workgroup = sixteen start candidates of one piece, wavefront = CT tiles of sixteen end candidates; v_mfma_f64_16x16x4
 // over KH CH steps of four.  The weights X (16 x K) alternate between two LDS buffers; the slab's fragments live in registers and
 // each is reloaded with the next slab's (or the next half's) right after its use.  The row blocks of a piece are dealt to one XCD,
@@ -262,7 +361,7 @@ __global__ void __launch_bounds__(NTH)
 trellis_product_kernel(const TrellisView v, const double *__restrict__ local, int max_pieces, int row_blocks, bool skip_last, int *__restrict__ flag,
                        double *__restrict__ M, int *__restrict__ exps)
 {
-    constexpr int W = NTH / 64, COLS = 4 * KH * CH, LDX = COLS + 4;
+    constexpr int W = NTH / 64, COLS = 4 * KH * CH, LDX = COLS + 2;      // (sixteen rows 4 odd banks apart)
     __shared__ double X[2][16 * LDX];
     __shared__ double top[2][W][16];
     __shared__ int bad;
@@ -832,7 +931,8 @@ trellis_posterior_kernel(const TrellisView v, const int *__restrict__ flag, cons
                          double *__restrict__ posterior, double *__restrict__ row_uses)
 {
     __shared__ double in[256], out[256], red[8];
-    __shared__ int edges[64], id0[256], id1[256];
+    __shared__ __align__(16) int edges[64];
+    __shared__ int id0[256], id1[256];
     __shared__ u64 uses[64];
     const int64_t t = v.c0 + blockIdx.x;
     const int K = v.K, Kp = v.Kp, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -878,8 +978,9 @@ trellis_posterior_kernel(const TrellisView v, const int *__restrict__ flag, cons
         }
     }
     if (tid < 64) uses[tid] = 0;
-    if (tid < n_buckets - 1) edges[tid] = bucket_edges[tid];
+    trellis_load_edges(edges, bucket_edges, n_buckets);
     __syncthreads();
+    const TrellisEdges look = trellis_edges(edges);
     if (!last && !dead) {
         const double *__restrict__ c = v.C + (t - v.c0) * K * Kp;
         u64 first = 0, far = 0;
@@ -892,7 +993,7 @@ trellis_posterior_kernel(const TrellisView v, const int *__restrict__ flag, cons
                 else p = va * x * out[b];
                 const u64 w = sample_fix(p, SNK_USES_UNIT);
                 if (!w) continue;
-                const int k = trellis_bucket(id1[b] - id0[a], edges, n_buckets);
+                const int k = trellis_bucket(id1[b] - id0[a], look);
                 if (k == 0) first += w;
                 else if (k == n_buckets - 1) far += w;
                 else atomicAdd(&uses[k], w);
@@ -1098,7 +1199,10 @@ trellis_path_kernel(const TrellisView v, const TrellisCosts c, const int *__rest
         }
         cost += sqrt(wave_sum(d2));
         int cls = c.n_classes ? (c.join_class ? c.join_class[t] : 0) : -1;
-        if (cls >= 0 && cls < c.n_classes) cost += c.bias[(int64_t)cls * c.n_buckets + trellis_bucket((int)(next - id), c.edges, c.n_buckets)];
+        if (cls >= 0 && cls < c.n_classes) {
+            const bool below = lane < c.n_buckets - 1 && (int)(next - id) >= c.edges[lane];
+            cost += c.bias[(int64_t)cls * c.n_buckets + __popcll(__ballot(below))];
+        }
     }
     if (lane == 0) { path[at] = id; row_cost[at] = cost; row_logp[at] = lp; }
 }
@@ -1133,22 +1237,22 @@ void launch_trellis_local(const TrellisView &v, double *local, double *least, in
     hipLaunchKernelGGL(trellis_local_kernel, dim3((unsigned)((v.rows + 3) / 4)), dim3(256), 0, s, v, local, least, flag);
 }
 
-// The widest tile a thread's registers hold is 7 x 7 cells (two workgroups a compute unit): K is cut into as few equal tiles.
+// The widest tile that a wavefront's registers hold is 7 x 2 tiles of 16 x 16 (two workgroups a compute unit): K is cut into as few
+// equal tiles of at most 112.
 void launch_trellis_costs(const TrellisView &v, const TrellisCosts &c, bool logs, int *flag, double *X, hipStream_t s)
 {
     if (v.rows < 2) return;
     const int n = (v.K + 111) / 112, rt = ((v.K + n - 1) / n + 15) / 16;
     const dim3 grid((unsigned)(v.rows - 1), n, n);
-#define SNK_COST(RT_)                                                                                                        \
+#define SNK_COST(RT_, RM_, CM_)                                                                                              \
     do {                                                                                                                     \
-        if (logs) hipLaunchKernelGGL((trellis_cost_kernel<RT_, true>), grid, dim3(256), 0, s, v, c, flag, X);                \
-        else hipLaunchKernelGGL((trellis_cost_kernel<RT_, false>), grid, dim3(256), 0, s, v, c, flag, X);                    \
+        if (logs) hipLaunchKernelGGL((trellis_cost_kernel<RT_, RM_, CM_, true>), grid, dim3(256), 0, s, v, c, flag, X);      \
+        else hipLaunchKernelGGL((trellis_cost_kernel<RT_, RM_, CM_, false>), grid, dim3(256), 0, s, v, c, flag, X);          \
     } while (0)
-    if (rt <= 2) SNK_COST(2);
-    else if (rt <= 4) SNK_COST(4);
-    else if (rt == 5) SNK_COST(5);
-    else if (rt == 6) SNK_COST(6);
-    else SNK_COST(7);
+    if (rt <= 2) SNK_COST(2, 1, 1);
+    else if (rt <= 4) SNK_COST(4, 2, 2);
+    else if (rt <= 6) SNK_COST(6, 3, 3);
+    else SNK_COST(7, 7, 2);
 #undef SNK_COST
 }
 
