@@ -163,6 +163,10 @@ __device__ __forceinline__ double quad_sum(double v)       // of each four lanes
     v += __longlong_as_double((long long)dpp_move<0x4e, 0xf>(0, SNK_BITS(v)));
     return v;
 }
+__device__ __forceinline__ double eight_sum(double v)      // of two neighbouring fours that hold a sum each, in all eight lanes
+{
+    return v + __longlong_as_double((long long)dpp_move<0x141, 0xf>(0, SNK_BITS(v)));
+}
 __device__ __forceinline__ double rows4_sum(double v)      // of the same lane of the four rows of 16, in all of them
 {
     v += __shfl_xor(v, 16, 64);

@@ -144,13 +144,13 @@ template <int RT, int RM, int CM, bool LOG>
 __global__ void __launch_bounds__(256, 2)
 trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__ flag, double *__restrict__ X)
 {
-    constexpr int N = 16 * RT, DC = 16, LD = DC + 2, PASS = (N + 63) / 64, WC = (RT + CM - 1) / CM, NEAR = 2048;      // WC wavefronts side by side; cells to take again
+    constexpr int N = 16 * RT, DC = 16, LD = DC + 2, PASS = (N + 63) / 64, WC = (RT + CM - 1) / CM;      // WC wavefronts side by side
     __shared__ __align__(16) double Es[N * LD], Ss[N * LD];
     __shared__ double nE[N], nS[N];
     __shared__ int idE[N], idS[N];                              // unit id, -1: cannot join
     __shared__ __align__(16) int edges[64];
     __shared__ double bias[64];
-    __shared__ unsigned short near_cell[NEAR];
+    __shared__ unsigned short near_cell[N * N];                 // cells to take again
     __shared__ unsigned int n_near;
     const int64_t t = v.c0 + blockIdx.x;
     const int u = trellis_utterance(v.off, v.first, v.n_utts, t);
@@ -175,9 +175,16 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
     }
     if (tid == 0) n_near = 0;
     __syncthreads();
-    int about = 0;                                              // the row that both sides are taken relative to
-    for (int i = 0; i < N; ++i)
-        if (idS[i] >= 0) { about = idS[i]; break; }
+    // the unit that both sides are taken relative to: the second row's first one that can join (of the whole row: a cell's value does
+    // not depend on the tiles)
+    int about = 0;
+    bool found = false;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int64_t id = lane + 64 * i < v.K ? v.cand[(t + 1) * v.K + lane + 64 * i] : -1;
+        const u64 can = __ballot(trellis_usable(id, v.n_units));
+        if (can && !found) { about = __builtin_amdgcn_readlane((int)id, __ffsll((long long)can) - 1); found = true; }
+    }
 
     const int q = tid & 3, r0 = tid >> 2;
     const float *pe[PASS], *ps[PASS], *pc = c.JC + (int64_t)about * c.Jp + 4 * q;
@@ -298,18 +305,15 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
 #pragma unroll
             for (int r = 0; r < 4; ++r)
                 if (again[r]) {
-                    if (at < NEAR) near_cell[at] = (unsigned short)((ti * 16 + g + 4 * r) * N + bl);
+                    near_cell[at] = (unsigned short)((ti * 16 + g + 4 * r) * N + bl);
                     ++at;
                 }
         }
     }
     __syncthreads();
-    // the near cells in differences, sixteen lanes each (more of them than the list holds: every cell)
-    const bool every = n_near > NEAR;
-    const int todo = every ? N * N : (int)n_near;
-    for (int i = tid >> 4; i < todo; i += 16) {
-        const int cell = every ? i : near_cell[i], al = cell / N, bl = cell % N, ie = idE[al], is = idS[bl], a = a0 + al, b = b0 + bl;
-        if ((ie | is) < 0) continue;
+    // the near cells in differences, sixteen lanes each
+    for (int i = tid >> 4; i < (int)n_near; i += 16) {
+        const int cell = near_cell[i], al = cell / N, bl = cell % N, ie = idE[al], is = idS[bl], a = a0 + al, b = b0 + bl;
         const double x = value(trellis_difference(c, ie, is), ie, is);
         if (c16 == 0 && a < v.K && b < v.Kp) out[(int64_t)a * v.Kp + b] = x;
     }
@@ -352,21 +356,22 @@ __device__ __forceinline__ TrellisPiece trellis_piece(const TrellisView &v, int 
     return p;
 }
 
-// 1. products: workgroup = sixteen start candidates of one piece, wavefront = CT tiles of sixteen end candidates; v_mfma_f64_16x16x4
-// over KH CH steps of four.  The weights X (16 x K) alternate between two LDS buffers; the slab's fragments live in registers and
-// each is reloaded with the next slab's (or the next half's) right after its use.  The row blocks of a piece are dealt to one XCD,
-// so that a slab comes from memory once and from that XCD's L2 for the others.
-template <int CT, int KH, int CH, int NTH>
+// 1. products: workgroup = 16 RB start candidates of one piece, wavefront = CT tiles of sixteen end candidates; v_mfma_f64_16x16x4
+// over KH CH steps of four.  The weights X alternate between two LDS buffers; the slab's fragments live in registers and each is
+// reloaded with the next slab's (or the next half's) right after its use.  The row blocks of a piece are dealt to one XCD, so that a
+// slab comes from memory once and from that XCD's L2 for the others.  RB 1: a step re-reads the slab for sixteen rows, 50 bytes a
+// cycle and compute unit, near what the L2 gives one; RB 2 halves that and is for launches that fill the chip either way.
+template <int CT, int KH, int CH, int RB, int NTH>
 __global__ void __launch_bounds__(NTH)
 trellis_product_kernel(const TrellisView v, const double *__restrict__ local, int max_pieces, int row_blocks, bool skip_last, int *__restrict__ flag,
                        double *__restrict__ M, int *__restrict__ exps)
 {
     constexpr int W = NTH / 64, COLS = 4 * KH * CH, LDX = COLS + 2;      // (sixteen rows 4 odd banks apart)
-    __shared__ double X[2][16 * LDX];
-    __shared__ double top[2][W][16];
+    __shared__ double X[2][16 * RB * LDX];
+    __shared__ double top[2][W][16 * RB];
     __shared__ int bad;
     const int j = blockIdx.x >> 3;
-    const int i0 = (j % row_blocks) * 16, flat = (j / row_blocks) * 8 + (blockIdx.x & 7);
+    const int i0 = (j % row_blocks) * 16 * RB, flat = (j / row_blocks) * 8 + (blockIdx.x & 7);
     if (flat >= max_pieces * v.n_utts) return;
     const TrellisPiece p = trellis_piece(v, flat / max_pieces, flat % max_pieces);
     if (p.k >= p.P || p.P == 1 || (skip_last && p.k == p.P - 1) || flag[p.u]) return;
@@ -393,76 +398,98 @@ trellis_product_kernel(const TrellisView v, const double *__restrict__ local, in
 #pragma unroll
             for (int c = 0; c < CT; ++c) load(1, 0, ks, c);
     }
-    for (int i = tid; i < 2 * 16 * LDX; i += NTH) (&X[0][0])[i] = 0.0;
+    for (int i = tid; i < 2 * 16 * RB * LDX; i += NTH) (&X[0][0])[i] = 0.0;
     if (tid == 0) bad = 0;
-    if (tid < W * 16) top[0][tid >> 4][tid & 15] = 0.0;
     __syncthreads();
     // the first slab: the start candidate's own cells
     bool small = false;
-    double m4[4] = {0.0, 0.0, 0.0, 0.0};
+    double most[RB][4];
+#pragma unroll
+    for (int h = 0; h < RB; ++h)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) most[h][r] = 0.0;
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
         if (col[c] >= Kp) continue;
         const double l = local[(first_row + 1) * Kp + col[c]];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int row = g + 4 * r;
-            const double x = i0 + row < K ? slab0[(int64_t)(i0 + row) * Kp + col[c]] * l : 0.0;
-            X[0][row * LDX + col[c]] = x;
-            m4[r] = fmax(m4[r], x);
-            small |= x > 0.0 && x < SNK_WEIGHT_LEAST;
-        }
+        for (int h = 0; h < RB; ++h)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int row = 16 * h + g + 4 * r;
+                const double x = i0 + row < K ? slab0[(int64_t)(i0 + row) * Kp + col[c]] * l : 0.0;
+                X[0][row * LDX + col[c]] = x;
+                most[h][r] = fmax(most[h][r], x);
+                small |= x > 0.0 && x < SNK_WEIGHT_LEAST;
+            }
     }
     auto row_max = [&](int at) {                                // largest weight of every row, per wavefront (lane 15 of each row of lanes has it)
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const double m = row16_max(m4[r]);
-            if (c16 == 15) top[at][wave][g + 4 * r] = m;
-        }
+        for (int h = 0; h < RB; ++h)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const double m = row16_max(most[h][r]);
+                if (c16 == 15) top[at][wave][16 * h + g + 4 * r] = m;
+            }
+    };
+    auto row_exponent = [&](int at, int row) -> int {
+        double m = top[at][0][row];
+#pragma unroll
+        for (int w = 1; w < W; ++w) m = fmax(m, top[at][w][row]);
+        return trellis_exponent(m);
     };
     row_max(0);
     __syncthreads();
-    int e4[4] = {0, 0, 0, 0};
+    auto read = [&](int at, int step, double (&x)[RB]) {
+#pragma unroll
+        for (int h = 0; h < RB; ++h) x[h] = X[at][(16 * h + c16) * LDX + step * 4 + g];
+    };
+    int e4[RB][4] = {};
     for (int s = 1; s < p.n; ++s) {
         const int from = (s - 1) & 1, to = s & 1;
-        f64x4 acc[CT];
+        f64x4 acc[RB][CT];
 #pragma unroll
-        for (int c = 0; c < CT; ++c) acc[c] = f64x4{0.0, 0.0, 0.0, 0.0};
+        for (int h = 0; h < RB; ++h)
+#pragma unroll
+            for (int c = 0; c < CT; ++c) acc[h][c] = f64x4{0.0, 0.0, 0.0, 0.0};
         double lw[CT];
 #pragma unroll
         for (int c = 0; c < CT; ++c) lw[c] = col[c] < Kp ? local[(first_row + s + 1) * Kp + col[c]] : 0.0;
+        double x[3][RB];
+        read(from, 0, x[0]);
+        read(from, 1, x[1]);
 #pragma unroll
         for (int half = 0; half < CH; ++half) {
             const int nslab = half + 1 < CH ? s : s + 1, nhalf = half + 1 < CH ? half + 1 : 0;
 #pragma unroll
             for (int ks = 0; ks < KH; ++ks) {
-                const double x = X[from][c16 * LDX + (half * KH + ks) * 4 + g];
+                // weights two steps ahead, products, reloads: in this order (left to itself the compiler moves the reloads behind the
+                // last product, where the next slab waits for them)
+                if (half * KH + ks + 2 < KH * CH) read(from, half * KH + ks + 2, x[(half * KH + ks + 2) % 3]);
 #pragma unroll
-                for (int c = 0; c < CT; ++c) {
-                    acc[c] = __builtin_amdgcn_mfma_f64_16x16x4f64(x, frag[ks][c], acc[c], 0, 0, 0);
-                    load(nslab, nhalf, ks, c);
-                }
+                for (int c = 0; c < CT; ++c)
+#pragma unroll
+                    for (int h = 0; h < RB; ++h) acc[h][c] = __builtin_amdgcn_mfma_f64_16x16x4f64(x[(half * KH + ks) % 3][h], frag[ks][c], acc[h][c], 0, 0, 0);
+#pragma unroll
+                for (int c = 0; c < CT; ++c) load(nslab, nhalf, ks, c);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
-        double f[4];
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            double m = top[from][0][g + 4 * r];
-#pragma unroll
-            for (int w = 1; w < W; ++w) m = fmax(m, top[from][w][g + 4 * r]);
-            const int e = trellis_exponent(m);
-            e4[r] += e;
-            f[r] = trellis_pow2(-e);
-            m4[r] = 0.0;
-        }
-#pragma unroll
-        for (int c = 0; c < CT; ++c)
+        for (int h = 0; h < RB; ++h)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const double x = (acc[c][r] * f[r]) * lw[c];
-                if (col[c] < Kp) X[to][(g + 4 * r) * LDX + col[c]] = x;
-                m4[r] = fmax(m4[r], x);
-                small |= x > 0.0 && x < SNK_WEIGHT_LEAST;
+                const int row = 16 * h + g + 4 * r, e = row_exponent(from, row);
+                const double f = trellis_pow2(-e);
+                e4[h][r] += e;
+                most[h][r] = 0.0;
+#pragma unroll
+                for (int c = 0; c < CT; ++c) {
+                    const double x = (acc[h][c][r] * f) * lw[c];
+                    if (col[c] < Kp) X[to][row * LDX + col[c]] = x;
+                    most[h][r] = fmax(most[h][r], x);
+                    small |= x > 0.0 && x < SNK_WEIGHT_LEAST;
+                }
             }
         row_max(to);
         __syncthreads();
@@ -473,32 +500,32 @@ trellis_product_kernel(const TrellisView v, const double *__restrict__ local, in
     // out: rows scaled to [1, 2), their exponents beside them
     const int at = (p.n - 1) & 1;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        const int row = g + 4 * r, i = i0 + row;
-        double m = top[at][0][row];
+    for (int h = 0; h < RB; ++h)
 #pragma unroll
-        for (int w = 1; w < W; ++w) m = fmax(m, top[at][w][row]);
-        const int e = trellis_exponent(m);
-        const double f = trellis_pow2(-e);
-        if (i < K) {
+        for (int r = 0; r < 4; ++r) {
+            const int row = 16 * h + g + 4 * r, i = i0 + row, e = row_exponent(at, row);
+            const double f = trellis_pow2(-e);
+            if (i < K) {
 #pragma unroll
-            for (int c = 0; c < CT; ++c)
-                if (col[c] < Kp) M[(p.at * K + i) * Kp + col[c]] = X[at][row * LDX + col[c]] * f;
-            if (wave == 0 && c16 == 0) exps[p.at * K + i] = e4[r] + e;
+                for (int c = 0; c < CT; ++c)
+                    if (col[c] < Kp) M[(p.at * K + i) * Kp + col[c]] = X[at][row * LDX + col[c]] * f;
+                if (wave == 0 && c16 == 0) exps[p.at * K + i] = e4[h][r] + e;
+            }
         }
-    }
 }
 
-// 2. the weights at the pieces' ends: a workgroup per utterance.  Forward: thread = (pair of columns, every PARTS-th row), backward:
-// Q threads a row, (row, every Q-th pair of columns).  A thread's cells come in H parts of R; each is reloaded with the next part's
-// right after its use.
-template <int R, int H, int Q>
-__global__ void __launch_bounds__(1024)
+// 2. the weights at the pieces' ends: a workgroup per utterance; what a step waits for is what it costs (two barriers, no sum in a row).
+// Forward: a wavefront owns 32 columns, CW of them side by side, RG such groups and the four rows of lanes in each split the rows.
+// Backward: Q threads a row.  A thread's cells come in H parts of R; each is reloaded with the next part's right after its use.  Every
+// wavefront keeps the weights of all candidates, S a lane, and scales them itself.
+template <int R, int H, int CW, int RG, int Q, int S, int NTH>
+__global__ void __launch_bounds__(NTH)
 trellis_ends_kernel(const TrellisView v, const double *__restrict__ local, const double *__restrict__ M, const int *__restrict__ exps,
                     int *__restrict__ flag, double *__restrict__ ends_out, int64_t *__restrict__ scaled_out)
 {
     constexpr bool BACK = Q > 0;
-    __shared__ double vec[256], part[2048], red[16];
+    constexpr int PARTS = BACK ? 1 : RG, STEP = BACK ? 2 * Q : 4 * RG;   // columns / rows between a thread's cells
+    __shared__ __align__(16) double vec[256], part[PARTS][256];
     __shared__ int bad;
     const TrellisPiece p = trellis_piece(v, blockIdx.x, 0);
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, K = v.K, Kp = v.Kp;
@@ -508,50 +535,80 @@ trellis_ends_kernel(const TrellisView v, const double *__restrict__ local, const
     const int *__restrict__ e0 = exps + p.at * K;
     double *__restrict__ ends = ends_out + p.at * Kp;
     if (tid == 0) bad = 0;
-    const int pairs = Kp >> 1, parts = 1024 / pairs;
-    const int b = BACK ? 2 * (tid % (BACK ? Q : 1)) : 2 * (tid % pairs), a = BACK ? tid / (BACK ? Q : 1) : tid / pairs;
-    const bool on = BACK ? a < K : a < parts;
+    const int group = BACK ? 0 : wave / (CW ? CW : 1);
+    const int b = BACK ? 2 * (tid % (BACK ? Q : 1)) : (wave % (CW ? CW : 1)) * 32 + 2 * (lane & 15), a = BACK ? tid / (BACK ? Q : 1) : group * 4 + (lane >> 4);
+    const bool on = BACK ? a < K : b < Kp && group < RG;
+    const int off = on ? (a * Kp + b) * 8 : 0x7ff00000;
     const int steps = p.P - 1, pieces = steps * H;
     f64x2 m[R];
     auto load = [&](int piece, int i) {                         // (rows beyond K and columns beyond Kp read as 0 or meet a weight of 0)
         piece = piece < pieces ? piece : pieces - 1;
         const int k = BACK ? p.P - 1 - piece / H : piece / H, n = (piece % H) * R + i;
         const __amdgpu_buffer_rsrc_t res = __builtin_amdgcn_make_buffer_rsrc(const_cast<double *>(m0 + (int64_t)k * K * Kp), 0, bytes, 0x00020000);
-        const int off = on ? (a * Kp + b) * 8 : 0x7ff00000;
-        const int more = min(BACK ? n * Q * 16 : n * parts * Kp * 8, bytes);
+        const int more = min(BACK ? n * STEP * 8 : n * STEP * Kp * 8, bytes);
         m[i] = __builtin_bit_cast(f64x2, __builtin_amdgcn_raw_buffer_load_b128(res, off, more, 0));
     };
-    double x = 0.0;                                             // weight of candidate tid
-    if (tid < Kp) {
-        x = BACK ? (tid < K ? 1.0 : 0.0) : local[p.r0 * Kp + tid];
-        ends[(int64_t)(BACK ? p.P - 1 : 0) * Kp + tid] = x;
+    double x[S];                                                // weights of candidates lane, lane + 64 ..
+    int e_next[S];
+    auto store = [&](int64_t k) {
+        if (wave == 0)
+#pragma unroll
+            for (int i = 0; i < S; ++i)
+                if (lane + 64 * i < Kp) ends[k * Kp + lane + 64 * i] = x[i];
+    };
+    auto exponents = [&](int s) {                               // (a step ahead, like the cells)
+        s = s < steps ? s : steps - 1;
+#pragma unroll
+        for (int i = 0; i < S; ++i) e_next[i] = s >= 0 && lane + 64 * i < K ? e0[(int64_t)(BACK ? p.P - 1 - s : s) * K + lane + 64 * i] : 0;
+    };
+#pragma unroll
+    for (int i = 0; i < S; ++i) {
+        const int c = lane + 64 * i;
+        x[i] = BACK ? (c < K ? 1.0 : 0.0) : c < Kp ? local[p.r0 * Kp + c] : 0.0;
     }
+    store(BACK ? p.P - 1 : 0);
+    if (tid < 256)
+        for (int i = 0; i < PARTS; ++i) part[i][tid] = 0.0;
     if (tid < 256) vec[tid] = 0.0;
     if (pieces > 0) {
 #pragma unroll
         for (int i = 0; i < R; ++i) load(0, i);
     }
+    exponents(0);
+    __syncthreads();
     int64_t scaled = 0;
     bool small = false;
-    // scales the candidates' weights y 2^e to at most 2: forward the exponents belong to what goes into a product, backward to what comes out
-    auto scale = [&](double y, int e) -> double {
-        const double t = wave_max(y > 0.0 ? (double)(e + trellis_exponent(y)) : -1e30);
-        if (lane == 0) red[wave] = t;
-        __syncthreads();
-        double most = red[0];
-        for (int i = 1; i < (Kp + 63) >> 6; ++i) most = fmax(most, red[i]);
-        if (!(most > -1e29)) return 0.0;
+    // scales the weights x 2^e to at most 2: forward the exponents belong to what goes into a product, backward to what comes out
+    auto scale = [&](const int (&e)[S]) {
+        int t[S];
+        double most = -1e30;
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            t[i] = e[i] + trellis_exponent(x[i]);
+            if (x[i] > 0.0) most = fmax(most, (double)t[i]);
+        }
+        most = wave_max(most);
+        if (!(most > -1e29)) return;                            // (nothing left: all are 0)
         scaled += (int64_t)most;
-        if (!(y > 0.0)) return 0.0;
-        const int have = trellis_exponent(y), d = have + e - (int)most;
-        if (d < -489) { small = true; return 0.0; }
-        return y * trellis_pow2(-have) * trellis_pow2(d);       // (y in [1, 2), then scaled down)
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            const int d = t[i] - (int)most;
+            const bool lost = x[i] > 0.0 && d < -489;
+            small |= lost;
+            x[i] = x[i] > 0.0 && !lost ? x[i] * trellis_pow2(-trellis_exponent(x[i])) * trellis_pow2(d) : 0.0;      // (to [1, 2), then down)
+        }
     };
     for (int s = 0; s < steps; ++s) {
         const int k = BACK ? p.P - 1 - s : s;
-        const int e = tid < K ? e0[(int64_t)k * K + tid] : 0;
-        if (!BACK) x = scale(x, e);
-        if (tid < Kp) vec[tid] = x;
+        int e[S];
+#pragma unroll
+        for (int i = 0; i < S; ++i) e[i] = e_next[i];
+        exponents(s + 1);
+        if (!BACK) scale(e);
+        if (wave == 0)
+#pragma unroll
+            for (int i = 0; i < S; ++i)
+                if (lane + 64 * i < Kp) vec[lane + 64 * i] = x[i];
         __syncthreads();
         f64x2 sum = {0.0, 0.0};
 #pragma unroll
@@ -560,29 +617,35 @@ trellis_ends_kernel(const TrellisView v, const double *__restrict__ local, const
             for (int i = 0; i < R; ++i) {
                 const int n = h * R + i;
                 if (BACK) {
-                    const int c = min(b + n * 2 * Q, 254);
-                    sum[0] = __fma_rn(vec[c], m[i][0], sum[0]);
-                    sum[1] = __fma_rn(vec[c + 1], m[i][1], sum[1]);
+                    const f64x2 w = *reinterpret_cast<const f64x2 *>(&vec[min(b + n * STEP, 254)]);
+                    sum[0] = __fma_rn(w[0], m[i][0], sum[0]);
+                    sum[1] = __fma_rn(w[1], m[i][1], sum[1]);
                 } else {
-                    const double w = vec[min(a + n * parts, 255)];
+                    const double w = vec[min(a + n * STEP, 255)];
                     sum[0] = __fma_rn(w, m[i][0], sum[0]);
                     sum[1] = __fma_rn(w, m[i][1], sum[1]);
                 }
                 load(s * H + h + 1, i);
+                if (H == 1 && (i & 1)) __builtin_amdgcn_sched_barrier(0);      // (the reloads stay beside the products)
             }
         if (BACK) {
-            double y = sum[0] + sum[1];
-#pragma unroll
-            for (int o = 1; o < Q; o <<= 1) y += __shfl_xor(y, o, 64);
-            if (on && b == 0) part[a] = y;
-        } else if (on) { part[a * Kp + b] = sum[0]; part[a * Kp + b + 1] = sum[1]; }
-        __syncthreads();
-        if (BACK) x = scale(tid < K ? part[tid] : 0.0, e);
-        else if (tid < Kp) {
-            x = 0.0;
-            for (int i = 0; i < parts; ++i) x += part[i * Kp + tid];
+            double y = quad_sum(sum[0] + sum[1]);
+            if (Q == 8) y = eight_sum(y);
+            if (on && b == 0) part[0][a] = y;
+        } else {
+            sum[0] = rows4_sum(sum[0]);
+            sum[1] = rows4_sum(sum[1]);
+            if (on && lane < 16) *reinterpret_cast<f64x2 *>(&part[group][b]) = sum;
         }
-        if (tid < Kp) ends[(int64_t)(BACK ? k - 1 : k + 1) * Kp + tid] = x;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < S; ++i) {
+            x[i] = part[0][lane + 64 * i];
+#pragma unroll
+            for (int g = 1; g < PARTS; ++g) x[i] += part[g][lane + 64 * i];
+        }
+        if (BACK) scale(e);
+        store(BACK ? k - 1 : k + 1);
     }
     if (small) bad = 1;
     __syncthreads();
@@ -672,12 +735,22 @@ trellis_forward_kernel(const TrellisView v, const double *__restrict__ local, co
             for (int ch = 0; ch < CH; ++ch) {
                 f64x2(&c)[KPM] = cell[(s * CH + ch) % NB];
                 const double *w = &cur[from][rows * R + ch * KPM];
+                double x[KPM];
 #pragma unroll
-                for (int i = 0; i < KPM; ++i) {
-                    sum[0] = __fma_rn(w[i], c[i][0], sum[0]);
-                    sum[1] = __fma_rn(w[i], c[i][1], sum[1]);
+                for (int i = 0; i < KPM; ++i) x[i] = w[i];
+                f64x2 more = {0.0, 0.0};
+#pragma unroll
+                for (int i = 0; i < KPM; i += 2) {              // (the reloads stay beside the products: see trellis_product_kernel)
+                    sum[0] = __fma_rn(x[i], c[i][0], sum[0]);
+                    sum[1] = __fma_rn(x[i], c[i][1], sum[1]);
+                    more[0] = __fma_rn(x[i + 1], c[i + 1][0], more[0]);
+                    more[1] = __fma_rn(x[i + 1], c[i + 1][1], more[1]);
                     load((now - 1) * CH + ch + NB, i, c[i]);
+                    load((now - 1) * CH + ch + NB, i + 1, c[i + 1]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+                sum[0] += more[0];
+                sum[1] += more[1];
             }
             sum[0] = rows4_sum(sum[0]);
             sum[1] = rows4_sum(sum[1]);
@@ -797,6 +870,7 @@ trellis_backward_kernel(const TrellisView v, const double *__restrict__ local, c
                     sum[0] = __fma_rn(x[0], c[i][0], sum[0]);
                     sum[1] = __fma_rn(x[1], c[i][1], sum[1]);
                     load((k + s) * CH + ch + NB, i, c[i], voff[(ch + NB) % CH]);
+                    if (i & 1) __builtin_amdgcn_sched_barrier(0);      // (the reloads stay beside the products)
                 }
                 double y = sum[0] + sum[1];
                 y = quad_sum(y) * f;
@@ -1238,11 +1312,14 @@ void launch_trellis_local(const TrellisView &v, double *local, double *least, in
 }
 
 // The widest tile that a wavefront's registers hold is 7 x 2 tiles of 16 x 16 (two workgroups a compute unit): K is cut into as few
-// equal tiles of at most 112.
+// equal tiles of at most 112 -- of at most 64 where that would leave less than two rounds of workgroups (599 pairs of rows of 100
+// candidates, 302 columns: 214 us instead of 249).
 void launch_trellis_costs(const TrellisView &v, const TrellisCosts &c, bool logs, int *flag, double *X, hipStream_t s)
 {
     if (v.rows < 2) return;
-    const int n = (v.K + 111) / 112, rt = ((v.K + n - 1) / n + 15) / 16;
+    int n = (v.K + 111) / 112;
+    if (v.K > 64 && (v.rows - 1) * n * n < 1024) n = (v.K + 63) / 64;
+    const int rt = ((v.K + n - 1) / n + 15) / 16;
     const dim3 grid((unsigned)(v.rows - 1), n, n);
 #define SNK_COST(RT_, RM_, CM_)                                                                                              \
     do {                                                                                                                     \
@@ -1272,25 +1349,33 @@ void launch_trellis_ends(const TrellisView &v, const double *local, bool both, i
 {
     const int n = v.pieces;
     if (n == 1) return;
-    const int row_blocks = (v.K + 15) / 16;
-    const dim3 grid((unsigned)((((int64_t)n * v.n_utts + 7) / 8) * 8 * row_blocks));
-#define SNK_PROD(CT_, KH_, CH_, NTH_) hipLaunchKernelGGL((trellis_product_kernel<CT_, KH_, CH_, NTH_>), grid, dim3(NTH_), 0, s, v, local, n, row_blocks, !both, flag, M, exps)
+    // (two workgroups a compute unit: beyond two rounds of them the larger row blocks, where the registers hold them)
+    const int64_t all = (((int64_t)n * v.n_utts + 7) / 8) * 8;
+    const int rb = v.K <= 128 && all * ((v.K + 15) / 16) >= 1024 ? 2 : 1, row_blocks = (v.K + 16 * rb - 1) / (16 * rb);
+    const dim3 grid((unsigned)(all * row_blocks));
+#define SNK_PROD(CT_, KH_, CH_, NTH_)                                                                                                             \
+    do {                                                                                                                                          \
+        if (rb == 2) hipLaunchKernelGGL((trellis_product_kernel<CT_, KH_, CH_, CH_ == 1 ? 2 : 1, NTH_>), grid, dim3(NTH_), 0, s, v, local, n, row_blocks, !both, flag, M, exps); \
+        else hipLaunchKernelGGL((trellis_product_kernel<CT_, KH_, CH_, 1, NTH_>), grid, dim3(NTH_), 0, s, v, local, n, row_blocks, !both, flag, M, exps);         \
+    } while (0)
     if (v.K <= 32) SNK_PROD(1, 8, 1, 128);
     else if (v.K <= 64) SNK_PROD(1, 16, 1, 256);
     else if (v.K <= 104) SNK_PROD(2, 26, 1, 256);
     else if (v.K <= 128) SNK_PROD(2, 32, 1, 256);
     else SNK_PROD(2, 26, 2, 448);
 #undef SNK_PROD
-#define SNK_ENDS(R_, H_, RB_, HB_, Q_)                                                                                                                    \
+#define SNK_ENDS(R_, H_, CW_, RG_, RB_, HB_, Q_, S_, NTH_)                                                                                           \
     do {                                                                                                                                              \
-        hipLaunchKernelGGL((trellis_ends_kernel<R_, H_, 0>), dim3(v.n_utts), dim3(1024), 0, s, v, local, M, exps, flag, ends_v, scaled);              \
-        if (both) hipLaunchKernelGGL((trellis_ends_kernel<RB_, HB_, Q_>), dim3(v.n_utts), dim3(1024), 0, s, v, local, M, exps, flag, ends_w, scaled); \
+        hipLaunchKernelGGL((trellis_ends_kernel<R_, H_, CW_, RG_, 0, S_, NTH_>), dim3(v.n_utts), dim3(NTH_), 0, s, v, local, M, exps, flag, ends_v, scaled);  \
+        if (both)                                                                                                                                     \
+            hipLaunchKernelGGL((trellis_ends_kernel<RB_, HB_, 0, 0, Q_, S_, 32 * ((Q_ == 8 ? 4 : 8) * Q_)>), dim3(v.n_utts), dim3(32 * ((Q_ == 8 ? 4 : 8) * Q_)), 0, s, v, local, M, \
+                               exps, flag, ends_w, scaled);                                                                                           \
     } while (0)
-    if (v.K <= 32) SNK_ENDS(1, 1, 2, 1, 8);
-    else if (v.K <= 64) SNK_ENDS(2, 1, 4, 1, 8);
-    else if (v.K <= 104) SNK_ENDS(6, 1, 7, 1, 8);
-    else if (v.K <= 128) SNK_ENDS(8, 1, 8, 1, 8);
-    else SNK_ENDS(8, 3, 13, 2, 4);
+    if (v.K <= 32) SNK_ENDS(2, 1, 1, 4, 2, 1, 8, 1, 256);
+    else if (v.K <= 64) SNK_ENDS(4, 1, 2, 4, 4, 1, 8, 1, 512);
+    else if (v.K <= 104) SNK_ENDS(7, 1, 4, 4, 7, 1, 8, 2, 1024);
+    else if (v.K <= 128) SNK_ENDS(8, 1, 4, 4, 8, 1, 8, 2, 1024);
+    else SNK_ENDS(13, 2, 7, 2, 13, 2, 4, 4, 896);
 #undef SNK_ENDS
 }
 
