@@ -273,6 +273,11 @@ sample_rows_block_kernel(const T *__restrict__ scores, int64_t stride, int64_t V
     for (int d = 0; d < n_draws; ++d) {
         const u64 t = sample_exceed(u[r * n_draws + d], total);
         // the tile: the first wavefront walks the tiles' sums
+        if (tid == 0) {
+            sh_digit = 0xffffffffu;
+            index[r * n_draws + d] = -1;
+            if (logp) logp[r * n_draws + d] = ninf;
+        }
         if (tid < 64) {
             u64 mass0 = 0, ties0 = 0;
             for (int64_t b = 0; b < n_tiles; b += 64) {
@@ -288,6 +293,7 @@ sample_rows_block_kernel(const T *__restrict__ scores, int64_t stride, int64_t V
             }
         }
         __syncthreads();
+        if (sh_digit == 0xffffffffu) { __syncthreads(); continue; }      // (only where the scores changed under the call)
         const int64_t base = (int64_t)sh_digit * TILE + (int64_t)tid * SNK_SAMPLE_VEC;
         const u64 mass0 = sh_a, ties0 = sh_b;
         u64 w[SNK_SAMPLE_VEC]; unsigned int q[SNK_SAMPLE_VEC];
@@ -335,7 +341,7 @@ struct RowState {
     double m, bin_scale;        // largest score, bins per unit of exponent
     double cut;                 // kept: above the cut, and the first n_tie equal to it
     u64 n_tie, total;           // total: mass of what the goals so far keep
-    u64 above, key_min, key_max;
+    u64 above;
     unsigned int listed, want_bin;
     int all, pad;
     u64 want;
@@ -363,35 +369,42 @@ __device__ __forceinline__ void chunk_scores(const T *__restrict__ p, int64_t lo
     const int skip = (int)(((16 - ((uintptr_t)(p + lo) & 15)) & 15) / sizeof(T));
     const int64_t a = lo + skip < hi ? lo + skip : hi, n = (hi - a) / VEC, b = a + n * VEC;
     if (lo + tid < a) f(score_load(p + lo + tid), lo + tid);
-    for (int64_t i = tid; i < n; i += NT) {
-        union { uint4 q; T v[VEC]; } u;
-        u.q = *reinterpret_cast<const uint4 *>(p + a + i * VEC);
+    // four loads in flight: what f does with a score can keep the next load from being moved ahead of it
+    for (int64_t i = tid; i < n; i += 4 * NT) {
+        union { uint4 q; T v[VEC]; } u[4];
 #pragma unroll
-        for (int j = 0; j < VEC; ++j) f(score_bits(u.v, j), a + i * VEC + j);
+        for (int k = 0; k < 4; ++k)
+            if (i + k * NT < n) u[k].q = *reinterpret_cast<const uint4 *>(p + a + (i + k * NT) * VEC);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (i + k * NT < n) {
+#pragma unroll
+                for (int j = 0; j < VEC; ++j) f(score_bits(u[k].v, j), a + (i + k * NT) * VEC + j);
+            }
     }
     if (b + tid < hi) f(score_load(p + b + tid), b + tid);
 }
 
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(512)
 rows_extremes_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, const RowsWork w)
 {
-    __shared__ double hi[4], lo[4];
+    __shared__ double hi[8], lo[8];
     const int64_t r = blockIdx.y, c = blockIdx.x;
     const int tid = threadIdx.x;
     const double inf = __builtin_inf();
     if (c == 0) {
-        for (int i = tid; i < w.bins; i += 256) { w.hist_mass[r * w.bins + i] = 0; w.hist_count[r * w.bins + i] = 0; }
+        for (int i = tid; i < w.bins; i += 512) { w.hist_mass[r * w.bins + i] = 0; w.hist_count[r * w.bins + i] = 0; }
         if (tid == 0) {
             RowState s;
-            s.m = -inf; s.bin_scale = 0.0; s.cut = -inf; s.n_tie = 0; s.total = 0; s.above = 0; s.key_min = ~0ull; s.key_max = 0;
+            s.m = -inf; s.bin_scale = 0.0; s.cut = -inf; s.n_tie = 0; s.total = 0; s.above = 0;
             s.listed = 0; s.want_bin = 0; s.all = 1; s.pad = 0; s.want = 0;
             w.state[r] = s;
             w.left[r] = 0;
         }
     }
     double m = -inf, n = inf;
-    chunk_scores<T, 256>(scores + r * stride, c * SNK_CHUNK, min((c + 1) * SNK_CHUNK, V), [&](double x, int64_t) {
+    chunk_scores<T, 512>(scores + r * stride, c * SNK_CHUNK, min((c + 1) * SNK_CHUNK, V), [&](double x, int64_t) {
         m = fmax(m, x);
         n = x > -inf ? fmin(n, x) : n;
     });
@@ -400,8 +413,9 @@ rows_extremes_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, co
     if ((tid & 63) == 0) { hi[tid >> 6] = m; lo[tid >> 6] = n; }
     __syncthreads();
     if (tid == 0) {
-        w.chunk_max[r * w.chunks + c] = fmax(fmax(hi[0], hi[1]), fmax(hi[2], hi[3]));
-        w.chunk_min[r * w.chunks + c] = fmin(fmin(lo[0], lo[1]), fmin(lo[2], lo[3]));
+        for (int i = 1; i < 8; ++i) { hi[0] = fmax(hi[0], hi[i]); lo[0] = fmin(lo[0], lo[i]); }
+        w.chunk_max[r * w.chunks + c] = hi[0];
+        w.chunk_min[r * w.chunks + c] = lo[0];
     }
 }
 
@@ -451,13 +465,16 @@ rows_histogram_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, S
 
 // by_mass 0: the top_k-th score; 1: where top_p of the mass kept so far is reached
 template <typename T>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(512)
 rows_boundary_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, SampleRule call, const double *__restrict__ rules, double unit, int by_mass,
                      const RowsWork w)
 {
-    __shared__ u64 sums[256], counts[256];
-    __shared__ u64 above_s, total_s;
+    constexpr int PER = SNK_BINS_MOST / 256;
+    constexpr unsigned int HITS = 2048;
+    __shared__ BlockScratch<512> scratch;
     __shared__ int bin_s;
+    __shared__ double hit[HITS], ends[16];
+    __shared__ unsigned int n_hit, place;
     const int64_t r = blockIdx.y, c = blockIdx.x;
     const int tid = threadIdx.x;
     const SampleRule rule = sample_rule(call, rules, r);
@@ -467,48 +484,82 @@ rows_boundary_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, Sa
     if (by_mass ? !(rule.top_p < 1.0) : !(rule.top_k > 0 && rule.top_k < V)) return;
     const u64 *__restrict__ mass = w.hist_mass + r * w.bins;
     const unsigned int *__restrict__ count = w.hist_count + r * w.bins;
+    // every workgroup finds the bin for itself: a thread sums its neighbouring bins, the sums are scanned, the bin is in one thread's
     const int per = w.bins >> 8;
-    u64 sm = 0, sc = 0;
-    for (int i = 0; i < per; ++i) { sm += mass[tid * per + i]; sc += count[tid * per + i]; }
-    sums[tid] = sm; counts[tid] = sc;
-    __syncthreads();
-    if (tid == 0) {
-        u64 tm = 0;
-        for (int i = 0; i < 256; ++i) tm += sums[i];
-        const u64 total = st->all ? tm : st->total;
-        const u64 want = by_mass ? sample_reach(rule.top_p, total) : (u64)rule.top_k;
-        const u64 *v = by_mass ? sums : counts;
-        u64 a = 0;
-        int bin = -1;
-        for (int i = 0; i < 256 && bin < 0; ++i) {
-            if (a + v[i] < want) { a += v[i]; continue; }
-            for (int j = i * per;; ++j) {
-                const u64 n = by_mass ? mass[j] : (u64)count[j];
-                if (a + n >= want) { bin = j; break; }
-                a += n;
+    u64 vm[PER], sm = 0, sc = 0;
+    unsigned int vc[PER];
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+        vm[i] = tid < 256 && i < per ? mass[tid * per + i] : 0;
+        vc[i] = tid < 256 && i < per ? count[tid * per + i] : 0;
+        sm += vm[i]; sc += vc[i];
+    }
+    if (tid == 0) bin_s = -1;
+    u64 um = sm, uc = sc, total_m, total_c;
+    block_scan2<512>(um, uc, total_m, total_c, scratch);
+    const u64 want = by_mass ? sample_reach(rule.top_p, st->all ? total_m : st->total) : (u64)rule.top_k;
+    const u64 upto = by_mass ? um : uc;
+    u64 a = upto - (by_mass ? sm : sc);
+    if (a < want && upto >= want) {
+        bool found = false;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+            const u64 n = by_mass ? vm[i] : vc[i];
+            if (!found && a + n >= want) {
+                found = true;
+                bin_s = tid * per + i;
+                if (c == 0) { st->want = want; st->above = a; st->want_bin = (unsigned int)(tid * per + i); }
             }
+            a += n;
         }
-        bin_s = bin; above_s = a; total_s = tm;
-        if (c == 0) { st->want = want; st->above = a; st->want_bin = (unsigned int)bin; if (bin < 0) st->total = tm; }
     }
     __syncthreads();
     const int bin = bin_s;
-    if (bin < 0) return;                                        // fewer scores than the goal: all are kept
-    chunk_scores<T, 256>(scores + r * stride, c * SNK_CHUNK, min((c + 1) * SNK_CHUNK, V), [&](double x, int64_t i) {
-        if (x == ninf) return;
+    if (bin < 0) {                                              // fewer scores than the goal: all are kept
+        if (c == 0 && tid == 0) { st->want_bin = (unsigned int)-1; st->total = total_m; }
+        return;
+    }
+    // the bin's scores by way of LDS: one place in the row's list is asked for by a workgroup, not one a score (atomics on one address
+    // from all XCDs take tens of nanoseconds each)
+    if (tid == 0) n_hit = 0;
+    __syncthreads();
+    const int64_t lo = c * SNK_CHUNK, hi = min((c + 1) * SNK_CHUNK, V);
+    auto of_bin = [&](double x) -> bool {
+        if (x == ninf) return false;
         const double e = sample_exponent(x, m, rule.inv_tau);
-        if (e < SNK_SAMPLE_FLOOR || score_bin(e, scale, w.bins) != bin || !sample_weight(e, unit)) return;
-        // (a bin of thousands of equal scores: one count a wavefront, no further extremes)
-        const u64 key = score_key<double>(x);
-        if (key < *(volatile u64 *)&st->key_min) atomicMin(&st->key_min, key);
-        if (key > *(volatile u64 *)&st->key_max) atomicMax(&st->key_max, key);
-        const u64 here = __ballot(1);
-        const int lead = __ffsll((long long)here) - 1, lane = tid & 63;
-        unsigned int at = 0;
-        if (lane == lead) at = atomicAdd(&st->listed, (unsigned int)__popcll(here));
-        at = __shfl(at, lead, 64) + (unsigned int)__popcll(here & ((1ull << lane) - 1));
-        if (at < w.list) w.list_x[r * w.list + at] = x;
+        return e >= SNK_SAMPLE_FLOOR && score_bin(e, scale, w.bins) == bin && sample_weight(e, unit) != 0;
+    };
+    double most = ninf, least = -ninf;
+    chunk_scores<T, 512>(scores + r * stride, lo, hi, [&](double x, int64_t) {
+        if (!of_bin(x)) return;
+        most = fmax(most, x);
+        least = fmin(least, x);
+        const unsigned int at = atomicAdd(&n_hit, 1u);
+        if (at < HITS) hit[at] = x;
     });
+    most = wave_max(most);
+    least = -wave_max(-least);
+    if ((tid & 63) == 0) { ends[tid >> 6] = most; ends[8 + (tid >> 6)] = least; }
+    __syncthreads();
+    const unsigned int n = n_hit;
+    if (tid == 0) {
+        for (int i = 1; i < 8; ++i) { most = fmax(most, ends[i]); least = fmin(least, ends[8 + i]); }
+        w.chunk_max[r * w.chunks + c] = most;
+        w.chunk_min[r * w.chunks + c] = least;
+        place = n ? atomicAdd(&st->listed, n) : 0;
+        n_hit = 0;
+    }
+    __syncthreads();
+    const unsigned int base = place;
+    if (n <= HITS) {
+        for (unsigned int i = tid; i < n; i += 512)
+            if (base + i < w.list) w.list_x[r * w.list + base + i] = hit[i];
+    } else
+        chunk_scores<T, 512>(scores + r * stride, lo, hi, [&](double x, int64_t) {
+            if (!of_bin(x)) return;
+            const unsigned int at = base + atomicAdd(&n_hit, 1u);
+            if (at < w.list) w.list_x[r * w.list + at] = x;
+        });
 }
 
 __global__ void __launch_bounds__(1024)
@@ -518,6 +569,7 @@ rows_select_kernel(int64_t V, SampleRule call, const double *__restrict__ rules,
     __shared__ u64 sh_above;
     __shared__ unsigned int sh_digit;
     __shared__ u64 red[16];
+    __shared__ double ends[32];
     const int64_t r = blockIdx.x;
     const int tid = threadIdx.x;
     const SampleRule rule = sample_rule(call, rules, r);
@@ -528,17 +580,26 @@ rows_select_kernel(int64_t V, SampleRule call, const double *__restrict__ rules,
     if ((int)st->want_bin < 0) return;
     const unsigned int n = st->listed;
     const u64 want = st->want;
-    u64 above = st->above, key = st->key_min;
+    double most = -__builtin_inf(), least = __builtin_inf();    // of the bin's scores
+    for (int i = tid; i < w.chunks; i += 1024) { most = fmax(most, w.chunk_max[r * w.chunks + i]); least = fmin(least, w.chunk_min[r * w.chunks + i]); }
+    most = wave_max(most);
+    least = -wave_max(-least);
+    if ((tid & 63) == 0) { ends[tid >> 6] = most; ends[16 + (tid >> 6)] = least; }
+    __syncthreads();
+    for (int i = 0; i < 16; ++i) { most = fmax(most, ends[i]); least = fmin(least, ends[16 + i]); }
+    const u64 key_min = score_key<double>(least), key_max = score_key<double>(most);
+    u64 above = st->above, key = key_min;
     u64 ties = n, each = 0;                                     // of the cut's own scores
-    if (st->key_min != st->key_max) {
+    if (key_min != key_max) {
         if (n > w.list) { if (tid == 0) w.left[r] = 1; return; }
         u64 prefix = 0;
         // (keys that differ share their leading bits: start at the first digit in which they do)
-        int top = 63 - __clzll((long long)(st->key_min ^ st->key_max));
+        int top = 63 - __clzll((long long)(key_min ^ key_max));
         top = (top >> 3) << 3;
         prefix = top + 8 < 64 ? (key >> (top + 8)) << (top + 8) : 0;
         for (int shift = top; shift >= 0; shift -= 8) {
             if (tid < 256) { hist_mass[tid] = 0; hist_count[tid] = 0; }
+            if (tid == 0) { sh_digit = 0; sh_above = above; }
             __syncthreads();
             for (unsigned int i = tid; i < n; i += 1024) {
                 const double x = w.list_x[r * w.list + i];
@@ -573,12 +634,12 @@ rows_select_kernel(int64_t V, SampleRule call, const double *__restrict__ rules,
     // the cut's value back from its key
     const double cut = __longlong_as_double((long long)((key >> 63) ? key & 0x7fffffffffffffffull : ~key));
     each = sample_weight(sample_exponent(cut, m, rule.inv_tau), unit);
-    const u64 n_tie = by_mass ? (want - above + each - 1) / each : want - above;
+    const u64 n_tie = by_mass ? (each ? (want - above + each - 1) / each : 0) : want - above;
     // the mass above the cut: whole bins, and the list's scores above it
     u64 mass = 0;
     const int bin = (int)st->want_bin;
     for (int i = tid; i < bin; i += 1024) mass += w.hist_mass[r * w.bins + i];
-    if (st->key_min != st->key_max)
+    if (key_min != key_max)
         for (unsigned int i = tid; i < n; i += 1024) {
             const double x = w.list_x[r * w.list + i];
             if (x > cut) mass += sample_weight(sample_exponent(x, m, rule.inv_tau), unit);
@@ -591,7 +652,7 @@ rows_select_kernel(int64_t V, SampleRule call, const double *__restrict__ rules,
         for (int i = 0; i < 16; ++i) t += red[i];
         st->cut = cut; st->n_tie = n_tie < ties ? n_tie : ties; st->all = 0;
         st->total = t + each * st->n_tie;
-        st->listed = 0; st->key_min = ~0ull; st->key_max = 0;
+        st->listed = 0;
     }
 }
 
@@ -636,14 +697,14 @@ rows_masses_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, Samp
 
 template <typename T>
 __global__ void __launch_bounds__(1024)
-rows_draw_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, const double *__restrict__ u, int n_draws, SampleRule call,
+rows_draw_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, const double *__restrict__ u, int n_draws, int draw0, SampleRule call,
                  const double *__restrict__ rules, double unit, const RowsWork w, int64_t *__restrict__ index, double *__restrict__ logp)
 {
     constexpr int EACH = SNK_CHUNK / 1024;
     __shared__ BlockScratch<1024> scratch;
     __shared__ u64 sh_mass, sh_ties;
     __shared__ int sh_chunk;
-    const int64_t r = blockIdx.x, at = r * n_draws + blockIdx.y;
+    const int64_t r = blockIdx.x, at = r * n_draws + draw0 + blockIdx.y;
     const int tid = threadIdx.x;
     const RowState st = w.state[r];
     if (w.left[r]) return;
@@ -666,6 +727,8 @@ rows_draw_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, const 
     const u64 total = total_m + each * (total_t < n_tie ? total_t : n_tie);
     const u64 t = sample_exceed(u[at], total);
     u64 am = cm - mass, an = ct - ties;
+    if (tid == 0) { sh_chunk = -1; index[at] = -1; if (logp) logp[at] = -__builtin_inf(); }
+    __syncthreads();
     for (int i = 0; i < per; ++i) {
         const int c = tid * per + i;
         if (c >= w.chunks) break;
@@ -676,6 +739,7 @@ rows_draw_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, const 
         if (lo <= t && t < hi) { sh_chunk = c; sh_mass = m0; sh_ties = t0; }
     }
     __syncthreads();
+    if (sh_chunk < 0) return;                                   // (only where the scores changed under the call: nothing is read beyond them)
     const T *__restrict__ p = scores + r * stride;
     const int64_t base = (int64_t)sh_chunk * SNK_CHUNK + tid * EACH;
     const u64 mass0 = sh_mass, ties0 = sh_ties;
@@ -742,15 +806,17 @@ static void launch_rows_split(const T *scores, int64_t stride, int64_t R, int64_
     w.list_x = (double *)take((size_t)R * w.list * 8);
     w.left = (int *)take(R * 4);
     const dim3 grid((unsigned)w.chunks, (unsigned)R);
-    hipLaunchKernelGGL((rows_extremes_kernel<T>), grid, dim3(256), 0, s, scores, stride, V, w);
+    hipLaunchKernelGGL((rows_extremes_kernel<T>), grid, dim3(512), 0, s, scores, stride, V, w);
     hipLaunchKernelGGL((rows_histogram_kernel<T>), grid, dim3(512), (size_t)w.bins * 12, s, scores, stride, V, rule, rules, unit, w);
     for (int by_mass = 0; by_mass < 2; ++by_mass) {
         if (!rules && (by_mass ? !(rule.top_p < 1.0) : !(rule.top_k > 0 && rule.top_k < V))) continue;
-        hipLaunchKernelGGL((rows_boundary_kernel<T>), grid, dim3(256), 0, s, scores, stride, V, rule, rules, unit, by_mass, w);
+        hipLaunchKernelGGL((rows_boundary_kernel<T>), grid, dim3(512), 0, s, scores, stride, V, rule, rules, unit, by_mass, w);
         hipLaunchKernelGGL(rows_select_kernel, dim3((unsigned)R), dim3(1024), 0, s, V, rule, rules, unit, by_mass, w);
     }
     hipLaunchKernelGGL((rows_masses_kernel<T>), grid, dim3(512), 0, s, scores, stride, V, rule, rules, unit, w);
-    hipLaunchKernelGGL((rows_draw_kernel<T>), dim3((unsigned)R, n_draws), dim3(1024), 0, s, scores, stride, V, u, n_draws, rule, rules, unit, w, index, logp);
+    for (int d = 0; d < n_draws; d += 32768)
+        hipLaunchKernelGGL((rows_draw_kernel<T>), dim3((unsigned)R, std::min(n_draws - d, 32768)), dim3(1024), 0, s, scores, stride, V, u, n_draws, d, rule,
+                           rules, unit, w, index, logp);
     hipLaunchKernelGGL((sample_rows_block_kernel<T, 1024>), dim3((unsigned)R), dim3(1024), 0, s, scores, stride, V, u, n_draws, rule, rules, unit, w.left,
                        index, logp);
 }
@@ -786,7 +852,9 @@ void launch_sample_rows(const void *scores, int dtype, int64_t stride, int64_t R
     k.top_k = rule.temperature > 0.0 ? rule.top_k : 1;
     k.top_p = rule.top_p;
     k.min_p = rule.min_p;
-    const int64_t step = work ? sample_rows_together(R, V) : R;
+    // a launch holds fewer than 2^32 threads, 64 a row or 1024
+    const int64_t most = V <= 1024 ? (int64_t)1 << 25 : (int64_t)1 << 21;
+    const int64_t step = std::min(work ? sample_rows_together(R, V) : R, most);
     const size_t width = dtype == 0 ? 8 : dtype == 1 ? 4 : 2;
     for (int64_t r = 0; r < R; r += step) {
         const int64_t n = R - r < step ? R - r : step;

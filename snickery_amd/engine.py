@@ -546,7 +546,7 @@ class HipSearchEngine(object):
         u (R,) or (R, draws): (index int64, log probability float64), both shaped like u.  temperature, top_k, top_p and min_p
         are numbers, or arrays of R for a rule per row."""
         rules = (temperature, top_k, top_p, min_p)
-        per_row = any(np.ndim(r) > 0 for r in rules)
+        per_row = any(not isinstance(r, (int, float)) and np.ndim(r) > 0 for r in rules)
         if getattr(scores, 'ndim', 0) != 2 or getattr(u, 'ndim', 0) not in (1, 2) or u.shape[0] != scores.shape[0]:
             raise SnkError('sample_rows: scores (R, V) and random numbers (R,) or (R, draws) expected')
         R, V = int(scores.shape[0]), int(scores.shape[1])
