@@ -169,6 +169,9 @@ int snk_set_position_bias(snk_handle h, const double *bias, int n_classes, int n
 }
 
 // ---- the trellis ------------------------------------------------------------------------------------------------------------------
+// a launch holds fewer than 2^32 threads, 256 a row; a group of utterances holds as many rows at most
+static const int64_t kTrellisMostRows = (int64_t)1 << 23;
+
 static int check_trellis(const char *who, snk_engine *h, const void *cand, const void *tdist, const int64_t *row_offsets, int n_utts, int K)
 {
     CHK(check_ready(h, false, true));
@@ -178,6 +181,8 @@ static int check_trellis(const char *who, snk_engine *h, const void *cand, const
     if (row_offsets[0] != 0) return fail("%s: row_offsets[0] must be 0 (got %lld)", who, (long long)row_offsets[0]);
     for (int v = 0; v < n_utts; ++v)
         if (row_offsets[v + 1] <= row_offsets[v]) return fail("%s: utterance %d has no rows", who, v);
+        else if (row_offsets[v + 1] - row_offsets[v] > kTrellisMostRows)
+            return fail("%s: utterance %d has %lld rows (at most %lld)", who, v, (long long)(row_offsets[v + 1] - row_offsets[v]), (long long)kTrellisMostRows);
     if (row_offsets[n_utts] > 0x7fffffff) return fail("%s: %lld rows", who, (long long)row_offsets[n_utts]);
     return 0;
 }
@@ -185,7 +190,23 @@ static int check_trellis(const char *who, snk_engine *h, const void *cand, const
 // Costs of the rows of as many utterances as fit the workspace, then `use` on them; group after group on the engine's stream.
 // 4 GB hold 53 000 rows of 100 candidates: larger groups would not fill the chip better, smaller ones would (a sentence alone
 // keeps a handful of compute units busy in the recursions).  An utterance that is longer than that is a group by itself.
+// (Launches over utterances times the pieces of the longest one: their product is bounded for the sake of short utterances beside a
+// very long one, which would otherwise meet mostly empty workgroups, and more of them than a launch holds.)
 static const size_t kTrellisGroupBytes = (size_t)4 << 30;
+static const int64_t kTrellisGroupUtts = 32768, kTrellisGroupPieces = 262144;
+
+static int trellis_group_end(const int64_t *off, int n_utts, int v0, size_t row_bytes)
+{
+    int64_t pieces = trellis_most_pieces(off + v0, 1);
+    int v1 = v0 + 1;
+    for (; v1 < n_utts && v1 - v0 < kTrellisGroupUtts; ++v1) {
+        const int64_t rows = off[v1 + 1] - off[v0];
+        if ((size_t)rows * row_bytes > kTrellisGroupBytes || rows > kTrellisMostRows) break;
+        pieces = std::max<int64_t>(pieces, trellis_most_pieces(off + v1, 1));
+        if (pieces * (v1 + 1 - v0) > kTrellisGroupPieces) break;
+    }
+    return v1;
+}
 
 struct TrellisCall {
     const char *who; bool timed;                    // stage timers (calls that wait for their results)
@@ -202,7 +223,13 @@ static int trellis_groups(snk_engine *h, const TrellisCall &q, Use use)
     const int Kp = roundup(q.K, 8);
     const size_t row_bytes = (size_t)q.K * Kp * sizeof(double);
     CHK(h->tr_off.ensure((size_t)(q.n_utts + 1) * sizeof(int64_t)));
-    CHK(h2d(h, h->tr_off.p, q.row_offsets, (size_t)(q.n_utts + 1) * sizeof(int64_t), h->stream));
+    // (by way of this frame: a queued copy straight out of a caller's pinned memory would still be read after a _dev call returned)
+    for (int v = 0; v <= q.n_utts; v += 2048) {
+        int64_t part[2048];
+        const size_t n = (size_t)std::min(q.n_utts + 1 - v, 2048) * sizeof(int64_t);
+        memcpy(part, q.row_offsets + v, n);
+        CHK(h2d(h, h->tr_off.as<int64_t>() + v, part, n, h->stream));
+    }
     CHK(h->tr_V.ensure((size_t)rows * Kp * sizeof(double)));
     CHK(h->tr_local.ensure((size_t)rows * Kp * sizeof(double)));
     CHK(h->tr_least.ensure((size_t)rows * sizeof(double)));
@@ -215,8 +242,7 @@ static int trellis_groups(snk_engine *h, const TrellisCall &q, Use use)
     c.n_classes = h->pb_classes; c.n_buckets = h->pb_buckets;
     c.bias_min = h->pb_classes > 0 ? h->pb_min : 0.0;
     for (int v0 = 0; v0 < q.n_utts;) {
-        int v1 = v0 + 1;
-        while (v1 < q.n_utts && (size_t)(q.row_offsets[v1 + 1] - q.row_offsets[v0]) * row_bytes <= kTrellisGroupBytes) ++v1;
+        const int v1 = trellis_group_end(q.row_offsets, q.n_utts, v0, row_bytes);
         TrellisView v;
         v.cand = q.cand; v.tdist = q.tdist; v.off = h->tr_off.as<int64_t>();
         v.first = v0; v.n_utts = v1 - v0; v.K = q.K; v.Kp = Kp;

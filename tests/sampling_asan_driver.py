@@ -117,12 +117,13 @@ for bias in (False, True):
         e.sample_paths(cand, dist, w, row_offsets=o, temperature=0.0)
         logz, post, uses = e.path_posterior(cand, dist, row_offsets=o)
         assert logz.shape == (n,) and post.shape == (T, K) and (uses.shape == (2, 5) if bias else uses is None)
-for call in (lambda c, d, **k: e.sample_paths(c, d, k.pop('u', w), **k), lambda c, d, **k: e.path_posterior(c, d, **k)):
+for call in (lambda c, d, **k: e.sample_paths(c, d, k.pop('u', w), **k), lambda c, d, u=None, **k: e.path_posterior(c, d, **k)):
     assert refused('has no rows', call, cand, dist, row_offsets=[0, 5, 5, 30])
     assert refused('has no rows', call, cand, dist, row_offsets=[0, 9, 5, 30])
     assert refused('row_offsets[0]', call, cand, dist, row_offsets=[1, 30])
     assert refused('row_offsets', call, cand, dist, row_offsets=[0, 29])
     assert refused('row_offsets', call, cand, dist, row_offsets=[30])
+    assert refused('8388609 rows', call, np.zeros((8388610, 1), np.int64), np.zeros((8388610, 1)), u=np.zeros((1, 8388610)), row_offsets=[0, 1, 8388610])
     assert refused('expected', call, cand[0], dist[0])
     assert refused('fit', call, cand, dist[:, :5])
     assert refused('fit', call, cand, dist, join_class=np.zeros(T - 1, np.int32))

@@ -236,6 +236,40 @@ def test_rows_on_another_stream_and_in_a_graph(engine):
             assert torch.equal(eager, i)
 
 
+def test_rows_of_many_draws(engine):
+    """More draws than a launch's second dimension holds."""
+    rng = np.random.RandomState(9)
+    for V, draws in ((1500, 70000), (40, 70000)):
+        x, u = rng.randn(2, V).astype(np.float32), rng.rand(2, draws)
+        i, lp = [a.cpu().numpy() for a in engine.sample_rows(on_gpu(x), on_gpu(u), top_p=0.9)]
+        some = np.r_[0:50, 32760:32780, 65530:65540, draws - 50:draws]
+        want, want_lp = o.sample_rows(as_f64(x), u[:, some], top_p=0.9)
+        assert np.array_equal(i[:, some], want)
+        assert np.all(np.abs(lp[:, some] - want_lp) <= logp_tolerance(V, np.abs(want_lp).max()))
+        assert i.min() >= 0
+
+
+@pytest.mark.parametrize('dtype', ['float32', 'float64', 'bfloat16'])
+@pytest.mark.parametrize('V', [20000, 70001])
+def test_rows_whose_boundary_is_one_chunks(engine, V, dtype):
+    """The scores among which the order reaches its goal: all in one chunk, one in each, more of them than a workgroup holds at once,
+    more than the list holds."""
+    rng = np.random.RandomState(V)
+    x = np.full((4, V), -30.0)
+    x[0, 8192:8192 + 3000] = rng.permutation(3000) / 4096.0          # side by side
+    x[1, ::8192] = rng.permutation(x[1, ::8192].size) / 64.0
+    x[2, :12000] = rng.permutation(12000) / 2.0 ** 20
+    x[3, :V - 1] = rng.permutation(V - 1) / 2.0 ** 24
+    if dtype == 'bfloat16':
+        import torch
+        x = torch.from_numpy(x).to(torch.bfloat16)
+    else:
+        x = x.astype(dtype)
+    u = rng.rand(4, 3)
+    for rule in (dict(top_k=2), dict(top_k=1999), dict(top_p=0.5), dict(top_k=9000, top_p=0.4), dict(temperature=0.01, top_p=0.7)):
+        check_rows(engine, x, u, **rule)
+
+
 # ---------------------------------------------------------------------------------------------------------------- trellis
 class Voice(object):
     def __init__(self, engine, Dj=9, n=400, seed=0):
@@ -510,6 +544,83 @@ def test_trellis_results_do_not_depend_on_the_batch(engine):
         assert z[0] == logz[i] and np.array_equal(q, post[a:b])
     again = v.engine.path_posterior(cand, dist, row_offsets=offs, join_class=cls, temperature=0.5)
     assert all(np.array_equal(a, b) for a, b in zip(again, (logz, post, uses)))
+
+
+@pytest.mark.parametrize('K', [64, 100, 130])
+def test_trellis_tiles_do_not_depend_on_the_batch(engine, K):
+    """A sentence by itself (small tiles, few workgroups) and among many others."""
+    v = Voice(engine, n=2000)
+    v.set_bias(2, 8)
+    lengths = [60, 26, 1, 150, 200, 90, 2, 170]
+    cand, dist, offs = v.candidates(lengths, K)
+    rng = np.random.RandomState(0)
+    u, cls = rng.rand(2, cand.shape[0]), rng.randint(0, 2, cand.shape[0]).astype(np.int32)
+    path, cost, logp = v.engine.sample_paths(cand, dist, u, row_offsets=offs, join_class=cls, temperature=0.5, top_p=0.9)
+    logz, post, _ = v.engine.path_posterior(cand, dist, row_offsets=offs, join_class=cls, temperature=0.5)
+    for i in (0, 1, 2, 6):
+        a, b = int(offs[i]), int(offs[i + 1])
+        p, c, l = v.engine.sample_paths(cand[a:b], dist[a:b], u[:, a:b], join_class=cls[a:b], temperature=0.5, top_p=0.9)
+        assert np.array_equal(p, path[:, a:b]) and np.array_equal(c[:, 0], cost[:, i]) and np.array_equal(l[:, 0], logp[:, i])
+        z, q, _ = v.engine.path_posterior(cand[a:b], dist[a:b], join_class=cls[a:b], temperature=0.5)
+        assert z[0] == logz[i] and np.array_equal(q, post[a:b])
+
+
+def test_trellis_of_many_utterances(engine):
+    """More utterances than a launch's second dimension holds, short ones beside a long one."""
+    v = Voice(engine)
+    rng = np.random.RandomState(0)
+    lengths = rng.randint(1, 4, 70001)
+    lengths[[5, 69000]] = 700, 900
+    cand, dist, offs = v.candidates(lengths, 2)
+    u = rng.rand(1, cand.shape[0])
+    path, cost, logp = v.engine.sample_paths(cand, dist, u, row_offsets=offs)
+    logz, post, _ = v.engine.path_posterior(cand, dist, row_offsets=offs)
+    usable = ((cand >= 1) & (cand < v.n - 1)).any(axis=1)        # rows of two units that cannot be joined leave a few utterances empty
+    alive = np.logical_and.reduceat(usable, offs[:-1])
+    rows_alive = np.repeat(alive, lengths)
+    assert 0 < (~alive).sum() < 20
+    assert np.array_equal(path[0] >= 0, rows_alive) and np.array_equal(np.isfinite(cost[0]), alive) and np.array_equal(np.isfinite(logz), alive)
+    assert not post[~rows_alive].any()
+    # a row's probabilities sum to 1: two of them, each with the error of the recursions (sum_tolerance, and 4 roundings more)
+    size = np.abs(logz[alive]).max() + 2.0 * 900
+    assert np.abs(post[rows_alive].sum(axis=1) - 1.0).max() <= 8.0 * sum_tolerance(900, 2, size)
+    for i in (0, 4, 5, 6, 32767, 32768, 32769, 65535, 65536, 68999, 69000, 69001, 70000):
+        a, b = int(offs[i]), int(offs[i + 1])
+        p, c, l = v.engine.sample_paths(cand[a:b], dist[a:b], u[:, a:b])
+        assert np.array_equal(p, path[:, a:b]) and c[0, 0] == cost[0, i] and l[0, 0] == logp[0, i]
+        z, q, _ = v.engine.path_posterior(cand[a:b], dist[a:b])
+        assert z[0] == logz[i] and np.array_equal(q, post[a:b])
+
+
+@pytest.mark.parametrize('Dj', [1, 33, 151, 302])
+def test_join_costs_of_far_and_near_units(engine, Dj):
+    """Frames that lie far from the origin, next to each other, and equal.  The engine may take a squared distance from products,
+    |e|^2 + |s|^2 - 2 e s, where that is above 2^-8 of |e|^2 + |s|^2; its Dj + 4 roundings of 2^-53 then cost 2^8 (Dj + 4) 2^-52
+    relative of the square, half that of the distance: so much of the largest join cost, once a row and for each sum that it enters."""
+    v = Voice(engine, Dj=Dj, n=300)
+    rng = np.random.RandomState(Dj)
+    JC = 3000.0 + rng.randn(301, Dj)
+    JC[100:200] = JC[100] + 1e-3 * rng.randn(100, Dj)
+    JC[200:250] = JC[200]
+    JC[250:260] = 0.0
+    v.JC = JC.astype(np.float32)
+    v.wj = v.wj / np.sqrt(Dj)
+    engine.upload_join_only(v.JC)
+    engine.set_weights(None, v.wj)
+    T, K = 30, 20
+    cand = rng.randint(0, 300, (T, K)).astype(np.int64)
+    cand[10:20] = rng.randint(100, 200, (10, K))
+    cand[20:25] = rng.randint(200, 250, (5, K))
+    dist = rng.rand(T, K)
+    furthest = np.sqrt((v.wj ** 2 * (v.JC.max(axis=0) - v.JC.min(axis=0)).astype(np.float64) ** 2).sum())
+    for near in (True, False):                              # without and with the frames at the origin
+        if not near:
+            cand[0, 0] = 255
+        z, p, _ = o.posterior(cand, dist, 1.0, **v.model())
+        logz, post, _ = engine.path_posterior(cand, dist)
+        tol = sum_tolerance(T, K, abs(z) + 2.0 * T) + T * furthest * (Dj + 4.0) * 2.0 ** -45
+        assert abs(logz[0] - z) <= tol
+        assert np.all(np.abs(post - p) <= 4.0 * tol)
 
 
 def test_trellis_on_another_stream(engine):
