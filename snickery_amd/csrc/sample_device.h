@@ -149,12 +149,12 @@ __device__ __forceinline__ double row16_max(double v)      // of each row of 16 
     v = dpp_max(v, dpp_move<0x118, 0xf>(SNK_BITS(v), SNK_BITS(v)));
     return v;
 }
-__device__ __forceinline__ double row16_sum(double v)      // of each row of 16 lanes, in all of them
+__device__ __forceinline__ double row16_sum(double v)      // of each row of 16 lanes, in all of them: mirrored, so that they agree to the last bit
 {
-    v += __longlong_as_double((long long)dpp_move<0x121, 0xf>(0, SNK_BITS(v)));     // rotations within the row
-    v += __longlong_as_double((long long)dpp_move<0x122, 0xf>(0, SNK_BITS(v)));
-    v += __longlong_as_double((long long)dpp_move<0x124, 0xf>(0, SNK_BITS(v)));
-    v += __longlong_as_double((long long)dpp_move<0x128, 0xf>(0, SNK_BITS(v)));
+    v += __longlong_as_double((long long)dpp_move<0xb1, 0xf>(0, SNK_BITS(v)));
+    v += __longlong_as_double((long long)dpp_move<0x4e, 0xf>(0, SNK_BITS(v)));
+    v += __longlong_as_double((long long)dpp_move<0x141, 0xf>(0, SNK_BITS(v)));
+    v += __longlong_as_double((long long)dpp_move<0x140, 0xf>(0, SNK_BITS(v)));
     return v;
 }
 __device__ __forceinline__ double quad_sum(double v)       // of each four lanes, in all of them

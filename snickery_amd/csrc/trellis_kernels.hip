@@ -44,29 +44,34 @@ __device__ __forceinline__ int trellis_utterance(const int64_t *__restrict__ off
     return u;
 }
 
-// Bucket of a distance: the number of edges up to it.  63 edges at most, in LDS behind INT_MAX padding: which eight of them it falls
-// among from every eighth (in registers), then those eight.  28 instructions and one LDS latency whatever the distance; a search by
-// halves waits for LDS five times.
-struct TrellisEdges { int head[7]; const int *all; };
+// Bucket of a distance: the number of edges up to it.  63 edges at most, in LDS behind INT_MAX padding: which sixteen of them it falls
+// among, which four of those, which of those: nine comparisons and two LDS latencies, where two steps of eight take fifteen and one
+// and a search by halves waits for LDS five times.
+#define SNK_EDGE_WORDS 80                                       // the edges, then every fourth one
+struct TrellisEdges { int head[3]; const int *all; };
 __device__ __forceinline__ TrellisEdges trellis_edges(const int *lds)
 {
     TrellisEdges e;
     e.all = lds;
 #pragma unroll
-    for (int i = 0; i < 7; ++i) e.head[i] = lds[8 * i + 7];
+    for (int i = 0; i < 3; ++i) e.head[i] = lds[16 * i + 15];
     return e;
 }
 __device__ __forceinline__ int trellis_bucket(int apart, const TrellisEdges &e)
 {
-    int k = 0;
-#pragma unroll
-    for (int i = 0; i < 7; ++i) k += apart >= e.head[i] ? 8 : 0;
-    const int4 x = *reinterpret_cast<const int4 *>(e.all + k), y = *reinterpret_cast<const int4 *>(e.all + k + 4);
-    return k + (apart >= x.x) + (apart >= x.y) + (apart >= x.z) + (apart >= x.w) + (apart >= y.x) + (apart >= y.y) + (apart >= y.z) + (apart >= y.w);
+    int k = 4 * ((apart >= e.head[0]) + (apart >= e.head[1]) + (apart >= e.head[2]));
+    const int4 x = *reinterpret_cast<const int4 *>(e.all + 64 + k);
+    k = 4 * (k + (apart >= x.x) + (apart >= x.y) + (apart >= x.z));
+    const int4 y = *reinterpret_cast<const int4 *>(e.all + k);
+    return k + (apart >= y.x) + (apart >= y.y) + (apart >= y.z);
 }
 __device__ __forceinline__ void trellis_load_edges(int *lds, const int *__restrict__ edges, int n_buckets)
 {
-    if (threadIdx.x < 64) lds[threadIdx.x] = (int)threadIdx.x < n_buckets - 1 ? edges[threadIdx.x] : 0x7fffffff;
+    const int i = threadIdx.x;
+    if (i >= 64) return;
+    const int e = i < n_buckets - 1 ? edges[i] : 0x7fffffff;
+    lds[i] = e;
+    if ((i & 3) == 3) lds[64 + (i >> 2)] = e;
 }
 
 __device__ __forceinline__ double trellis_pow2(int e)           // 2^e, -1022 <= e <= 1023
@@ -128,39 +133,103 @@ __device__ __forceinline__ double trellis_difference(const TrellisCosts &c, int 
 {
     const float *__restrict__ pe = c.JC + (int64_t)(end + 1) * c.Jp, *__restrict__ ps = c.JC + (int64_t)start * c.Jp;
     double d2 = 0.0;
-    for (int j = 4 * (threadIdx.x & 15); j < c.Dj; j += 64) {   // (rows are padded to multiples of four columns)
-        const float4 e = *reinterpret_cast<const float4 *>(pe + j), s = *reinterpret_cast<const float4 *>(ps + j);
-        const float e4[4] = {e.x, e.y, e.z, e.w}, s4[4] = {s.x, s.y, s.z, s.w};
+    for (int j0 = 0; j0 < c.Dj; j0 += 128) {                    // (rows are padded to multiples of four columns; a lane beyond them reads their last four)
+        float4 e[2], s[2];
+        double w[2][4];
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            const double w = j + k < c.Dj ? c.wj[j + k] : 0.0, d = (double)e4[k] * w - (double)s4[k] * w;
-            d2 = __fma_rn(d, d, d2);
+        for (int h = 0; h < 2; ++h) {
+            const int j = j0 + 64 * h + 4 * (threadIdx.x & 15), at = min(j, c.Jp - 4);
+            e[h] = *reinterpret_cast<const float4 *>(pe + at);
+            s[h] = *reinterpret_cast<const float4 *>(ps + at);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) w[h][k] = j + k < c.Dj ? c.wj[j + k] : 0.0;
+        }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const float e4[4] = {e[h].x, e[h].y, e[h].z, e[h].w}, s4[4] = {s[h].x, s[h].y, s[h].z, s[h].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const double d = (double)e4[k] * w[h][k] - (double)s4[k] * w[h][k];
+                d2 = __fma_rn(d, d, d2);
+            }
         }
     }
     return row16_sum(d2);
 }
 
-template <int RT, int RM, int CM, bool LOG>
-__global__ void __launch_bounds__(256, 2)
+// A constant that the compiler keeps in scalar registers: written as a number it is moved into a pair of vector registers for every
+// multiply-add that adds it, two of three instructions of the polynomial below.
+#define SNK_SCALAR(name_, value_) double name_ = value_; asm("" : "+s"(name_))
+
+// exp(x), -SNK_COST_RANGE <= x <= 0, to about a unit in the last place: 2^(n / 32) from a table in LDS times a series of degree 6 in
+// what is left, |r| <= ln 2 / 64 (the next term is below 2^-58)
+__device__ const double trellis_powers[32] = {                  // 2^(j / 32)
+    0x1.0000000000000p+0, 0x1.059b0d3158574p+0, 0x1.0b5586cf9890fp+0, 0x1.11301d0125b51p+0, 0x1.172b83c7d517bp+0, 0x1.1d4873168b9aap+0,
+    0x1.2387a6e756238p+0, 0x1.29e9df51fdee1p+0, 0x1.306fe0a31b715p+0, 0x1.371a7373aa9cbp+0, 0x1.3dea64c123422p+0, 0x1.44e086061892dp+0,
+    0x1.4bfdad5362a27p+0, 0x1.5342b569d4f82p+0, 0x1.5ab07dd485429p+0, 0x1.6247eb03a5585p+0, 0x1.6a09e667f3bcdp+0, 0x1.71f75e8ec5f74p+0,
+    0x1.7a11473eb0187p+0, 0x1.82589994cce13p+0, 0x1.8ace5422aa0dbp+0, 0x1.93737b0cdc5e5p+0, 0x1.9c49182a3f090p+0, 0x1.a5503b23e255dp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b7f76f2fb5e47p+0, 0x1.c199bdd85529cp+0, 0x1.cb720dcef9069p+0, 0x1.d5818dcfba487p+0, 0x1.dfc97337b9b5fp+0,
+    0x1.ea4afa2a490dap+0, 0x1.f50765b6e4540p+0};
+__device__ __forceinline__ double trellis_exp(double x, const double *powers)
+{
+    SNK_SCALAR(per, 46.16624130844682903552);                   // 32 / ln 2
+    SNK_SCALAR(whole, 6755399441055744.0);                      // 1.5 2^52: a sum with it has its integer in the low bits
+    SNK_SCALAR(hi, -6.93147180369123816490e-01 / 32);
+    SNK_SCALAR(lo, -1.90821492927058770002e-10 / 32);
+    SNK_SCALAR(c6, 1.38888888888888888889e-03);
+    SNK_SCALAR(c5, 8.33333333333333333333e-03);
+    SNK_SCALAR(c4, 4.16666666666666666667e-02);
+    SNK_SCALAR(c3, 1.66666666666666666667e-01);
+    const double t = __fma_rn(x, per, whole), n = t - whole;
+    const int i = (int)__double_as_longlong(t);
+    const double r = __fma_rn(n, lo, __fma_rn(n, hi, x)), power = powers[i & 31];
+    double p = __fma_rn(r, c6, c5);
+    p = __fma_rn(p, r, c4);
+    p = __fma_rn(p, r, c3);
+    p = __fma_rn(p, r, 0.5);
+    p = __fma_rn(p, r, 1.0);
+    p = __fma_rn(power, p * r, power);
+    return __longlong_as_double(__double_as_longlong(p) + ((long long)(i >> 5) << 52));
+}
+
+// sqrt(x), x >= 0, to a unit in the last place, infinite for neither: the reciprocal root refined by Goldschmidt's step and a
+// correction by the remainder.  Below 2^-1000 it is 2^-500.
+__device__ __forceinline__ double trellis_root(double x)
+{
+    x = fmax(x, 0x1p-1000);
+    const double y = __builtin_amdgcn_rsq(x);
+    double g = x * y, h = 0.5 * y;
+    const double r = __fma_rn(-h, g, 0.5);
+    g = __fma_rn(g, r, g);
+    h = __fma_rn(h, r, h);
+    return __fma_rn(__fma_rn(-g, g, x), h, g);
+}
+
+template <int RT, int RM, int CM, int NTH, int OCC, bool LOG>
+__global__ void __launch_bounds__(NTH, OCC)
 trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__ flag, double *__restrict__ X)
 {
-    constexpr int N = 16 * RT, DC = 16, LD = DC + 2, PASS = (N + 63) / 64, WC = (RT + CM - 1) / CM;      // WC wavefronts side by side
-    __shared__ __align__(16) double Es[N * LD], Ss[N * LD];
+    constexpr int N = 16 * RT, DC = 16, LD = DC + 2, NW = NTH / 64, NR = NTH / 4, PASS = (N + NR - 1) / NR;
+    constexpr int WC = (RT + CM - 1) / CM;                      // wavefronts side by side
+    __shared__ __align__(16) double Es[2 * N * LD];             // of the first row's candidates, then of the second's
+    __shared__ double powers[32];
     __shared__ double nE[N], nS[N];
     __shared__ int idE[N], idS[N];                              // unit id, -1: cannot join
-    __shared__ __align__(16) int edges[64];
+    __shared__ __align__(16) int edges[SNK_EDGE_WORDS];
     __shared__ double bias[64];
-    __shared__ unsigned short near_cell[N * N];                 // cells to take again
     __shared__ unsigned int n_near;
+    double *const Ss = Es + N * LD;
+    unsigned short *const near_cell = reinterpret_cast<unsigned short *>(Es);           // cells to take again, when the products are done
+    static_assert(N * N * sizeof(short) <= sizeof Es, "a list of every cell");
     const int64_t t = v.c0 + blockIdx.x;
     const int u = trellis_utterance(v.off, v.first, v.n_utts, t);
     if (t + 1 == v.off[u + 1]) return;
     if (LOG && !flag[u]) return;
     const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, g = lane >> 4;
-    const int wave = ((tid >> 6) + blockIdx.x) & 3;             // (the last wavefront has fewer tiles: not always on the same SIMD)
+    const int wave = ((tid >> 6) + blockIdx.x) % NW;            // (the last wavefronts have fewer tiles or none: not always on the same SIMD)
     const int row0 = (wave / WC) * RM, col0 = (wave % WC) * CM;
     const int a0 = blockIdx.y * N, b0 = blockIdx.z * N;
-    for (int i = tid; i < 2 * N; i += 256) {
+    for (int i = tid; i < 2 * N; i += NTH) {
         const bool second = i >= N;
         const int k = second ? b0 + i - N : a0 + i;
         const int64_t id = k < v.K ? v.cand[(t + (second ? 1 : 0)) * v.K + k] : -1;
@@ -174,6 +243,7 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
         if (cls >= 0 && tid < c.n_buckets) bias[tid] = c.bias[(int64_t)cls * c.n_buckets + tid];
     }
     if (tid == 0) n_near = 0;
+    if (!LOG && tid < 32) powers[tid] = trellis_powers[tid];
     __syncthreads();
     // the unit that both sides are taken relative to: the second row's first one that can join (of the whole row: a cell's value does
     // not depend on the tiles)
@@ -192,7 +262,7 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
     double w[4], ne[PASS], ns[PASS];
 #pragma unroll
     for (int p = 0; p < PASS; ++p) {
-        const int r = r0 + 64 * p < N ? r0 + 64 * p : 0;
+        const int r = r0 + NR * p < N ? r0 + NR * p : 0;
         pe[p] = c.JC + (int64_t)(idE[r] >= 0 ? idE[r] + 1 : about) * c.Jp + 4 * q;
         ps[p] = c.JC + (int64_t)(idS[r] >= 0 ? idS[r] : about) * c.Jp + 4 * q;
         ne[p] = 0.0; ns[p] = 0.0;
@@ -219,15 +289,15 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
         const float c4[4] = {fc.x, fc.y, fc.z, fc.w};
 #pragma unroll
         for (int p = 0; p < PASS; ++p) {
-            const int r = r0 + 64 * p;
+            const int r = r0 + NR * p;
             if (r < N) {
                 const float e4[4] = {fe[p].x, fe[p].y, fe[p].z, fe[p].w}, s4[4] = {fs[p].x, fs[p].y, fs[p].z, fs[p].w};
                 double de[4], ds[4];
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     const double m = (double)c4[e] * w[e];
-                    de[e] = (double)e4[e] * w[e] - m;
-                    ds[e] = (double)s4[e] * w[e] - m;
+                    de[e] = __fma_rn((double)e4[e], w[e], -m);
+                    ds[e] = __fma_rn((double)s4[e], w[e], -m);
                     ne[p] = __fma_rn(de[e], de[e], ne[p]);
                     ns[p] = __fma_rn(ds[e], ds[e], ns[p]);
                 }
@@ -256,22 +326,25 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
     }
 #pragma unroll
     for (int p = 0; p < PASS; ++p) {
-        const int r = r0 + 64 * p;
+        const int r = r0 + NR * p;
         const double e = quad_sum(ne[p]), s = quad_sum(ns[p]);
-        if (r < N && q == 0) { nE[r] = e; nS[r] = s; }
+        if (r < N && q == 0) {                                  // what cannot join is infinitely far
+            nE[r] = idE[r] >= 0 ? e : __builtin_inf();
+            nS[r] = idS[r] >= 0 ? s : __builtin_inf();
+        }
     }
     __syncthreads();
     bool wide = false;
     double *__restrict__ out = X + (t - v.c0) * v.K * v.Kp;
     const TrellisEdges look = trellis_edges(edges);
-    auto value = [&](double d2, int ie, int is) -> double {     // a cell from the squared distance; ie, is < 0: cannot join
-        const bool ok = (ie | is) >= 0;
-        double cost = sqrt(d2);
+    auto value = [&](double d2, int ie, int is) -> double {     // a cell from the squared distance, infinite: cannot join
+        double cost = LOG ? sqrt(d2) : trellis_root(d2);
         if (cls >= 0) cost += bias[trellis_bucket(is - ie, look)];
-        if (LOG) return ok ? -cost * v.inv_tau : -__builtin_inf();
+        if (LOG) return -cost * v.inv_tau;
+        const bool ok = cost < __builtin_inf();                 // (the root of an infinite square is not a number)
         const double x = (c.bias_min - cost) * v.inv_tau;
-        wide |= ok && x < -SNK_COST_RANGE && cost < __builtin_inf();
-        return ok && cost < __builtin_inf() ? sample_exp(fmax(x, -SNK_COST_RANGE)) : 0.0;
+        wide |= ok && x < -SNK_COST_RANGE;
+        return ok ? trellis_exp(fmax(x, -SNK_COST_RANGE), powers) : 0.0;
     };
     // (a loop over the tiles, not RM CM copies of its body; a wavefront's k-th tile is picked by uniform branches)
 #pragma unroll 1
@@ -292,7 +365,7 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
         for (int r = 0; r < 4; ++r) {
             const int al = ti * 16 + g + 4 * r, ie = idE[al], a = a0 + al;
             const double both = nE[al] + sn, d2 = __fma_rn(-2.0, p[r], both);
-            again[r] = (ie | is) >= 0 && d2 < SNK_COST_NEAR * both;
+            again[r] = d2 < SNK_COST_NEAR * both;
             any += again[r] ? 1 : 0;
             const double x = value(fmax(d2, 0.0), ie, is);
             if (a < v.K && b < v.Kp) out[(int64_t)a * v.Kp + b] = x;
@@ -311,11 +384,20 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
         }
     }
     __syncthreads();
-    // the near cells in differences, sixteen lanes each
-    for (int i = tid >> 4; i < (int)n_near; i += 16) {
-        const int cell = near_cell[i], al = cell / N, bl = cell % N, ie = idE[al], is = idS[bl], a = a0 + al, b = b0 + bl;
-        const double x = value(trellis_difference(c, ie, is), ie, is);
-        if (c16 == 0 && a < v.K && b < v.Kp) out[(int64_t)a * v.Kp + b] = x;
+    // the near cells in differences, sixteen lanes each: up to sixteen one after the other, then each lane has one of its own to weigh
+    for (int base = 0, left = (int)n_near; left > 0; base += 64 * NW, left -= 64 * NW) {
+        const int each = (min(left, 64 * NW) + 4 * NW - 1) / (4 * NW), first = base + (tid >> 4) * each, n = min(each, (int)n_near - first);
+        double d2 = 0.0;
+        for (int i = 0; i < n; ++i) {
+            const int cell = near_cell[first + i];
+            const double d = trellis_difference(c, idE[cell / N], idS[cell % N]);
+            if (c16 == i) d2 = d;
+        }
+        if (c16 < n) {
+            const int cell = near_cell[first + c16], al = cell / N, bl = cell % N, a = a0 + al, b = b0 + bl;
+            const double x = value(d2, idE[al], idS[bl]);
+            if (a < v.K && b < v.Kp) out[(int64_t)a * v.Kp + b] = x;
+        }
     }
     if (!LOG && wide) flag[u] = 1;
 }
@@ -1005,7 +1087,7 @@ trellis_posterior_kernel(const TrellisView v, const int *__restrict__ flag, cons
                          double *__restrict__ posterior, double *__restrict__ row_uses)
 {
     __shared__ double in[256], out[256], red[8];
-    __shared__ __align__(16) int edges[64];
+    __shared__ __align__(16) int edges[SNK_EDGE_WORDS];
     __shared__ int id0[256], id1[256];
     __shared__ u64 uses[64];
     const int64_t t = v.c0 + blockIdx.x;
@@ -1321,15 +1403,15 @@ void launch_trellis_costs(const TrellisView &v, const TrellisCosts &c, bool logs
     if (v.K > 64 && (v.rows - 1) * n * n < 1024) n = (v.K + 63) / 64;
     const int rt = ((v.K + n - 1) / n + 15) / 16;
     const dim3 grid((unsigned)(v.rows - 1), n, n);
-#define SNK_COST(RT_, RM_, CM_)                                                                                              \
+#define SNK_COST(RT_, RM_, CM_, NTH_, OCC_)                                                                                            \
     do {                                                                                                                     \
-        if (logs) hipLaunchKernelGGL((trellis_cost_kernel<RT_, RM_, CM_, true>), grid, dim3(256), 0, s, v, c, flag, X);      \
-        else hipLaunchKernelGGL((trellis_cost_kernel<RT_, RM_, CM_, false>), grid, dim3(256), 0, s, v, c, flag, X);          \
+        if (logs) hipLaunchKernelGGL((trellis_cost_kernel<RT_, RM_, CM_, NTH_, OCC_, true>), grid, dim3(NTH_), 0, s, v, c, flag, X);      \
+        else hipLaunchKernelGGL((trellis_cost_kernel<RT_, RM_, CM_, NTH_, OCC_, false>), grid, dim3(NTH_), 0, s, v, c, flag, X);          \
     } while (0)
-    if (rt <= 2) SNK_COST(2, 1, 1);
-    else if (rt <= 4) SNK_COST(4, 2, 2);
-    else if (rt <= 6) SNK_COST(6, 3, 3);
-    else SNK_COST(7, 7, 2);
+    if (rt <= 2) SNK_COST(2, 1, 1, 256, 4);
+    else if (rt <= 4) SNK_COST(4, 2, 2, 256, 4);
+    else if (rt <= 6) SNK_COST(6, 3, 3, 256, 3);
+    else SNK_COST(7, 7, 1, 512, 4);
 #undef SNK_COST
 }
 
