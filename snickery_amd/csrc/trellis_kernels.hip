@@ -123,8 +123,9 @@ trellis_local_kernel(const TrellisView v, double *__restrict__ local, double *__
 // one of the tile's units, so that the norms are those of the candidates' spread and not of their distance from the origin.  Where
 // the difference is small against the norms -- a unit and its natural successor join at exactly 0 -- the product form cancels: a
 // cell below SNK_COST_NEAR of them is taken again in differences.  The others carry a relative error of at most Dj 2^-53 / SNK_COST_NEAR.
-// A wavefront owns RM x CM tiles of 16 x 16; 16 columns of the two sets of rows go through LDS at a time, weighted and widened on
-// the way, the next 16 are in flight meanwhile.
+// A wavefront owns RM x CM tiles of 16 x 16; DC columns of the two sets of rows go through LDS at a time, weighted and widened on
+// the way, the next ones are in flight meanwhile: 32, a cache line of a row (197 us for 600 rows of 100 candidates and 302 columns, 206
+// with 16), or 16 in the larger tiles, whose registers hold no more (2.55 ms for 9600 rows, 2.73 with 32 and spills).
 #define SNK_COST_NEAR 0x1p-8
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
@@ -205,11 +206,11 @@ __device__ __forceinline__ double trellis_root(double x)
     return __fma_rn(__fma_rn(-g, g, x), h, g);
 }
 
-template <int RT, int RM, int CM, int NTH, int OCC, bool LOG>
+template <int RT, int RM, int CM, int NTH, int OCC, int DC, bool LOG>
 __global__ void __launch_bounds__(NTH, OCC)
 trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__ flag, double *__restrict__ X)
 {
-    constexpr int N = 16 * RT, DC = 16, LD = DC + 2, NW = NTH / 64, NR = NTH / 4, PASS = (N + NR - 1) / NR;
+    constexpr int N = 16 * RT, QL = DC / 4, LD = DC + 2, NW = NTH / 64, NR = NTH / QL, PASS = (N + NR - 1) / NR;
     constexpr int WC = (RT + CM - 1) / CM;                      // wavefronts side by side
     __shared__ __align__(16) double Es[2 * N * LD];             // of the first row's candidates, then of the second's
     __shared__ double powers[32];
@@ -256,7 +257,7 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
         if (can && !found) { about = __builtin_amdgcn_readlane((int)id, __ffsll((long long)can) - 1); found = true; }
     }
 
-    const int q = tid & 3, r0 = tid >> 2;
+    const int q = tid & (QL - 1), r0 = tid / QL;            // a thread takes four columns of the rows r0, r0 + NR, ..
     const float *pe[PASS], *ps[PASS], *pc = c.JC + (int64_t)about * c.Jp + 4 * q;
     float4 fe[PASS], fs[PASS], fc;
     double w[4], ne[PASS], ns[PASS];
@@ -310,6 +311,7 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
         if (col + DC < c.Dj) fetch(col + DC);
 #pragma unroll
         for (int ks = 0; ks < DC / 4; ++ks) {
+            if (col + 4 * ks >= c.Dj) break;
             double fa[RM], fb[CM];
 #pragma unroll
             for (int i = 0; i < RM; ++i) fa[i] = row0 + i < RT ? Es[((row0 + i) * 16 + c16) * LD + 4 * ks + g] : 0.0;
@@ -327,7 +329,8 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
 #pragma unroll
     for (int p = 0; p < PASS; ++p) {
         const int r = r0 + NR * p;
-        const double e = quad_sum(ne[p]), s = quad_sum(ns[p]);
+        double e = quad_sum(ne[p]), s = quad_sum(ns[p]);
+        if (QL == 8) { e = eight_sum(e); s = eight_sum(s); }
         if (r < N && q == 0) {                                  // what cannot join is infinitely far
             nE[r] = idE[r] >= 0 ? e : __builtin_inf();
             nS[r] = idS[r] >= 0 ? s : __builtin_inf();
@@ -1403,15 +1406,15 @@ void launch_trellis_costs(const TrellisView &v, const TrellisCosts &c, bool logs
     if (v.K > 64 && (v.rows - 1) * n * n < 1024) n = (v.K + 63) / 64;
     const int rt = ((v.K + n - 1) / n + 15) / 16;
     const dim3 grid((unsigned)(v.rows - 1), n, n);
-#define SNK_COST(RT_, RM_, CM_, NTH_, OCC_)                                                                                            \
+#define SNK_COST(RT_, RM_, CM_, NTH_, OCC_, DC_)                                                                                            \
     do {                                                                                                                     \
-        if (logs) hipLaunchKernelGGL((trellis_cost_kernel<RT_, RM_, CM_, NTH_, OCC_, true>), grid, dim3(NTH_), 0, s, v, c, flag, X);      \
-        else hipLaunchKernelGGL((trellis_cost_kernel<RT_, RM_, CM_, NTH_, OCC_, false>), grid, dim3(NTH_), 0, s, v, c, flag, X);          \
+        if (logs) hipLaunchKernelGGL((trellis_cost_kernel<RT_, RM_, CM_, NTH_, OCC_, DC_, true>), grid, dim3(NTH_), 0, s, v, c, flag, X);      \
+        else hipLaunchKernelGGL((trellis_cost_kernel<RT_, RM_, CM_, NTH_, OCC_, DC_, false>), grid, dim3(NTH_), 0, s, v, c, flag, X);          \
     } while (0)
-    if (rt <= 2) SNK_COST(2, 1, 1, 256, 4);
-    else if (rt <= 4) SNK_COST(4, 2, 2, 256, 4);
-    else if (rt <= 6) SNK_COST(6, 3, 3, 256, 3);
-    else SNK_COST(7, 7, 1, 512, 4);
+    if (rt <= 2) SNK_COST(2, 1, 1, 256, 4, 32);
+    else if (rt <= 4) SNK_COST(4, 2, 2, 256, 4, 32);
+    else if (rt <= 6) SNK_COST(6, 3, 3, 256, 3, 16);
+    else SNK_COST(7, 7, 1, 512, 4, 16);
 #undef SNK_COST
 }
 
