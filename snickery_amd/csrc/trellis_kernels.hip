@@ -129,6 +129,14 @@ trellis_local_kernel(const TrellisView v, double *__restrict__ local, double *__
 #define SNK_COST_NEAR 0x1p-8
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
+// weight of a column; 0 behind the last.  (Loads from a clamped place, here and of the rows: a load that is left out behind a condition
+// goes through the stack's address space.)
+__device__ __forceinline__ double trellis_weight(const TrellisCosts &c, int j)
+{
+    const double w = c.wj[min(j, c.Dj - 1)];
+    return j < c.Dj ? w : 0.0;
+}
+
 // sum of squared differences of a pair of join rows by a row of sixteen lanes; in every one of them
 __device__ __forceinline__ double trellis_difference(const TrellisCosts &c, int end, int start)
 {
@@ -143,7 +151,7 @@ __device__ __forceinline__ double trellis_difference(const TrellisCosts &c, int 
             e[h] = *reinterpret_cast<const float4 *>(pe + at);
             s[h] = *reinterpret_cast<const float4 *>(ps + at);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) w[h][k] = j + k < c.Dj ? c.wj[j + k] : 0.0;
+            for (int k = 0; k < 4; ++k) w[h][k] = trellis_weight(c, j + k);
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -211,7 +219,8 @@ __global__ void __launch_bounds__(NTH, OCC)
 trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__ flag, double *__restrict__ X)
 {
     constexpr int N = 16 * RT, QL = DC / 4, LD = DC + 2, NW = NTH / 64, NR = NTH / QL, PASS = (N + NR - 1) / NR;
-    constexpr int WC = (RT + CM - 1) / CM;                      // wavefronts side by side
+    constexpr int WC = RT / CM;                                 // wavefronts side by side
+    static_assert(RT % RM == 0 && RT % CM == 0 && (RT / RM) * WC <= NW, "every tile has its wavefront");
     __shared__ __align__(16) double Es[2 * N * LD];             // of the first row's candidates, then of the second's
     __shared__ double powers[32];
     __shared__ double nE[N], nS[N];
@@ -227,8 +236,9 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
     if (t + 1 == v.off[u + 1]) return;
     if (LOG && !flag[u]) return;
     const int tid = threadIdx.x, lane = tid & 63, c16 = lane & 15, g = lane >> 4;
-    const int wave = ((tid >> 6) + blockIdx.x) % NW;            // (the last wavefronts have fewer tiles or none: not always on the same SIMD)
+    const int wave = ((tid >> 6) + blockIdx.x) % NW;            // (one of eight has no tiles: not always on the same SIMD)
     const int row0 = (wave / WC) * RM, col0 = (wave % WC) * CM;
+    const bool busy = row0 < RT;
     const int a0 = blockIdx.y * N, b0 = blockIdx.z * N;
     for (int i = tid; i < 2 * N; i += NTH) {
         const bool second = i >= N;
@@ -269,16 +279,15 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
         ne[p] = 0.0; ns[p] = 0.0;
     }
     auto fetch = [&](int col) {
-        const bool in = col + 4 * q < c.Jp;
-        const float4 zero = make_float4(0.f, 0.f, 0.f, 0.f);
-        fc = in ? *reinterpret_cast<const float4 *>(pc + col) : zero;
+        const int at = min(col, c.Jp - 4 - 4 * q);              // (rows are padded to multiples of four columns)
+        fc = *reinterpret_cast<const float4 *>(pc + at);
 #pragma unroll
         for (int p = 0; p < PASS; ++p) {
-            fe[p] = in ? *reinterpret_cast<const float4 *>(pe[p] + col) : zero;
-            fs[p] = in ? *reinterpret_cast<const float4 *>(ps[p] + col) : zero;
+            fe[p] = *reinterpret_cast<const float4 *>(pe[p] + at);
+            fs[p] = *reinterpret_cast<const float4 *>(ps[p] + at);
         }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) w[e] = col + 4 * q + e < c.Dj ? c.wj[col + 4 * q + e] : 0.0;
+        for (int e = 0; e < 4; ++e) w[e] = trellis_weight(c, col + 4 * q + e);
     };
     f64x4 acc[RM][CM];
 #pragma unroll
@@ -309,20 +318,20 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
         }
         __syncthreads();
         if (col + DC < c.Dj) fetch(col + DC);
+        if (busy) {
 #pragma unroll
-        for (int ks = 0; ks < DC / 4; ++ks) {
-            if (col + 4 * ks >= c.Dj) break;
-            double fa[RM], fb[CM];
+            for (int ks = 0; ks < DC / 4; ++ks) {
+                if (col + 4 * ks >= c.Dj) break;
+                double fa[RM], fb[CM];
 #pragma unroll
-            for (int i = 0; i < RM; ++i) fa[i] = row0 + i < RT ? Es[((row0 + i) * 16 + c16) * LD + 4 * ks + g] : 0.0;
+                for (int i = 0; i < RM; ++i) fa[i] = Es[((row0 + i) * 16 + c16) * LD + 4 * ks + g];
 #pragma unroll
-            for (int j = 0; j < CM; ++j)
-                if (col0 + j < RT) {                            // (uniform)
-                    fb[j] = Ss[((col0 + j) * 16 + c16) * LD + 4 * ks + g];
+                for (int j = 0; j < CM; ++j) fb[j] = Ss[((col0 + j) * 16 + c16) * LD + 4 * ks + g];
 #pragma unroll
-                    for (int i = 0; i < RM; ++i)
-                        if (row0 + i < RT) acc[i][j] = __builtin_amdgcn_mfma_f64_16x16x4f64(fa[i], fb[j], acc[i][j], 0, 0, 0);
-                }
+                for (int j = 0; j < CM; ++j)
+#pragma unroll
+                    for (int i = 0; i < RM; ++i) acc[i][j] = __builtin_amdgcn_mfma_f64_16x16x4f64(fa[i], fb[j], acc[i][j], 0, 0, 0);
+            }
         }
         __syncthreads();
     }
@@ -351,7 +360,7 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
     };
     // (a loop over the tiles, not RM CM copies of its body; a wavefront's k-th tile is picked by uniform branches)
 #pragma unroll 1
-    for (int k = 0; k < RM * CM; ++k) {
+    for (int k = 0; k < (busy ? RM * CM : 0); ++k) {
         f64x4 p = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
         for (int i = 0; i < RM; ++i)
@@ -359,7 +368,6 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
             for (int j = 0; j < CM; ++j)
                 if (i * CM + j == k) p = acc[i][j];
         const int ti = row0 + k / CM, tj = col0 + k % CM;
-        if (ti >= RT || tj >= RT) continue;
         const int bl = tj * 16 + c16, is = idS[bl], b = b0 + bl;
         const double sn = nS[bl];
         bool again[4];
