@@ -121,8 +121,8 @@ trellis_local_kernel(const TrellisView v, double *__restrict__ local, double *__
 // |e - s|^2 = |e|^2 + |s|^2 - 2 e.s on the float64 matrix pipe: half the instructions of the difference form (one fused multiply-add
 // a column instead of a subtraction and one), which ran at two thirds of the vector pipe's rate.  Both sides are taken relative to
 // one of the tile's units, so that the norms are those of the candidates' spread and not of their distance from the origin.  Where
-// the difference is small against the norms -- a unit and its natural successor join at exactly 0 -- the product form cancels: a
-// cell below SNK_COST_NEAR of them is taken again in differences.  The others carry a relative error of at most Dj 2^-53 / SNK_COST_NEAR.
+// the difference is small against the norms -- neighbouring frames -- the product form cancels: a cell below SNK_COST_NEAR of them is taken
+// again in differences.  A unit and its natural successor join at exactly 0.  The others carry a relative error of at most Dj 2^-53 / SNK_COST_NEAR.
 // A wavefront owns RM x CM tiles of 16 x 16; DC columns of the two sets of rows go through LDS at a time, weighted and widened on
 // the way, the next ones are in flight meanwhile: 32, a cache line of a row (197 us for 600 rows of 100 candidates and 302 columns, 206
 // with 16), or 16 in the larger tiles, whose registers hold no more (2.55 ms for 9600 rows, 2.73 with 32 and spills).
@@ -375,8 +375,8 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int al = ti * 16 + g + 4 * r, ie = idE[al], a = a0 + al;
-            const double both = nE[al] + sn, d2 = __fma_rn(-2.0, p[r], both);
-            again[r] = d2 < SNK_COST_NEAR * both;
+            const double both = nE[al] + sn, apart = __fma_rn(-2.0, p[r], both), d2 = is == ie + 1 ? 0.0 : apart;   // (natural: the same frame)
+            again[r] = apart < SNK_COST_NEAR * both && is != ie + 1;
             any += again[r] ? 1 : 0;
             const double x = value(fmax(d2, 0.0), ie, is);
             if (a < v.K && b < v.Kp) out[(int64_t)a * v.Kp + b] = x;
