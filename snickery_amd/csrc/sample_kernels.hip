@@ -70,13 +70,13 @@ sample_rows_wave_kernel(const T *__restrict__ scores, int64_t stride, int64_t R,
     for (int e = 0; e < E; ++e) row.w[e] = x[e] == ninf ? 0 : sample_weight(sample_exponent(x[e], m, rule.inv_tau), unit);
     wave_row_keep<E>(x, rule, unit, row);
     const double log_total = log((double)row.total / unit);
-    for (int d = 0; d < n_draws; ++d) {
-        int l, s;
-        const int pick = wave_row_pick<E>(row, u[r * n_draws + d], l, s);
-        const double lp = sample_exponent(wave_row_value<E>(x, l, s), m, rule.inv_tau) - log_total;
-        if (lane == 0) {
-            index[r * n_draws + d] = pick;
-            if (logp) logp[r * n_draws + d] = lp;
+    for (int d0 = 0; d0 < n_draws; d0 += 64) {                  // a lane has a draw
+        const int n = n_draws - d0 < 64 ? n_draws - d0 : 64;
+        const int64_t at = r * n_draws + d0 + lane;
+        const int pick = wave_row_picks<E>(row, lane < n ? u[at] : 0.0, n);
+        if (lane < n) {
+            index[at] = pick;
+            if (logp) logp[at] = sample_exponent(score_load(p + pick), m, rule.inv_tau) - log_total;
         }
     }
 }

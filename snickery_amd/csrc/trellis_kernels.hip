@@ -1240,10 +1240,10 @@ trellis_pointer_kernel(const TrellisView v, const int *__restrict__ flag, const 
     if (last) {                                                 // the path's end
         if (blockIdx.y || wave) return;
         const bool any = trellis_row<E>(vt, logs, rule, x, row, m);
-        for (int s = 0; s < n_draws; ++s) {
-            int l, slot, k = -1;
-            if (any) k = wave_row_pick<E>(row, greedy ? 0.0 : u[(int64_t)s * all_rows + t], l, slot);
-            if (lane == 0) root[(int64_t)s * all_utts + utt] = k;
+        for (int s = lane; s - lane < n_draws; s += 64) {       // a lane has a draw
+            const double r = greedy || s >= n_draws ? 0.0 : u[(int64_t)s * all_rows + t];
+            const int k = any ? wave_row_picks<E>(row, r, min(n_draws - (s - lane), 64)) : -1;
+            if (s < n_draws) root[(int64_t)s * all_utts + utt] = k;
         }
         return;
     }
@@ -1253,6 +1253,7 @@ trellis_pointer_kernel(const TrellisView v, const int *__restrict__ flag, const 
         const int a = i >> 5, b = i & 31;
         cells[b * LDA + a] = b0 + b < K ? c[a * Kp + b0 + b] : 0.0;
     }
+    const double first = greedy || lane >= n_draws ? 0.0 : u[(int64_t)lane * all_rows + t];
     __syncthreads();
     for (int b = wave; b < SNK_POINTER_COLUMNS && b0 + b < K; b += 4) {
         double p[E];
@@ -1263,10 +1264,10 @@ trellis_pointer_kernel(const TrellisView v, const int *__restrict__ flag, const 
             p[e] = logs ? vt[e] + cell : vt[e] * cell;
         }
         const bool any = trellis_row<E>(p, logs, rule, x, row, m);
-        for (int s = 0; s < n_draws; ++s) {
-            int l, slot, k = 0;                                 // (a candidate nothing leads to is on no path)
-            if (any) k = wave_row_pick<E>(row, greedy ? 0.0 : u[(int64_t)s * all_rows + t], l, slot);
-            if (lane == 0) pointer[((int64_t)s * all_rows + t) * K + b0 + b] = (unsigned char)k;
+        for (int s = lane; s - lane < n_draws; s += 64) {
+            const double r = s < 64 ? first : greedy || s >= n_draws ? 0.0 : u[(int64_t)s * all_rows + t];
+            const int k = any ? wave_row_picks<E>(row, r, min(n_draws - (s - lane), 64)) : 0;        // (a candidate nothing leads to is on no path)
+            if (s < n_draws) pointer[((int64_t)s * all_rows + t) * K + b0 + b] = (unsigned char)k;
         }
     }
 }
