@@ -136,7 +136,10 @@ int snk_knn_viterbi(snk_handle h, const double *Q, int64_t T, int D, int K,
 int snk_knn_viterbi_batch(snk_handle h, const double *Q, const int64_t *row_offsets,
                           int n_utts, int D, int K,
                           int64_t *path_out, int64_t *path_len_out, double *cost_out);
-/* optional: page-lock a host buffer that is uploaded repeatedly (queued instead of blocking copies) */
+/* optional: page-locked memory for a host buffer that is uploaded repeatedly (queued instead of blocking copies); snk_host_register
+ * locks memory that exists already, which not every system lets a process do (an error then) */
+int snk_host_alloc(size_t bytes, void **ptr_out);
+int snk_host_free(void *ptr);
 int snk_host_register(void *ptr, size_t bytes);
 int snk_host_unregister(void *ptr);
 /* The same in two halves: submit() queues the whole batch and returns, collect() waits for it.  Three

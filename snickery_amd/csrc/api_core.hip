@@ -62,7 +62,7 @@ int staged_d2h(snk_engine *h, hipStream_t st, const D2HPart *parts, int n)
 
 // ---------------------------------------------------------------------------
 // Host <-> device copies.  The GPU (its DMA engines, the runtime's copy kernels) only ever touches page-locked memory
-// that THIS library allocated (hipHostMalloc) or that the caller registered (snk_host_register): caller buffers are
+// that THIS library allocated (hipHostMalloc, snk_host_alloc) or that the caller registered (snk_host_register): caller buffers are
 // ordinary pageable memory (numpy arrays, stack variables), and handing those to hipMemcpyAsync makes the runtime pin
 // and map them on the fly -- a process that frees and reuses such memory all the time (a Python test session, a tuning
 // loop) was seen to die with "Memory access fault by GPU node ... on address <an address of the host heap>" inside an
@@ -760,7 +760,26 @@ int no_batch_in_flight(snk_engine *h, const char *who)
 int snk_host_register(void *ptr, size_t bytes)
 {
     if (!ptr || !bytes) return fail("snk_host_register: null/empty buffer");
-    HIPCHK(hipHostRegister(ptr, bytes, hipHostRegisterDefault));
+    const hipError_t e = hipHostRegister(ptr, bytes, hipHostRegisterDefault);
+    if (e == hipSuccess) return 0;
+    (void)hipGetLastError();                               // (a later call would report it as its own)
+    return fail("snk_host_register: %s (snk_host_alloc gives page-locked memory of its own)", hipGetErrorString(e));
+}
+
+int snk_host_alloc(size_t bytes, void **ptr_out)
+{
+    if (!bytes || !ptr_out) return fail("snk_host_alloc: null/empty buffer");
+    *ptr_out = nullptr;
+    const hipError_t e = hipHostMalloc(ptr_out, bytes, hipHostMallocDefault);
+    if (e == hipSuccess) return 0;
+    (void)hipGetLastError();
+    return fail("snk_host_alloc: %zu bytes: %s", bytes, hipGetErrorString(e));
+}
+
+int snk_host_free(void *ptr)
+{
+    if (!ptr) return fail("snk_host_free: null buffer");
+    HIPCHK(hipHostFree(ptr));
     return 0;
 }
 

@@ -6,6 +6,8 @@ in ``snickery_amd.synthesiser``: same argument meaning, numpy in / numpy out.
 """
 import ctypes
 import os
+import weakref
+
 import numpy as np
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -77,6 +79,8 @@ _SIGNATURES = {
                                         ctypes.c_double, _c_i64p, _c_f64p, _c_i64p]),
     'snk_set_column_selection': (ctypes.c_int, [ctypes.c_void_p, ctypes.POINTER(ctypes.c_int), ctypes.c_int,
                                                 ctypes.POINTER(ctypes.c_int), ctypes.c_int]),
+    'snk_host_alloc': (ctypes.c_int, [ctypes.c_size_t, ctypes.POINTER(ctypes.c_void_p)]),
+    'snk_host_free': (ctypes.c_int, [ctypes.c_void_p]),
     'snk_host_register': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_size_t]),
     'snk_host_unregister': (ctypes.c_int, [ctypes.c_void_p]),
     'snk_knn_viterbi_batch_submit': (ctypes.c_int, [ctypes.c_void_p, _c_f64p, _c_i64p, ctypes.c_int, ctypes.c_int,
@@ -204,21 +208,20 @@ class QueryBatch(object):
         return len(self.lengths)
 
     def pin(self):
-        """Page-lock the rows (hipHostRegister): uploads of this batch are then queued on the stream
-        instead of making the host wait for it.  Undone when the batch is garbage collected."""
-        if not getattr(self, '_pinned', False):
+        """Move the rows to page-locked memory: uploads of this batch are then queued on the stream instead of making the host
+        wait for it.  The memory is given back when neither the batch nor a subset taken of it since uses it any more."""
+        if not getattr(self, '_pinned', False) and self.Q.nbytes:
             lib = load_library()
-            if lib.snk_host_register(ctypes.c_void_p(self.Q.ctypes.data), self.Q.nbytes) != 0:
+            p = ctypes.c_void_p()
+            if lib.snk_host_alloc(self.Q.nbytes, ctypes.byref(p)) != 0:
                 raise SnkError(lib.snk_last_error().decode('utf-8', 'replace'))
+            memory = (ctypes.c_double * self.Q.size).from_address(p.value)
+            weakref.finalize(memory, lib.snk_host_free, p)
+            rows = np.frombuffer(memory, dtype=np.float64).reshape(self.Q.shape)
+            rows[:] = self.Q
+            self.Q = rows
             self._pinned = True
         return self
-
-    def __del__(self):
-        if getattr(self, '_pinned', False):
-            try:
-                load_library().snk_host_unregister(ctypes.c_void_p(self.Q.ctypes.data))
-            except Exception:
-                pass
 
     def subset(self, lo, hi):
         """Utterances lo..hi-1 as a batch of their own (a view of the same rows)."""
