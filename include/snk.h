@@ -322,7 +322,7 @@ int snk_copy_to_device(void *dst_dev, const void *src_host, int64_t bytes);
  *   index_out (R, n_draws) int64; logp_out (R, n_draws) float64, or NULL: log of the drawn weight over the kept weight
  * Draws are reproducible: sums of weights are whole numbers, the same in any order.  V is at most 2^24.
  * The _dev form takes device memory throughout and puts its kernels on `stream` (a hipStream_t; NULL: the default stream)
- * without waiting, and can be captured into a graph (rows of more than 1024 scores then take a slower form that needs none
+ * without waiting, and can be captured into a graph (rows of more than 8192 scores then take a slower form that needs none
  * of the engine's workspace).  It cannot look at device memory first: a number
  * u below 0 or NaN draws the first kept index, one of 1 or more the last; a row rule without meaning counts as off (a temperature
  * as 0). */

@@ -1,7 +1,7 @@
 // C ABI of libsnkhip.so, part 6: draws and probabilities over the candidates of a preselection (include/snk.h snk_sample_rows,
 // snk_set_position_bias, snk_sample_paths, snk_path_posterior).
 //
-// Streams.  snk_sample_rows_dev puts its kernels straight on the caller's stream; rows of more than 1024 scores use the engine's
+// Streams.  snk_sample_rows_dev puts its kernels straight on the caller's stream; rows of more than 8192 scores use the engine's
 // row workspace, which a later call on another stream waits for.  The trellis calls
 // use the engine's workspaces, so their kernels run on the engine's main stream, in the order of the calls; a _dev call makes that
 // stream wait for what the caller's stream holds and the caller's stream for the results, without a host wait in between.

@@ -322,6 +322,218 @@ sample_rows_block_kernel(const T *__restrict__ scores, int64_t stride, int64_t V
     }
 }
 
+__device__ __forceinline__ int score_bin(double e, double scale, int bins)
+{
+    const double b = -e * scale;
+    return b < (double)(bins - 1) ? (int)b : bins - 1;
+}
+
+// ---- rows of up to 8 NT scores: a workgroup each, the row in registers ---------------------------------------------------------------
+// One read of the row and one launch.  A prefix of the order is found as below for longer rows -- the bin of the exponent in which the
+// count or the mass reaches its goal, then the place among that bin's scores by radix on their keys -- but bins and digits are in LDS
+// and the scores never leave the registers: no list, nothing left over, no workspace that a captured graph would share.  A thread's
+// scores are neighbours, so that the ranks of equal ones and the kept mass are scans over the threads.  128 registers at most, some
+// spilled: with 190 and none the rows of 2048 and 4096 scores took 86 and 115 us instead of 74 and 78.  Bound by the scans' and the
+// radix's barriers, some 30 of them.  float32, top_p 0.9, 8.4 million scores in all:
+//     scores a row     1025   2000   4096   8192 us, one row 8192
+//     this              139     78     78    117              27
+//     passes below      677    370    214    147              50
+// Sixteen scores a thread, rows of 16384: 169 us, the passes below 125.
+#define SNK_HELD_MOST 8192
+template <typename T, int NT, int EACH>
+__global__ void __launch_bounds__(NT, 4)
+sample_rows_held_kernel(const T *__restrict__ scores, int64_t stride, int V, const double *__restrict__ u, int n_draws, SampleRule call,
+                        const double *__restrict__ rules, double unit, int64_t *__restrict__ index, double *__restrict__ logp)
+{
+    constexpr int BINS = 1024, PER = BINS / NT, NW = NT / 64;
+    __shared__ BlockScratch<NT> scratch;
+    __shared__ u64 bin_mass[BINS], digit_mass[256], sh_above;
+    __shared__ unsigned int bin_count[BINS], digit_count[256];
+    __shared__ double ends[2 * NW];
+    __shared__ int sh_bin, sh_digit;
+    const int tid = threadIdx.x, at = tid * EACH;
+    const int64_t r = blockIdx.x;
+    const SampleRule rule = sample_rule(call, rules, r);
+    const T *__restrict__ p = scores + r * stride;
+    const double inf = __builtin_inf();
+    double x[EACH];
+    if ((((uintptr_t)p) & 15) == 0 && at + EACH <= V) {
+        union { uint4 w[EACH * sizeof(T) / 16]; T v[EACH]; } raw;
+#pragma unroll
+        for (int j = 0; j < (int)(EACH * sizeof(T) / 16); ++j) raw.w[j] = reinterpret_cast<const uint4 *>(p + at)[j];
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) x[j] = score_load(raw.v + j);
+    } else {
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) x[j] = at + j < V ? score_load(p + at + j) : -inf;
+    }
+    // largest and smallest of the scores that `in` marks
+    auto extremes = [&](unsigned int in, double &most, double &least) {
+        most = -inf; least = inf;
+#pragma unroll
+        for (int j = 0; j < EACH; ++j)
+            if ((in >> j) & 1) { most = fmax(most, x[j]); least = fmin(least, x[j]); }
+        most = wave_max(most);
+        least = -wave_max(-least);
+        __syncthreads();
+        if ((tid & 63) == 0) { ends[tid >> 6] = most; ends[NW + (tid >> 6)] = least; }
+        __syncthreads();
+        for (int i = 0; i < NW; ++i) { most = fmax(most, ends[i]); least = fmin(least, ends[NW + i]); }
+    };
+    unsigned int in = 0;
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) in |= x[j] > -inf ? 1u << j : 0;
+    double m, least;
+    extremes(in, m, least);
+    if (m == -inf) {
+        for (int d = tid; d < n_draws; d += NT) {
+            index[r * n_draws + d] = -1;
+            if (logp) logp[r * n_draws + d] = m;
+        }
+        return;
+    }
+    u64 q[EACH];                                                // weights; 0: not kept
+    unsigned int bins[EACH / 2];                                // two scores' bins a word
+    const bool counted = rule.top_k > 0 && rule.top_k < V, shared = rule.top_p < 1.0;
+    const double range = fmin(-sample_exponent(least, m, rule.inv_tau), -SNK_SAMPLE_FLOOR);
+    const double scale = range > 0.0 ? fmin((double)BINS / range, 1e300) : 0.0;
+    for (int i = tid; i < BINS; i += NT) { bin_mass[i] = 0; bin_count[i] = 0; }
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+        const double e = sample_exponent(x[j], m, rule.inv_tau);
+        q[j] = x[j] == -inf ? 0 : sample_weight(e, unit);
+        const unsigned int b = q[j] ? score_bin(e, scale, BINS) : 0;
+        if (q[j] && (counted || shared)) {
+            atomicAdd(&bin_mass[b], q[j]);
+            atomicAdd(&bin_count[b], 1u);
+        }
+        bins[j / 2] = j & 1 ? bins[j / 2] | b << 16 : b;
+    }
+    __syncthreads();
+    u64 total = 0;                                              // mass that top_k keeps
+#pragma unroll 1
+    for (int by_mass = 0; by_mass < 2; ++by_mass) {
+        if (by_mass ? !shared : !counted) continue;
+        // the bin
+        u64 vm[PER], vc[PER], sm = 0, sc = 0, total_m, total_c;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) { vm[i] = bin_mass[tid * PER + i]; vc[i] = bin_count[tid * PER + i]; sm += vm[i]; sc += vc[i]; }
+        if (tid == 0) sh_bin = -1;
+        u64 um = sm, uc = sc;
+        block_scan2<NT>(um, uc, total_m, total_c, scratch);
+        const u64 want = by_mass ? sample_reach(rule.top_p, total ? total : total_m) : (u64)rule.top_k;
+        const u64 upto = by_mass ? um : uc;
+        u64 a = upto - (by_mass ? sm : sc);
+        if (a < want && upto >= want) {
+            bool found = false;
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+                const u64 n = by_mass ? vm[i] : vc[i];
+                if (!found && a + n >= want) { found = true; sh_bin = tid * PER + i; sh_above = a; }
+                a += n;
+            }
+        }
+        __syncthreads();
+        const int bin = sh_bin;
+        u64 above = sh_above;
+        __syncthreads();
+        if (bin < 0) continue;                                  // fewer scores than the goal
+        // its scores, and the one among them at which the order reaches the goal
+        in = 0;
+#pragma unroll
+        for (int j = 0; j < EACH; ++j)
+            in |= q[j] && (int)((bins[j / 2] >> (j & 1 ? 16 : 0)) & 0xffff) == bin ? 1u << j : 0;
+        double high, low;
+        extremes(in, high, low);
+        const u64 key_min = score_key<double>(low), key_max = score_key<double>(high);
+        u64 key = key_min;
+        if (key_min != key_max) {
+            // (keys that differ share their leading bits: start at the first digit in which they do)
+            int shift = ((63 - __clzll((long long)(key_min ^ key_max))) >> 3) << 3;
+            u64 prefix = shift + 8 < 64 ? (key_min >> (shift + 8)) << (shift + 8) : 0;
+            for (; shift >= 0; shift -= 8) {
+                for (int i = tid; i < 256; i += NT) { digit_mass[i] = 0; digit_count[i] = 0; }
+                if (tid == 0) { sh_digit = 0; sh_above = above; }
+                __syncthreads();
+#pragma unroll
+                for (int j = 0; j < EACH; ++j)
+                    if ((in >> j) & 1) {
+                        double v = x[j];
+                        asm volatile("" : "+v"(v));             // (or all the keys are made before the loop and kept beside the scores)
+                        const u64 k = score_key<double>(v);
+                        if (shift + 8 < 64 && (k >> (shift + 8)) != (prefix >> (shift + 8))) continue;
+                        const int digit = (int)((k >> shift) & 255);
+                        if (by_mass) atomicAdd(&digit_mass[digit], q[j]);
+                        else atomicAdd(&digit_count[digit], 1u);
+                    }
+                __syncthreads();
+                if (tid < 64) {
+                    // lane l: digits 255 - 4 l .. 252 - 4 l, from the top
+                    u64 v[4], sum = 0;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) { const int d = 255 - (4 * tid + j); v[j] = by_mass ? digit_mass[d] : (u64)digit_count[d]; sum += v[j]; }
+                    const u64 reach = wave_scan_add(sum), hit = __ballot(above + reach >= want);
+                    if (hit && tid == __ffsll((long long)hit) - 1) {
+                        u64 b = above + reach - sum;
+                        for (int j = 0; j < 4; ++j) {
+                            if (b + v[j] >= want) { sh_digit = 255 - (4 * tid + j); sh_above = b; break; }
+                            b += v[j];
+                        }
+                    }
+                }
+                __syncthreads();
+                above = sh_above;
+                prefix |= (u64)sh_digit << shift;
+                __syncthreads();
+            }
+            key = prefix;
+        }
+        const double cut = __longlong_as_double((long long)((key >> 63) ? key & 0x7fffffffffffffffull : ~key));
+        const u64 each = sample_weight(sample_exponent(cut, m, rule.inv_tau), unit);
+        u64 n_tie = by_mass ? (each ? (want - above + each - 1) / each : 0) : want - above;
+        u64 ties = 0, mass = 0, all_ties, all_mass;
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) {
+            if (q[j] && x[j] == cut) ++ties;
+            if (x[j] > cut) mass += q[j];
+        }
+        u64 rank = ties;
+        block_scan2<NT>(rank, mass, all_ties, all_mass, scratch);
+        rank -= ties;                                           // equal ones before this thread's
+        if (n_tie > all_ties) n_tie = all_ties;
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) {
+            const bool tie = q[j] && x[j] == cut;
+            if (x[j] < cut || (tie && rank >= n_tie)) q[j] = 0;
+            rank += tie ? 1 : 0;
+        }
+        total = all_mass + each * n_tie;
+    }
+    u64 mass = 0, none = 0, kept, unused;
+#pragma unroll
+    for (int j = 0; j < EACH; ++j) {
+        if (rule.min_p > 0.0 && (double)q[j] < rule.min_p * unit) q[j] = 0;
+        mass += q[j];
+    }
+    u64 upto = mass;
+    block_scan2<NT>(upto, none, kept, unused, scratch);
+    const double log_kept = logp ? log((double)kept / unit) : 0.0;
+    for (int d = 0; d < n_draws; ++d) {
+        const u64 t = sample_exceed(u[r * n_draws + d], kept);
+        if (t >= upto || t < upto - mass) continue;
+        u64 c = upto - mass;
+        int pick = at;                                          // weights that do not reach t are passed over
+#pragma unroll
+        for (int j = 0; j < EACH - 1; ++j) {
+            c += q[j];
+            pick += c <= t ? 1 : 0;
+        }
+        index[r * n_draws + d] = pick;
+        if (logp) logp[r * n_draws + d] = sample_exponent(score_load(p + pick), m, rule.inv_tau) - log_kept;
+    }
+}
+
 // ---- longer rows, every pass over all of the chip ----------------------------------------------------------------------------------
 // A row is cut into chunks of SNK_CHUNK scores, a workgroup each:
 //   extremes   the chunks' largest and smallest score
@@ -417,12 +629,6 @@ rows_extremes_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, co
         w.chunk_max[r * w.chunks + c] = hi[0];
         w.chunk_min[r * w.chunks + c] = lo[0];
     }
-}
-
-__device__ __forceinline__ int score_bin(double e, double scale, int bins)
-{
-    const double b = -e * scale;
-    return b < (double)(bins - 1) ? (int)b : bins - 1;
 }
 
 template <typename T>
@@ -772,10 +978,10 @@ static int64_t rows_chunks(int64_t V) { return (V + SNK_CHUNK - 1) / SNK_CHUNK; 
 static unsigned int rows_list(int64_t V) { return V < SNK_LIST ? (unsigned int)V : SNK_LIST; }
 #define SNK_ALIGNED(bytes_) (((size_t)(bytes_) + 255) & ~(size_t)255)
 
-// rows of more than 1024 scores: bytes of workspace a row takes, and how many rows go together at most (2 GB)
+// rows that no workgroup holds: bytes of workspace a row takes, and how many rows go together at most (2 GB)
 size_t sample_rows_work_bytes(int64_t V)
 {
-    if (V <= 1024) return 0;
+    if (V <= SNK_HELD_MOST) return 0;
     const size_t c = (size_t)rows_chunks(V), b = (size_t)rows_bins(V);
     return sizeof(RowState) + c * (2 * sizeof(double) + sizeof(u64) + sizeof(unsigned int)) + b * 12 + rows_list(V) * sizeof(double) + sizeof(int);
 }
@@ -786,7 +992,7 @@ int64_t sample_rows_together(int64_t R, int64_t V)
     const int64_t most = (int64_t)(((size_t)2 << 30) / each);
     return std::min<int64_t>(R, std::max<int64_t>(1, std::min<int64_t>(most, 32768)));
 }
-size_t sample_rows_work(int64_t rows, int64_t V) { return V <= 1024 ? 0 : rows * sample_rows_work_bytes(V) + 16 * 256; }
+size_t sample_rows_work(int64_t rows, int64_t V) { return V <= SNK_HELD_MOST ? 0 : rows * sample_rows_work_bytes(V) + 16 * 256; }
 
 template <typename T>
 static void launch_rows_split(const T *scores, int64_t stride, int64_t R, int64_t V, const double *u, int n_draws, const SampleRule &rule,
@@ -830,16 +1036,22 @@ static void launch_sample_t(const T *scores, int64_t stride, int64_t R, int64_t 
     if (s_bits > 51) s_bits = 51;
     const double unit = (double)(1ull << s_bits);
 #define SNK_WAVE(E_) hipLaunchKernelGGL((sample_rows_wave_kernel<T, E_>), dim3((unsigned)((R + 3) / 4)), dim3(256), 0, s, scores, stride, R, (int)V, u, n_draws, rule, rules, unit, index, logp)
+#define SNK_HELD(NT_, EACH_) hipLaunchKernelGGL((sample_rows_held_kernel<T, NT_, EACH_>), dim3((unsigned)R), dim3(NT_), 0, s, scores, stride, (int)V, u, n_draws, rule, rules, unit, index, logp)
     if (V <= 64) SNK_WAVE(1);
     else if (V <= 128) SNK_WAVE(2);
     else if (V <= 256) SNK_WAVE(4);
     else if (V <= 512) SNK_WAVE(8);
     else if (V <= 1024) SNK_WAVE(16);
-    else if (work) launch_rows_split(scores, stride, R, V, u, n_draws, rule, rules, unit, work, index, logp, s);
+    else if (V <= SNK_HELD_MOST) {
+        if (V <= 2048) SNK_HELD(256, 8);
+        else if (V <= 4096) SNK_HELD(512, 8);
+        else SNK_HELD(1024, 8);
+    } else if (work) launch_rows_split(scores, stride, R, V, u, n_draws, rule, rules, unit, work, index, logp, s);
     else
         hipLaunchKernelGGL((sample_rows_block_kernel<T, 1024>), dim3((unsigned)R), dim3(1024), 0, s, scores, stride, V, u, n_draws, rule, rules, unit,
                            (const int *)nullptr, index, logp);
 #undef SNK_WAVE
+#undef SNK_HELD
 }
 
 int64_t sample_rows_max() { return (int64_t)SNK_SAMPLE_TILES * 1024 * SNK_SAMPLE_VEC; }

@@ -236,10 +236,32 @@ def test_rows_on_another_stream_and_in_a_graph(engine):
             assert torch.equal(eager, i)
 
 
+def test_long_rows_in_a_graph(engine):
+    """Rows whose workspace a graph would share with later calls: captured, replayed between eager calls of other sizes."""
+    import torch
+    rng = np.random.RandomState(8)
+    side = torch.cuda.Stream()
+    x, u = [rng.randn(6, 20000).astype(np.float32) for _ in range(3)], [rng.rand(6, 2) for _ in range(3)]
+    want = [o.sample_rows(a, b, top_k=300, top_p=0.9)[0] for a, b in zip(x, u)]
+    with torch.cuda.stream(side):
+        gx, gu = on_gpu(x[0]), on_gpu(u[0])
+    side.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        i, _ = engine.sample_rows(gx, gu, top_k=300, top_p=0.9)
+    for n in range(3):
+        gx.copy_(on_gpu(x[n])); gu.copy_(on_gpu(u[n]))
+        graph.replay()
+        eager, _ = engine.sample_rows(on_gpu(x[n]), on_gpu(u[n]), top_k=300, top_p=0.9)
+        engine.sample_rows(on_gpu(rng.randn(2, 70000)), on_gpu(rng.rand(2, 1)), top_p=0.5)
+        torch.cuda.synchronize()
+        assert np.array_equal(i.cpu().numpy(), want[n]) and torch.equal(eager, i)
+
+
 def test_rows_of_many_draws(engine):
     """More draws than a launch's second dimension holds."""
     rng = np.random.RandomState(9)
-    for V, draws in ((1500, 70000), (40, 70000)):
+    for V, draws in ((9000, 70000), (1500, 70000), (40, 70000)):
         x, u = rng.randn(2, V).astype(np.float32), rng.rand(2, draws)
         i, lp = [a.cpu().numpy() for a in engine.sample_rows(on_gpu(x), on_gpu(u), top_p=0.9)]
         some = np.r_[0:50, 32760:32780, 65530:65540, draws - 50:draws]
@@ -247,6 +269,41 @@ def test_rows_of_many_draws(engine):
         assert np.array_equal(i[:, some], want)
         assert np.all(np.abs(lp[:, some] - want_lp) <= logp_tolerance(V, np.abs(want_lp).max()))
         assert i.min() >= 0
+
+
+@pytest.mark.parametrize('dtype', ['float32', 'float64', 'float16', 'bfloat16'])
+@pytest.mark.parametrize('V', [1025, 2047, 2048, 2049, 4095, 4097, 8191, 8192, 8193])
+def test_rows_at_the_borders_of_the_workgroups_sizes(engine, V, dtype):
+    rng = np.random.RandomState(V)
+    x, u = scores_of(rng, 5, V, dtype), rng.rand(5, 2)
+    x[1, :] = -np.inf
+    x[2, :] = -np.inf
+    x[2, V - 1] = 3.0
+    x[3, :V // 2] = x[3, 0]                                  # equal ones
+    for rule in RULES:
+        check_rows(engine, x, u, **rule)
+
+
+@pytest.mark.parametrize('V', [1500, 5000, 8000])
+def test_rows_in_a_workgroup_whose_scores_crowd(engine, V):
+    """Every score in one bin but for one that stretches the range; equal in all but the last bits; few different ones."""
+    rng = np.random.RandomState(V)
+    x = np.zeros((5, V))
+    x[0] = rng.permutation(V) * 2.0 ** -52 + 1.0
+    x[1] = rng.permutation(V) / 2.0 ** 30
+    x[1, V // 3] = -30.0
+    x[2] = rng.randint(0, 3, V) * 2.0 ** -40
+    x[3] = 7.0
+    x[4] = -rng.rand(V) * 40.0
+    u = rng.rand(5, 70)                                     # more draws than a wavefront has lanes
+    for rule in (dict(top_k=V // 2), dict(top_k=1), dict(top_p=0.37), dict(top_p=1e-9), dict(top_k=V - 1, top_p=0.999), dict(top_k=100, top_p=0.5, min_p=0.9)):
+        check_rows(engine, x, u, **rule)
+
+
+@pytest.mark.parametrize('V', [30, 900])
+def test_rows_of_a_hundred_draws(engine, V):
+    rng = np.random.RandomState(V)
+    check_rows(engine, rng.randn(7, V), rng.rand(7, 100), top_p=0.8)
 
 
 @pytest.mark.parametrize('dtype', ['float32', 'float64', 'bfloat16'])
