@@ -322,16 +322,18 @@ int snk_copy_to_device(void *dst_dev, const void *src_host, int64_t bytes);
  *   index_out (R, n_draws) int64; logp_out (R, n_draws) float64, or NULL: log of the drawn weight over the kept weight
  * Draws are reproducible: sums of weights are whole numbers, the same in any order.  V is at most 2^24.
  * The _dev form takes device memory throughout and puts its kernels on `stream` (a hipStream_t; NULL: the default stream)
- * without waiting, and can be captured into a graph (rows of more than 8192 scores then take a slower form that needs none
- * of the engine's workspace).  It cannot look at device memory first: a number
- * u below 0 or NaN draws the first kept index, one of 1 or more the last; a row rule without meaning counts as off (a temperature
- * as 0). */
+ * without waiting, and can be captured into a graph.  Rows of more than 8192 scores use a workspace: `workspace`, device memory of
+ * at least snk_sample_rows_workspace(R, V) bytes (0: none needed), aligned to 16, that nothing else uses until the call's kernels
+ * are done; or NULL for the engine's own, which a graph cannot share with later calls -- a captured call without a workspace takes a
+ * slower form.  It cannot look at device memory first: a number u below 0 or NaN draws the first kept index, one of 1 or more the
+ * last; a row rule without meaning counts as off (a temperature as 0). */
 int snk_sample_rows(snk_handle h, const void *scores, int dtype, int64_t R, int64_t V, int64_t row_stride, const double *u, int n_draws,
                     double temperature, int64_t top_k, double top_p, double min_p, const double *row_rules,
                     int64_t *index_out, double *logp_out);
 int snk_sample_rows_dev(snk_handle h, const void *scores_dev, int dtype, int64_t R, int64_t V, int64_t row_stride, const double *u_dev,
                         int n_draws, double temperature, int64_t top_k, double top_p, double min_p, const double *row_rules_dev,
-                        int64_t *index_dev_out, double *logp_dev_out, void *stream);
+                        int64_t *index_dev_out, double *logp_dev_out, void *workspace, size_t workspace_bytes, void *stream);
+size_t snk_sample_rows_workspace(int64_t R, int64_t V);
 
 /* A bias on the relative position of consecutive units of a path, by buckets: joining unit i to unit j adds
  * bias[class, bucket(j - i)] to the join cost, bucket(d) = number of edges <= d, class = the join's own (join_class below).

@@ -1,8 +1,8 @@
 // C ABI of libsnkhip.so, part 6: draws and probabilities over the candidates of a preselection (include/snk.h snk_sample_rows,
 // snk_set_position_bias, snk_sample_paths, snk_path_posterior).
 //
-// Streams.  snk_sample_rows_dev puts its kernels straight on the caller's stream; rows of more than 8192 scores use the engine's
-// row workspace, which a later call on another stream waits for.  The trellis calls
+// Streams.  snk_sample_rows_dev puts its kernels straight on the caller's stream; rows of more than 8192 scores use the caller's
+// workspace or the engine's, which a later call on another stream waits for.  The trellis calls
 // use the engine's workspaces, so their kernels run on the engine's main stream, in the order of the calls; a _dev call makes that
 // stream wait for what the caller's stream holds and the caller's stream for the results, without a host wait in between.
 #include "snk_engine.h"
@@ -119,7 +119,7 @@ int snk_sample_rows(snk_handle h, const void *scores, int dtype, int64_t R, int6
 
 int snk_sample_rows_dev(snk_handle h, const void *scores_dev, int dtype, int64_t R, int64_t V, int64_t row_stride, const double *u_dev,
                         int n_draws, double temperature, int64_t top_k, double top_p, double min_p, const double *row_rules_dev,
-                        int64_t *index_dev_out, double *logp_dev_out, void *stream)
+                        int64_t *index_dev_out, double *logp_dev_out, void *workspace, size_t workspace_bytes, void *stream)
 {
     const char *who = "snk_sample_rows_dev";
     if (!h) return fail("null handle");
@@ -127,15 +127,25 @@ int snk_sample_rows_dev(snk_handle h, const void *scores_dev, int dtype, int64_t
     if (R == 0) return 0;
     if (!scores_dev || !u_dev || !index_dev_out) return fail("%s: null argument", who);
     if (!row_rules_dev) CHK(check_rule(who, temperature, top_k, top_p, min_p));
+    const size_t need = snk_sample_rows_workspace(R, V);
+    if (workspace && ((uintptr_t)workspace & 15)) return fail("%s: the workspace is not aligned to 16 bytes", who);
+    if (workspace && workspace_bytes < need) return fail("%s: a workspace of %zu bytes, %zu needed", who, workspace_bytes, need);
     DeviceGuard device;
     CHK(device.enter(h->device));
     const SampleRuleHost rule = {temperature, top_k, top_p, min_p};
-    char *work;
-    CHK(rows_workspace(h, who, R, V, (hipStream_t)stream, &work));
+    char *work = need ? (char *)workspace : nullptr;
+    const bool own = !work;
+    if (own) CHK(rows_workspace(h, who, R, V, (hipStream_t)stream, &work));
     launch_sample_rows(scores_dev, dtype, row_stride, R, V, u_dev, n_draws, rule, row_rules_dev, work, index_dev_out, logp_dev_out, (hipStream_t)stream);
     HIPCHK(hipGetLastError());
-    if (work) CHK(rows_workspace_used(h, (hipStream_t)stream));
+    if (own && work) CHK(rows_workspace_used(h, (hipStream_t)stream));
     return 0;
+}
+
+size_t snk_sample_rows_workspace(int64_t R, int64_t V)
+{
+    if (R < 1 || V < 1 || V > sample_rows_max()) return 0;
+    return sample_rows_work(sample_rows_together(R, V), V);
 }
 
 int snk_set_position_bias(snk_handle h, const double *bias, int n_classes, int n_buckets, const int64_t *edges)

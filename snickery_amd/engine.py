@@ -46,7 +46,8 @@ _SIGNATURES = {
                                        ctypes.c_void_p, ctypes.c_void_p]),
     'snk_sample_rows_dev': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_int, ctypes.c_int64, ctypes.c_int64, ctypes.c_int64, ctypes.c_void_p,
                                            ctypes.c_int, ctypes.c_double, ctypes.c_int64, ctypes.c_double, ctypes.c_double, ctypes.c_void_p,
-                                           ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p]),
+                                           ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
+    'snk_sample_rows_workspace': (ctypes.c_size_t, [ctypes.c_int64, ctypes.c_int64]),
     'snk_set_position_bias': (ctypes.c_int, [ctypes.c_void_p, _c_f64p, ctypes.c_int, ctypes.c_int, _c_i64p]),
     'snk_sample_paths': (ctypes.c_int, [ctypes.c_void_p, ctypes.c_void_p, ctypes.c_void_p, _c_i64p, ctypes.c_int, ctypes.c_int, ctypes.c_void_p,
                                         ctypes.c_void_p, ctypes.c_int, ctypes.c_double, ctypes.c_int64, ctypes.c_double, ctypes.c_double,
@@ -574,9 +575,14 @@ class HipSearchEngine(object):
             index = torch.empty(u.shape, dtype=torch.int64, device=scores.device)
             logp = torch.empty(u.shape, dtype=torch.float64, device=scores.device)
             rule = (1.0, 0, 1.0, 0.0) if per_row else self._rule(*rules)
+            work = None
+            if V > 1024 and torch.cuda.is_current_stream_capturing():       # the graph's own, not the engine's
+                need = self._lib.snk_sample_rows_workspace(R, V)
+                work = torch.empty(need, dtype=torch.uint8, device=scores.device) if need else None
             self._check(self._lib.snk_sample_rows_dev(
                 self._h, scores.data_ptr(), _SCORE_TYPES[name], R, V, scores.stride(0) if R > 1 else V, u.data_ptr(), draws, *rule,
-                table.data_ptr() if per_row else None, index.data_ptr(), logp.data_ptr(), self._stream()))
+                table.data_ptr() if per_row else None, index.data_ptr(), logp.data_ptr(), None if work is None else work.data_ptr(),
+                0 if work is None else work.numel(), self._stream()))
             return index, logp
         scores = np.asarray(scores)
         if str(scores.dtype) not in _SCORE_TYPES:

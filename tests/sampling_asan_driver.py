@@ -71,7 +71,7 @@ def p(a):
 
 
 index, logp = np.zeros((5, 3), np.int64), np.zeros((5, 3))
-for fn in (lambda *a: lib.snk_sample_rows(*a), lambda *a: lib.snk_sample_rows_dev(*a, None)):
+for fn in (lambda *a: lib.snk_sample_rows(*a), lambda *a: lib.snk_sample_rows_dev(*a, None, 0, None)):
     def call(scores=p(x), dtype=0, R=5, V=40, stride=40, u_=p(u), n=3, t=1.0, k=0, tp=1.0, mp=0.0, out=p(index), h=e._h):
         return fn(h, scores, dtype, R, V, stride, u_, n, t, k, tp, mp, None, out, p(logp))
     assert call() == 0
@@ -96,6 +96,23 @@ assert refused('bias 7', e.set_position_bias, np.where(np.arange(15).reshape(3, 
 assert refused('bias 7', e.set_position_bias, np.where(np.arange(15).reshape(3, 5) == 7, -np.inf, 0.0), edges)
 assert refused('classes', e.set_position_bias, np.zeros((65536, 1)))
 e.set_position_bias(None)
+
+# ---- a caller's workspace for long rows ----
+long_rows, lu, li = np.zeros((3, 20000)), np.full((3, 1), 0.5), np.zeros((3, 1), np.int64)
+need = lib.snk_sample_rows_workspace(3, 20000)
+assert need > 0 and lib.snk_sample_rows_workspace(3, 8192) == 0 and lib.snk_sample_rows_workspace(0, 20000) == 0
+assert lib.snk_sample_rows_workspace(3, (1 << 24) + 1) == 0 and lib.snk_sample_rows_workspace(100000, 20000) < 3 << 30
+room = np.zeros(need // 8 + 4)
+first = room.ctypes.data + (-room.ctypes.data) % 16
+
+
+def long_call(ws, n):
+    return lib.snk_sample_rows_dev(e._h, p(long_rows), 0, 3, 20000, 20000, p(lu), 1, 1.0, 5, 0.9, 0.0, None, p(li), None, ws, n, None)
+
+
+assert long_call(first, need) == 0 and long_call(None, 0) == 0
+assert long_call(first + 8, need) != 0 and b'aligned' in lib.snk_last_error()
+assert long_call(first, need - 1) != 0 and b'needed' in lib.snk_last_error()
 
 # ---- trellis ----
 T, K, N, Dj = 30, 12, 500, 21

@@ -258,6 +258,26 @@ def test_long_rows_in_a_graph(engine):
         assert np.array_equal(i.cpu().numpy(), want[n]) and torch.equal(eager, i)
 
 
+def test_long_rows_captured_without_a_workspace(engine):
+    """The C call without a workspace under capture: the form that needs none."""
+    import torch
+    rng = np.random.RandomState(4)
+    x, u = rng.randn(4, 9001), rng.rand(4, 2)
+    want = o.sample_rows(x, u, top_k=100, top_p=0.8, min_p=0.01)[0]
+    gx, gu = on_gpu(x), on_gpu(u)
+    index = torch.full((4, 2), -7, dtype=torch.int64, device='cuda')
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        stream = torch.cuda.current_stream().cuda_stream
+        assert engine._lib.snk_sample_rows_dev(engine._h, gx.data_ptr(), 0, 4, 9001, 9001, gu.data_ptr(), 2, 1.0, 100, 0.8, 0.01, None, index.data_ptr(), None,
+                                               None, 0, stream) == 0
+    for _ in range(3):
+        index.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert np.array_equal(index.cpu().numpy(), want)
+
+
 def test_rows_of_many_draws(engine):
     """More draws than a launch's second dimension holds."""
     rng = np.random.RandomState(9)
