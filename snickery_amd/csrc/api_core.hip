@@ -292,6 +292,7 @@ int snk_destroy(snk_handle h)
 static int upload_join(snk_engine *h, const float *JC_unw, int64_t Njc, int Dj)
 {
     if (!JC_unw || Njc < 2 || Dj < 1) return fail("upload: bad join matrix (Njc=%lld Dj=%d)", (long long)Njc, Dj);
+    CHK(trellis_settled(h));
     h->Njc = Njc; h->Dj = Dj; h->Djpad = roundup(Dj, 32);
     h->Jp = roundup(Dj, 4);     // 16-byte aligned rows, zero-filled padding (greedy scan: 128-bit loads)
     CHK(h->JC_unw.ensure((size_t)Njc * h->Jp * sizeof(float)));
@@ -637,6 +638,7 @@ int snk_set_weights(snk_handle h, const double *wt, int n_wt, const double *wj, 
     if (h->have_join) {
         if (!wj || n_wj != h->Dj)
             return fail("snk_set_weights: join weight vector has %d entries, join_contexts has %d columns", n_wj, h->Dj);
+        CHK(trellis_settled(h));
         CHK(h->wj.ensure((size_t)n_wj * sizeof(double)));
         std::vector<double> eff(wj, wj + n_wj);
         if (!h->jsel.empty()) {

@@ -2,9 +2,9 @@
 // snk_set_position_bias, snk_sample_paths, snk_path_posterior).
 //
 // Streams.  snk_sample_rows_dev puts its kernels straight on the caller's stream; rows of more than 8192 scores use the caller's
-// workspace or the engine's, which a later call on another stream waits for.  The trellis calls
-// use the engine's workspaces, so their kernels run on the engine's main stream, in the order of the calls; a _dev call makes that
-// stream wait for what the caller's stream holds and the caller's stream for the results, without a host wait in between.
+// workspace or the engine's, which a later call on another stream waits for.  The _dev trellis calls too run on the caller's stream: an
+// event behind each makes the next one, on whatever stream, and every call that changes what they read (join frames, weights, bias)
+// wait for its use of the workspaces.  (On the engine's stream, with an event either way, a call took 30 us more of the host's time.)
 #include "snk_engine.h"
 
 // the caller's device again when a _dev call returns
@@ -163,6 +163,7 @@ int snk_set_position_bias(snk_handle h, const double *bias, int n_classes, int n
     for (int64_t i = 0; i < n; ++i)
         if (!(bias[i] > -INFINITY)) return fail("%s: bias %lld is %g (finite, or +inf to forbid)", who, (long long)i, bias[i]);
     HIPCHK(hipSetDevice(h->device));
+    CHK(trellis_settled(h));
     h->pb_classes = 0;
     CHK(h->pb_bias.ensure((size_t)n * sizeof(double)));
     CHK(h->pb_edges.ensure(64 * sizeof(int)));
@@ -223,6 +224,7 @@ struct TrellisCall {
     const int64_t *cand; const double *tdist; const int64_t *row_offsets; const int32_t *join_class;
     int n_utts, K;
     double temperature;
+    hipStream_t stream;
 };
 
 // `use` gets the group's view (cells not made yet), the costs' parts
@@ -233,19 +235,12 @@ static int trellis_groups(snk_engine *h, const TrellisCall &q, Use use)
     const int Kp = roundup(q.K, 8);
     const size_t row_bytes = (size_t)q.K * Kp * sizeof(double);
     CHK(h->tr_off.ensure((size_t)(q.n_utts + 1) * sizeof(int64_t)));
-    // (by way of this frame: a queued copy straight out of a caller's pinned memory would still be read after a _dev call returned)
-    for (int v = 0; v <= q.n_utts; v += 2048) {
-        int64_t part[2048];
-        const size_t n = (size_t)std::min(q.n_utts + 1 - v, 2048) * sizeof(int64_t);
-        memcpy(part, q.row_offsets + v, n);
-        CHK(h2d(h, h->tr_off.as<int64_t>() + v, part, n, h->stream));
-    }
     CHK(h->tr_V.ensure((size_t)rows * Kp * sizeof(double)));
     CHK(h->tr_local.ensure((size_t)rows * Kp * sizeof(double)));
     CHK(h->tr_least.ensure((size_t)rows * sizeof(double)));
     CHK(h->tr_flag.ensure((size_t)q.n_utts * sizeof(int)));
     // temperature 0: every utterance goes through the launches that keep the largest term
-    HIPCHK(hipMemsetAsync(h->tr_flag.p, q.temperature > 0.0 ? 0 : 1, (size_t)q.n_utts * sizeof(int), h->stream));
+    launch_trellis_offsets(q.row_offsets, q.n_utts, q.temperature > 0.0 ? 0 : 1, h->tr_off.as<int64_t>(), h->tr_flag.as<int>(), q.stream);
     TrellisCosts c;
     c.JC = h->JC_unw.as<float>(); c.Jp = h->Jp; c.Dj = h->Dj; c.wj = h->wj.as<double>();
     c.join_class = q.join_class; c.bias = h->pb_bias.as<double>(); c.edges = h->pb_edges.as<int>();
@@ -289,23 +284,23 @@ static int sample_paths_device(snk_engine *h, const TrellisCall &q, const double
         double *V = h->tr_V.as<double>(), *X = h->tr_C.as<double>();
         if (sum) {
             {
-                StageTimer t(h, h->stream, q.timed ? TM_JOIN : -1);
-                launch_trellis_local(v, h->tr_local.as<double>(), h->tr_least.as<double>(), flag, h->stream);
-                launch_trellis_costs(v, c, false, flag, X, h->stream);
+                StageTimer t(h, q.stream, q.timed ? TM_JOIN : -1);
+                launch_trellis_local(v, h->tr_local.as<double>(), h->tr_least.as<double>(), flag, q.stream);
+                launch_trellis_costs(v, c, false, flag, X, q.stream);
             }
-            StageTimer t(h, h->stream, q.timed ? TM_TRELLIS_SUM : -1);
+            StageTimer t(h, q.stream, q.timed ? TM_TRELLIS_SUM : -1);
             launch_trellis_ends(v, h->tr_local.as<double>(), false, flag, h->tr_M.as<double>(), h->tr_exps.as<int>(), h->tr_ends_v.as<double>(),
-                                h->tr_ends_w.as<double>(), h->tr_scaled.as<int64_t>(), h->stream);
+                                h->tr_ends_w.as<double>(), h->tr_scaled.as<int64_t>(), q.stream);
             launch_trellis_forward(v, h->tr_local.as<double>(), h->tr_least.as<double>(), c.bias_min, h->tr_ends_v.as<double>(), h->tr_scaled.as<int64_t>(),
-                                   flag, V, nullptr, h->stream);
+                                   flag, V, nullptr, q.stream);
         }
         {
-            StageTimer t(h, h->stream, q.timed ? TM_TRELLIS_SUM : -1);
-            launch_trellis_costs(v, c, true, flag, X, h->stream);
-            launch_trellis_forward_log(v, sum, flag, V, nullptr, h->stream);
+            StageTimer t(h, q.stream, q.timed ? TM_TRELLIS_SUM : -1);
+            launch_trellis_costs(v, c, true, flag, X, q.stream);
+            launch_trellis_forward_log(v, sum, flag, V, nullptr, q.stream);
         }
-        StageTimer t(h, h->stream, q.timed ? TM_TRELLIS_DRAW : -1);
-        launch_trellis_draw(v, c, rule, flag, V, u, n_draws, rows, q.n_utts, h->tr_draw.as<char>(), path, cost, logp, h->stream);
+        StageTimer t(h, q.stream, q.timed ? TM_TRELLIS_DRAW : -1);
+        launch_trellis_draw(v, c, rule, flag, V, u, n_draws, rows, q.n_utts, h->tr_draw.as<char>(), path, cost, logp, q.stream);
         return 0;
     });
 }
@@ -319,27 +314,27 @@ static int path_posterior_device(snk_engine *h, const TrellisCall &q, double *lo
         int *flag = h->tr_flag.as<int>();
         double *V = h->tr_V.as<double>(), *W = h->tr_W.as<double>(), *X = h->tr_C.as<double>(), *local = h->tr_local.as<double>();
         {
-            StageTimer t(h, h->stream, q.timed ? TM_JOIN : -1);
-            launch_trellis_local(v, local, h->tr_least.as<double>(), flag, h->stream);
-            launch_trellis_costs(v, c, false, flag, X, h->stream);
+            StageTimer t(h, q.stream, q.timed ? TM_JOIN : -1);
+            launch_trellis_local(v, local, h->tr_least.as<double>(), flag, q.stream);
+            launch_trellis_costs(v, c, false, flag, X, q.stream);
         }
         {
-            StageTimer t(h, h->stream, q.timed ? TM_TRELLIS_SUM : -1);
+            StageTimer t(h, q.stream, q.timed ? TM_TRELLIS_SUM : -1);
             launch_trellis_ends(v, local, true, flag, h->tr_M.as<double>(), h->tr_exps.as<int>(), h->tr_ends_v.as<double>(), h->tr_ends_w.as<double>(),
-                                h->tr_scaled.as<int64_t>(), h->stream);
+                                h->tr_scaled.as<int64_t>(), q.stream);
             launch_trellis_forward(v, local, h->tr_least.as<double>(), c.bias_min, h->tr_ends_v.as<double>(), h->tr_scaled.as<int64_t>(), flag, V, logz,
-                                   h->stream);
-            launch_trellis_backward(v, local, h->tr_ends_w.as<double>(), flag, W, h->stream);
-            launch_trellis_costs(v, c, true, flag, X, h->stream);
-            launch_trellis_forward_log(v, true, flag, V, logz, h->stream);
-            launch_trellis_backward_log(v, flag, W, h->stream);
+                                   q.stream);
+            launch_trellis_backward(v, local, h->tr_ends_w.as<double>(), flag, W, q.stream);
+            launch_trellis_costs(v, c, true, flag, X, q.stream);
+            launch_trellis_forward_log(v, true, flag, V, logz, q.stream);
+            launch_trellis_backward_log(v, flag, W, q.stream);
         }
-        StageTimer t(h, h->stream, q.timed ? TM_TRELLIS_POST : -1);
+        StageTimer t(h, q.stream, q.timed ? TM_TRELLIS_POST : -1);
         launch_trellis_posterior(v, flag, V, W, h->tr_ends_w.as<double>(), local, logz, h->pb_edges.as<int>(), h->pb_buckets, posterior,
-                                 uses ? h->tr_row_uses.as<double>() : nullptr, h->stream);
+                                 uses ? h->tr_row_uses.as<double>() : nullptr, q.stream);
         return 0;
     }));
-    if (uses) launch_trellis_uses(h->tr_row_uses.as<double>(), q.join_class, rows, h->pb_classes, h->pb_buckets, uses, h->stream);
+    if (uses) launch_trellis_uses(h->tr_row_uses.as<double>(), q.join_class, rows, h->pb_classes, h->pb_buckets, uses, q.stream);
     HIPCHK(hipGetLastError());
     return 0;
 }
@@ -360,27 +355,41 @@ static int upload_trellis(snk_engine *h, const int64_t *cand, const double *tdis
     return 0;
 }
 
-// the engine's stream behind what the caller's stream holds; refused while that stream is being captured: a captured call would
-// share the engine's workspaces with every later one
-static int trellis_enter(snk_engine *h, const char *who, hipStream_t caller)
+// before a trellis call's work on stream s: behind the workspaces' last use and behind what the engine's stream holds.  Refused while s
+// is being captured: a captured call would share the engine's workspaces with every later one
+static int trellis_enter(snk_engine *h, const char *who, hipStream_t s)
 {
     hipStreamCaptureStatus st = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(caller, &st) != hipSuccess || st != hipStreamCaptureStatusNone) {
+    if (hipStreamIsCapturing(s, &st) != hipSuccess || st != hipStreamCaptureStatusNone) {
         (void)hipGetLastError();
         return fail("%s: the stream is being captured (this call uses the engine's workspaces)", who);
     }
-    if (!h->tr_in) {
-        HIPCHK(hipEventCreateWithFlags(&h->tr_in, hipEventDisableTiming));
-        HIPCHK(hipEventCreateWithFlags(&h->tr_done, hipEventDisableTiming));
-    }
-    HIPCHK(hipEventRecord(h->tr_in, caller));
-    HIPCHK(hipStreamWaitEvent(h->stream, h->tr_in, 0));
+    if (!h->tr_in) HIPCHK(hipEventCreateWithFlags(&h->tr_in, hipEventDisableTiming));
+    if (!h->tr_done) HIPCHK(hipEventCreateWithFlags(&h->tr_done, hipEventDisableTiming));
+    if (h->tr_used) HIPCHK(hipStreamWaitEvent(s, h->tr_done, 0));
+    if (s == h->stream) return 0;
+    const hipError_t idle = hipStreamQuery(h->stream);
+    if (idle == hipSuccess) return 0;
+    if (idle != hipErrorNotReady) HIPCHK(idle);
+    (void)hipGetLastError();
+    HIPCHK(hipEventRecord(h->tr_in, h->stream));
+    HIPCHK(hipStreamWaitEvent(s, h->tr_in, 0));
     return 0;
 }
-static int trellis_leave(snk_engine *h, hipStream_t caller)
+// behind it, whether or not all of it was queued
+static int trellis_leave(snk_engine *h, hipStream_t s, int result)
 {
-    HIPCHK(hipEventRecord(h->tr_done, h->stream));
-    HIPCHK(hipStreamWaitEvent(caller, h->tr_done, 0));
+    const hipError_t e = hipEventRecord(h->tr_done, s);
+    if (e == hipSuccess) h->tr_used = true;
+    else (void)hipStreamSynchronize(s);
+    if (result) return result;
+    HIPCHK(e);
+    return 0;
+}
+int trellis_settled(snk_engine *h)
+{
+    if (h->tr_used) HIPCHK(hipEventSynchronize(h->tr_done));
+    h->tr_used = false;
     return 0;
 }
 
@@ -403,13 +412,14 @@ int snk_sample_paths(snk_handle h, const int64_t *cand, const double *tdist, con
     CHK(check_randoms(who, u, rows * n_draws));
     HIPCHK(hipSetDevice(h->device));
     const size_t np = (size_t)n_draws * rows * 8, nc = (size_t)n_draws * n_utts * 8;
+    CHK(trellis_enter(h, who, h->stream));
     CHK(h->tr_u.ensure(np));
     CHK(h->tr_out.ensure(np + 2 * nc));
     CHK(upload_trellis(h, cand, tdist, rows, K, join_class));
     CHK(h2d(h, h->tr_u.p, u, np, h->stream));
     char *out = h->tr_out.as<char>();
     const TrellisCall q = {who, true, h->tr_cand.as<int64_t>(), h->tr_tdist.as<double>(), row_offsets, join_class ? h->tr_class.as<int32_t>() : nullptr,
-                           n_utts, K, temperature};
+                           n_utts, K, temperature, h->stream};
     CHK(sample_paths_device(h, q, h->tr_u.as<double>(), n_draws, rule, (int64_t *)out, (double *)(out + np),
                             logp_out ? (double *)(out + np + nc) : nullptr));
     D2HPart parts[3] = {{path_out, out, np}, {cost_out, out + np, nc}, {logp_out, out + np + nc, logp_out ? nc : 0}};
@@ -429,9 +439,8 @@ int snk_sample_paths_dev(snk_handle h, const int64_t *cand_dev, const double *td
     DeviceGuard device;
     CHK(device.enter(h->device));
     CHK(trellis_enter(h, who, (hipStream_t)stream));
-    const TrellisCall q = {who, false, cand_dev, tdist_dev, row_offsets, join_class_dev, n_utts, K, temperature};
-    CHK(sample_paths_device(h, q, u_dev, n_draws, rule, path_dev_out, cost_dev_out, logp_dev_out));
-    return trellis_leave(h, (hipStream_t)stream);
+    const TrellisCall q = {who, false, cand_dev, tdist_dev, row_offsets, join_class_dev, n_utts, K, temperature, (hipStream_t)stream};
+    return trellis_leave(h, (hipStream_t)stream, sample_paths_device(h, q, u_dev, n_draws, rule, path_dev_out, cost_dev_out, logp_dev_out));
 }
 
 static int check_posterior(const char *who, snk_engine *h, double temperature, const void *logz, const void *posterior, const void *uses)
@@ -451,11 +460,12 @@ int snk_path_posterior(snk_handle h, const int64_t *cand, const double *tdist, c
     HIPCHK(hipSetDevice(h->device));
     const int64_t rows = row_offsets[n_utts];
     const size_t nz = (size_t)n_utts * 8, np = (size_t)rows * K * 8, nu = uses_out ? (size_t)h->pb_classes * h->pb_buckets * 8 : 0;
+    CHK(trellis_enter(h, who, h->stream));
     CHK(h->tr_out.ensure(nz + np + nu));
     CHK(upload_trellis(h, cand, tdist, rows, K, join_class));
     char *out = h->tr_out.as<char>();
     const TrellisCall q = {who, true, h->tr_cand.as<int64_t>(), h->tr_tdist.as<double>(), row_offsets, join_class ? h->tr_class.as<int32_t>() : nullptr,
-                           n_utts, K, temperature};
+                           n_utts, K, temperature, h->stream};
     CHK(path_posterior_device(h, q, (double *)out, (double *)(out + nz), uses_out ? (double *)(out + nz + np) : nullptr));
     D2HPart parts[3] = {{logz_out, out, nz}, {posterior_out, out + nz, np}, {uses_out, out + nz + np, nu}};
     CHK(staged_d2h(h, h->stream, parts, 3));
@@ -473,7 +483,6 @@ int snk_path_posterior_dev(snk_handle h, const int64_t *cand_dev, const double *
     DeviceGuard device;
     CHK(device.enter(h->device));
     CHK(trellis_enter(h, who, (hipStream_t)stream));
-    const TrellisCall q = {who, false, cand_dev, tdist_dev, row_offsets, join_class_dev, n_utts, K, temperature};
-    CHK(path_posterior_device(h, q, logz_dev_out, posterior_dev_out, uses_dev_out));
-    return trellis_leave(h, (hipStream_t)stream);
+    const TrellisCall q = {who, false, cand_dev, tdist_dev, row_offsets, join_class_dev, n_utts, K, temperature, (hipStream_t)stream};
+    return trellis_leave(h, (hipStream_t)stream, path_posterior_device(h, q, logz_dev_out, posterior_dev_out, uses_dev_out));
 }

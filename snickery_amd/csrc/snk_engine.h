@@ -453,7 +453,8 @@ struct snk_engine {
     double pb_min = 0.0;                   // the smallest finite bias, at most 0
     DevBuf tr_off, tr_cand, tr_tdist, tr_class, tr_u, tr_C, tr_V, tr_W, tr_local, tr_least, tr_flag, tr_draw, tr_row_uses, tr_out;
     DevBuf tr_M, tr_exps, tr_ends_v, tr_ends_w, tr_scaled;      // the pieces of the recursions
-    hipEvent_t tr_in = nullptr, tr_done = nullptr;      // hand-over between a caller's stream and the engine's
+    hipEvent_t tr_in = nullptr, tr_done = nullptr;      // what the engine's stream held before a trellis call; end of the last one
+    bool tr_used = false;
     DevBuf vstats;             // [0] cells refined, [1] steps with a refinement, [2] exact costs computed there
     // pass 1 of the sparse path, second form (joinfast_kernels.hip: join_lb2_kernel): float32 copy of the weighted join rows,
     // built at the first sparse recursion after snk_set_weights; [0] of jw_umax: bits of the largest row norm
@@ -520,6 +521,7 @@ int reorder_units(snk_engine *h);
 // state checks (api_core.hip)
 int check_ready(snk_engine *h, bool need_target, bool need_join);
 int no_batch_in_flight(snk_engine *h, const char *who);
+int trellis_settled(snk_engine *h);                          // trellis calls on callers' streams are done (api_sample.hip)
 inline int roundup(int64_t v, int64_t m) { return (int)(((v + m - 1) / m) * m); }
 
 // error of ONE v_mfma_f32_32x32x16_bf16, as a fraction of the sum of its |products| and |C|, that the bf16-split bound

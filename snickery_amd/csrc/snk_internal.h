@@ -381,6 +381,7 @@ struct TrellisCosts {         // what the cost of a join is made of
 };
 void launch_trellis_local(const TrellisView &v, double *local, double *least, int *flag, hipStream_t s);
 void launch_trellis_costs(const TrellisView &v, const TrellisCosts &c, bool logs, int *flag, double *X, hipStream_t s);
+void launch_trellis_offsets(const int64_t *off_host, int n_utts, int flag_value, int64_t *off, int *flag, hipStream_t s);
 int trellis_most_pieces(const int64_t *off, int n_utts);
 size_t trellis_piece_places(const TrellisView &v);    // entries of the pieces' tables: products (K x Kp), exponents (K), ends (Kp)
 void launch_trellis_ends(const TrellisView &v, const double *local, bool both, int *flag, double *M, int *exps, double *ends_v, double *ends_w,

@@ -84,6 +84,16 @@ __device__ __forceinline__ int trellis_exponent(double m)
     return m > 0.0 ? (int)(((u64)__double_as_longlong(m) >> 52) & 0x7ff) - 1023 : 0;
 }
 
+// ---- an utterance's first row and flag.  The offsets travel as arguments: a copy would need a page-locked place that lives on -----------
+struct TrellisOffsets { int64_t v[256]; };
+__global__ void __launch_bounds__(256)
+trellis_offsets_kernel(const TrellisOffsets part, int first, int n_utts, int flag_value, int64_t *__restrict__ off, int *__restrict__ flag)
+{
+    const int i = first + threadIdx.x;
+    if (i <= n_utts) off[i] = part.v[threadIdx.x];
+    if (i < n_utts) flag[i] = flag_value;
+}
+
 // ---- local weights: a wavefront per row ---------------------------------------------------------------------------------------------
 __global__ void __launch_bounds__(256)
 trellis_local_kernel(const TrellisView v, double *__restrict__ local, double *__restrict__ least, int *__restrict__ flag)
@@ -1401,6 +1411,15 @@ trellis_total_kernel(const TrellisView v, const int *__restrict__ root, const do
 }
 
 // ---- launches ---------------------------------------------------------------------------------------------------------------------------
+void launch_trellis_offsets(const int64_t *off_host, int n_utts, int flag_value, int64_t *off, int *flag, hipStream_t s)
+{
+    for (int v = 0; v <= n_utts; v += 256) {
+        TrellisOffsets part;
+        for (int i = 0; i < 256; ++i) part.v[i] = v + i <= n_utts ? off_host[v + i] : 0;
+        hipLaunchKernelGGL(trellis_offsets_kernel, dim3(1), dim3(256), 0, s, part, v, n_utts, flag_value, off, flag);
+    }
+}
+
 void launch_trellis_local(const TrellisView &v, double *local, double *least, int *flag, hipStream_t s)
 {
     hipLaunchKernelGGL(trellis_local_kernel, dim3((unsigned)((v.rows + 3) / 4)), dim3(256), 0, s, v, local, least, flag);

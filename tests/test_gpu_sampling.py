@@ -723,6 +723,47 @@ def test_trellis_on_another_stream(engine):
         assert np.array_equal(both.cpu().numpy(), np.concatenate([want[1].ravel(), want[2].ravel()]))
 
 
+def test_trellis_calls_on_streams_at_once_and_changes_behind_them(engine):
+    """Calls on two streams in turn share the workspaces, and so does one that waits; a bias, weights and frames that change right
+    behind a queued call are not seen by it."""
+    import torch
+    v = Voice(engine)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    rng = np.random.RandomState(2)
+    work = []
+    for n, (T, K) in enumerate(((200, 40), (30, 90), (400, 20), (25, 25), (300, 40), (60, 64))):
+        v.set_bias(1, 4 + n % 3, seed=n)
+        v.wj = 0.3 + rng.rand(v.wj.size)
+        engine.set_weights(None, v.wj)
+        if n == 3:
+            v.JC = v.JC[::-1].copy()
+            engine.upload_join_only(v.JC)
+            engine.set_weights(None, v.wj)
+        cand, dist, offs = v.candidates([T, 3], K, seed=n)
+        u = rng.rand(1, T + 3)
+        with torch.cuda.stream(streams[n % 2]):
+            args = on_gpu(cand), on_gpu(dist), on_gpu(u)
+            big = torch.rand((1024, 1024), device='cuda')
+            for _ in range(6):
+                big = big @ big * 1e-3                      # the call is still waiting when the next one is made
+            got = engine.sample_paths(*args, row_offsets=offs)
+            post = engine.path_posterior(*args[:2], row_offsets=offs)
+        work.append((got, post, cand, dist, offs, u, v.model()))
+        if n == 4:                                          # one that waits, between the two
+            host = engine.path_posterior(cand, dist, row_offsets=offs)
+            torch.cuda.synchronize()
+            assert all(np.array_equal(a, b.cpu().numpy()) for a, b in zip(host, post))
+    torch.cuda.synchronize()
+    for got, post, cand, dist, offs, u, model in work:
+        for i in range(2):
+            a, b = int(offs[i]), int(offs[i + 1])
+            want, c, lp = o.sample_path(cand[a:b], dist[a:b], u[0, a:b], 1.0, **model)
+            assert np.array_equal(got[0].cpu().numpy()[0, a:b], want)
+            z, p, _ = o.posterior(cand[a:b], dist[a:b], 1.0, **model)
+            tol = sum_tolerance(b - a, cand.shape[1], abs(z) + 2.0 * (b - a))
+            assert abs(post[0].cpu().numpy()[i] - z) <= tol and np.all(np.abs(post[1].cpu().numpy()[a:b] - p) <= 4.0 * tol)
+
+
 def test_trellis_refuses_a_stream_under_capture(engine):
     import torch
     import snickery_amd
