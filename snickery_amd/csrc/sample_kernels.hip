@@ -36,6 +36,9 @@ __device__ __forceinline__ typename ScoreKey<T>::type score_key(double x)
 }
 
 // ---- rows of up to 64 E scores: a wavefront each ------------------------------------------------------------------------------
+// A row is read once, its sums are data-parallel moves within the wavefront, and a lane has a draw.  One row of 30: 2.8 us, a launch;
+// 600 rows of 100, top_p 0.9: 9 us; 19200 rows of 100, top_k 40, top_p 0.95, min_p 0.02, 8 draws: 51 us, 0.4 TB/s: bound by the search
+// for the cuts (wave_row_keep).  8.4 million float32 scores, top_p 0.9: 128 us in rows of 128, 87 of 256, 83 of 512, 99 of 1024.
 template <typename T, int E>
 __global__ void __launch_bounds__(256)
 sample_rows_wave_kernel(const T *__restrict__ scores, int64_t stride, int64_t R, int V, const double *__restrict__ u, int n_draws,
@@ -81,7 +84,9 @@ sample_rows_wave_kernel(const T *__restrict__ scores, int64_t stride, int64_t R,
     }
 }
 
-// ---- longer rows without a workspace: a workgroup each, the row read once per pass ---------------------------------------------------------------------
+// ---- longer rows without a workspace: a workgroup each, the row read once per pass ------------------------------------------------------
+// For rows that the passes below leave over and for captured calls without a workspace.  Bound by what one compute unit reads: a row of
+// 1048576 float32 3.3 ms, 37 rows of 50003 179 us.
 #define SNK_SAMPLE_TILES 4096
 #define SNK_SAMPLE_VEC 4
 
@@ -544,7 +549,11 @@ sample_rows_held_kernel(const T *__restrict__ scores, int64_t stride, int V, con
 //   draw       the chunk, then the score that a random number falls on
 // top_k and top_p take a boundary / select pair each.  Counts and masses are integers: neither the order of the atomics nor the cutting
 // shows in a result.  A boundary bin of equal scores needs no list; one of more than SNK_LIST different ones (or a workspace that a
-// captured graph would have to share) leaves the row to the kernel above.
+// captured graph would have to share) leaves the row to the kernel above.  us a pass, for 1 row of 1048576 float32, 37 of 50003 float32
+// (top_p 0.95: 7.4 MB, 1.5 us at a copy's rate) and 128 of 131071 bfloat16 (top_k 50 and top_p 0.9: 34 MB, 6.6 us):
+//     extremes 6, 6, 13    histogram 13, 11, 37    boundary 12, 12, 2 x 32    select 10, 13, 2 x 5    masses 8, 11, 17    draw 13, 13, 10
+// The first two are launches and the latency of a few dependent reads each; the third is bound by the float64 work on every score (weight
+// and bin) and by the boundary's two rounds of workgroups, each of which finds the bin for itself.
 #define SNK_CHUNK 8192
 #define SNK_LIST 16384
 #define SNK_BINS_MOST 4096

@@ -94,7 +94,7 @@ trellis_offsets_kernel(const TrellisOffsets part, int first, int n_utts, int fla
     if (i < n_utts) flag[i] = flag_value;
 }
 
-// ---- local weights: a wavefront per row ---------------------------------------------------------------------------------------------
+// ---- local weights: a wavefront per row; 9600 rows of 100: 9 us, 2.5 TB/s ---------------------------------------------------------------------------------------------
 __global__ void __launch_bounds__(256)
 trellis_local_kernel(const TrellisView v, double *__restrict__ local, double *__restrict__ least, int *__restrict__ flag)
 {
@@ -130,12 +130,15 @@ trellis_local_kernel(const TrellisView v, double *__restrict__ local, double *__
 // ---- costs: a workgroup per pair of rows and tile of 16 RT x 16 RT cells ------------------------------------------------------------
 // |e - s|^2 = |e|^2 + |s|^2 - 2 e.s on the float64 matrix pipe: half the instructions of the difference form (one fused multiply-add
 // a column instead of a subtraction and one), which ran at two thirds of the vector pipe's rate.  Both sides are taken relative to
-// one of the tile's units, so that the norms are those of the candidates' spread and not of their distance from the origin.  Where
+// one unit of the second row, so that the norms are those of the candidates' spread and not of their distance from the origin.  Where
 // the difference is small against the norms -- neighbouring frames -- the product form cancels: a cell below SNK_COST_NEAR of them is taken
 // again in differences.  A unit and its natural successor join at exactly 0.  The others carry a relative error of at most Dj 2^-53 / SNK_COST_NEAR.
 // A wavefront owns RM x CM tiles of 16 x 16; DC columns of the two sets of rows go through LDS at a time, weighted and widened on
 // the way, the next ones are in flight meanwhile: 32, a cache line of a row (197 us for 600 rows of 100 candidates and 302 columns, 206
-// with 16), or 16 in the larger tiles, whose registers hold no more (2.55 ms for 9600 rows, 2.73 with 32 and spills).
+// with 16, before what follows), or 16 in the larger tiles, whose registers hold no more (2.55 ms for 9600 rows, 2.73 with 32 and
+// spills).  9600 rows of 100 candidates, 302 columns: 2.14 ms, 27 TFLOP/s of a large product's 62 (34 with the cells that pad K to
+// 112); bound by the float64 units, which the products hold 43 % of the time and weighing the cells, staging and padding the most of
+// the rest: neither overlaps with products of another wavefront.  1200 rows of 200, 151 columns: 0.68 ms.
 #define SNK_COST_NEAR 0x1p-8
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
@@ -463,7 +466,8 @@ __device__ __forceinline__ TrellisPiece trellis_piece(const TrellisView &v, int 
 // over KH CH steps of four.  The weights X alternate between two LDS buffers; the slab's fragments live in registers and each is
 // reloaded with the next slab's (or the next half's) right after its use.  The row blocks of a piece are dealt to one XCD, so that a
 // slab comes from memory once and from that XCD's L2 for the others.  RB 1: a step re-reads the slab for sixteen rows, 50 bytes a
-// cycle and compute unit, near what the L2 gives one; RB 2 halves that and is for launches that fill the chip either way.
+// cycle and compute unit, near what the L2 gives one; RB 2 halves that and is for launches that fill the chip either way.  9600 rows of
+// 100: 0.71 ms, 27 TFLOP/s (37 with the padding); 1200 rows of 200: 0.62 ms; 600 of 100: 71 us, 24 steps of 3 us.
 template <int CT, int KH, int CH, int RB, int NTH>
 __global__ void __launch_bounds__(NTH)
 trellis_product_kernel(const TrellisView v, const double *__restrict__ local, int max_pieces, int row_blocks, bool skip_last, int *__restrict__ flag,
@@ -620,7 +624,8 @@ trellis_product_kernel(const TrellisView v, const double *__restrict__ local, in
 // 2. the weights at the pieces' ends: a workgroup per utterance; what a step waits for is what it costs (two barriers, no sum in a row).
 // Forward: a wavefront owns 32 columns, CW of them side by side, RG such groups and the four rows of lanes in each split the rows.
 // Backward: Q threads a row.  A thread's cells come in H parts of R; each is reloaded with the next part's right after its use.  Every
-// wavefront keeps the weights of all candidates, S a lane, and scales them itself.
+// wavefront keeps the weights of all candidates, S a lane, and scales them itself.  Bound by a step's latency: 25 pieces of 100
+// candidates 47 us, both directions of 18 pieces of 50 20 us each.
 template <int R, int H, int CW, int RG, int Q, int S, int NTH>
 __global__ void __launch_bounds__(NTH)
 trellis_ends_kernel(const TrellisView v, const double *__restrict__ local, const double *__restrict__ M, const int *__restrict__ exps,
@@ -760,7 +765,8 @@ trellis_ends_kernel(const TrellisView v, const double *__restrict__ local, const
 
 // 3. forward.  A wavefront owns 32 columns (two a lane); its four rows of 16 lanes split the predecessors, so a step's sums end inside
 // the wavefront and a step costs one barrier.  A thread's KPM CH predecessors come in CH parts; every cell's register is reloaded
-// with a later slab's right after its use (NB parts ahead).
+// with a later slab's right after its use (NB parts ahead).  9600 rows of 100: 172 us, 4.5 TB/s of a copy's 5.1: bound by memory;
+// 600 rows: 38 us, 24 steps.
 template <int KPM, int CH, int NB, int NTH>
 __global__ void __launch_bounds__(NTH)
 trellis_forward_kernel(const TrellisView v, const double *__restrict__ local, const double *__restrict__ least, double bias_min,
@@ -890,7 +896,7 @@ trellis_forward_kernel(const TrellisView v, const double *__restrict__ local, co
     }
 }
 
-// 3. backward: a wavefront owns CH x 16 predecessors, four lanes share each one's successors
+// 3. backward: a wavefront owns CH x 16 predecessors, four lanes share each one's successors.  9600 rows of 100: 188 us, 4.1 TB/s
 template <int KC, int CH, int NB, int NTH>
 __global__ void __launch_bounds__(NTH)
 trellis_backward_kernel(const TrellisView v, const double *__restrict__ local, const double *__restrict__ ends, int *__restrict__ flag,
@@ -1101,7 +1107,8 @@ trellis_backward_log_kernel(const TrellisView v, const int *__restrict__ flag, d
 
 // ---- posteriors: a workgroup per row ---------------------------------------------------------------------------------------------------
 // The row's bucket uses are integers in units of 2^-50: their sums are the same in any order.  The two outermost buckets take most
-// cells and are summed in registers; the others go to LDS.
+// cells and are summed in registers; the others go to LDS.  9600 rows of 100: 0.31 ms, 2.5 TB/s: bound by the cells' vector work (bucket,
+// integer sums), 174 us for 1200 rows of 200.
 __global__ void __launch_bounds__(256)
 trellis_posterior_kernel(const TrellisView v, const int *__restrict__ flag, const double *__restrict__ V, const double *__restrict__ Wt,
                          const double *__restrict__ ends, const double *__restrict__ local, const double *__restrict__ logz, const int *__restrict__ bucket_edges, int n_buckets,
@@ -1183,7 +1190,8 @@ trellis_posterior_kernel(const TrellisView v, const int *__restrict__ flag, cons
     if (tid < n_buckets) row_uses[t * n_buckets + tid] = (double)uses[tid] * (1.0 / SNK_USES_UNIT);
 }
 
-// uses[class, bucket] = sum over the rows of the class: a workgroup per class and bucket, the rows in a fixed order
+// uses[class, bucket] = sum over the rows of the class: a workgroup per class and bucket, the rows in a fixed order (9600 rows of 32
+// buckets, 3 classes: 30 us, each workgroup reads its column alone)
 __global__ void __launch_bounds__(256)
 trellis_uses_kernel(const double *__restrict__ row_uses, const int32_t *__restrict__ join_class, int64_t rows, int n_buckets,
                     double *__restrict__ uses)
@@ -1205,7 +1213,8 @@ trellis_uses_kernel(const double *__restrict__ row_uses, const int32_t *__restri
 // ---- draws -----------------------------------------------------------------------------------------------------------------------------
 // The random number of a row does not depend on the candidate behind it, so the predecessor of EVERY candidate is drawn at once,
 // all rows side by side (the weights and their truncation once per candidate, whatever the number of draws); what is left of the
-// chain is following those pointers.
+// chain is following those pointers.  9600 rows of 100 candidates, four draws: 1.30 ms for the 960 000 weighted rows, 1.36 ns each as in
+// sample_rows (51 us for 19200): bound by the search's dependent chain (sample_device.h), 0.6 TB/s of cells.
 //
 // Weights of the row of scores V[t,.] (E[t,.,after]) / alpha + X: x in the order of the scores, -inf: takes no part.
 template <int E>
@@ -1285,6 +1294,7 @@ trellis_pointer_kernel(const TrellisView v, int shift, const int *__restrict__ f
 
 // Follows the pointers of an utterance and draw: a workgroup each, as many rows at a time as LDS holds.  The rows are cut into
 // pieces of 32: all K ways through every piece side by side, then the pieces' ends one after the other, then the pieces side by side.
+// 600 rows of 100: 14 us, a chain of 600 loads from LDS would take 40.
 #define SNK_CHASE_BYTES (128 * 1024)
 #define SNK_CHASE_PIECE 32
 __global__ void __launch_bounds__(512)
@@ -1333,7 +1343,7 @@ trellis_chase_kernel(const TrellisView v, const unsigned char *__restrict__ poin
 }
 
 // Unit, cost and log probability of every row of a path: a wavefront per row and draw.  The join cost is taken from the units
-// themselves, in differences: the cells only hold its exponential.
+// themselves, in differences: the cells only hold its exponential.  9600 rows, four draws: 106 us, most of it the row's truncation again.
 template <int E>
 __global__ void __launch_bounds__(256)
 trellis_path_kernel(const TrellisView v, const TrellisCosts c, const int *__restrict__ flag, const double *__restrict__ V, SampleRule rule,
@@ -1425,14 +1435,14 @@ void launch_trellis_local(const TrellisView &v, double *local, double *least, in
     hipLaunchKernelGGL(trellis_local_kernel, dim3((unsigned)((v.rows + 3) / 4)), dim3(256), 0, s, v, local, least, flag);
 }
 
-// The widest tile that a wavefront's registers hold is 7 x 2 tiles of 16 x 16 (two workgroups a compute unit): K is cut into as few
-// equal tiles of at most 112 -- of at most 64 where that would leave less than two rounds of workgroups (599 pairs of rows of 100
-// candidates, 302 columns: 214 us instead of 249).
+// A wavefront's registers hold 7 tiles of 16 x 16 (two workgroups of eight wavefronts a compute unit): K is cut into as few equal
+// tiles of at most 112 -- of at most 64 where that would leave less than three quarters of the workgroups that run at once (posteriors
+// of 100 candidates, 302 columns, with tiles of 64 and of 112: 100 rows 233 and 258 us, 300 rows 349 and 363, 450 rows 430 and 409).
 void launch_trellis_costs(const TrellisView &v, const TrellisCosts &c, bool logs, int *flag, double *X, hipStream_t s)
 {
     if (v.rows < 2) return;
     int n = (v.K + 111) / 112;
-    if (v.K > 64 && (v.rows - 1) * n * n < 1024) n = (v.K + 63) / 64;
+    if (v.K > 64 && (v.rows - 1) * n * n < 384) n = (v.K + 63) / 64;
     const int rt = ((v.K + n - 1) / n + 15) / 16;
     const dim3 grid((unsigned)(v.rows - 1), n, n);
 #define SNK_COST(RT_, RM_, CM_, NTH_, OCC_, DC_)                                                                                            \
