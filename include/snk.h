@@ -353,9 +353,11 @@ int snk_set_position_bias(snk_handle h, const double *bias, int n_classes, int n
  *   path_out (n_draws, rows) int64 unit ids, -1 throughout an utterance without a complete path
  *   cost_out (n_draws, n_utts) float64 (+inf there); logp_out likewise, or NULL: log of the product of the truncated
  *   probabilities (-inf there)
- * K up to 208; an utterance of a single row is a draw from its target costs.
- * The _dev form takes device memory (row_offsets excepted), waits for what `stream` holds and makes `stream` wait for the
- * results, without a host wait; it refuses a stream that is being captured. */
+ * K up to 208, n_draws up to 65535, an utterance up to 2^23 rows; one of a single row is a draw from its target costs.  Results of an
+ * utterance do not depend on the others of the call.  Join costs are float64, within (Dj + 4) 2^-45 relative of the exact ones.
+ * The _dev form takes device memory (row_offsets excepted) and puts its kernels on `stream` without a host wait.  It uses the engine's
+ * workspaces: later calls, on any stream, are ordered behind it, and it refuses a stream that is being captured.  It cannot look at
+ * device memory first: numbers u as in snk_sample_rows_dev. */
 int snk_sample_paths(snk_handle h, const int64_t *cand, const double *tdist, const int64_t *row_offsets, int n_utts, int K,
                      const int32_t *join_class, const double *u, int n_draws, double temperature, int64_t top_k, double top_p,
                      double min_p, int64_t *path_out, double *cost_out, double *logp_out);
