@@ -81,7 +81,7 @@ __device__ __forceinline__ double sample_exp(double e)
 
 __device__ __forceinline__ u64 sample_weight(double e, double unit)
 {
-    return e < SNK_SAMPLE_FLOOR ? 0ull : sample_fix(sample_exp(e), unit);
+    return e >= SNK_SAMPLE_FLOOR ? sample_fix(sample_exp(e), unit) : 0ull;     // (an exponent that is not a number weighs nothing)
 }
 
 // thresholds: the mass a prefix has to reach (top_p) / to exceed (a draw)

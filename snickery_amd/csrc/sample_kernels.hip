@@ -227,7 +227,7 @@ sample_rows_block_kernel(const T *__restrict__ scores, int64_t stride, int64_t V
         const Key k = score_key<T>(x);
         if (!all && k < cut) return;
         const double e = sample_exponent(x, m, rule.inv_tau);
-        if (e < SNK_SAMPLE_FLOOR) return;
+        if (!(e >= SNK_SAMPLE_FLOOR)) return;
         const double v = sample_exp(e);
         if (use_min && (double)sample_fix(v, unit) < rule.min_p * unit) return;
         if (!all && k == cut) { tie = 1; return; }

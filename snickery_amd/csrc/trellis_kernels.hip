@@ -30,10 +30,10 @@ typedef double f64x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ bool trellis_usable(int64_t id, int64_t n_units) { return id >= 1 && id < n_units - 1; }
 __device__ __forceinline__ bool trellis_takes_part(int64_t id, double d, int64_t n_units) { return trellis_usable(id, n_units) && d - d == 0.0; }
 
-// -d / tau of a candidate that takes part
+// -d / tau of a candidate that takes part, kept finite (a sum over 2^23 rows stays so)
 __device__ __forceinline__ double trellis_local(int64_t id, double d, int64_t n_units, double inv_tau)
 {
-    return trellis_takes_part(id, d, n_units) ? -d * inv_tau : -__builtin_inf();
+    return trellis_takes_part(id, d, n_units) ? fmin(fmax(-d * inv_tau, -1e300), 1e300) : -__builtin_inf();
 }
 
 // utterance of a row (first .. first + n - 1): off[u] <= t < off[u + 1]
@@ -1224,7 +1224,7 @@ __device__ __forceinline__ bool trellis_row(const double (&p)[E], bool logs, con
     m = ninf;
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-        x[e] = logs || p[e] > 0.0 ? p[e] : ninf;
+        x[e] = p[e] > (logs ? ninf : 0.0) ? p[e] : ninf;        // (neither NaN)
         m = fmax(m, x[e]);
     }
     m = wave_max(m);
@@ -1378,8 +1378,9 @@ trellis_path_kernel(const TrellisView v, const TrellisCosts c, const int *__rest
     const double lp = (logs ? sample_exponent(mine, m, 1.0) : mine == m ? 0.0 : log(mine * (1.0 / m))) - log((double)row.total / SNK_SAMPLE_UNIT);
     double cost = v.tdist[t * K + k];
     const int64_t id = v.cand[t * K + k];
-    if (!last) {
-        const int64_t next = v.cand[(t + 1) * K + after];
+    const int64_t next = last ? -1 : v.cand[(t + 1) * K + after];
+    if (!last && (!trellis_usable(id, v.n_units) || !trellis_usable(next, v.n_units))) cost = __builtin_inf();    // (not one of these was drawn:
+    else if (!last) {                                                                                             // the candidates changed under the call)
         const float *__restrict__ pe = c.JC + (id + 1) * c.Jp, *__restrict__ ps = c.JC + next * c.Jp;
         double d2 = 0.0;
         for (int j = lane; j < c.Dj; j += 64) {

@@ -291,6 +291,32 @@ def test_rows_of_many_draws(engine):
         assert i.min() >= 0
 
 
+def test_rows_whose_exponents_are_no_numbers(engine):
+    """A temperature of infinity (a rule in device memory) and a row that +inf shares: 0 times infinity weighs nothing."""
+    import torch
+    rng = np.random.RandomState(5)
+    for V in (50, 1000, 5000, 20000):
+        x = rng.randn(4, V)
+        x[0, [V // 2, V - 1]] = np.inf
+        x[1, :3] = np.inf
+        x[2, 7] = -np.inf
+        gx, gu = on_gpu(x), on_gpu(rng.rand(4, 40))
+        tau = on_gpu(np.full(4, np.inf))
+        for rule in (dict(), dict(top_k=5), dict(top_p=0.5), dict(top_k=5, top_p=0.5, min_p=0.1)):
+            graph = torch.cuda.CUDAGraph()
+            i, _ = engine.sample_rows(gx, gu, temperature=tau, **{k: on_gpu(np.full(4, float(w))) for k, w in rule.items()})
+            rules = on_gpu(np.array([[np.inf, rule.get('top_k', 0), rule.get('top_p', 1.0), rule.get('min_p', 0.0)]] * 4))
+            j = torch.empty_like(i)
+            with torch.cuda.graph(graph):                       # (without a workspace)
+                assert engine._lib.snk_sample_rows_dev(engine._h, gx.data_ptr(), 0, 4, V, V, gu.data_ptr(), 40, 1.0, 0, 1.0, 0.0, rules.data_ptr(), j.data_ptr(),
+                                                       None, None, 0, torch.cuda.current_stream().cuda_stream) == 0
+            graph.replay()
+            torch.cuda.synchronize()
+            i, j = i.cpu().numpy(), j.cpu().numpy()
+            assert np.array_equal(i, j) and np.all((i >= 0) & (i < V))
+            assert set(i[0]) <= {V // 2, V - 1} and set(i[1]) <= {0, 1, 2} and 7 not in i[2]
+
+
 @pytest.mark.parametrize('dtype', ['float32', 'float64', 'float16', 'bfloat16'])
 @pytest.mark.parametrize('V', [1025, 2047, 2048, 2049, 4095, 4097, 8191, 8192, 8193])
 def test_rows_at_the_borders_of_the_workgroups_sizes(engine, V, dtype):
@@ -480,6 +506,25 @@ def test_trellis_of_extreme_temperatures(engine):
     for tau in (1e-2, 1.0):
         check_paths(v, cand, dist, offs, u, temperature=tau)
         check_posterior(v, cand, dist, offs, temperature=tau)
+
+
+def test_trellis_of_costs_that_overflow(engine):
+    """Costs over a temperature that float64 does not hold, either sign, and a bias of that size: units of the candidates, or none."""
+    v = Voice(engine)
+    cand, dist, offs = v.candidates([30, 5], 20)
+    rng = np.random.RandomState(1)
+    u = rng.rand(3, 35)
+    for scale, tau, bias in ((1e300, 1e-10, 0.0), (-1e300, 1e-10, 0.0), (-1e308, 1e-300, 0.0), (1.0, 1e-300, 0.0), (1.0, 0.5, -1e308), (1.0, 1e-10, 1e308),
+                             (-1e300, 1e-300, -1e300)):
+        d = dist * scale
+        d[rng.rand(*d.shape) < 0.3] *= -1.0
+        engine.set_position_bias(np.array([[0.0, bias]]), [1])
+        for t in (tau, 0.0):
+            path, cost, logp = engine.sample_paths(cand, d, u, row_offsets=offs, temperature=t, top_p=0.9)
+            drawn = (path[:, :, None] == cand[None]).any(axis=2)
+            assert np.all(drawn | (path == -1))
+        logz, post, uses = engine.path_posterior(cand, d, row_offsets=offs, temperature=tau)
+        assert post.shape == cand.shape and uses.shape == (1, 2)
 
 
 def test_trellis_without_a_complete_path(engine):
