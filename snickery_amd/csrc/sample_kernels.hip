@@ -551,9 +551,9 @@ sample_rows_held_kernel(const T *__restrict__ scores, int64_t stride, int V, con
 // shows in a result.  A boundary bin of equal scores needs no list; one of more than SNK_LIST different ones (or a workspace that a
 // captured graph would have to share) leaves the row to the kernel above.  us a pass, for 1 row of 1048576 float32, 37 of 50003 float32
 // (top_p 0.95: 7.4 MB, 1.5 us at a copy's rate) and 128 of 131071 bfloat16 (top_k 50 and top_p 0.9: 34 MB, 6.6 us):
-//     extremes 6, 6, 13    histogram 13, 11, 37    boundary 12, 12, 2 x 32    select 10, 13, 2 x 5    masses 8, 11, 17    draw 13, 13, 10
+//     extremes 6, 5, 13    histogram 13, 11, 36    boundary 12, 11, 2 x 20    select 10, 11, 2 x 5    masses 8, 11, 17    draw 13, 13, 10
 // The first two are launches and the latency of a few dependent reads each; the third is bound by the float64 work on every score (weight
-// and bin) and by the boundary's two rounds of workgroups, each of which finds the bin for itself.
+// and bin, tested again for the boundary).
 #define SNK_CHUNK 8192
 #define SNK_LIST 16384
 #define SNK_BINS_MOST 4096
@@ -570,12 +570,13 @@ struct RowState {
 
 struct RowsWork {
     RowState *state;
-    double *chunk_max, *chunk_min;          // [rows][chunks]
+    double *chunk_max, *chunk_min;          // [rows][spans]
     u64 *hist_mass; unsigned int *hist_count;   // [rows][bins]
     double *list_x;                         // [rows][list]
     u64 *chunk_mass; unsigned int *chunk_ties;
     int *left;                              // rows for the kernel above
-    int bins, chunks;
+    int64_t span;                           // scores that a workgroup of the first passes takes: chunks, as many as leave workgroups enough
+    int bins, chunks, spans;
     unsigned int list;                      // entries of a row's list: SNK_LIST, or the row's length
 };
 
@@ -625,7 +626,7 @@ rows_extremes_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, co
         }
     }
     double m = -inf, n = inf;
-    chunk_scores<T, 512>(scores + r * stride, c * SNK_CHUNK, min((c + 1) * SNK_CHUNK, V), [&](double x, int64_t) {
+    chunk_scores<T, 512>(scores + r * stride, c * w.span, min((c + 1) * w.span, V), [&](double x, int64_t) {
         m = fmax(m, x);
         n = x > -inf ? fmin(n, x) : n;
     });
@@ -635,8 +636,8 @@ rows_extremes_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, co
     __syncthreads();
     if (tid == 0) {
         for (int i = 1; i < 8; ++i) { hi[0] = fmax(hi[0], hi[i]); lo[0] = fmin(lo[0], lo[i]); }
-        w.chunk_max[r * w.chunks + c] = hi[0];
-        w.chunk_min[r * w.chunks + c] = lo[0];
+        w.chunk_max[r * w.spans + c] = hi[0];
+        w.chunk_min[r * w.spans + c] = lo[0];
     }
 }
 
@@ -653,7 +654,7 @@ rows_histogram_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, S
     const double inf = __builtin_inf();
     const SampleRule rule = sample_rule(call, rules, r);
     double m = -inf, n = inf;
-    for (int i = tid; i < w.chunks; i += 512) { m = fmax(m, w.chunk_max[r * w.chunks + i]); n = fmin(n, w.chunk_min[r * w.chunks + i]); }
+    for (int i = tid; i < w.spans; i += 512) { m = fmax(m, w.chunk_max[r * w.spans + i]); n = fmin(n, w.chunk_min[r * w.spans + i]); }
     m = wave_max(m);
     n = -wave_max(-n);
     if ((tid & 63) == 0) { hi[tid >> 6] = m; lo[tid >> 6] = n; }
@@ -664,7 +665,7 @@ rows_histogram_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, S
     const double range = fmin(-sample_exponent(n, m, rule.inv_tau), -SNK_SAMPLE_FLOOR);
     const double scale = range > 0.0 ? fmin((double)w.bins / range, 1e300) : 0.0;
     if (c == 0 && tid == 0) { w.state[r].m = m; w.state[r].bin_scale = scale; }
-    chunk_scores<T, 512>(scores + r * stride, c * SNK_CHUNK, min((c + 1) * SNK_CHUNK, V), [&](double x, int64_t) {
+    chunk_scores<T, 512>(scores + r * stride, c * w.span, min((c + 1) * w.span, V), [&](double x, int64_t) {
         if (x == -inf) return;
         const double e = sample_exponent(x, m, rule.inv_tau);
         const u64 q = sample_weight(e, unit);
@@ -738,7 +739,7 @@ rows_boundary_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, Sa
     // from all XCDs take tens of nanoseconds each)
     if (tid == 0) n_hit = 0;
     __syncthreads();
-    const int64_t lo = c * SNK_CHUNK, hi = min((c + 1) * SNK_CHUNK, V);
+    const int64_t lo = c * w.span, hi = min((c + 1) * w.span, V);
     auto of_bin = [&](double x) -> bool {
         if (x == ninf) return false;
         const double e = sample_exponent(x, m, rule.inv_tau);
@@ -759,8 +760,8 @@ rows_boundary_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, Sa
     const unsigned int n = n_hit;
     if (tid == 0) {
         for (int i = 1; i < 8; ++i) { most = fmax(most, ends[i]); least = fmin(least, ends[8 + i]); }
-        w.chunk_max[r * w.chunks + c] = most;
-        w.chunk_min[r * w.chunks + c] = least;
+        w.chunk_max[r * w.spans + c] = most;
+        w.chunk_min[r * w.spans + c] = least;
         place = n ? atomicAdd(&st->listed, n) : 0;
         n_hit = 0;
     }
@@ -796,7 +797,7 @@ rows_select_kernel(int64_t V, SampleRule call, const double *__restrict__ rules,
     const unsigned int n = st->listed;
     const u64 want = st->want;
     double most = -__builtin_inf(), least = __builtin_inf();    // of the bin's scores
-    for (int i = tid; i < w.chunks; i += 1024) { most = fmax(most, w.chunk_max[r * w.chunks + i]); least = fmin(least, w.chunk_min[r * w.chunks + i]); }
+    for (int i = tid; i < w.spans; i += 1024) { most = fmax(most, w.chunk_max[r * w.spans + i]); least = fmin(least, w.chunk_min[r * w.spans + i]); }
     most = wave_max(most);
     least = -wave_max(-least);
     if ((tid & 63) == 0) { ends[tid >> 6] = most; ends[16 + (tid >> 6)] = least; }
@@ -982,8 +983,17 @@ rows_draw_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, const 
     }
 }
 
-static int rows_bins(int64_t V) { int b = 256; while (b < SNK_BINS_MOST && b * 256 < V) b <<= 1; return b; }
+static int rows_bins(int64_t V) { int b = 1024; while (b < SNK_BINS_MOST && b * 256 < V) b <<= 1; return b; }
 static int64_t rows_chunks(int64_t V) { return (V + SNK_CHUNK - 1) / SNK_CHUNK; }
+// What every workgroup of the first three passes does besides its scores -- the row's largest, the histogram, the boundary's bin -- is as
+// much work as a chunk or two.  So a workgroup takes several chunks where 512 workgroups are left, half of what runs at once (boundary of
+// 128 rows of 131071 bfloat16: 33 us with a chunk each, 24 with two, 20 with four).
+static int64_t rows_span(int64_t R, int64_t V)
+{
+    int64_t span = SNK_CHUNK;
+    while (span < 8 * SNK_CHUNK && R * ((V + 2 * span - 1) / (2 * span)) >= 512) span *= 2;
+    return span;
+}
 static unsigned int rows_list(int64_t V) { return V < SNK_LIST ? (unsigned int)V : SNK_LIST; }
 #define SNK_ALIGNED(bytes_) (((size_t)(bytes_) + 255) & ~(size_t)255)
 
@@ -1010,6 +1020,8 @@ static void launch_rows_split(const T *scores, int64_t stride, int64_t R, int64_
     RowsWork w;
     w.bins = rows_bins(V);
     w.chunks = (int)rows_chunks(V);
+    w.span = rows_span(R, V);
+    w.spans = (int)((V + w.span - 1) / w.span);
     size_t at = 0;
     auto take = [&](size_t bytes) { char *p = work + at; at += SNK_ALIGNED(bytes); return p; };
     const size_t n = (size_t)R * w.chunks;
@@ -1020,12 +1032,12 @@ static void launch_rows_split(const T *scores, int64_t stride, int64_t R, int64_
     w.list = rows_list(V);
     w.list_x = (double *)take((size_t)R * w.list * 8);
     w.left = (int *)take(R * 4);
-    const dim3 grid((unsigned)w.chunks, (unsigned)R);
-    hipLaunchKernelGGL((rows_extremes_kernel<T>), grid, dim3(512), 0, s, scores, stride, V, w);
-    hipLaunchKernelGGL((rows_histogram_kernel<T>), grid, dim3(512), (size_t)w.bins * 12, s, scores, stride, V, rule, rules, unit, w);
+    const dim3 grid((unsigned)w.chunks, (unsigned)R), spans((unsigned)w.spans, (unsigned)R);
+    hipLaunchKernelGGL((rows_extremes_kernel<T>), spans, dim3(512), 0, s, scores, stride, V, w);
+    hipLaunchKernelGGL((rows_histogram_kernel<T>), spans, dim3(512), (size_t)w.bins * 12, s, scores, stride, V, rule, rules, unit, w);
     for (int by_mass = 0; by_mass < 2; ++by_mass) {
         if (!rules && (by_mass ? !(rule.top_p < 1.0) : !(rule.top_k > 0 && rule.top_k < V))) continue;
-        hipLaunchKernelGGL((rows_boundary_kernel<T>), grid, dim3(512), 0, s, scores, stride, V, rule, rules, unit, by_mass, w);
+        hipLaunchKernelGGL((rows_boundary_kernel<T>), spans, dim3(512), 0, s, scores, stride, V, rule, rules, unit, by_mass, w);
         hipLaunchKernelGGL(rows_select_kernel, dim3((unsigned)R), dim3(1024), 0, s, V, rule, rules, unit, by_mass, w);
     }
     hipLaunchKernelGGL((rows_masses_kernel<T>), grid, dim3(512), 0, s, scores, stride, V, rule, rules, unit, w);
