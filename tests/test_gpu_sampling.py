@@ -278,6 +278,28 @@ def test_long_rows_captured_without_a_workspace(engine):
         assert np.array_equal(index.cpu().numpy(), want)
 
 
+@pytest.mark.parametrize('R,V', [(600, 9000), (300, 40000), (520, 70001)])
+def test_rows_of_many_long_rows(engine, R, V):
+    """A workgroup takes more of a row where rows are many: the same results as a few rows at a time."""
+    import torch
+    g = torch.Generator(device='cuda').manual_seed(V)
+    x = torch.randn((R, V), device='cuda', generator=g)
+    x[1::7] *= 1e-6                                         # one bin holds all of them
+    x[2::7, : V - 5] = 0.25
+    x[3::7] = torch.floor(x[3::7] * 3.0)
+    x[4::7, 100:] = float('-inf')
+    x[5] = float('nan')
+    u = torch.rand((R, 2), device='cuda', dtype=torch.float64, generator=g)
+    for rule in (dict(top_p=0.9), dict(top_k=V // 3, top_p=0.5), dict(top_k=40, min_p=0.01)):
+        i, lp = engine.sample_rows(x, u, **rule)
+        for a in range(0, R, 97):
+            j, lq = engine.sample_rows(x[a:a + 4], u[a:a + 4], **rule)
+            assert torch.equal(i[a:a + 4], j) and torch.equal(lp[a:a + 4], lq)
+        few = [1, 2, 3, 4, 5, R - 1]
+        want, _ = o.sample_rows(x[few].double().cpu().numpy(), u[few].cpu().numpy(), **rule)
+        assert np.array_equal(i[few].cpu().numpy(), want)
+
+
 def test_rows_of_many_draws(engine):
     """More draws than a launch's second dimension holds."""
     rng = np.random.RandomState(9)
