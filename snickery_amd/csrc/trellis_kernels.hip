@@ -462,23 +462,23 @@ __device__ __forceinline__ TrellisPiece trellis_piece(const TrellisView &v, int 
     return p;
 }
 
-// 1. products: workgroup = 16 RB start candidates of one piece, wavefront = CT tiles of sixteen end candidates; v_mfma_f64_16x16x4
+// 1. products: workgroup = sixteen start candidates of one piece, wavefront = CT tiles of sixteen end candidates; v_mfma_f64_16x16x4
 // over KH CH steps of four.  The weights X alternate between two LDS buffers; the slab's fragments live in registers and each is
 // reloaded with the next slab's (or the next half's) right after its use.  The row blocks of a piece are dealt to one XCD, so that a
-// slab comes from memory once and from that XCD's L2 for the others.  RB 1: a step re-reads the slab for sixteen rows, 50 bytes a
-// cycle and compute unit, near what the L2 gives one; RB 2 halves that and is for launches that fill the chip either way.  9600 rows of
-// 100: 0.71 ms, 27 TFLOP/s (37 with the padding); 1200 rows of 200: 0.62 ms; 600 of 100: 71 us, 24 steps of 3 us.
-template <int CT, int KH, int CH, int RB, int NTH>
-__global__ void __launch_bounds__(NTH)
+// slab comes from memory once and from that XCD's L2 for the others: a step re-reads the slab for sixteen rows, 50 bytes a cycle and
+// compute unit.  Thirty-two rows halve that but leave two workgroups a compute unit where sixteen leave three: 0.72 against 0.63 ms for
+// 9600 rows of 100 (30 TFLOP/s, 36 with the padding); 1200 rows of 200: 0.62 ms; 600 of 100: 71 us, 24 steps of 3 us.
+template <int CT, int KH, int CH, int NTH>
+__global__ void __launch_bounds__(NTH, NTH == 256 && KH <= 26 ? 3 : 2)
 trellis_product_kernel(const TrellisView v, const double *__restrict__ local, int max_pieces, int row_blocks, bool skip_last, int *__restrict__ flag,
                        double *__restrict__ M, int *__restrict__ exps)
 {
     constexpr int W = NTH / 64, COLS = 4 * KH * CH, LDX = COLS + 2;      // (sixteen rows 4 odd banks apart)
-    __shared__ double X[2][16 * RB * LDX];
-    __shared__ double top[2][W][16 * RB];
+    __shared__ double X[2][16 * LDX];
+    __shared__ double top[2][W][16];
     __shared__ int bad;
     const int j = blockIdx.x >> 3;
-    const int i0 = (j % row_blocks) * 16 * RB, flat = (j / row_blocks) * 8 + (blockIdx.x & 7);
+    const int i0 = (j % row_blocks) * 16, flat = (j / row_blocks) * 8 + (blockIdx.x & 7);
     if (flat >= max_pieces * v.n_utts) return;
     const TrellisPiece p = trellis_piece(v, flat / max_pieces, flat % max_pieces);
     if (p.k >= p.P || p.P == 1 || (skip_last && p.k == p.P - 1) || flag[p.u]) return;
@@ -505,39 +505,33 @@ trellis_product_kernel(const TrellisView v, const double *__restrict__ local, in
 #pragma unroll
             for (int c = 0; c < CT; ++c) load(1, 0, ks, c);
     }
-    for (int i = tid; i < 2 * 16 * RB * LDX; i += NTH) (&X[0][0])[i] = 0.0;
+    for (int i = tid; i < 2 * 16 * LDX; i += NTH) (&X[0][0])[i] = 0.0;
     if (tid == 0) bad = 0;
     __syncthreads();
     // the first slab: the start candidate's own cells
     bool small = false;
-    double most[RB][4];
+    double most[4];
 #pragma unroll
-    for (int h = 0; h < RB; ++h)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) most[h][r] = 0.0;
+    for (int r = 0; r < 4; ++r) most[r] = 0.0;
 #pragma unroll
     for (int c = 0; c < CT; ++c) {
         if (col[c] >= Kp) continue;
         const double l = local[(first_row + 1) * Kp + col[c]];
 #pragma unroll
-        for (int h = 0; h < RB; ++h)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 16 * h + g + 4 * r;
-                const double x = i0 + row < K ? slab0[(int64_t)(i0 + row) * Kp + col[c]] * l : 0.0;
-                X[0][row * LDX + col[c]] = x;
-                most[h][r] = fmax(most[h][r], x);
-                small |= x > 0.0 && x < SNK_WEIGHT_LEAST;
-            }
+        for (int r = 0; r < 4; ++r) {
+            const int row = g + 4 * r;
+            const double x = i0 + row < K ? slab0[(int64_t)(i0 + row) * Kp + col[c]] * l : 0.0;
+            X[0][row * LDX + col[c]] = x;
+            most[r] = fmax(most[r], x);
+            small |= x > 0.0 && x < SNK_WEIGHT_LEAST;
+        }
     }
     auto row_max = [&](int at) {                                // largest weight of every row, per wavefront (lane 15 of each row of lanes has it)
 #pragma unroll
-        for (int h = 0; h < RB; ++h)
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const double m = row16_max(most[h][r]);
-                if (c16 == 15) top[at][wave][16 * h + g + 4 * r] = m;
-            }
+        for (int r = 0; r < 4; ++r) {
+            const double m = row16_max(most[r]);
+            if (c16 == 15) top[at][wave][g + 4 * r] = m;
+        }
     };
     auto row_exponent = [&](int at, int row) -> int {
         double m = top[at][0][row];
@@ -547,24 +541,17 @@ trellis_product_kernel(const TrellisView v, const double *__restrict__ local, in
     };
     row_max(0);
     __syncthreads();
-    auto read = [&](int at, int step, double (&x)[RB]) {
-#pragma unroll
-        for (int h = 0; h < RB; ++h) x[h] = X[at][(16 * h + c16) * LDX + step * 4 + g];
-    };
-    int e4[RB][4] = {};
+    auto read = [&](int at, int step) { return X[at][c16 * LDX + step * 4 + g]; };
+    int e4[4] = {};
     for (int s = 1; s < p.n; ++s) {
         const int from = (s - 1) & 1, to = s & 1;
-        f64x4 acc[RB][CT];
+        f64x4 acc[CT];
 #pragma unroll
-        for (int h = 0; h < RB; ++h)
-#pragma unroll
-            for (int c = 0; c < CT; ++c) acc[h][c] = f64x4{0.0, 0.0, 0.0, 0.0};
+        for (int c = 0; c < CT; ++c) acc[c] = f64x4{0.0, 0.0, 0.0, 0.0};
         double lw[CT];
 #pragma unroll
         for (int c = 0; c < CT; ++c) lw[c] = col[c] < Kp ? local[(first_row + s + 1) * Kp + col[c]] : 0.0;
-        double x[3][RB];
-        read(from, 0, x[0]);
-        read(from, 1, x[1]);
+        double x[3] = {read(from, 0), read(from, 1), 0.0};
 #pragma unroll
         for (int half = 0; half < CH; ++half) {
             const int nslab = half + 1 < CH ? s : s + 1, nhalf = half + 1 < CH ? half + 1 : 0;
@@ -572,32 +559,28 @@ trellis_product_kernel(const TrellisView v, const double *__restrict__ local, in
             for (int ks = 0; ks < KH; ++ks) {
                 // weights two steps ahead, products, reloads: in this order (left to itself the compiler moves the reloads behind the
                 // last product, where the next slab waits for them)
-                if (half * KH + ks + 2 < KH * CH) read(from, half * KH + ks + 2, x[(half * KH + ks + 2) % 3]);
+                if (half * KH + ks + 2 < KH * CH) x[(half * KH + ks + 2) % 3] = read(from, half * KH + ks + 2);
 #pragma unroll
-                for (int c = 0; c < CT; ++c)
-#pragma unroll
-                    for (int h = 0; h < RB; ++h) acc[h][c] = __builtin_amdgcn_mfma_f64_16x16x4f64(x[(half * KH + ks) % 3][h], frag[ks][c], acc[h][c], 0, 0, 0);
+                for (int c = 0; c < CT; ++c) acc[c] = __builtin_amdgcn_mfma_f64_16x16x4f64(x[(half * KH + ks) % 3], frag[ks][c], acc[c], 0, 0, 0);
 #pragma unroll
                 for (int c = 0; c < CT; ++c) load(nslab, nhalf, ks, c);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
 #pragma unroll
-        for (int h = 0; h < RB; ++h)
+        for (int r = 0; r < 4; ++r) {
+            const int row = g + 4 * r, e = row_exponent(from, row);
+            const double f = trellis_pow2(-e);
+            e4[r] += e;
+            most[r] = 0.0;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int row = 16 * h + g + 4 * r, e = row_exponent(from, row);
-                const double f = trellis_pow2(-e);
-                e4[h][r] += e;
-                most[h][r] = 0.0;
-#pragma unroll
-                for (int c = 0; c < CT; ++c) {
-                    const double x = (acc[h][c][r] * f) * lw[c];
-                    if (col[c] < Kp) X[to][row * LDX + col[c]] = x;
-                    most[h][r] = fmax(most[h][r], x);
-                    small |= x > 0.0 && x < SNK_WEIGHT_LEAST;
-                }
+            for (int c = 0; c < CT; ++c) {
+                const double x = (acc[c][r] * f) * lw[c];
+                if (col[c] < Kp) X[to][row * LDX + col[c]] = x;
+                most[r] = fmax(most[r], x);
+                small |= x > 0.0 && x < SNK_WEIGHT_LEAST;
             }
+        }
         row_max(to);
         __syncthreads();
     }
@@ -607,18 +590,16 @@ trellis_product_kernel(const TrellisView v, const double *__restrict__ local, in
     // out: rows scaled to [1, 2), their exponents beside them
     const int at = (p.n - 1) & 1;
 #pragma unroll
-    for (int h = 0; h < RB; ++h)
+    for (int r = 0; r < 4; ++r) {
+        const int row = g + 4 * r, i = i0 + row, e = row_exponent(at, row);
+        const double f = trellis_pow2(-e);
+        if (i < K) {
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const int row = 16 * h + g + 4 * r, i = i0 + row, e = row_exponent(at, row);
-            const double f = trellis_pow2(-e);
-            if (i < K) {
-#pragma unroll
-                for (int c = 0; c < CT; ++c)
-                    if (col[c] < Kp) M[(p.at * K + i) * Kp + col[c]] = X[at][row * LDX + col[c]] * f;
-                if (wave == 0 && c16 == 0) exps[p.at * K + i] = e4[h][r] + e;
-            }
+            for (int c = 0; c < CT; ++c)
+                if (col[c] < Kp) M[(p.at * K + i) * Kp + col[c]] = X[at][row * LDX + col[c]] * f;
+            if (wave == 0 && c16 == 0) exps[p.at * K + i] = e4[r] + e;
         }
+    }
 }
 
 // 2. the weights at the pieces' ends: a workgroup per utterance; what a step waits for is what it costs (two barriers, no sum in a row).
@@ -1474,15 +1455,11 @@ void launch_trellis_ends(const TrellisView &v, const double *local, bool both, i
 {
     const int n = v.pieces;
     if (n == 1) return;
-    // (two workgroups a compute unit: beyond two rounds of them the larger row blocks, where the registers hold them)
     const int64_t all = (((int64_t)n * v.n_utts + 7) / 8) * 8;
-    const int rb = v.K <= 128 && all * ((v.K + 15) / 16) >= 1024 ? 2 : 1, row_blocks = (v.K + 16 * rb - 1) / (16 * rb);
+    const int row_blocks = (v.K + 15) / 16;
     const dim3 grid((unsigned)(all * row_blocks));
 #define SNK_PROD(CT_, KH_, CH_, NTH_)                                                                                                             \
-    do {                                                                                                                                          \
-        if (rb == 2) hipLaunchKernelGGL((trellis_product_kernel<CT_, KH_, CH_, CH_ == 1 ? 2 : 1, NTH_>), grid, dim3(NTH_), 0, s, v, local, n, row_blocks, !both, flag, M, exps); \
-        else hipLaunchKernelGGL((trellis_product_kernel<CT_, KH_, CH_, 1, NTH_>), grid, dim3(NTH_), 0, s, v, local, n, row_blocks, !both, flag, M, exps);         \
-    } while (0)
+    hipLaunchKernelGGL((trellis_product_kernel<CT_, KH_, CH_, NTH_>), grid, dim3(NTH_), 0, s, v, local, n, row_blocks, !both, flag, M, exps)
     if (v.K <= 32) SNK_PROD(1, 8, 1, 128);
     else if (v.K <= 64) SNK_PROD(1, 16, 1, 256);
     else if (v.K <= 104) SNK_PROD(2, 26, 1, 256);
