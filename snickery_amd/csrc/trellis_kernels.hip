@@ -467,7 +467,9 @@ __device__ __forceinline__ TrellisPiece trellis_piece(const TrellisView &v, int 
 // reloaded with the next slab's (or the next half's) right after its use.  The row blocks of a piece are dealt to one XCD, so that a
 // slab comes from memory once and from that XCD's L2 for the others: a step re-reads the slab for sixteen rows, 50 bytes a cycle and
 // compute unit.  Thirty-two rows halve that but leave two workgroups a compute unit where sixteen leave three: 0.72 against 0.63 ms for
-// 9600 rows of 100 (30 TFLOP/s, 36 with the padding); 1200 rows of 200: 0.62 ms; 600 of 100: 71 us, 24 steps of 3 us.
+// 9600 rows of 100 (30 TFLOP/s, 36 with the padding); 1200 rows of 200: 0.62 ms; 600 of 100: 71 us, 24 steps of 3 us.  Sizes of their own
+// for 80 and 160 candidates: 350 instead of 430 us and 2.3 instead of 3.1 ms for 9600 rows.  CT 1 where the registers of CT 2 leave one
+// wavefront a SIMD (2.3 against 2.5 ms), not below (0.74 against 0.63 ms).
 template <int CT, int KH, int CH, int NTH>
 __global__ void __launch_bounds__(NTH, NTH == 256 && KH <= 26 ? 3 : 2)
 trellis_product_kernel(const TrellisView v, const double *__restrict__ local, int max_pieces, int row_blocks, bool skip_last, int *__restrict__ flag,
@@ -1462,8 +1464,10 @@ void launch_trellis_ends(const TrellisView &v, const double *local, bool both, i
     hipLaunchKernelGGL((trellis_product_kernel<CT_, KH_, CH_, NTH_>), grid, dim3(NTH_), 0, s, v, local, n, row_blocks, !both, flag, M, exps)
     if (v.K <= 32) SNK_PROD(1, 8, 1, 128);
     else if (v.K <= 64) SNK_PROD(1, 16, 1, 256);
+    else if (v.K <= 80) SNK_PROD(2, 20, 1, 192);
     else if (v.K <= 104) SNK_PROD(2, 26, 1, 256);
     else if (v.K <= 128) SNK_PROD(2, 32, 1, 256);
+    else if (v.K <= 160) SNK_PROD(1, 20, 2, 640);
     else SNK_PROD(2, 26, 2, 448);
 #undef SNK_PROD
 #define SNK_ENDS(R_, H_, CW_, RG_, RB_, HB_, Q_, S_, NTH_)                                                                                           \
