@@ -468,7 +468,7 @@ __device__ __forceinline__ TrellisPiece trellis_piece(const TrellisView &v, int 
 // slab comes from memory once and from that XCD's L2 for the others: a step re-reads the slab for sixteen rows, 50 bytes a cycle and
 // compute unit.  Thirty-two rows halve that but leave two workgroups a compute unit where sixteen leave three: 0.72 against 0.63 ms for
 // 9600 rows of 100 (30 TFLOP/s, 36 with the padding); 1200 rows of 200: 0.62 ms; 600 of 100: 71 us, 24 steps of 3 us.  Sizes of their own
-// for 80 and 160 candidates: 350 instead of 430 us and 2.3 instead of 3.1 ms for 9600 rows.  CT 1 where the registers of CT 2 leave one
+// for 80 and 160 candidates: 350 instead of 445 us and 2.3 instead of 3.1 ms for 9600 rows.  CT 1 where the registers of CT 2 leave one
 // wavefront a SIMD (2.3 against 2.5 ms), not below (0.74 against 0.63 ms).
 template <int CT, int KH, int CH, int NTH>
 __global__ void __launch_bounds__(NTH, NTH == 256 && KH <= 26 ? 3 : 2)
