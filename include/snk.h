@@ -347,7 +347,7 @@ int snk_set_position_bias(snk_handle h, const double *bias, int n_classes, int n
  * candidates cand / tdist (row_offsets[n_utts], K) of n_utts utterances (as snk_viterbi_batch; candidates of a unit that cannot
  * join or without a finite target cost take no part).  Each path is drawn from its end: the last candidate from its marginal,
  * every one before from its probability given the one behind it, each of these distributions truncated by top_k, top_p and
- * min_p as in snk_sample_rows.  temperature 0: the cheapest path (ties as in snk_viterbi).
+ * min_p as in snk_sample_rows.  temperature 0: the cheapest path (ties as in snk_viterbi); one below 1e-250 counts as that.
  *   join_class (rows) int32, or NULL (class 0): class of the join from row r to row r + 1; outside 0 .. n_classes - 1: no bias
  *   u (n_draws, rows) float64 in [0, 1)
  *   path_out (n_draws, rows) int64 unit ids, -1 throughout an utterance without a complete path

@@ -253,7 +253,7 @@ static int trellis_groups(snk_engine *h, const TrellisCall &q, Use use)
         v.first = v0; v.n_utts = v1 - v0; v.K = q.K; v.Kp = Kp;
         v.c0 = q.row_offsets[v0]; v.rows = q.row_offsets[v1] - q.row_offsets[v0];
         v.n_units = h->Njc - 1;
-        v.inv_tau = q.temperature > 0.0 ? 1.0 / q.temperature : 1.0;
+        v.inv_tau = q.temperature > 0.0 ? std::min(1.0 / q.temperature, 1e250) : 1.0;      // (0 times it is 0, costs times it keep their order)
         v.pieces = trellis_most_pieces(q.row_offsets + v0, v.n_utts);
         if (v.pieces > 1) {
             const size_t n = trellis_piece_places(v);

@@ -549,6 +549,20 @@ def test_trellis_of_costs_that_overflow(engine):
         assert post.shape == cand.shape and uses.shape == (1, 2)
 
 
+@pytest.mark.parametrize('tau', [1e-300, 1e-310, 5e-324])
+def test_trellis_of_a_temperature_whose_inverse_overflows(engine, tau):
+    """The cheapest path, as at temperature 0; all of the probability is its."""
+    v = Voice(engine)
+    cand, dist, offs = v.candidates([30, 1, 7], 20)
+    rng = np.random.RandomState(1)
+    cheapest, cost, _ = engine.sample_paths(cand, dist, rng.rand(1, 38), row_offsets=offs, temperature=0.0)
+    path, c, logp = engine.sample_paths(cand, dist, rng.rand(3, 38), row_offsets=offs, temperature=tau)
+    assert np.array_equal(path, np.repeat(cheapest, 3, axis=0)) and np.array_equal(c, np.repeat(cost, 3, axis=0)) and not logp.any()
+    # float32 and float64 rows in the same limit
+    x = rng.randn(5, 30)
+    assert np.array_equal(engine.sample_rows(x, rng.rand(5), temperature=tau)[0], x.argmax(axis=1))
+
+
 def test_trellis_without_a_complete_path(engine):
     v = Voice(engine)
     cand, dist, offs = v.candidates([6, 4, 1, 5], 5, pad=False)
@@ -670,6 +684,16 @@ def test_recursions_in_pieces(engine, lengths, K):
     for tau in (0.3, 2.0):
         check_posterior(v, cand, dist, offs, cls, tau)
         check_paths(v, cand, dist, offs, u, cls, temperature=tau, top_p=0.9)
+
+
+@pytest.mark.parametrize('T,K', [(30000, 3), (5000, 33)])
+def test_trellis_of_a_long_utterance(engine, T, K):
+    v = Voice(engine, n=2000)
+    v.set_bias(1, 8)
+    cand, dist, offs = v.candidates([T], K)
+    u = np.random.RandomState(3).rand(1, T)
+    check_posterior(v, cand, dist, offs, temperature=0.7)
+    check_paths(v, cand, dist, offs, u, temperature=0.7, top_p=0.95)
 
 
 def test_trellis_results_do_not_depend_on_the_batch(engine):
