@@ -300,6 +300,34 @@ def test_rows_of_many_long_rows(engine, R, V):
         assert np.array_equal(i[few].cpu().numpy(), want)
 
 
+@pytest.mark.parametrize('V', [100, 1000, 5000, 20000])
+def test_rows_past_offsets_of_32_bits(engine, V):
+    import torch
+    g = torch.Generator(device='cuda').manual_seed(1)
+    stride = (1 << 31) + 4096 + 8
+    memory = torch.zeros(2 * stride + V, dtype=torch.float16, device='cuda')
+    rows = memory.as_strided((3, V), (stride, 1))
+    x = torch.randn((3, V), device='cuda', generator=g).half()
+    rows.copy_(x)
+    u = torch.rand((3, 2), device='cuda', dtype=torch.float64, generator=g)
+    i, lp = engine.sample_rows(rows, u, top_p=0.8)
+    j, lq = engine.sample_rows(x, u, top_p=0.8)
+    assert torch.equal(i, j) and torch.equal(lp, lq)
+
+
+@pytest.mark.parametrize('R,V', [((1 << 25) + 7, 2), ((1 << 21) + 3, 1025)])
+def test_more_rows_than_a_launch_holds(engine, R, V):
+    """Equal scores: every weight is 2^s, the draw is the quotient by it of the mass below u."""
+    import torch
+    x = torch.zeros((R, V), dtype=torch.float16, device='cuda')
+    u = torch.rand(R, device='cuda', dtype=torch.float64, generator=torch.Generator(device='cuda').manual_seed(0))
+    i, lp = engine.sample_rows(x, u)
+    s = min(51, 62 - int(np.ceil(np.log2(V))))
+    want = torch.div(torch.floor(u * float(V << s)).to(torch.int64), 1 << s, rounding_mode='floor')
+    assert torch.equal(i, want)
+    assert (lp + np.log(V)).abs().max().item() <= logp_tolerance(V, np.log(V))
+
+
 def test_rows_of_many_draws(engine):
     """More draws than a launch's second dimension holds."""
     rng = np.random.RandomState(9)
@@ -684,6 +712,26 @@ def test_recursions_in_pieces(engine, lengths, K):
     for tau in (0.3, 2.0):
         check_posterior(v, cand, dist, offs, cls, tau)
         check_paths(v, cand, dist, offs, u, cls, temperature=tau, top_p=0.9)
+
+
+def test_trellis_of_more_than_four_gigabytes(engine):
+    """Cells of one utterance past offsets of 32 bits: the cheapest path against the search's own, probabilities that sum to 1."""
+    T, K = 13000, 208
+    v = Voice(engine, n=5000)
+    cand, dist, offs = v.candidates([T], K, pad=False)
+    assert T * K * K * 8 > 1 << 32
+    u = np.random.RandomState(0).rand(1, T)
+    path, cost, _ = engine.sample_paths(cand, dist, u, temperature=0.0)
+    _, want_cost = engine.viterbi(cand, dist)
+    product = (v.JC.shape[1] + 4.0) * 2.0 ** -45             # of a join cost by products, relative: the choice between paths that near
+    assert abs(cost[0, 0] - want_cost) <= (2.0 ** -52 * 4.0 * T + 2.0 * product) * want_cost
+    logz, post, _ = engine.path_posterior(cand, dist, temperature=0.8)
+    size = abs(logz[0]) + 2.0 * T / 0.8
+    assert np.abs(post.sum(axis=1) - 1.0).max() <= 8.0 * sum_tolerance(T, K, size) and post.min() >= 0.0
+    path, cost, logp = engine.sample_paths(cand, dist, u, temperature=0.8)
+    assert (path[0][:, None] == cand).any(axis=1).all() and cost[0, 0] > want_cost and logp[0, 0] < 0.0
+    # without a truncation the log probability is the path's own
+    assert abs(logp[0, 0] - (-cost[0, 0] / 0.8 - logz[0])) <= 2.0 * T * logp_tolerance(K) + 4.0 * sum_tolerance(T, K, size) + 4.0 * product * cost[0, 0] / 0.8
 
 
 @pytest.mark.parametrize('T,K', [(30000, 3), (5000, 33)])
