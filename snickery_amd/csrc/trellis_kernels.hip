@@ -132,14 +132,16 @@ trellis_local_kernel(const TrellisView v, double *__restrict__ local, double *__
 // a column instead of a subtraction and one), which ran at two thirds of the vector pipe's rate.  Both sides are taken relative to
 // one unit of the second row, so that the norms are those of the candidates' spread and not of their distance from the origin.  Where
 // the difference is small against the norms -- neighbouring frames -- the product form cancels: a cell below SNK_COST_NEAR of them is taken
-// again in differences.  A unit and its natural successor join at exactly 0.  The others carry a relative error of at most Dj 2^-53 / SNK_COST_NEAR.
+// again in differences.  A unit and its natural successor join at exactly 0.  The others carry a relative error of at most Dj 2^-53 / SNK_COST_NEAR,
+// an absolute one of 2^5 Dj 2^-53 of the norms' root.  (2^-8: 2.20 ms for 9600 rows of 100, half the error of the posteriors; 2^-10: 2.11 and
+// 1.2e-14 at most over 335 rows of 50, where logarithms of float64 err by 2e-13.)
 // A wavefront owns RM x CM tiles of 16 x 16; DC columns of the two sets of rows go through LDS at a time, weighted and widened on
 // the way, the next ones are in flight meanwhile: 32, a cache line of a row (197 us for 600 rows of 100 candidates and 302 columns, 206
 // with 16, before what follows), or 16 in the larger tiles, whose registers hold no more (2.55 ms for 9600 rows, 2.73 with 32 and
-// spills).  9600 rows of 100 candidates, 302 columns: 2.14 ms, 27 TFLOP/s of a large product's 62 (34 with the cells that pad K to
+// spills).  9600 rows of 100 candidates, 302 columns: 2.11 ms, 27 TFLOP/s of a large product's 62 (35 with the cells that pad K to
 // 112); bound by the float64 units, which the products hold 43 % of the time and weighing the cells, staging and padding the most of
-// the rest: neither overlaps with products of another wavefront.  1200 rows of 200, 151 columns: 0.68 ms.
-#define SNK_COST_NEAR 0x1p-8
+// the rest: neither overlaps with products of another wavefront.  1200 rows of 200, 151 columns: 0.66 ms.
+#define SNK_COST_NEAR 0x1p-10
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
 // weight of a column; 0 behind the last.  (Loads from a clamped place, here and of the rows: a load that is left out behind a condition

@@ -811,8 +811,10 @@ def test_trellis_of_many_utterances(engine):
 @pytest.mark.parametrize('Dj', [1, 33, 151, 302])
 def test_join_costs_of_far_and_near_units(engine, Dj):
     """Frames that lie far from the origin, next to each other, and equal.  The engine may take a squared distance from products,
-    |e|^2 + |s|^2 - 2 e s, where that is above 2^-8 of |e|^2 + |s|^2; its Dj + 4 roundings of 2^-53 then cost 2^8 (Dj + 4) 2^-52
-    relative of the square, half that of the distance: so much of the largest join cost, once a row and for each sum that it enters."""
+    |e|^2 + |s|^2 - 2 e s, where that is above 2^-10 of n = |e|^2 + |s|^2.  Its Dj + 4 roundings of 2^-53 are (Dj + 4) 2^-52 n of the
+    square, (Dj + 4) 2^-53 n / c of a distance c >= 2^-5 sqrt(n): at most (Dj + 4) 2^-48 sqrt(n), n at most twice the square of the
+    largest distance about the unit that both are taken relative to.  Below 2^-45 (Dj + 4) of the largest join cost, four times that:
+    once a row and for each sum that it enters."""
     v = Voice(engine, Dj=Dj, n=300)
     rng = np.random.RandomState(Dj)
     JC = 3000.0 + rng.randn(301, Dj)
