@@ -355,7 +355,7 @@ int snk_set_position_bias(snk_handle h, const double *bias, int n_classes, int n
  *   probabilities (-inf there)
  * K up to 208, n_draws up to 65535, an utterance up to 2^23 rows; one of a single row is a draw from its target costs.  Results of an
  * utterance do not depend on the others of the call.  Join costs are float64, within (Dj + 4) 2^-43 relative of the exact ones and (Dj + 4)
- * 2^-47 of the largest.
+ * 2^-47 of the largest; a join over a frame that is not finite, or whose distance float64 does not hold, is forbidden.
  * The _dev form takes device memory (row_offsets excepted) and puts its kernels on `stream` without a host wait.  It uses the engine's
  * workspaces: later calls, on any stream, are ordered behind it, and it refuses a stream that is being captured.  It cannot look at
  * device memory first: numbers u as in snk_sample_rows_dev. */

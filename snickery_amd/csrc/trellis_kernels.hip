@@ -135,6 +135,9 @@ trellis_local_kernel(const TrellisView v, double *__restrict__ local, double *__
 // again in differences.  A unit and its natural successor join at exactly 0.  The others carry a relative error of at most Dj 2^-53 / SNK_COST_NEAR,
 // an absolute one of 2^5 Dj 2^-53 of the norms' root.  (2^-8: 2.20 ms for 9600 rows of 100, half the error of the posteriors; 2^-10: 2.11 and
 // 1.2e-14 at most over 335 rows of 50, where logarithms of float64 err by 2e-13.)
+// Frames that are not finite: a distance that is infinite or no number joins nothing.  The product form says so only while the unit that both
+// sides are taken relative to is finite; where it is not, or a frame brings an infinity of its own into a product, a cell's value is no
+// number, and every such cell of units that can join counts as near: the differences, which know its own two frames alone, decide.
 // A wavefront owns RM x CM tiles of 16 x 16; DC columns of the two sets of rows go through LDS at a time, weighted and widened on
 // the way, the next ones are in flight meanwhile: 32, a cache line of a row (197 us for 600 rows of 100 candidates and 302 columns, 206
 // with 16, before what follows), or 16 in the larger tiles, whose registers hold no more (2.55 ms for 9600 rows, 2.73 with 32 and
@@ -367,7 +370,7 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
     auto value = [&](double d2, int ie, int is) -> double {     // a cell from the squared distance, infinite: cannot join
         double cost = LOG ? sqrt(d2) : trellis_root(d2);
         if (cls >= 0) cost += bias[trellis_bucket(is - ie, look)];
-        if (LOG) return -cost * v.inv_tau;
+        if (LOG) return cost < __builtin_inf() ? -cost * v.inv_tau : -__builtin_inf();
         const bool ok = cost < __builtin_inf();                 // (the root of an infinite square is not a number)
         const double x = (c.bias_min - cost) * v.inv_tau;
         wide |= ok && x < -SNK_COST_RANGE;
@@ -390,10 +393,11 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int al = ti * 16 + g + 4 * r, ie = idE[al], a = a0 + al;
-            const double both = nE[al] + sn, apart = __fma_rn(-2.0, p[r], both), d2 = is == ie + 1 ? 0.0 : apart;   // (natural: the same frame)
-            again[r] = apart < SNK_COST_NEAR * both && is != ie + 1;
+            const double both = nE[al] + sn, apart = __fma_rn(-2.0, p[r], both);
+            const bool natural = is == ie + 1;                  // (the same frame)
+            again[r] = (ie | is) >= 0 && (natural ? !(both < __builtin_inf()) : !(apart >= SNK_COST_NEAR * both));      // (true of what is no number)
             any += again[r] ? 1 : 0;
-            const double x = value(fmax(d2, 0.0), ie, is);
+            const double x = value(natural ? 0.0 : fmax(apart, 0.0), ie, is);
             if (a < v.K && b < v.Kp) out[(int64_t)a * v.Kp + b] = x;
         }
         if (__ballot(any)) {
@@ -421,7 +425,7 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
         }
         if (c16 < n) {
             const int cell = near_cell[first + c16], al = cell / N, bl = cell % N, a = a0 + al, b = b0 + bl;
-            const double x = value(d2, idE[al], idS[bl]);
+            const double x = value(d2 < __builtin_inf() ? d2 : __builtin_inf(), idE[al], idS[bl]);
             if (a < v.K && b < v.Kp) out[(int64_t)a * v.Kp + b] = x;
         }
     }
