@@ -237,6 +237,8 @@ __global__ void __launch_bounds__(NTH, OCC)
 trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__ flag, double *__restrict__ X)
 {
     constexpr int N = 16 * RT, QL = DC / 4, LD = DC + 2, NW = NTH / 64, NR = NTH / QL, PASS = (N + NR - 1) / NR;
+    constexpr int HALF = 32 / DC;                               // sums of a norm that a thread keeps: see below
+    static_assert(HALF * DC == 32 && HALF <= 2, "a norm has eight sums");
     constexpr int WC = RT / CM;                                 // wavefronts side by side
     static_assert(RT % RM == 0 && RT % CM == 0 && (RT / RM) * WC <= NW, "every tile has its wavefront");
     __shared__ __align__(16) double Es[2 * N * LD];             // of the first row's candidates, then of the second's
@@ -288,14 +290,27 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
     const int q = tid & (QL - 1), r0 = tid / QL;            // a thread takes four columns of the rows r0, r0 + NR, ..
     const float *pe[PASS], *ps[PASS], *pc = c.JC + (int64_t)about * c.Jp + 4 * q;
     float4 fe[PASS], fs[PASS], fc;
-    double w[4], ne[PASS], ns[PASS];
+    // A norm is the sum of eight, of the columns 4 i .. 4 i + 3 of every 32, whatever the tile: with 32 columns at a time a thread has one
+    // of them, with 16 two, which take turns.  So a cell is the same to the last bit in every tile, and an utterance's results do not
+    // depend on how many rows stand beside it.
+    double w[4], ne[HALF][PASS], ns[HALF][PASS];
 #pragma unroll
     for (int p = 0; p < PASS; ++p) {
         const int r = r0 + NR * p < N ? r0 + NR * p : 0;
         pe[p] = c.JC + (int64_t)(idE[r] >= 0 ? idE[r] + 1 : about) * c.Jp + 4 * q;
         ps[p] = c.JC + (int64_t)(idS[r] >= 0 ? idS[r] : about) * c.Jp + 4 * q;
-        ne[p] = 0.0; ns[p] = 0.0;
+#pragma unroll
+        for (int h = 0; h < HALF; ++h) ne[h][p] = ns[h][p] = 0.0;
     }
+    auto turn = [&]() {                                         // the other half of 32 columns is next
+        if (HALF == 2)
+#pragma unroll
+            for (int p = 0; p < PASS; ++p) {
+                const double e = ne[0][p], s = ns[0][p];
+                ne[0][p] = ne[HALF - 1][p]; ns[0][p] = ns[HALF - 1][p];
+                ne[HALF - 1][p] = e; ns[HALF - 1][p] = s;
+            }
+    };
     auto fetch = [&](int col) {
         const int at = min(col, c.Jp - 4 - 4 * q);              // (rows are padded to multiples of four columns)
         fc = *reinterpret_cast<const float4 *>(pc + at);
@@ -326,14 +341,15 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
                     const double m = (double)c4[e] * w[e];
                     de[e] = __fma_rn((double)e4[e], w[e], -m);
                     ds[e] = __fma_rn((double)s4[e], w[e], -m);
-                    ne[p] = __fma_rn(de[e], de[e], ne[p]);
-                    ns[p] = __fma_rn(ds[e], ds[e], ns[p]);
+                    ne[0][p] = __fma_rn(de[e], de[e], ne[0][p]);
+                    ns[0][p] = __fma_rn(ds[e], ds[e], ns[0][p]);
                 }
                 f64x2 *te = reinterpret_cast<f64x2 *>(&Es[r * LD + 4 * q]), *ts = reinterpret_cast<f64x2 *>(&Ss[r * LD + 4 * q]);
                 te[0] = f64x2{de[0], de[1]}; te[1] = f64x2{de[2], de[3]};
                 ts[0] = f64x2{ds[0], ds[1]}; ts[1] = f64x2{ds[2], ds[3]};
             }
         }
+        turn();
         __syncthreads();
         if (col + DC < c.Dj) fetch(col + DC);
         if (busy) {
@@ -353,10 +369,12 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
         }
         __syncthreads();
     }
+    if (((c.Dj + DC - 1) / DC) & 1) turn();
 #pragma unroll
     for (int p = 0; p < PASS; ++p) {
         const int r = r0 + NR * p;
-        double e = quad_sum(ne[p]), s = quad_sum(ns[p]);
+        double e = quad_sum(ne[0][p]), s = quad_sum(ns[0][p]);
+        if (HALF == 2) { e += quad_sum(ne[HALF - 1][p]); s += quad_sum(ns[HALF - 1][p]); }
         if (QL == 8) { e = eight_sum(e); s = eight_sum(s); }
         if (r < N && q == 0) {                                  // what cannot join is infinitely far
             nE[r] = idE[r] >= 0 ? e : __builtin_inf();
