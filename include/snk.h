@@ -320,7 +320,8 @@ int snk_copy_to_device(void *dst_dev, const void *src_host, int64_t bytes);
  * probability -inf; +inf shares the row among its holders.
  *   row_rules (R, 4) float64, or NULL: temperature, top_k, top_p, min_p of each row instead of the call's
  *   index_out (R, n_draws) int64; logp_out (R, n_draws) float64, or NULL: log of the drawn weight over the kept weight
- * Draws are reproducible: sums of weights are whole numbers, the same in any order.  V is at most 2^24.
+ * Draws are reproducible: sums of weights are whole numbers, the same in any order.  A weight is rounded to a multiple of 2^-51 of the
+ * largest (2^-50 in rows of more than 4096 scores): V 2^-52 of the mass (V 2^-51) at most is moved or lost.  V is at most 2^24.
  * The _dev form takes device memory throughout and puts its kernels on `stream` (a hipStream_t; NULL: the default stream)
  * without waiting, and can be captured into a graph.  Rows of more than 8192 scores use a workspace: `workspace`, device memory of
  * at least snk_sample_rows_workspace(R, V) bytes (0: none needed), aligned to 16, that nothing else uses until the call's kernels

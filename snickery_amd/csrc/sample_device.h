@@ -8,15 +8,18 @@
 //     draw = the smallest kept i with  sum_{j <= i, kept} w_j  >  u * sum_{kept} w_j
 //
 // A draw is a whole number: it has to come out the same however the row is split over lanes and workgroups.  So masses are
-// 64-bit integers, w_i rounded to nearest in units of 2^-s: integer sums are exact in any order, and every comparison above is
-// one between integers.  s <= 51 leaves the rounding of one weight at half a unit of float64's last place next to 1 (the weights
-// themselves are computed in float64); rows of more than 2^11 scores take s = 62 - ceil(log2 V), so that a sum never overflows.
+// integers, w_i rounded to nearest in units of 2^-s: integer sums are exact in any order, and every comparison above is one between
+// integers.  s = 51 leaves the rounding of one weight at a unit of float64's last place next to 1 (the weights themselves are computed in
+// float64), and the sums of up to 4096 of them in 64 bits; rows of more scores take s = 50, whose sums of up to 8192 fit, and
+// longer sums a second word (sample_sum below).  A row's largest weight is 1, so that V 2^-(s+1) is also the share of the mass that
+// rounding can move: 2e-13 of 208 scores, 5e-10 of 2^20, 7e-9 of 2^24.
 #pragma once
 #include "snk_internal.h"
 
 namespace snk {
 
 typedef unsigned long long u64;
+typedef unsigned __int128 u128;
 
 struct SampleRule {             // what a row is truncated by, in the form the kernels use
     double inv_tau;             // +inf: temperature 0 (with top_k 1: the lowest index of the maximum)
@@ -96,6 +99,45 @@ __device__ __forceinline__ u64 sample_exceed(double u, u64 total)
     const double t = floor(u * (double)total);
     if (!(t > 0.0)) return 0;
     return t >= (double)total ? total - 1 : (u64)t;
+}
+
+// ---- sums of up to 2^24 weights of up to 2^50, in two words that any order of additions leaves the same: `mass`, the sum modulo 2^64, and
+// `more`, the sum of the weights' upper parts (w >> 40, 34 bits) below a count (24 bits).  What the lower parts add up to is less than 2^64
+// and therefore known from both.  (A word for the carry alone would need atomics that return what they found.)
+#define SNK_MORE_ONE (1ull << 36)
+__device__ __forceinline__ u64 sample_more(u64 w) { return w >> 40; }
+__device__ __forceinline__ u64 sample_count(u64 more) { return more >> 36; }
+__device__ __forceinline__ u128 sample_sum(u64 mass, u64 more)
+{
+    const u64 upper = more & (SNK_MORE_ONE - 1);
+    return ((u128)upper << 40) + (mass - (upper << 40));
+}
+__device__ __forceinline__ double sample_double(u128 v) { return __fma_rn((double)(u64)(v >> 64), 18446744073709551616.0, (double)(u64)v); }
+__device__ __forceinline__ u128 sample_whole(double t)          // of a whole number, 0 <= t < 2^96
+{
+    const double upper = floor(t * 0x1p-32);
+    return ((u128)(u64)upper << 32) + (u64)__fma_rn(-upper, 4294967296.0, t);
+}
+__device__ __forceinline__ u128 sample_reach(double top_p, u128 total)
+{
+    const double all = sample_double(total), t = ceil(top_p * all);
+    const u128 v = t >= all ? total : sample_whole(t);
+    return v < 1 ? 1 : v;
+}
+__device__ __forceinline__ u128 sample_exceed(double u, u128 total)
+{
+    const double all = sample_double(total), t = floor(u * all);
+    if (!(t > 0.0)) return 0;
+    return t >= all ? total - 1 : sample_whole(t);
+}
+// how many weights of `each` reach `need`: the quotient in float64, then put right (it is below 2^25)
+__device__ __forceinline__ u64 sample_ties(u128 need, u64 each)
+{
+    if (!each) return 0;
+    u64 n = (u64)(sample_double(need) / (double)each);
+    while ((u128)n * each < need) ++n;
+    while (n && (u128)(n - 1) * each >= need) --n;
+    return n;
 }
 
 // ---- wavefront sums and maxima on the data-parallel moves: a step costs two moves and one operation, where a shuffle through

@@ -87,8 +87,8 @@ sample_rows_wave_kernel(const T *__restrict__ scores, int64_t stride, int64_t R,
 // ---- longer rows without a workspace: a workgroup each, the row read once per pass ------------------------------------------------------
 // For rows that the passes below leave over and for captured calls without a workspace.  Bound by what one compute unit reads: a row of
 // 1048576 float32 3.3 ms, 37 rows of 50003 179 us.
-#define SNK_SAMPLE_TILES 4096
-#define SNK_SAMPLE_VEC 4
+#define SNK_SAMPLE_TILES 2048
+#define SNK_SAMPLE_VEC 8
 
 template <int NT> struct BlockScratch {
     u64 mass[NT / 64];
@@ -138,10 +138,9 @@ sample_rows_block_kernel(const T *__restrict__ scores, int64_t stride, int64_t V
     constexpr int BITS = ScoreKey<T>::bits;
     constexpr int64_t TILE = (int64_t)NT * SNK_SAMPLE_VEC;
     __shared__ BlockScratch<NT> scratch;
-    __shared__ u64 hist_mass[256];
-    __shared__ unsigned int hist_count[256];
-    __shared__ u64 tile_mass[SNK_SAMPLE_TILES];
-    __shared__ unsigned int tile_ties[SNK_SAMPLE_TILES];
+    __shared__ u64 hist_mass[256], hist_more[256];
+    __shared__ u64 tile_mass[SNK_SAMPLE_TILES], tile_more[SNK_SAMPLE_TILES];      // the count: scores equal to the cut
+    __shared__ u128 sh_above;
     __shared__ u64 sh_a, sh_b;
     __shared__ unsigned int sh_digit;
 
@@ -167,11 +166,12 @@ sample_rows_block_kernel(const T *__restrict__ scores, int64_t stride, int64_t V
     Key cut = 0;
     bool all = true;
     u64 n_tie = 0;
-    auto search = [&](bool by_mass, u64 want) -> bool {          // false: fewer than `want`: the prefix is the whole row
+    auto search = [&](bool by_mass, u128 want) -> bool {         // false: fewer than `want`: the prefix is the whole row
         Key prefix = 0;
-        u64 above = 0;
+        u128 above = 0;
+        auto amount = [&](u64 mass, u64 more) -> u128 { return by_mass ? sample_sum(mass, more) : (u128)sample_count(more); };
         for (int shift = BITS - 8; shift >= 0; shift -= 8) {
-            for (int i = tid; i < 256; i += NT) { hist_count[i] = 0; hist_mass[i] = 0; }
+            for (int i = tid; i < 256; i += NT) { hist_more[i] = 0; hist_mass[i] = 0; }
             __syncthreads();
             for (int64_t i = tid; i < V; i += NT) {
                 const double x = score_load(p + i);
@@ -179,40 +179,40 @@ sample_rows_block_kernel(const T *__restrict__ scores, int64_t stride, int64_t V
                 const Key k = score_key<T>(x);
                 if (shift + 8 < BITS && (k >> (shift + 8)) != (prefix >> (shift + 8))) continue;
                 const int digit = (int)((k >> shift) & 255);
+                u64 w = 0;
                 if (by_mass) {
-                    const u64 w = sample_weight(sample_exponent(x, m, rule.inv_tau), unit);
+                    w = sample_weight(sample_exponent(x, m, rule.inv_tau), unit);
                     if (w) atomicAdd(&hist_mass[digit], w);
                 }
-                atomicAdd(&hist_count[digit], 1u);
+                atomicAdd(&hist_more[digit], SNK_MORE_ONE + sample_more(w));
             }
             __syncthreads();
             if (tid < 64) {
                 // lane l: digits 255 - 4 l .. 252 - 4 l, from the top
-                u64 v[4], sum = 0;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) { const int d = 255 - (4 * tid + j); v[j] = by_mass ? hist_mass[d] : (u64)hist_count[d]; sum += v[j]; }
-                const u64 upto = wave_scan_add(sum);
-                const u64 hit = __ballot(above + upto >= want);
+                u64 mass = 0, more = 0;
+                for (int j = 0; j < 4; ++j) { const int d = 255 - (4 * tid + j); mass += hist_mass[d]; more += hist_more[d]; }
+                const u64 upto_mass = wave_scan_add(mass), upto_more = wave_scan_add(more);
+                const u64 hit = __ballot(above + amount(upto_mass, upto_more) >= want);
                 if (!hit) { if (tid == 0) sh_digit = 256; }
                 else if (tid == __ffsll((long long)hit) - 1) {
-                    u64 a = above + upto - sum;
+                    u128 a = above + amount(upto_mass - mass, upto_more - more);
                     for (int j = 0; j < 4; ++j) {
-                        if (a + v[j] >= want) { sh_digit = 255 - (4 * tid + j); sh_a = a; break; }
-                        a += v[j];
+                        const int d = 255 - (4 * tid + j);
+                        const u128 v = amount(hist_mass[d], hist_more[d]);
+                        if (a + v >= want) { sh_digit = d; sh_above = a; break; }
+                        a += v;
                     }
                 }
             }
             __syncthreads();
             const unsigned int digit = sh_digit;
             if (digit == 256) { __syncthreads(); return false; }
-            above = sh_a;
+            above = sh_above;
             prefix |= (Key)digit << shift;
-            if (shift == 0) {
-                const u64 c = hist_count[digit];
-                if (by_mass) {
-                    const u64 each = hist_mass[digit] / c;
-                    n_tie = (want - above + each - 1) / each;
-                } else n_tie = want - above;
+            if (shift == 0) {                                   // (equal scores, equal weights)
+                const u64 more = hist_more[digit], c = sample_count(more), upper = (more & (SNK_MORE_ONE - 1)) / c;
+                const u64 each = (upper << 40) + (hist_mass[digit] - ((upper * c) << 40)) / c;
+                n_tie = by_mass ? sample_ties(want - above, each) : (u64)(want - above);
             }
             __syncthreads();
         }
@@ -235,48 +235,47 @@ sample_rows_block_kernel(const T *__restrict__ scores, int64_t stride, int64_t V
     };
     const int64_t n_tiles = (V + TILE - 1) / TILE;
     u64 w_tie = 0;
-    auto totals = [&](bool use_min) -> u64 {
-        if (tid == 0) { sh_a = 0; sh_b = 0; }
-        for (int i = tid; i < n_tiles; i += NT) { tile_mass[i] = 0; tile_ties[i] = 0; }
+    auto totals = [&](bool use_min) -> u128 {
+        if (tid == 0) sh_b = 0;
+        for (int i = tid; i < n_tiles; i += NT) { tile_mass[i] = 0; tile_more[i] = 0; }
         __syncthreads();
         u64 tw = 0;
         for (int64_t t = 0; t < n_tiles; ++t) {
-            u64 mass = 0;
-            unsigned int ties = 0;
+            u64 mass = 0, more = 0;
             for (int j = 0; j < SNK_SAMPLE_VEC; ++j) {
                 const int64_t i = t * TILE + (int64_t)j * NT + tid;
                 if (i >= V) break;
                 const double x = score_load(p + i);
                 u64 w; unsigned int q;
                 element(x, use_min, w, q);
-                mass += w; ties += q;
+                mass += w; more += sample_more(w) + (q ? SNK_MORE_ONE : 0);
                 if (q) tw = sample_weight(sample_exponent(x, m, rule.inv_tau), unit);
             }
             mass = wave_add(mass);
-            const u64 all_ties = wave_add((u64)ties);
+            more = wave_add(more);
             if ((tid & 63) == 0) {
                 if (mass) atomicAdd(&tile_mass[t], mass);
-                if (all_ties) atomicAdd(&tile_ties[t], (unsigned int)all_ties);
+                if (more) atomicAdd(&tile_more[t], more);
             }
         }
         if (tw) sh_b = tw;                                      // (every holder writes the same value)
         __syncthreads();
         w_tie = sh_b;
-        u64 mass = 0, ties = 0, tm, tt;
-        for (int i = tid; i < n_tiles; i += NT) { mass += tile_mass[i]; ties += tile_ties[i]; }
-        block_scan2<NT>(mass, ties, tm, tt, scratch);
-        return tm + w_tie * (tt < n_tie ? tt : n_tie);
+        u64 mass = 0, more = 0, tm, tt;
+        for (int i = tid; i < n_tiles; i += NT) { mass += tile_mass[i]; more += tile_more[i]; }
+        block_scan2<NT>(mass, more, tm, tt, scratch);
+        return sample_sum(tm, tt) + (u128)w_tie * min(sample_count(tt), n_tie);
     };
-    if (rule.top_k > 0 && rule.top_k < V) search(false, (u64)rule.top_k);
+    if (rule.top_k > 0 && rule.top_k < V) search(false, (u128)rule.top_k);
     if (rule.top_p < 1.0) {
-        const u64 total = totals(false);
+        const u128 total = totals(false);
         search(true, sample_reach(rule.top_p, total));
     }
-    const u64 total = totals(rule.min_p > 0.0);
-    const double log_total = log((double)total / unit);
+    const u128 total = totals(rule.min_p > 0.0);
+    const double log_total = log(sample_double(total) / unit);
 
     for (int d = 0; d < n_draws; ++d) {
-        const u64 t = sample_exceed(u[r * n_draws + d], total);
+        const u128 t = sample_exceed(u[r * n_draws + d], total);
         // the tile: the first wavefront walks the tiles' sums
         if (tid == 0) {
             sh_digit = 0xffffffffu;
@@ -284,23 +283,28 @@ sample_rows_block_kernel(const T *__restrict__ scores, int64_t stride, int64_t V
             if (logp) logp[r * n_draws + d] = ninf;
         }
         if (tid < 64) {
-            u64 mass0 = 0, ties0 = 0;
+            u64 mass0 = 0, more0 = 0;
             for (int64_t b = 0; b < n_tiles; b += 64) {
-                const u64 mass = b + tid < n_tiles ? tile_mass[b + tid] : 0, ties = b + tid < n_tiles ? tile_ties[b + tid] : 0;
-                const u64 cm = mass0 + wave_scan_add(mass), ct = ties0 + wave_scan_add(ties);
-                const u64 hit = __ballot(cm + w_tie * (ct < n_tie ? ct : n_tie) > t);
+                const u64 mass = b + tid < n_tiles ? tile_mass[b + tid] : 0, more = b + tid < n_tiles ? tile_more[b + tid] : 0;
+                const u64 cm = mass0 + wave_scan_add(mass), ct = more0 + wave_scan_add(more);
+                const u64 hit = __ballot(sample_sum(cm, ct) + (u128)w_tie * min(sample_count(ct), n_tie) > t);
                 if (hit) {
                     const int l = __ffsll((long long)hit) - 1;
-                    if (tid == l) { sh_digit = (unsigned int)(b + l); sh_a = cm - mass; sh_b = ct - ties; }
+                    if (tid == l) {                             // what is left of t in the tile, and the equal scores before it
+                        const u64 before = sample_count(ct - more);
+                        sh_digit = (unsigned int)(b + l);
+                        sh_a = (u64)(t - (sample_sum(cm - mass, ct - more) + (u128)w_tie * min(before, n_tie)));
+                        sh_b = before;
+                    }
                     break;
                 }
-                mass0 = __shfl(cm, 63, 64); ties0 = __shfl(ct, 63, 64);
+                mass0 = wave_lane(cm, 63); more0 = wave_lane(ct, 63);
             }
         }
         __syncthreads();
         if (sh_digit == 0xffffffffu) { __syncthreads(); continue; }      // (only where the scores changed under the call)
         const int64_t base = (int64_t)sh_digit * TILE + (int64_t)tid * SNK_SAMPLE_VEC;
-        const u64 mass0 = sh_a, ties0 = sh_b;
+        const u64 goal = sh_a, ties0 = sh_b, kept0 = min(ties0, n_tie);
         u64 w[SNK_SAMPLE_VEC]; unsigned int q[SNK_SAMPLE_VEC];
         double x[SNK_SAMPLE_VEC];
         u64 mass = 0, ties = 0;
@@ -312,13 +316,13 @@ sample_rows_block_kernel(const T *__restrict__ scores, int64_t stride, int64_t V
         }
         u64 cm = mass, ct = ties, ignore_a, ignore_b;
         block_scan2<NT>(cm, ct, ignore_a, ignore_b, scratch);
-        u64 am = mass0 + cm - mass, at = ties0 + ct - ties;
+        u64 am = cm - mass, at = ties0 + ct - ties;
 #pragma unroll
         for (int j = 0; j < SNK_SAMPLE_VEC; ++j) {
-            const u64 lo = am + w_tie * (at < n_tie ? at : n_tie);
+            const u64 lo = am + w_tie * (min(at, n_tie) - kept0);
             am += w[j]; at += q[j];
-            const u64 hi = am + w_tie * (at < n_tie ? at : n_tie);
-            if (lo <= t && t < hi) {
+            const u64 hi = am + w_tie * (min(at, n_tie) - kept0);
+            if (lo <= goal && goal < hi) {
                 index[r * n_draws + d] = base + j;
                 if (logp) logp[r * n_draws + d] = sample_exponent(x[j], m, rule.inv_tau) - log_total;
             }
@@ -555,25 +559,25 @@ sample_rows_held_kernel(const T *__restrict__ scores, int64_t stride, int V, con
 // The first two are launches and the latency of a few dependent reads each; the third is bound by the float64 work on every score (weight
 // and bin, tested again for the boundary).
 #define SNK_CHUNK 8192
-#define SNK_LIST 16384
+#define SNK_LIST 16383                          // (weights of 2^50 that 64 bits can add)
 #define SNK_BINS_MOST 4096
 
 struct RowState {
     double m, bin_scale;        // largest score, bins per unit of exponent
     double cut;                 // kept: above the cut, and the first n_tie equal to it
-    u64 n_tie, total;           // total: mass of what the goals so far keep
-    u64 above;
+    u64 n_tie;
+    u128 total;                 // mass of what the goals so far keep
+    u128 above, want;
     unsigned int listed, want_bin;
     int all, pad;
-    u64 want;
 };
 
 struct RowsWork {
     RowState *state;
     double *chunk_max, *chunk_min;          // [rows][spans]
-    u64 *hist_mass; unsigned int *hist_count;   // [rows][bins]
+    u64 *hist_mass, *hist_more;             // [rows][bins]
     double *list_x;                         // [rows][list]
-    u64 *chunk_mass; unsigned int *chunk_ties;
+    u64 *chunk_mass, *chunk_more;           // the count: scores equal to the cut
     int *left;                              // rows for the kernel above
     int64_t span;                           // scores that a workgroup of the first passes takes: chunks, as many as leave workgroups enough
     int bins, chunks, spans;
@@ -616,7 +620,7 @@ rows_extremes_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, co
     const int tid = threadIdx.x;
     const double inf = __builtin_inf();
     if (c == 0) {
-        for (int i = tid; i < w.bins; i += 512) { w.hist_mass[r * w.bins + i] = 0; w.hist_count[r * w.bins + i] = 0; }
+        for (int i = tid; i < w.bins; i += 512) { w.hist_mass[r * w.bins + i] = 0; w.hist_more[r * w.bins + i] = 0; }
         if (tid == 0) {
             RowState s;
             s.m = -inf; s.bin_scale = 0.0; s.cut = -inf; s.n_tie = 0; s.total = 0; s.above = 0;
@@ -647,8 +651,7 @@ rows_histogram_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, S
 {
     extern __shared__ __align__(16) unsigned char smem[];
     __shared__ double hi[8], lo[8];
-    u64 *mass = reinterpret_cast<u64 *>(smem);
-    unsigned int *count = reinterpret_cast<unsigned int *>(mass + w.bins);
+    u64 *mass = reinterpret_cast<u64 *>(smem), *more = mass + w.bins;
     const int64_t r = blockIdx.y, c = blockIdx.x;
     const int tid = threadIdx.x;
     const double inf = __builtin_inf();
@@ -658,7 +661,7 @@ rows_histogram_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, S
     m = wave_max(m);
     n = -wave_max(-n);
     if ((tid & 63) == 0) { hi[tid >> 6] = m; lo[tid >> 6] = n; }
-    for (int i = tid; i < w.bins; i += 512) { mass[i] = 0; count[i] = 0; }
+    for (int i = tid; i < w.bins; i += 512) { mass[i] = 0; more[i] = 0; }
     __syncthreads();
     for (int i = 0; i < 8; ++i) { m = fmax(m, hi[i]); n = fmin(n, lo[i]); }
     if (m == -inf) return;                                      // an empty row
@@ -672,11 +675,11 @@ rows_histogram_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, S
         if (!q) return;
         const int b = score_bin(e, scale, w.bins);
         atomicAdd(&mass[b], q);
-        atomicAdd(&count[b], 1u);
+        atomicAdd(&more[b], SNK_MORE_ONE + sample_more(q));
     });
     __syncthreads();
     for (int i = tid; i < w.bins; i += 512)
-        if (count[i]) { atomicAdd(&w.hist_mass[r * w.bins + i], mass[i]); atomicAdd(&w.hist_count[r * w.bins + i], count[i]); }
+        if (more[i]) { atomicAdd(&w.hist_mass[r * w.bins + i], mass[i]); atomicAdd(&w.hist_more[r * w.bins + i], more[i]); }
 }
 
 // by_mass 0: the top_k-th score; 1: where top_p of the mass kept so far is reached
@@ -685,7 +688,7 @@ __global__ void __launch_bounds__(512)
 rows_boundary_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, SampleRule call, const double *__restrict__ rules, double unit, int by_mass,
                      const RowsWork w)
 {
-    constexpr int PER = SNK_BINS_MOST / 256;
+    constexpr int PER = SNK_BINS_MOST / 512;
     constexpr unsigned int HITS = 2048;
     __shared__ BlockScratch<512> scratch;
     __shared__ int bin_s;
@@ -699,28 +702,27 @@ rows_boundary_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, Sa
     if (m == ninf || w.left[r]) return;
     if (by_mass ? !(rule.top_p < 1.0) : !(rule.top_k > 0 && rule.top_k < V)) return;
     const u64 *__restrict__ mass = w.hist_mass + r * w.bins;
-    const unsigned int *__restrict__ count = w.hist_count + r * w.bins;
+    const u64 *__restrict__ more = w.hist_more + r * w.bins;
     // every workgroup finds the bin for itself: a thread sums its neighbouring bins, the sums are scanned, the bin is in one thread's
-    const int per = w.bins >> 8;
-    u64 vm[PER], sm = 0, sc = 0;
-    unsigned int vc[PER];
+    const int per = w.bins >> 9;
+    u64 vm[PER], vc[PER], sm = 0, sc = 0;
 #pragma unroll
     for (int i = 0; i < PER; ++i) {
-        vm[i] = tid < 256 && i < per ? mass[tid * per + i] : 0;
-        vc[i] = tid < 256 && i < per ? count[tid * per + i] : 0;
+        vm[i] = i < per ? mass[tid * per + i] : 0;
+        vc[i] = i < per ? more[tid * per + i] : 0;
         sm += vm[i]; sc += vc[i];
     }
     if (tid == 0) bin_s = -1;
     u64 um = sm, uc = sc, total_m, total_c;
     block_scan2<512>(um, uc, total_m, total_c, scratch);
-    const u64 want = by_mass ? sample_reach(rule.top_p, st->all ? total_m : st->total) : (u64)rule.top_k;
-    const u64 upto = by_mass ? um : uc;
-    u64 a = upto - (by_mass ? sm : sc);
-    if (a < want && upto >= want) {
+    auto amount = [&](u64 sum, u64 also) -> u128 { return by_mass ? sample_sum(sum, also) : (u128)sample_count(also); };
+    const u128 want = by_mass ? sample_reach(rule.top_p, st->all ? sample_sum(total_m, total_c) : st->total) : (u128)rule.top_k;
+    u128 a = amount(um - sm, uc - sc);
+    if (a < want && amount(um, uc) >= want) {
         bool found = false;
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
-            const u64 n = by_mass ? vm[i] : vc[i];
+            const u128 n = amount(vm[i], vc[i]);
             if (!found && a + n >= want) {
                 found = true;
                 bin_s = tid * per + i;
@@ -732,7 +734,7 @@ rows_boundary_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, Sa
     __syncthreads();
     const int bin = bin_s;
     if (bin < 0) {                                              // fewer scores than the goal: all are kept
-        if (c == 0 && tid == 0) { st->want_bin = (unsigned int)-1; st->total = total_m; }
+        if (c == 0 && tid == 0) { st->want_bin = (unsigned int)-1; st->total = sample_sum(total_m, total_c); }
         return;
     }
     // the bin's scores by way of LDS: one place in the row's list is asked for by a workgroup, not one a score (atomics on one address
@@ -784,7 +786,7 @@ rows_select_kernel(int64_t V, SampleRule call, const double *__restrict__ rules,
     __shared__ u64 hist_mass[256], hist_count[256];
     __shared__ u64 sh_above;
     __shared__ unsigned int sh_digit;
-    __shared__ u64 red[16];
+    __shared__ u64 red[32];
     __shared__ double ends[32];
     const int64_t r = blockIdx.x;
     const int tid = threadIdx.x;
@@ -795,7 +797,7 @@ rows_select_kernel(int64_t V, SampleRule call, const double *__restrict__ rules,
     if (by_mass ? !(rule.top_p < 1.0) : !(rule.top_k > 0 && rule.top_k < V)) return;
     if ((int)st->want_bin < 0) return;
     const unsigned int n = st->listed;
-    const u64 want = st->want;
+    u128 need = st->want - st->above;                           // of the bin
     double most = -__builtin_inf(), least = __builtin_inf();    // of the bin's scores
     for (int i = tid; i < w.spans; i += 1024) { most = fmax(most, w.chunk_max[r * w.spans + i]); least = fmin(least, w.chunk_min[r * w.spans + i]); }
     most = wave_max(most);
@@ -804,11 +806,12 @@ rows_select_kernel(int64_t V, SampleRule call, const double *__restrict__ rules,
     __syncthreads();
     for (int i = 0; i < 16; ++i) { most = fmax(most, ends[i]); least = fmin(least, ends[16 + i]); }
     const u64 key_min = score_key<double>(least), key_max = score_key<double>(most);
-    u64 above = st->above, key = key_min;
+    u64 key = key_min;
     u64 ties = n, each = 0;                                     // of the cut's own scores
     if (key_min != key_max) {
         if (n > w.list) { if (tid == 0) w.left[r] = 1; return; }
-        u64 prefix = 0;
+        u64 prefix = 0, above = 0;
+        const u64 want = (u64)need;                             // (the list's sums fit 64 bits)
         // (keys that differ share their leading bits: start at the first digit in which they do)
         int top = 63 - __clzll((long long)(key_min ^ key_max));
         top = (top >> 3) << 3;
@@ -846,28 +849,31 @@ rows_select_kernel(int64_t V, SampleRule call, const double *__restrict__ rules,
             __syncthreads();
         }
         key = prefix;
+        need = want - above;
     }
     // the cut's value back from its key
     const double cut = __longlong_as_double((long long)((key >> 63) ? key & 0x7fffffffffffffffull : ~key));
     each = sample_weight(sample_exponent(cut, m, rule.inv_tau), unit);
-    const u64 n_tie = by_mass ? (each ? (want - above + each - 1) / each : 0) : want - above;
+    const u64 n_tie = by_mass ? sample_ties(need, each) : (u64)need;
     // the mass above the cut: whole bins, and the list's scores above it
-    u64 mass = 0;
+    u64 mass = 0, more = 0;
     const int bin = (int)st->want_bin;
-    for (int i = tid; i < bin; i += 1024) mass += w.hist_mass[r * w.bins + i];
+    for (int i = tid; i < bin; i += 1024) { mass += w.hist_mass[r * w.bins + i]; more += w.hist_more[r * w.bins + i]; }
     if (key_min != key_max)
         for (unsigned int i = tid; i < n; i += 1024) {
             const double x = w.list_x[r * w.list + i];
-            if (x > cut) mass += sample_weight(sample_exponent(x, m, rule.inv_tau), unit);
+            const u64 q = x > cut ? sample_weight(sample_exponent(x, m, rule.inv_tau), unit) : 0;
+            mass += q; more += sample_more(q);
         }
     mass = wave_add(mass);
-    if ((tid & 63) == 0) red[tid >> 6] = mass;
+    more = wave_add(more);
+    if ((tid & 63) == 0) { red[tid >> 6] = mass; red[16 + (tid >> 6)] = more; }
     __syncthreads();
     if (tid == 0) {
-        u64 t = 0;
-        for (int i = 0; i < 16; ++i) t += red[i];
+        u64 t = 0, also = 0;
+        for (int i = 0; i < 16; ++i) { t += red[i]; also += red[16 + i]; }
         st->cut = cut; st->n_tie = n_tie < ties ? n_tie : ties; st->all = 0;
-        st->total = t + each * st->n_tie;
+        st->total = sample_sum(t, also) + (u128)each * st->n_tie;
         st->listed = 0;
     }
 }
@@ -893,21 +899,21 @@ rows_masses_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, Samp
     const RowState st = w.state[r];
     if (st.m == -__builtin_inf() || w.left[r]) return;
     const SampleRule rule = sample_rule(call, rules, r);
-    u64 mass = 0, ties = 0;
+    u64 mass = 0, more = 0;
     chunk_scores<T, 512>(scores + r * stride, c * SNK_CHUNK, min((c + 1) * SNK_CHUNK, V), [&](double x, int64_t) {
         u64 q; unsigned int t;
         row_element(x, st, rule, unit, q, t);
-        mass += q; ties += t;
+        mass += q; more += sample_more(q) + (t ? SNK_MORE_ONE : 0);
     });
     mass = wave_add(mass);
-    ties = wave_add(ties);
-    if ((tid & 63) == 0) { sm[tid >> 6] = mass; sc[tid >> 6] = ties; }
+    more = wave_add(more);
+    if ((tid & 63) == 0) { sm[tid >> 6] = mass; sc[tid >> 6] = more; }
     __syncthreads();
     if (tid == 0) {
         u64 a = 0, b = 0;
         for (int i = 0; i < 8; ++i) { a += sm[i]; b += sc[i]; }
         w.chunk_mass[r * w.chunks + c] = a;
-        w.chunk_ties[r * w.chunks + c] = (unsigned int)b;
+        w.chunk_more[r * w.chunks + c] = b;
     }
 }
 
@@ -918,7 +924,7 @@ rows_draw_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, const 
 {
     constexpr int EACH = SNK_CHUNK / 1024;
     __shared__ BlockScratch<1024> scratch;
-    __shared__ u64 sh_mass, sh_ties;
+    __shared__ u64 sh_goal, sh_ties;
     __shared__ int sh_chunk;
     const int64_t r = blockIdx.x, at = r * n_draws + draw0 + blockIdx.y;
     const int tid = threadIdx.x;
@@ -933,35 +939,34 @@ rows_draw_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, const 
     const u64 n_tie = st.all || (double)each < rule.min_p * unit ? 0 : st.n_tie;
     // chunks: a thread takes `per` neighbours
     const int per = (w.chunks + 1023) / 1024;
-    u64 mass = 0, ties = 0, total_m, total_t;
+    u64 mass = 0, more = 0, total_m, total_t;
     for (int i = 0; i < per; ++i) {
         const int c = tid * per + i;
-        if (c < w.chunks) { mass += w.chunk_mass[r * w.chunks + c]; ties += w.chunk_ties[r * w.chunks + c]; }
+        if (c < w.chunks) { mass += w.chunk_mass[r * w.chunks + c]; more += w.chunk_more[r * w.chunks + c]; }
     }
-    u64 cm = mass, ct = ties;
+    u64 cm = mass, ct = more;
     block_scan2<1024>(cm, ct, total_m, total_t, scratch);
-    const u64 total = total_m + each * (total_t < n_tie ? total_t : n_tie);
-    const u64 t = sample_exceed(u[at], total);
-    u64 am = cm - mass, an = ct - ties;
+    auto kept = [&](u64 sum, u64 also) -> u128 { return sample_sum(sum, also) + (u128)each * min(sample_count(also), n_tie); };
+    const u128 total = kept(total_m, total_t), t = sample_exceed(u[at], total);
+    u64 am = cm - mass, an = ct - more;
     if (tid == 0) { sh_chunk = -1; index[at] = -1; if (logp) logp[at] = -__builtin_inf(); }
     __syncthreads();
     for (int i = 0; i < per; ++i) {
         const int c = tid * per + i;
         if (c >= w.chunks) break;
-        const u64 lo = am + each * (an < n_tie ? an : n_tie);
-        const u64 m0 = am, t0 = an;
-        am += w.chunk_mass[r * w.chunks + c]; an += w.chunk_ties[r * w.chunks + c];
-        const u64 hi = am + each * (an < n_tie ? an : n_tie);
-        if (lo <= t && t < hi) { sh_chunk = c; sh_mass = m0; sh_ties = t0; }
+        const u128 lo = kept(am, an);
+        const u64 t0 = sample_count(an);
+        am += w.chunk_mass[r * w.chunks + c]; an += w.chunk_more[r * w.chunks + c];
+        if (lo <= t && t < kept(am, an)) { sh_chunk = c; sh_goal = (u64)(t - lo); sh_ties = t0; }
     }
     __syncthreads();
     if (sh_chunk < 0) return;                                   // (only where the scores changed under the call: nothing is read beyond them)
     const T *__restrict__ p = scores + r * stride;
     const int64_t base = (int64_t)sh_chunk * SNK_CHUNK + tid * EACH;
-    const u64 mass0 = sh_mass, ties0 = sh_ties;
+    const u64 goal = sh_goal, ties0 = sh_ties, kept0 = min(ties0, n_tie);      // what is left of t in the chunk; equal scores before it
     double x[EACH];
-    u64 q[EACH]; unsigned int k[EACH];
-    mass = 0; ties = 0;
+    u64 q[EACH], ties = 0; unsigned int k[EACH];
+    mass = 0;
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
         x[i] = base + i < V ? score_load(p + base + i) : -__builtin_inf();
@@ -970,15 +975,15 @@ rows_draw_kernel(const T *__restrict__ scores, int64_t stride, int64_t V, const 
     }
     cm = mass; ct = ties;
     block_scan2<1024>(cm, ct, total_m, total_t, scratch);
-    am = mass0 + cm - mass; an = ties0 + ct - ties;
+    am = cm - mass; an = ties0 + ct - ties;
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
-        const u64 lo = am + each * (an < n_tie ? an : n_tie);
+        const u64 lo = am + each * (min(an, n_tie) - kept0);
         am += q[i]; an += k[i];
-        const u64 hi = am + each * (an < n_tie ? an : n_tie);
-        if (lo <= t && t < hi) {
+        const u64 hi = am + each * (min(an, n_tie) - kept0);
+        if (lo <= goal && goal < hi) {
             index[at] = base + i;
-            if (logp) logp[at] = sample_exponent(x[i], st.m, rule.inv_tau) - log((double)total / unit);
+            if (logp) logp[at] = sample_exponent(x[i], st.m, rule.inv_tau) - log(sample_double(total) / unit);
         }
     }
 }
@@ -1002,7 +1007,7 @@ size_t sample_rows_work_bytes(int64_t V)
 {
     if (V <= SNK_HELD_MOST) return 0;
     const size_t c = (size_t)rows_chunks(V), b = (size_t)rows_bins(V);
-    return sizeof(RowState) + c * (2 * sizeof(double) + sizeof(u64) + sizeof(unsigned int)) + b * 12 + rows_list(V) * sizeof(double) + sizeof(int);
+    return sizeof(RowState) + c * (2 * sizeof(double) + 2 * sizeof(u64)) + b * 2 * sizeof(u64) + rows_list(V) * sizeof(double) + sizeof(int);
 }
 int64_t sample_rows_together(int64_t R, int64_t V)
 {
@@ -1027,14 +1032,18 @@ static void launch_rows_split(const T *scores, int64_t stride, int64_t R, int64_
     const size_t n = (size_t)R * w.chunks;
     w.state = (RowState *)take(R * sizeof(RowState));
     w.chunk_max = (double *)take(n * 8); w.chunk_min = (double *)take(n * 8);
-    w.chunk_mass = (u64 *)take(n * 8); w.chunk_ties = (unsigned int *)take(n * 4);
-    w.hist_mass = (u64 *)take((size_t)R * w.bins * 8); w.hist_count = (unsigned int *)take((size_t)R * w.bins * 4);
+    w.chunk_mass = (u64 *)take(n * 8); w.chunk_more = (u64 *)take(n * 8);
+    w.hist_mass = (u64 *)take((size_t)R * w.bins * 8); w.hist_more = (u64 *)take((size_t)R * w.bins * 8);
     w.list = rows_list(V);
     w.list_x = (double *)take((size_t)R * w.list * 8);
     w.left = (int *)take(R * 4);
     const dim3 grid((unsigned)w.chunks, (unsigned)R), spans((unsigned)w.spans, (unsigned)R);
     hipLaunchKernelGGL((rows_extremes_kernel<T>), spans, dim3(512), 0, s, scores, stride, V, w);
-    hipLaunchKernelGGL((rows_histogram_kernel<T>), spans, dim3(512), (size_t)w.bins * 12, s, scores, stride, V, rule, rules, unit, w);
+    const size_t bins_lds = (size_t)w.bins * 16;                // (with the workgroup's own few words beyond 64 KB at the most bins)
+    static size_t attr_set[32] = {0};
+    lds_attr_ensure(attr_set, bins_lds, [&] {
+        (void)hipFuncSetAttribute(reinterpret_cast<const void *>(&rows_histogram_kernel<T>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bins_lds); });
+    hipLaunchKernelGGL((rows_histogram_kernel<T>), spans, dim3(512), bins_lds, s, scores, stride, V, rule, rules, unit, w);
     for (int by_mass = 0; by_mass < 2; ++by_mass) {
         if (!rules && (by_mass ? !(rule.top_p < 1.0) : !(rule.top_k > 0 && rule.top_k < V))) continue;
         hipLaunchKernelGGL((rows_boundary_kernel<T>), spans, dim3(512), 0, s, scores, stride, V, rule, rules, unit, by_mass, w);
@@ -1052,10 +1061,7 @@ template <typename T>
 static void launch_sample_t(const T *scores, int64_t stride, int64_t R, int64_t V, const double *u, int n_draws, const SampleRule &rule,
                             const double *rules, char *work, int64_t *index, double *logp, hipStream_t s)
 {
-    int s_bits = 62;
-    for (int64_t v = 1; v < V; v <<= 1) --s_bits;
-    if (s_bits > 51) s_bits = 51;
-    const double unit = (double)(1ull << s_bits);
+    const double unit = V <= 4096 ? SNK_SAMPLE_UNIT : 0.5 * SNK_SAMPLE_UNIT;      // (sample_device.h: what the sums hold)
 #define SNK_WAVE(E_) hipLaunchKernelGGL((sample_rows_wave_kernel<T, E_>), dim3((unsigned)((R + 3) / 4)), dim3(256), 0, s, scores, stride, R, (int)V, u, n_draws, rule, rules, unit, index, logp)
 #define SNK_HELD(NT_, EACH_) hipLaunchKernelGGL((sample_rows_held_kernel<T, NT_, EACH_>), dim3((unsigned)R), dim3(NT_), 0, s, scores, stride, (int)V, u, n_draws, rule, rules, unit, index, logp)
     if (V <= 64) SNK_WAVE(1);

@@ -94,3 +94,104 @@ def test_large_tiles_of_many_columns(engine, K, Dj):
         assert np.all(np.abs(post[a:b] - p) <= 4.0 * tol)
         want, c, _ = o.sample_path(cand[a:b], dist[a:b], u[0, a:b], 0.7, top_k=30, top_p=0.9, **v.model())
         assert np.array_equal(path[0, a:b], want) and abs(cost[0, i] - c) <= 2.0 ** -52 * 4.0 * T * max(abs(c), 1.0)
+
+
+# ---- rows under one peak -----------------------------------------------------------------------------------------------------------------
+def peak_and_tail(V, depth, dtype='float32'):
+    """One score `depth` above V - 1 equal ones, and the tail's weight each: depths in eighths are exact in every type."""
+    x = np.full((1, V), -depth, dtype=dtype)
+    x[0, 0] = 0.0
+    return x, float(np.exp(-np.float64(depth)))
+
+
+@pytest.mark.parametrize('V,depth,dtype', [(4096, 26.5, 'float64'), (8192, 26.5, 'float32'), (8193, 27.0, 'float64'), (100003, 27.0, 'float32'),
+                                           (1 << 20, 30.0, 'float32'), (1 << 20, 30.0, 'float16'), (1 << 24, 27.5, 'float32'), (1 << 24, 33.0, 'float32')])
+def test_a_long_tail_under_one_peak_keeps_its_mass(engine, V, depth, dtype):
+    """Weights are rounded to multiples of 2^-50 at the coarsest: the mass up to a score is off by at most V 2^-51, its index by that
+    over the tail's weight, a log probability by twice that (the drawn score's own, and the mass')."""
+    x, w = peak_and_tail(V, depth, dtype)
+    mass = 1.0 + (V - 1) * w
+    slack = V * 2.0 ** -51
+    for part in (0.25, 0.5, 0.9):
+        goal = part * (V - 1)                                   # scores of the tail below the drawn one
+        u = np.array([[(1.0 + (goal + 0.5) * w) / mass]])
+        for got in (engine.sample_rows(x, u), [a.cpu().numpy() for a in engine.sample_rows(on_gpu(x), on_gpu(u))]):
+            index, logp = int(got[0][0, 0]), float(got[1][0, 0])
+            assert abs(index - 1 - goal) <= 1.0 + (slack + 4.0 * 2.0 ** -53 * mass) / w, (index, goal)
+            assert abs(logp - (-depth - np.log(mass))) <= 2.0 * slack + 64.0 * 2.0 ** -53 * (1.0 + depth)
+        # a share of the mass that ends inside the tail: nothing behind it is drawn, something next to it is
+        share = float(u[0, 0])
+        last = 1.0 - 2.0 ** -53
+        got = engine.sample_rows(on_gpu(x), on_gpu(np.array([[last]])), top_p=share)
+        assert abs(int(got[0][0, 0]) - 1 - goal) <= 2.0 + 2.0 * (slack + 4.0 * 2.0 ** -53 * mass) / w
+        assert abs(float(got[1][0, 0]) - (-depth - np.log(1.0 + goal * w))) <= 4.0 * slack + w + 64.0 * 2.0 ** -53 * (1.0 + depth)
+
+
+def test_a_long_tail_in_a_captured_call_without_a_workspace(engine):
+    import torch
+    V, depth = 1 << 22, 29.0
+    x, w = peak_and_tail(V, depth)
+    mass, slack = 1.0 + (V - 1) * w, V * 2.0 ** -51
+    goal = 0.7 * (V - 1)
+    share = (1.0 + (goal + 0.5) * w) / mass
+    gx, gu = on_gpu(x), on_gpu(np.array([[share, 1.0 - 2.0 ** -53, 0.0]]))
+    index = torch.full((2, 3), -7, dtype=torch.int64, device='cuda')
+    logp = torch.zeros((2, 3), dtype=torch.float64, device='cuda')
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        stream = torch.cuda.current_stream().cuda_stream
+        for n, top_p in enumerate((1.0, share)):
+            assert engine._lib.snk_sample_rows_dev(engine._h, gx.data_ptr(), 1, 1, V, V, gu.data_ptr(), 3, 1.0, 0, top_p, 0.0, None, index[n].data_ptr(),
+                                                   logp[n].data_ptr(), None, 0, stream) == 0
+    for _ in range(3):
+        index.fill_(-7)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = index.cpu().numpy()
+        near = 2.0 + 2.0 * (slack + 4.0 * 2.0 ** -53 * mass) / w
+        assert abs(got[0, 0] - 1 - goal) <= near and abs(got[0, 1] - (V - 1)) <= near and got[0, 2] == 0
+        assert abs(got[1, 1] - 1 - goal) <= near and got[1, 2] == 0
+    # the same calls with a workspace: the same draws
+    for n, top_p in enumerate((1.0, share)):
+        i, lp = engine.sample_rows(gx, gu, top_p=top_p)
+        assert torch.equal(i[0], index[n]) and torch.equal(lp[0], logp[n])
+
+
+@pytest.mark.parametrize('V', [2048, 4096, 8191, 8192, 8193, 65536, 1 << 20, 1 << 24])
+@pytest.mark.parametrize('dtype', ['float32', 'bfloat16'])
+def test_rows_of_equal_scores(engine, V, dtype):
+    """Every weight is 1, the largest mass that a row can have: a draw is floor(u V), exactly (V and u are whole multiples of powers of
+    two whose product float64 holds)."""
+    import torch
+    x = torch.full((2, V), 0.25, dtype=getattr(torch, dtype), device='cuda')
+    u = np.array([[0.0, 0.125, 0.5, 1.0 - 2.0 ** -26], [0.75, 0.875, 1.0 - 2.0 ** -25, 2.0 ** -26]])
+    exact = (np.floor(u * V)).astype(np.int64)
+    i, lp = engine.sample_rows(x, on_gpu(u))
+    assert np.array_equal(i.cpu().numpy(), exact)
+    assert np.all(np.abs(lp.cpu().numpy() + np.log(V)) <= 8.0 * 2.0 ** -53 * (1.0 + np.log(V)))
+    for rule, n in ((dict(top_k=V // 2), V // 2), (dict(top_p=0.5), (V + 1) // 2), (dict(top_k=V // 2, top_p=0.5), (V // 2 + 1) // 2),
+                    (dict(top_k=V - 1, min_p=1.0), V - 1)):
+        i, lp = engine.sample_rows(x, on_gpu(u), **rule)
+        assert np.array_equal(i.cpu().numpy(), np.floor(u * n).astype(np.int64)), rule
+        assert np.all(np.abs(lp.cpu().numpy() + np.log(n)) <= 8.0 * 2.0 ** -53 * (1.0 + np.log(n)))
+
+
+@pytest.mark.parametrize('V', [8192, 20000, 300000])
+def test_rows_of_scores_within_a_hair(engine, V):
+    """Weights of almost 1 that all differ, the largest masses of a list and of a bin; equal to the rows cut shorter by top_k."""
+    rng = np.random.RandomState(V)
+    x = -(rng.permutation(V) + 1.0)[None, :] * 2.0 ** -40
+    order = np.argsort(-x[0], kind='stable')
+    u = rng.rand(1, 5)
+    for k in (1, 1000, V // 2, V - 1):
+        kept = np.sort(order[:k])
+        w = np.exp(x[0, kept] - x[0].max())
+        c = np.cumsum(w.astype(np.longdouble))
+        want = kept[np.searchsorted(c, (u[0] * c[-1]).astype(np.longdouble), side='right')]
+        i, _ = engine.sample_rows(on_gpu(x), on_gpu(u), top_k=k)
+        assert np.array_equal(i.cpu().numpy()[0], want)
+        # the same prefix by its mass: between the k-th score's and the one's before
+        mass = np.cumsum(np.exp(x[0, order] - x[0].max()).astype(np.longdouble))
+        share = float((mass[k - 1] - 0.5) / mass[-1])
+        i, _ = engine.sample_rows(on_gpu(x), on_gpu(u), top_p=share)
+        assert np.array_equal(i.cpu().numpy()[0], want)
