@@ -393,11 +393,14 @@ int trellis_settled(snk_engine *h)
     return 0;
 }
 
-static int check_draws(const char *who, const void *u, int n_draws, const SampleRuleHost &rule, const void *path, const void *cost)
+// (a temperature whose inverse the costs cannot be multiplied by is that of the cheapest path, ties and all)
+static int check_draws(const char *who, const void *u, int n_draws, SampleRuleHost &rule, const void *path, const void *cost)
 {
     if (!u || !path || !cost) return fail("%s: null argument", who);
     if (n_draws < 1 || n_draws > 65535) return fail("%s: %d draws (1 .. 65535)", who, n_draws);
-    return check_rule(who, rule.temperature, rule.top_k, rule.top_p, rule.min_p);
+    CHK(check_rule(who, rule.temperature, rule.top_k, rule.top_p, rule.min_p));
+    if (rule.temperature < 1e-250) rule.temperature = 0.0;
+    return 0;
 }
 
 int snk_sample_paths(snk_handle h, const int64_t *cand, const double *tdist, const int64_t *row_offsets, int n_utts, int K,
@@ -405,7 +408,7 @@ int snk_sample_paths(snk_handle h, const int64_t *cand, const double *tdist, con
                      int64_t *path_out, double *cost_out, double *logp_out)
 {
     const char *who = "snk_sample_paths";
-    const SampleRuleHost rule = {temperature, top_k, top_p, min_p};
+    SampleRuleHost rule = {temperature, top_k, top_p, min_p};
     CHK(check_trellis(who, h, cand, tdist, row_offsets, n_utts, K));
     CHK(check_draws(who, u, n_draws, rule, path_out, cost_out));
     const int64_t rows = row_offsets[n_utts];
@@ -419,7 +422,7 @@ int snk_sample_paths(snk_handle h, const int64_t *cand, const double *tdist, con
     CHK(h2d(h, h->tr_u.p, u, np, h->stream));
     char *out = h->tr_out.as<char>();
     const TrellisCall q = {who, true, h->tr_cand.as<int64_t>(), h->tr_tdist.as<double>(), row_offsets, join_class ? h->tr_class.as<int32_t>() : nullptr,
-                           n_utts, K, temperature, h->stream};
+                           n_utts, K, rule.temperature, h->stream};
     CHK(sample_paths_device(h, q, h->tr_u.as<double>(), n_draws, rule, (int64_t *)out, (double *)(out + np),
                             logp_out ? (double *)(out + np + nc) : nullptr));
     D2HPart parts[3] = {{path_out, out, np}, {cost_out, out + np, nc}, {logp_out, out + np + nc, logp_out ? nc : 0}};
@@ -433,13 +436,13 @@ int snk_sample_paths_dev(snk_handle h, const int64_t *cand_dev, const double *td
                          double min_p, int64_t *path_dev_out, double *cost_dev_out, double *logp_dev_out, void *stream)
 {
     const char *who = "snk_sample_paths_dev";
-    const SampleRuleHost rule = {temperature, top_k, top_p, min_p};
+    SampleRuleHost rule = {temperature, top_k, top_p, min_p};
     CHK(check_trellis(who, h, cand_dev, tdist_dev, row_offsets, n_utts, K));
     CHK(check_draws(who, u_dev, n_draws, rule, path_dev_out, cost_dev_out));
     DeviceGuard device;
     CHK(device.enter(h->device));
     CHK(trellis_enter(h, who, (hipStream_t)stream));
-    const TrellisCall q = {who, false, cand_dev, tdist_dev, row_offsets, join_class_dev, n_utts, K, temperature, (hipStream_t)stream};
+    const TrellisCall q = {who, false, cand_dev, tdist_dev, row_offsets, join_class_dev, n_utts, K, rule.temperature, (hipStream_t)stream};
     return trellis_leave(h, (hipStream_t)stream, sample_paths_device(h, q, u_dev, n_draws, rule, path_dev_out, cost_dev_out, logp_dev_out));
 }
 

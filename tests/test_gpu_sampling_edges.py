@@ -195,3 +195,19 @@ def test_rows_of_scores_within_a_hair(engine, V):
         share = float((mass[k - 1] - 0.5) / mass[-1])
         i, _ = engine.sample_rows(on_gpu(x), on_gpu(u), top_p=share)
         assert np.array_equal(i.cpu().numpy()[0], want)
+
+
+# ---- temperature zero ------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('tau', [9.9e-251, 1e-300, 5e-324])
+def test_a_temperature_that_counts_as_zero_breaks_ties_like_it(engine, tau):
+    v = Voice(engine)
+    cand, dist, offs = v.candidates([12, 5], 9, pad=False)
+    cand[:, 5], dist[:, 5] = cand[:, 2], dist[:, 2]             # the same unit twice in every row, as cheap
+    cand[:, 7], dist[:, 7] = cand[:, 2], dist[:, 2]
+    dist[:, 2] -= 3.0
+    dist[:, 5], dist[:, 7] = dist[:, 2], dist[:, 2]
+    u = np.random.RandomState(0).rand(4, 17)
+    want = engine.sample_paths(cand, dist, u, row_offsets=offs, temperature=0.0)
+    for got in (engine.sample_paths(cand, dist, u, row_offsets=offs, temperature=tau),
+                [a.cpu().numpy() for a in engine.sample_paths(on_gpu(cand), on_gpu(dist), on_gpu(u), row_offsets=offs, temperature=tau)]):
+        assert all(np.array_equal(a, b) for a, b in zip(got, want)) and not got[2].any()
