@@ -372,7 +372,9 @@ int snk_sample_paths_dev(snk_handle h, const int64_t *cand_dev, const double *td
  *   posterior_out (rows, K)  probability of every candidate:  d logZ / d tdist = -posterior / temperature
  *   uses_out (n_classes, n_buckets), or NULL: expected uses of every entry of the position bias, summed over the utterances:
  *                            d logZ / d bias = -uses / temperature
- * An utterance without a complete path has posteriors 0 and adds no uses. */
+ * An utterance without a complete path has posteriors 0 and adds no uses.  A row's posteriors sum to 1 at any temperature (what the
+ * costs over a very small one round away decides between its candidates).  Uses are sums of the probabilities of pairs, each rounded to
+ * a multiple of 2^-50: a bucket that no pair uses by 2^-51 has none. */
 int snk_path_posterior(snk_handle h, const int64_t *cand, const double *tdist, const int64_t *row_offsets, int n_utts, int K,
                        const int32_t *join_class, double temperature, double *logz_out, double *posterior_out, double *uses_out);
 int snk_path_posterior_dev(snk_handle h, const int64_t *cand_dev, const double *tdist_dev, const int64_t *row_offsets, int n_utts, int K,

@@ -388,7 +388,7 @@ trellis_cost_kernel(const TrellisView v, const TrellisCosts c, int *__restrict__
     auto value = [&](double d2, int ie, int is) -> double {     // a cell from the squared distance, infinite: cannot join
         double cost = LOG ? sqrt(d2) : trellis_root(d2);
         if (cls >= 0) cost += bias[trellis_bucket(is - ie, look)];
-        if (LOG) return cost < __builtin_inf() ? -cost * v.inv_tau : -__builtin_inf();
+        if (LOG) return cost < __builtin_inf() ? fmin(fmax(-cost * v.inv_tau, -1e300), 1e300) : -__builtin_inf();      // (as trellis_local)
         const bool ok = cost < __builtin_inf();                 // (the root of an infinite square is not a number)
         const double x = (c.bias_min - cost) * v.inv_tau;
         wide |= ok && x < -SNK_COST_RANGE;
@@ -1011,11 +1011,13 @@ trellis_backward_kernel(const TrellisView v, const double *__restrict__ local, c
 }
 
 // ---- the flagged utterances in logarithms (SUM false: temperature 0, the largest term of every sum) ----------------------------------
+// Every row of the sums is taken relative to the largest weight of the row before (after) it: a row's differences stay the size of a step's
+// costs over tau, where the whole path's would round to more than the differences themselves once tau is 2^-50 of them.
 template <bool SUM>
 __global__ void __launch_bounds__(1024)
 trellis_forward_log_kernel(const TrellisView v, const int *__restrict__ flag, double *__restrict__ alpha, double *__restrict__ logz)
 {
-    __shared__ double cur[256], part_max[1024], part_sum[1024];
+    __shared__ double cur[256], part_max[1024], part_sum[1024], row_top[2][4];
     const int u = v.first + blockIdx.x;
     if (!flag[u]) return;
     const int K = v.K, Kp = v.Kp, tid = threadIdx.x;
@@ -1024,13 +1026,27 @@ trellis_forward_log_kernel(const TrellisView v, const int *__restrict__ flag, do
     const int64_t r0 = v.off[u], T = v.off[u + 1] - r0;
     const double ninf = -__builtin_inf();
     const bool mine = b < K && part < P;
-    if (tid < K) {
-        const double x = trellis_local(v.cand[r0 * K + tid], v.tdist[r0 * K + tid], v.n_units, v.inv_tau);
-        cur[tid] = x;
-        alpha[r0 * Kp + tid] = x;
-    }
+    double scaled = 0.0;                                        // what the rows were taken relative to
+    auto publish = [&](int64_t t, double x) {                   // by the first 256 threads; x -inf beyond K
+        if (tid < K) {
+            cur[tid] = x;
+            alpha[(r0 + t) * Kp + tid] = x;
+        }
+        if (SUM) {
+            x = wave_max(x);
+            if ((tid & 63) == 0) row_top[t & 1][tid >> 6] = x;
+        }
+    };
+    if (tid < 256) publish(0, tid < K ? trellis_local(v.cand[r0 * K + tid], v.tdist[r0 * K + tid], v.n_units, v.inv_tau) : ninf);
     __syncthreads();
     for (int64_t t = 0; t + 1 < T; ++t) {
+        double base = 0.0;
+        if (SUM) {
+            const double *m = row_top[t & 1];
+            base = fmax(fmax(m[0], m[1]), fmax(m[2], m[3]));
+            if (base == ninf) base = 0.0;
+            scaled += base;
+        }
         const double *__restrict__ c = v.C + (r0 + t - v.c0) * K * Kp + b;
         double top = ninf, sum = 0.0;
         if (mine) {
@@ -1041,20 +1057,20 @@ trellis_forward_log_kernel(const TrellisView v, const int *__restrict__ flag, do
         part_max[tid] = top;
         part_sum[tid] = sum;
         __syncthreads();
-        if (tid < K) {
-            double all = ninf;
-            for (int q = 0; q < P; ++q) all = fmax(all, part_max[q * KB + tid]);
-            double x = all;
-            if (SUM && all > ninf) {
-                double s = 0.0;
-                for (int q = 0; q < P; ++q)
-                    if (part_max[q * KB + tid] > ninf) s += part_sum[q * KB + tid] * exp(part_max[q * KB + tid] - all);
-                x = all + log(s);
+        if (tid < 256) {
+            double x = ninf;
+            if (tid < K) {
+                for (int q = 0; q < P; ++q) x = fmax(x, part_max[q * KB + tid]);
+                if (SUM && x > ninf) {
+                    double s = 0.0;
+                    for (int q = 0; q < P; ++q)
+                        if (part_max[q * KB + tid] > ninf) s += part_sum[q * KB + tid] * exp(part_max[q * KB + tid] - x);
+                    x = (x - base) + log(s);
+                }
+                const int64_t at = (r0 + t + 1) * K + tid;
+                x += trellis_local(v.cand[at], v.tdist[at], v.n_units, v.inv_tau);
             }
-            const int64_t at = (r0 + t + 1) * K + tid;
-            x += trellis_local(v.cand[at], v.tdist[at], v.n_units, v.inv_tau);
-            cur[tid] = x;
-            alpha[(r0 + t + 1) * Kp + tid] = x;
+            publish(t + 1, x);
         }
         __syncthreads();
     }
@@ -1064,27 +1080,35 @@ trellis_forward_log_kernel(const TrellisView v, const int *__restrict__ flag, do
         double s = 0.0;
         if (all > ninf)
             for (int a = 0; a < K; ++a) s += exp(cur[a] - all);
-        logz[u] = all > ninf ? all + log(s) : ninf;
+        logz[u] = all > ninf ? scaled + (all + log(s)) : ninf;
     }
 }
 
 __global__ void __launch_bounds__(1024)
 trellis_backward_log_kernel(const TrellisView v, const int *__restrict__ flag, double *__restrict__ beta)
 {
-    __shared__ double into[2][256];
+    __shared__ double into[2][256], row_top[2][16];
     const int u = v.first + blockIdx.x;
     if (!flag[u]) return;
     const int K = v.K, Kp = v.Kp, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t r0 = v.off[u], T = v.off[u + 1] - r0;
     const double ninf = -__builtin_inf();
+    double top_into = ninf;
     if (tid < K) {
         const int64_t at = (r0 + T - 1) * K + tid;
         beta[(r0 + T - 1) * Kp + tid] = 0.0;
-        into[(T - 1) & 1][tid] = trellis_local(v.cand[at], v.tdist[at], v.n_units, v.inv_tau);
+        top_into = trellis_local(v.cand[at], v.tdist[at], v.n_units, v.inv_tau);
+        into[(T - 1) & 1][tid] = top_into;
     }
+    top_into = wave_max(top_into);
+    if (lane == 0) row_top[(T - 1) & 1][wave] = top_into;
     __syncthreads();
     for (int64_t t = T - 2; t >= 0; --t) {
         const double *next = into[(t + 1) & 1];
+        double base = ninf;
+        for (int i = 0; i < 16; ++i) base = fmax(base, row_top[(t + 1) & 1][i]);
+        if (base == ninf) base = 0.0;
+        top_into = ninf;
         for (int a = wave; a < K; a += 16) {
             const double *__restrict__ c = v.C + (r0 + t - v.c0) * K * Kp + (int64_t)a * Kp;
             double x[4], top = ninf;
@@ -1102,12 +1126,15 @@ trellis_backward_log_kernel(const TrellisView v, const int *__restrict__ flag, d
                 s = wave_sum(s);
             }
             if (lane == 0) {
-                const double y = top > ninf ? top + log(s) : ninf;
+                const double y = top > ninf ? (top - base) + log(s) : ninf;
                 const int64_t at = (r0 + t) * K + a;
                 beta[(r0 + t) * Kp + a] = y;
-                into[t & 1][a] = y + trellis_local(v.cand[at], v.tdist[at], v.n_units, v.inv_tau);
+                const double x = y + trellis_local(v.cand[at], v.tdist[at], v.n_units, v.inv_tau);
+                into[t & 1][a] = x;
+                top_into = fmax(top_into, x);
             }
         }
+        if (lane == 0) row_top[t & 1][wave] = top_into;
         __syncthreads();
     }
 }
@@ -1132,10 +1159,19 @@ trellis_posterior_kernel(const TrellisView v, const int *__restrict__ flag, cons
     const double ninf = -__builtin_inf(), z = logz[u];
     const bool dead = !(z > ninf);
     if (logs) {
+        // of the row's own sum, and a candidate's share among what follows it (below) of that candidate's: both sum to 1, however large the
+        // exponents and what they round away
+        const double x = tid < K ? V[t * Kp + tid] + Wt[t * Kp + tid] : ninf, m = wave_max(x);
+        if (lane == 0) red[wave] = m;
+        __syncthreads();
+        const double most = fmax(fmax(red[0], red[1]), fmax(red[2], red[3]));
+        const double e = x > ninf ? exp(x - most) : 0.0, s = wave_sum(e);
+        if (lane == 0) red[4 + wave] = s;
+        __syncthreads();
         if (tid < K) {
-            const double a = V[t * Kp + tid];
-            posterior[t * K + tid] = dead ? 0.0 : exp(a + Wt[t * Kp + tid] - z);
-            in[tid] = a - z;
+            const double p = dead ? 0.0 : e / ((red[4] + red[5]) + (red[6] + red[7]));
+            posterior[t * K + tid] = p;
+            in[tid] = p;
         }
     } else {
         // sum_a v w of the row, and the power of two that the backward step into this row took out
@@ -1175,20 +1211,37 @@ trellis_posterior_kernel(const TrellisView v, const int *__restrict__ flag, cons
     if (!last && !dead) {
         const double *__restrict__ c = v.C + (t - v.c0) * K * Kp;
         u64 first = 0, far = 0;
+        auto add = [&](double p, int a, int b) {
+            const u64 w = sample_fix(p, SNK_USES_UNIT);
+            if (!w) return;
+            const int k = trellis_bucket(id1[b] - id0[a], look);
+            if (k == 0) first += w;
+            else if (k == n_buckets - 1) far += w;
+            else atomicAdd(&uses[k], w);
+        };
         for (int a = wave; a < K; a += 4) {
             const double va = in[a];
-            for (int b = lane; b < K; b += 64) {
-                const double x = c[a * Kp + b];
-                double p;
-                if (logs) p = exp(va + x + out[b]);
-                else p = va * x * out[b];
-                const u64 w = sample_fix(p, SNK_USES_UNIT);
-                if (!w) continue;
-                const int k = trellis_bucket(id1[b] - id0[a], look);
-                if (k == 0) first += w;
-                else if (k == n_buckets - 1) far += w;
-                else atomicAdd(&uses[k], w);
-            }
+            if (logs) {
+                double x[4], m = ninf, s = 0.0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int b = lane + 64 * j;
+                    x[j] = b < K ? c[a * Kp + b] + out[b] : ninf;
+                    m = fmax(m, x[j]);
+                }
+                m = wave_max(m);
+                if (!(va > 0.0 && m > ninf)) continue;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    x[j] = x[j] > ninf ? exp(x[j] - m) : 0.0;
+                    s += x[j];
+                }
+                s = va / wave_sum(s);
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    if (x[j] > 0.0) add(x[j] * s, a, lane + 64 * j);
+            } else
+                for (int b = lane; b < K; b += 64) add(va * c[a * Kp + b] * out[b], a, b);
         }
         if (first) atomicAdd(&uses[0], first);
         if (far) atomicAdd(&uses[n_buckets - 1], far);

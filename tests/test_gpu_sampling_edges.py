@@ -211,3 +211,42 @@ def test_a_temperature_that_counts_as_zero_breaks_ties_like_it(engine, tau):
     for got in (engine.sample_paths(cand, dist, u, row_offsets=offs, temperature=tau),
                 [a.cpu().numpy() for a in engine.sample_paths(on_gpu(cand), on_gpu(dist), on_gpu(u), row_offsets=offs, temperature=tau)]):
         assert all(np.array_equal(a, b) for a, b in zip(got, want)) and not got[2].any()
+
+
+# ---- tiny temperatures ---------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('tau', [1e-6, 1e-10, 1e-13, 1e-16, 1e-30])
+def test_posteriors_of_tiny_temperatures_are_probabilities(engine, tau):
+    """Path costs of up to 1e32 temperatures: what the exponents round away is more than 1, but a row's probabilities sum to 1, and where
+    the cheapest path is alone by more than all roundings they are its."""
+    v = Voice(engine)
+    v.set_bias(1, 8)
+    cand, dist, offs = v.candidates([30, 1, 12], 20)
+    cand[:, 10:] = np.where(cand[:, 10:] > 0, cand[:, 10:], 5)
+    path, cost, _ = engine.sample_paths(cand, dist, np.zeros((1, 43)), row_offsets=offs, temperature=0.0)
+    logz, post, uses = engine.path_posterior(cand, dist, row_offsets=offs, temperature=tau)
+    # a row's sum: K quotients and their sum, rounded K + 2 times
+    assert np.all(np.abs(post.sum(axis=1) - 1.0) <= 32.0 * 2.0 ** -53 * 20)
+    want = (cand == path[0][:, None]) & (post > 0.0)
+    assert np.array_equal(cand[np.arange(43), post.argmax(axis=1)], path[0])
+    assert np.all(np.abs((post * want).sum(axis=1) - 1.0) <= 1e-12)
+    steps = np.zeros(uses.shape)
+    for a, b in zip(offs[:-1], offs[1:]):
+        for t in range(a, b - 1):
+            steps[0, int(np.searchsorted(v.edges, path[0, t + 1] - path[0, t], side='right'))] += 1.0
+    assert np.all(np.abs(uses - steps) <= 1e-9)
+    # six roundings a row, of values of up to the whole sum: 1 / tau, the target cost and the join cost times it, their sum, the row's relative
+    # weight and what it is relative to
+    assert np.all(np.abs(logz + cost[0] / tau) <= 6.0 * np.diff(offs) * 2.0 ** -53 * cost[0] / tau + 5.0)
+
+
+@pytest.mark.parametrize('scale,tau,bias', [(1e300, 1e-10, 0.0), (-1e300, 1e-10, 0.0), (-1e308, 1e-300, 0.0), (1.0, 0.5, -1e308), (1.0, 1e-10, 1e308), (1.0, 1e-10, -1e308)])
+def test_posteriors_of_costs_that_overflow_are_probabilities(engine, scale, tau, bias):
+    v = Voice(engine)
+    cand, dist, offs = v.candidates([30, 5], 20, pad=False)
+    cand = np.clip(cand, 1, v.n - 2)
+    rng = np.random.RandomState(1)
+    d = dist * (scale * np.where(rng.rand(35, 20) < 0.3, -0.4, 0.4))
+    engine.set_position_bias(np.array([[0.0, bias]]), [1])
+    logz, post, uses = engine.path_posterior(cand, d, row_offsets=offs, temperature=tau)
+    assert np.all(np.abs(post.sum(axis=1) - 1.0) <= 32.0 * 2.0 ** -53 * 20) and not np.isnan(logz).any()
+    assert abs(uses.sum() - 33.0) <= 33.0 * 20 * 20 * 2.0 ** -51 + 1e-13      # a join between each two rows; K K cells a row, rounded to 2^-50
