@@ -502,12 +502,12 @@ trellis_product_kernel(const TrellisView v, const double *__restrict__ local, in
     constexpr int W = NTH / 64, COLS = 4 * KH * CH, LDX = COLS + 2;      // (sixteen rows 4 odd banks apart)
     __shared__ double X[2][16 * LDX];
     __shared__ double top[2][W][16];
-    __shared__ int bad;
-    const int j = blockIdx.x >> 3;
+    __shared__ int bad, done;                                   // done: another piece's workgroup may flag the utterance at any time, so one
+    const int j = blockIdx.x >> 3;                              // thread looks for all
     const int i0 = (j % row_blocks) * 16, flat = (j / row_blocks) * 8 + (blockIdx.x & 7);
     if (flat >= max_pieces * v.n_utts) return;
     const TrellisPiece p = trellis_piece(v, flat / max_pieces, flat % max_pieces);
-    if (p.k >= p.P || p.P == 1 || (skip_last && p.k == p.P - 1) || flag[p.u]) return;
+    if (p.k >= p.P || p.P == 1 || (skip_last && p.k == p.P - 1)) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c16 = lane & 15, g = lane >> 4;
     const int K = v.K, Kp = v.Kp, slab_bytes = K * Kp * 8;
     const int64_t first_row = p.r0 + (int64_t)p.k * p.L;
@@ -532,8 +532,9 @@ trellis_product_kernel(const TrellisView v, const double *__restrict__ local, in
             for (int c = 0; c < CT; ++c) load(1, 0, ks, c);
     }
     for (int i = tid; i < 2 * 16 * LDX; i += NTH) (&X[0][0])[i] = 0.0;
-    if (tid == 0) bad = 0;
+    if (tid == 0) { bad = 0; done = flag[p.u]; }
     __syncthreads();
+    if (done) return;
     // the first slab: the start candidate's own cells
     bool small = false;
     double most[4];
@@ -785,9 +786,9 @@ trellis_forward_kernel(const TrellisView v, const double *__restrict__ local, co
     __shared__ __align__(16) double cur[2][4 * R];
     __shared__ double top[2][W];
     __shared__ double part[NTH];
-    __shared__ int bad;
+    __shared__ int bad, done;
     const TrellisPiece p = trellis_piece(v, blockIdx.y, blockIdx.x);
-    if (p.k >= p.P || flag[p.u]) return;
+    if (p.k >= p.P) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int b = wave * 32 + (lane & 15) * 2, rows = lane >> 4;
     const int K = v.K, Kp = v.Kp, n = p.n;
@@ -796,8 +797,9 @@ trellis_forward_kernel(const TrellisView v, const double *__restrict__ local, co
     const int voff = b < Kp ? (rows * R * Kp + b) * 8 : 0x7ff00000;
     const int64_t first_row = p.r0 + (int64_t)p.k * p.L;
     for (int i = tid; i < 8 * R; i += NTH) (&cur[0][0])[i] = 0.0;
-    if (tid == 0) bad = 0;
+    if (tid == 0) { bad = 0; done = flag[p.u]; }
     __syncthreads();
+    if (done) return;
 
     f64x2 cell[NB][KPM];
     const int pieces = n * CH;
@@ -913,9 +915,9 @@ trellis_backward_kernel(const TrellisView v, const double *__restrict__ local, c
     static_assert(NB % CH == 0 || CH % NB == 0, "a step's parts go round the buffers");
     __shared__ __align__(16) double cur[2][8 * KC];
     __shared__ double top[2][W];
-    __shared__ int bad;
+    __shared__ int bad, done;
     const TrellisPiece p = trellis_piece(v, blockIdx.y, blockIdx.x);
-    if (p.k >= p.P || flag[p.u]) return;
+    if (p.k >= p.P) return;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int q = lane & 3, K = v.K, Kp = v.Kp, n = p.n;
     const int slab_bytes = K * Kp * 8;
@@ -927,8 +929,9 @@ trellis_backward_kernel(const TrellisView v, const double *__restrict__ local, c
         voff[ch] = a[ch] < K ? (a[ch] * Kp + 2 * q) * 8 : 0x7ff00000;
     }
     for (int i = tid; i < 16 * KC; i += NTH) (&cur[0][0])[i] = 0.0;
-    if (tid == 0) bad = 0;
+    if (tid == 0) { bad = 0; done = flag[p.u]; }
     __syncthreads();
+    if (done) return;
     f64x2 cell[NB][KC];
     const int pieces = n * CH;                                  // from the last slab down
     const double *__restrict__ slab0 = v.C + (first_row - v.c0) * ((int64_t)K * Kp);
