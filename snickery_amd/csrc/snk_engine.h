@@ -21,11 +21,15 @@ using namespace snk;
 int fail(const char *fmt, ...);                 // sets the thread's error message (snk_last_error), returns 1
 const std::string &last_error_string();
 
+// The runtime keeps a call's error until it is asked for the last one: an error that is reported here is taken back there, or the next
+// call's check behind its launches would report it as its own.
+inline const char *hip_error(hipError_t e) { (void)hipGetLastError(); return hipGetErrorString(e); }
+
 #define HIPCHK(expr)                                                                         \
     do {                                                                                     \
         hipError_t e_ = (expr);                                                              \
         if (e_ != hipSuccess)                                                                \
-            return fail("%s failed: %s (%s:%d)", #expr, hipGetErrorString(e_), __FILE__, __LINE__); \
+            return fail("%s failed: %s (%s:%d)", #expr, hip_error(e_), __FILE__, __LINE__);  \
     } while (0)
 
 #define CHK(expr)                    \
@@ -69,7 +73,7 @@ struct DevBuf {
         if (p) { (void)hipFree(p); p = nullptr; bytes = 0; }
         size_t want = need + need / 8 + 256;
         hipError_t e = hipMalloc(&p, want);
-        if (e != hipSuccess) { p = nullptr; return fail("hipMalloc(%zu) failed: %s", want, hipGetErrorString(e)); }
+        if (e != hipSuccess) { p = nullptr; return fail("hipMalloc(%zu) failed: %s", want, hip_error(e)); }
         bytes = want;
         return 0;
     }
@@ -82,7 +86,7 @@ struct DevBuf {
             // plain allocations of exactly the bytes asked for, filled with 0xFF: separates "relies on fresh memory being
             // zero / on the growth slack" from what the unmapped neighbours of modes 1 and 2 catch
             hipError_t e3 = hipMalloc(&p, need);
-            if (e3 != hipSuccess) { p = nullptr; return fail("hipMalloc(%zu) failed: %s", need, hipGetErrorString(e3)); }
+            if (e3 != hipSuccess) { p = nullptr; return fail("hipMalloc(%zu) failed: %s", need, hip_error(e3)); }
             (void)hipMemset(p, 0xFF, need);
             (void)hipDeviceSynchronize();
             bytes = need;
@@ -96,21 +100,21 @@ struct DevBuf {
         prop.location.id = dev;
         size_t gran = 0;
         hipError_t e = hipMemGetAllocationGranularity(&gran, &prop, hipMemAllocationGranularityMinimum);
-        if (e != hipSuccess || gran == 0) return fail("SNK_GUARD: hipMemGetAllocationGranularity: %s", hipGetErrorString(e));
+        if (e != hipSuccess || gran == 0) return fail("SNK_GUARD: hipMemGetAllocationGranularity: %s", hip_error(e));
         const size_t mapped = ((need + gran - 1) / gran) * gran;
         e = hipMemAddressReserve(&va, mapped + 2 * gran, gran, nullptr, 0);
-        if (e != hipSuccess) { va = nullptr; return fail("SNK_GUARD: hipMemAddressReserve(%zu): %s", mapped + 2 * gran, hipGetErrorString(e)); }
+        if (e != hipSuccess) { va = nullptr; return fail("SNK_GUARD: hipMemAddressReserve(%zu): %s", mapped + 2 * gran, hip_error(e)); }
         va_bytes = mapped + 2 * gran;
         e = hipMemCreate(&mh, mapped, &prop, 0);
-        if (e != hipSuccess) { (void)hipMemAddressFree(va, va_bytes); va = nullptr; return fail("SNK_GUARD: hipMemCreate(%zu): %s", mapped, hipGetErrorString(e)); }
+        if (e != hipSuccess) { (void)hipMemAddressFree(va, va_bytes); va = nullptr; return fail("SNK_GUARD: hipMemCreate(%zu): %s", mapped, hip_error(e)); }
         char *base = (char *)va + gran;
         e = hipMemMap(base, mapped, 0, mh, 0);
-        if (e != hipSuccess) return fail("SNK_GUARD: hipMemMap: %s", hipGetErrorString(e));
+        if (e != hipSuccess) return fail("SNK_GUARD: hipMemMap: %s", hip_error(e));
         hipMemAccessDesc acc{};
         acc.location = prop.location;
         acc.flags = hipMemAccessFlagsProtReadWrite;
         e = hipMemSetAccess(base, mapped, &acc, 1);
-        if (e != hipSuccess) return fail("SNK_GUARD: hipMemSetAccess: %s", hipGetErrorString(e));
+        if (e != hipSuccess) return fail("SNK_GUARD: hipMemSetAccess: %s", hip_error(e));
         map_bytes = mapped;
         guarded = true;
         (void)hipMemset(base, 0xFF, mapped);
@@ -152,7 +156,7 @@ struct HostBuf {        // pinned host staging (pageable D2H of > ~64 KB pins th
         size_t want = need + need / 4 + 4096;
         if (want < ((size_t)8 << 20)) want = (size_t)8 << 20;     // pinned allocations cost milliseconds
         hipError_t e = hipHostMalloc(&p, want, hipHostMallocDefault);
-        if (e != hipSuccess) { p = nullptr; return fail("hipHostMalloc(%zu) failed: %s", want, hipGetErrorString(e)); }
+        if (e != hipSuccess) { p = nullptr; return fail("hipHostMalloc(%zu) failed: %s", want, hip_error(e)); }
         bytes = want;
         return 0;
     }

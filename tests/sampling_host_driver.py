@@ -1,0 +1,58 @@
+"""The host side of the sampling entry points after refused and failed calls, through the sanitizer build of `make asan-host` (no device,
+kernels never run).  Run by tests/test_sampling_host.py in a child process; prints SAMPLING-HOST-OK."""
+import os
+import sys
+
+import numpy as np
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+sys.path.insert(0, ROOT)
+assert os.environ.get('SNK_LIBRARY', '').endswith('libsnkhip_host_asan.so'), 'run through tests/test_sampling_host.py'
+import snickery_amd                                   # noqa: E402
+from snickery_amd import SnkError                     # noqa: E402
+from snickery_amd.engine import load_library          # noqa: E402
+
+lib = load_library()
+rng = np.random.RandomState(0)
+
+
+def refused(part, fn, *a, **k):
+    """The call raises SnkError with `part` in its message."""
+    try:
+        fn(*a, **k)
+    except SnkError as e:
+        assert part in str(e), (part, str(e))
+        return True
+    return False
+
+
+e = snickery_amd.HipSearchEngine(0)
+N, Dj, T, K = 500, 21, 30, 12
+e.upload_join_only(rng.randn(N + 1, Dj).astype(np.float32))
+e.set_weights(None, np.full(Dj, 0.1))
+cand, dist, u = rng.randint(0, N, (T, K)), rng.rand(T, K), rng.rand(2, T)
+x = rng.randn(5, 40)
+
+# ---- a call that asks for more memory than there is: its error is its own, not that of the calls behind it ----
+rows = 20000                                          # one utterance: rows x 208 x 208 costs of 8 bytes
+wide = np.ones((rows, 208), np.int64)
+index = np.zeros((5, 1), np.int64)
+
+
+def rows_on_the_device():                             # ("device" memory is the host's here)
+    return lib.snk_sample_rows_dev(e._h, x.ctypes.data, 0, 5, 40, 40, u.ctypes.data, 1, 1.0, 0, 1.0, 0.0, None, index.ctypes.data, None, None, 0, None)
+
+
+assert rows_on_the_device() == 0
+for call in (lambda: e.path_posterior(wide, np.zeros((rows, 208))), lambda: e.sample_paths(wide, np.zeros((rows, 208)), np.zeros((1, rows)))):
+    assert refused('hipMalloc', call)
+    assert rows_on_the_device() == 0, lib.snk_last_error()
+    assert refused('hipMalloc', call)
+    e.sample_rows(x, rng.rand(5))
+    assert refused('hipMalloc', call)
+    e.sample_paths(cand, dist, u)
+    assert refused('hipMalloc', call)
+    e.path_posterior(cand, dist)
+
+e.close()
+print('SAMPLING-HOST-OK')

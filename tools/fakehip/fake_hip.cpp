@@ -18,6 +18,8 @@ static long g_launches = 0;
 static dim3 g_grid, g_block;
 static size_t g_shmem = 0;
 static hipStream_t g_stream = nullptr;
+static thread_local hipError_t g_last = hipSuccess;       // kept until it is asked for, as the real runtime does
+static hipError_t failed(hipError_t e) { g_last = e; return e; }
 
 extern "C" {
 
@@ -39,7 +41,7 @@ hipError_t __hipPopCallConfiguration(dim3 *grid, dim3 *block, size_t *shmem, hip
 hipError_t hipLaunchKernel(const void *, dim3 grid, dim3 block, void **, size_t, hipStream_t)
 {
     // a launch with an empty grid or block is an error on the real runtime too
-    if (!grid.x || !grid.y || !grid.z || !block.x || !block.y || !block.z) return hipErrorInvalidConfiguration;
+    if (!grid.x || !grid.y || !grid.z || !block.x || !block.y || !block.z) return failed(hipErrorInvalidConfiguration);
     ++g_launches;
     return hipSuccess;
 }
@@ -61,7 +63,7 @@ hipError_t hipGetDevicePropertiesR0600(hipDeviceProp_t *p, int d)
     p->warpSize = 64;
     return hipSuccess;
 }
-hipError_t hipGetLastError() { return hipSuccess; }
+hipError_t hipGetLastError() { const hipError_t e = g_last; g_last = hipSuccess; return e; }
 const char *hipGetErrorString(hipError_t e) { return e == hipSuccess ? "no error" : "fake-hip error"; }
 hipError_t hipDeviceSynchronize() { return hipSuccess; }
 hipError_t hipMemGetInfo(size_t *f, size_t *t) { *f = (size_t)200 << 30; *t = (size_t)288 << 30; return hipSuccess; }
@@ -70,9 +72,9 @@ hipError_t hipMalloc(void **p, size_t n)
 {
     // "device" memory: a plain host block (the sanitizer's red zones sit around it); sizes beyond what the CPU box has fail
     // like an out-of-memory device
-    if (n > ((size_t)6 << 30)) { *p = nullptr; return hipErrorOutOfMemory; }
+    if (n > ((size_t)6 << 30)) { *p = nullptr; return failed(hipErrorOutOfMemory); }
     *p = calloc(n ? n : 1, 1);
-    if (!*p) return hipErrorOutOfMemory;
+    if (!*p) return failed(hipErrorOutOfMemory);
     std::lock_guard<std::mutex> l(g_m);
     g_dev[*p] = n;
     return hipSuccess;
@@ -87,7 +89,7 @@ hipError_t hipFree(void *p)
 hipError_t hipHostMalloc(void **p, size_t n, unsigned int)
 {
     *p = calloc(n ? n : 1, 1);
-    if (!*p) return hipErrorOutOfMemory;
+    if (!*p) return failed(hipErrorOutOfMemory);
     std::lock_guard<std::mutex> l(g_m);
     g_host[*p] = n;
     return hipSuccess;
