@@ -616,9 +616,8 @@ class HipSearchEngine(object):
         e = np.ascontiguousarray(edges, dtype=np.int64)
         if b.ndim != 2 or b.size == 0 or e.shape != (b.shape[1] - 1,):
             raise SnkError('set_position_bias: bias (classes, buckets) and buckets - 1 edges expected')
-        self._bias_shape = None
         self._check(self._lib.snk_set_position_bias(self._h, _ptr(b, _c_f64p), b.shape[0], b.shape[1], _ptr(e, _c_i64p)))
-        self._bias_shape = b.shape
+        self._bias_shape = b.shape                      # (a bias that is refused leaves the one before)
 
     def _trellis(self, candidates, distances, row_offsets, join_class):
         """(on device, candidates, distances, offsets, classes or None, pointers of the three)"""

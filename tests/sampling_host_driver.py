@@ -54,5 +54,13 @@ for call in (lambda: e.path_posterior(wide, np.zeros((rows, 208))), lambda: e.sa
     assert refused('hipMalloc', call)
     e.path_posterior(cand, dist)
 
+# ---- a position bias that is refused leaves the one before, and its gradient ----
+e.set_position_bias(np.zeros((2, 3)), [0, 1])
+for bad in ((np.full((4, 2), np.nan), [0]), (np.zeros((1, 4)), [0, 2, 1]), (np.zeros((1, 65)), np.arange(64)), (np.zeros(3), [0])):
+    assert refused('', e.set_position_bias, *bad)
+    assert e.path_posterior(cand, dist)[2].shape == (2, 3)
+e.set_position_bias(None)
+assert e.path_posterior(cand, dist)[2] is None
+
 e.close()
 print('SAMPLING-HOST-OK')
