@@ -522,13 +522,20 @@ class HipSearchEngine(object):
 
     # -- draws and probabilities over the candidates ---------------------------
     # Every method takes numpy arrays (and returns them: the results are there when it returns) or torch tensors on the engine's
-    # GPU (and returns tensors; the work is queued on torch's current stream).
-    def _tensor(self, a, dtype, shape, what):
+    # GPU (and returns tensors; the work is queued on torch's current stream).  Results carry no gradient: a tensor that asks for
+    # one is refused (path_posterior returns what d logZ is made of).
+    def _on_device(self, a, what):
         import torch
         if not _is_device(a):
             raise SnkError('%s: expected a tensor on the GPU, like the other arguments' % what)
         if a.device.index != self.device:
             raise SnkError('%s is on %s, the engine on device %d' % (what, a.device, self.device))
+        if a.requires_grad and torch.is_grad_enabled():
+            raise SnkError('%s requires a gradient, which does not pass through this call: detach it, or call under torch.no_grad()' % what)
+
+    def _tensor(self, a, dtype, shape, what):
+        import torch
+        self._on_device(a, what)
         if tuple(a.shape) != tuple(shape):
             raise SnkError('%s has the shape %s, expected %s' % (what, tuple(a.shape), tuple(shape)))
         if a.dtype != getattr(torch, dtype):
@@ -560,8 +567,7 @@ class HipSearchEngine(object):
             name = str(scores.dtype).replace('torch.', '')
             if name not in _SCORE_TYPES:
                 raise SnkError('sample_rows: scores of type %s' % scores.dtype)
-            if scores.device.index != self.device:
-                raise SnkError('scores are on %s, the engine on device %d' % (scores.device, self.device))
+            self._on_device(scores, 'scores')
             if V > 1 and scores.stride(1) != 1 or R > 1 and scores.stride(0) < V:
                 scores = scores.contiguous()
             u = self._tensor(u, 'float64', u.shape, 'u')

@@ -250,3 +250,29 @@ def test_posteriors_of_costs_that_overflow_are_probabilities(engine, scale, tau,
     logz, post, uses = engine.path_posterior(cand, d, row_offsets=offs, temperature=tau)
     assert np.all(np.abs(post.sum(axis=1) - 1.0) <= 32.0 * 2.0 ** -53 * 20) and not np.isnan(logz).any()
     assert abs(uses.sum() - 33.0) <= 33.0 * 20 * 20 * 2.0 ** -51 + 1e-13      # a join between each two rows; K K cells a row, rounded to 2^-50
+
+
+# ---- autograd -----------------------------------------------------------------------------------------------------------------------------
+def test_tensors_that_ask_for_a_gradient_are_refused(engine):
+    import torch
+    from snickery_amd import SnkError
+    v = Voice(engine)
+    cand, dist, offs = v.candidates([5], 6, pad=False)
+    rng = np.random.RandomState(0)
+    c, d, u, x = on_gpu(cand), on_gpu(dist).requires_grad_(), on_gpu(rng.rand(2, 5)), on_gpu(rng.randn(5, 6)).requires_grad_()
+    for call in (lambda d, x: engine.path_posterior(c, d), lambda d, x: engine.sample_paths(c, d, u), lambda d, x: engine.sample_rows(x, u.t().contiguous())):
+        with pytest.raises(SnkError, match='gradient'):
+            call(d, x)
+        with pytest.raises(SnkError, match='gradient'):
+            call(2.0 * d, 2.0 * x)
+        want = call(d.detach(), x.detach())
+        with torch.no_grad():
+            got = call(d, x)
+        assert all(b is None or torch.equal(a, b) for a, b in zip(got, want))
+    # the gradient that a program puts together itself
+    logz, post, _ = engine.path_posterior(c, d.detach(), temperature=0.5)
+    h = 2.0 ** -14
+    e = torch.zeros_like(post)
+    e[2, 3] = h
+    slope = (engine.path_posterior(c, d.detach() + e, temperature=0.5)[0] - engine.path_posterior(c, d.detach() - e, temperature=0.5)[0]) / (2.0 * h)
+    assert abs(float(slope) + float(post[2, 3]) / 0.5) <= h * h / 6.0 / 0.5 ** 3 + 2.0 ** -40 / h
