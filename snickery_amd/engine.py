@@ -572,12 +572,22 @@ class HipSearchEngine(object):
                 scores = scores.contiguous()
             u = self._tensor(u, 'float64', u.shape, 'u')
             table = None
+            per_row = per_row or any(_is_device(r) for r in rules)          # (a number there is not fetched)
             if per_row:
-                cols = [r.to(dtype=torch.float64, device=scores.device) if torch.is_tensor(r) else
-                        torch.as_tensor(np.asarray(r, dtype=np.float64)).to(scores.device) for r in rules]
-                if any(c.ndim and tuple(c.shape) != (R,) for c in cols):
-                    raise SnkError('sample_rows: a rule per row needs %d entries' % R)
-                table = torch.stack([c.expand(R) for c in cols], 1).contiguous()
+                table = torch.empty((R, 4), dtype=torch.float64, device=scores.device)
+                for k, (r, what) in enumerate(zip(rules, ('temperature', 'top_k', 'top_p', 'min_p'))):
+                    if not _is_device(r) and np.ndim(r) == 0:
+                        table[:, k].fill_(float(r))                         # (no copy from the host: a graph may be recording)
+                        continue
+                    if _is_device(r):
+                        self._on_device(r, what)
+                    elif torch.cuda.is_current_stream_capturing():
+                        raise SnkError('%s: a rule per row has to be on the GPU for a call that is captured' % what)
+                    else:
+                        r = torch.as_tensor(np.asarray(r, dtype=np.float64))
+                    if tuple(r.shape) not in ((), (R,)):
+                        raise SnkError('sample_rows: a rule per row needs %d entries' % R)
+                    table[:, k] = r.to(scores.device)
             index = torch.empty(u.shape, dtype=torch.int64, device=scores.device)
             logp = torch.empty(u.shape, dtype=torch.float64, device=scores.device)
             rule = (1.0, 0, 1.0, 0.0) if per_row else self._rule(*rules)

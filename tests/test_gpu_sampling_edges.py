@@ -276,3 +276,44 @@ def test_tensors_that_ask_for_a_gradient_are_refused(engine):
     e[2, 3] = h
     slope = (engine.path_posterior(c, d.detach() + e, temperature=0.5)[0] - engine.path_posterior(c, d.detach() - e, temperature=0.5)[0]) / (2.0 * h)
     assert abs(float(slope) + float(post[2, 3]) / 0.5) <= h * h / 6.0 / 0.5 ** 3 + 2.0 ** -40 / h
+
+
+# ---- rules of rows --------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize('V', [100, 3000, 20000])
+def test_a_rule_per_row_in_a_graph(engine, V):
+    """Some rules a tensor, the others numbers, recorded once and replayed with other rules."""
+    import torch
+    rng = np.random.RandomState(V)
+    R = 6
+    x, u = rng.randn(R, V).astype(np.float32), rng.rand(R, 2)
+    gx, gu = on_gpu(x), on_gpu(u)
+    tau, k = on_gpu(np.full(R, 1.0)), on_gpu(np.full(R, 3))
+    one = torch.full((), 0.9, dtype=torch.float64, device='cuda')             # a single number on the GPU: for every row
+    engine.sample_rows(gx, gu, temperature=tau, top_k=k, top_p=0.9)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a = engine.sample_rows(gx, gu, temperature=tau, top_k=0, top_p=0.9, min_p=1e-3)
+        b = engine.sample_rows(gx, gu, temperature=0.7, top_k=k, top_p=one)
+    for n in range(3):
+        t, m = 0.2 + rng.rand(R), rng.randint(1, 50, R)
+        tau.copy_(on_gpu(t)); k.copy_(on_gpu(m))
+        graph.replay()
+        torch.cuda.synchronize()
+        for got, rule in ((a, dict(temperature=t, top_p=0.9, min_p=1e-3)), (b, dict(temperature=0.7, top_k=m, top_p=0.9))):
+            want, lp = o.sample_rows(x, u, **rule)
+            assert np.array_equal(got[0].cpu().numpy(), want)
+            eager = engine.sample_rows(gx, gu, **rule)                        # numpy rules, copied
+            assert torch.equal(eager[0], got[0]) and torch.equal(eager[1], got[1])
+
+
+def test_rules_of_rows_refused(engine):
+    import torch
+    from snickery_amd import SnkError
+    x, u = torch.zeros((4, 10), device='cuda'), torch.zeros((4,), dtype=torch.float64, device='cuda')
+    for bad in (torch.ones(3, device='cuda'), torch.ones((4, 1), device='cuda'), np.ones(5), np.ones((1, 4)), [1.0, 2.0]):
+        with pytest.raises(SnkError, match='entries'):
+            engine.sample_rows(x, u, temperature=bad)
+    with pytest.raises(SnkError, match='gradient'):
+        engine.sample_rows(x, u, temperature=torch.ones(4, device='cuda', requires_grad=True))
+    assert engine.sample_rows(x, u, temperature=[1.0, 0.5, 2.0, 0.0])[0].tolist() == [0, 0, 0, 0]
