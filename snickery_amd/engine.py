@@ -203,24 +203,38 @@ class QueryBatch(object):
         self.lengths = [int(m.shape[0]) for m in mats]
         self.offsets = np.zeros(len(mats) + 1, dtype=np.int64)
         self.offsets[1:] = np.cumsum(self.lengths)
-        self.Q = np.ascontiguousarray(np.vstack(mats))
+        self._rows = np.ascontiguousarray(np.vstack(mats))
+        self._of = None                                 # a subset: the batch it was taken of, its first and last row
 
     def __len__(self):
         return len(self.lengths)
 
+    @property
+    def Q(self):
+        """The rows as they are uploaded: write here to search other ones (pin() moves them)."""
+        if self._of is None:
+            return self._rows
+        batch, a, b = self._of
+        return batch.Q[a:b]
+
     def pin(self):
-        """Move the rows to page-locked memory: uploads of this batch are then queued on the stream instead of making the host
-        wait for it.  The memory is given back when neither the batch nor a subset taken of it since uses it any more."""
-        if not getattr(self, '_pinned', False) and self.Q.nbytes:
+        """Copy the rows to page-locked memory and use them there from now on: uploads of this batch, and of its subsets, are then
+        queued on the stream instead of making the host wait for it.  The array that Q was before is not uploaded any more and
+        cannot be written through (a view of it that the caller made can): take Q again.  The memory is given back when neither the
+        batch nor a subset of it uses it any more.  A subset is moved with the batch that it was taken of."""
+        if self._of is not None:
+            self._of[0].pin()
+        elif not getattr(self, '_pinned', False) and self._rows.nbytes:
             lib = load_library()
             p = ctypes.c_void_p()
-            if lib.snk_host_alloc(self.Q.nbytes, ctypes.byref(p)) != 0:
+            if lib.snk_host_alloc(self._rows.nbytes, ctypes.byref(p)) != 0:
                 raise SnkError(lib.snk_last_error().decode('utf-8', 'replace'))
-            memory = (ctypes.c_double * self.Q.size).from_address(p.value)
+            memory = (ctypes.c_double * self._rows.size).from_address(p.value)
             weakref.finalize(memory, lib.snk_host_free, p)
-            rows = np.frombuffer(memory, dtype=np.float64).reshape(self.Q.shape)
-            rows[:] = self.Q
-            self.Q = rows
+            rows = np.frombuffer(memory, dtype=np.float64).reshape(self._rows.shape)
+            rows[:] = self._rows
+            self._rows.flags.writeable = False
+            self._rows = rows
             self._pinned = True
         return self
 
@@ -229,7 +243,8 @@ class QueryBatch(object):
         b = QueryBatch.__new__(QueryBatch)
         b.lengths = self.lengths[lo:hi]
         b.offsets = self.offsets[lo:hi + 1] - self.offsets[lo]
-        b.Q = self.Q[self.offsets[lo]:self.offsets[hi]]
+        a = 0 if self._of is None else self._of[1]
+        b._of = (self if self._of is None else self._of[0], a + int(self.offsets[lo]), a + int(self.offsets[hi]))
         return b
 
 

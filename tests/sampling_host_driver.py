@@ -62,5 +62,26 @@ for bad in ((np.full((4, 2), np.nan), [0]), (np.zeros((1, 4)), [0, 2, 1]), (np.z
 e.set_position_bias(None)
 assert e.path_posterior(cand, dist)[2] is None
 
+# ---- query rows moved to page-locked memory: what is written afterwards is what is searched ----
+utts = [rng.randn(n, 5) for n in (4, 1, 7)]
+batch = snickery_amd.QueryBatch(utts)
+before, early = batch.Q, batch.subset(1, 3)
+assert np.array_equal(early.Q, np.vstack(utts[1:])) and np.shares_memory(early.Q, before)
+batch.pin()
+assert not np.shares_memory(batch.Q, before) and np.array_equal(batch.Q, np.vstack(utts))
+try:
+    before[0, 0] = 1.0                                # the rows are elsewhere: not a silent search of the old ones
+    raise AssertionError('the array from before the move can be written')
+except ValueError:
+    pass
+batch.Q[:] = 2.0
+late = batch.subset(0, 2).subset(1, 2)
+assert np.all(early.Q == 2.0) and early.Q.shape == (8, 5) and np.all(late.Q == 2.0) and late.Q.shape == (1, 5) and late.offsets.tolist() == [0, 1]
+assert np.shares_memory(early.Q, batch.Q) and np.shares_memory(late.Q, batch.Q)
+other = snickery_amd.QueryBatch(utts)
+part = other.subset(0, 1).pin()                       # a subset takes its batch along
+assert np.shares_memory(part.Q, other.Q) and other._pinned and other.pin().Q is other.Q
+assert snickery_amd.QueryBatch([np.zeros((0, 5))]).pin().Q.shape == (0, 5)
+
 e.close()
 print('SAMPLING-HOST-OK')
