@@ -10,7 +10,8 @@ With Z the partition function of the path model exp(-cost / temperature) and n t
 
 is convex, and its gradient is n * goal - uses, `uses` being the expected uses of a bucket that engine.path_posterior returns.
 Every iteration moves a bias by rate * temperature * log(uses / (n * goal)), a scaled step down that gradient; a bucket whose goal is
-0 is forbidden (+inf).
+0 is forbidden (+inf).  A bucket that no two candidates of the tune set offer stays at 0, and its goal goes to the others of its class in
+proportion: nothing is to be learned of it, and F would have its bias fall without end.
 
     position_goals = {'edges': [0, 1, 2], 'goals': [0.1, 0.0, 0.7, 0.2], 'classes': {...}}       # goals: a list, or one per class
     unit_sampling = {'temperature': 0.5}
@@ -23,8 +24,8 @@ import numpy as np
 
 
 def bias_step(bias, uses, goals, temperature, rate, floor=1e-6):
-    """One iteration: the moved bias and the gradient n goal - uses of F at the old one.  A share below `floor` counts as that
-    (a bucket that no candidate offers would otherwise run away); a class without joins stays as it is."""
+    """One iteration: the moved bias and the gradient n goal - uses of F at the old one.  A share below `floor` counts as that, which
+    bounds the step of a bucket that is hardly used; a class without joins stays as it is."""
     n = uses.sum(axis=1, keepdims=True)
     gradient = n * goals - uses
     share = np.where(n > 0.0, uses / np.where(n > 0.0, n, 1.0), goals)
@@ -61,6 +62,14 @@ def train_position_bias(synth, goals, edges, classes=None, n_tune=10, max_epochs
     synth.set_position_bias(bias, edges, classes)
     per_utt = [synth.join_classes(w, len(c)) for w, c in zip(names, cands)]
     join_class = None if per_utt[0] is None else np.concatenate(per_utt)
+    # At a temperature far above every cost all paths weigh the same: what is used there is what the candidates offer.
+    ceiling = 1e6 * max(1.0, float(np.abs(dist[np.isfinite(dist)]).max(initial=0.0)))
+    offered = synth.engine.path_posterior(cand, dist, row_offsets=offs, join_class=join_class, temperature=ceiling)[2] > 0.0
+    wanted, goals = goals > 0.0, np.where(offered, goals, 0.0)
+    for c, k in zip(*np.nonzero(wanted & ~offered)):
+        report('## class %d: no candidates offer bucket %d' % (c, k))
+    left = goals.sum(axis=1, keepdims=True)
+    goals = goals / np.where(left > 0.0, left, 1.0)
     losses, uses = [], None
     for epoch in range(max_epochs):
         logz, _, uses = synth.engine.path_posterior(cand, dist, row_offsets=offs, join_class=join_class, temperature=temperature)
@@ -74,7 +83,8 @@ def train_position_bias(synth, goals, edges, classes=None, n_tune=10, max_epochs
             break
         bias, _ = bias_step(bias, uses, goals, temperature, rate)
         # a constant over a class's buckets changes no probability: the smallest stays at 0
-        bias = bias - np.where(np.isfinite(bias), bias, np.inf).min(axis=1, keepdims=True)
+        least = np.where(np.isfinite(bias), bias, np.inf).min(axis=1, keepdims=True)
+        bias = np.where(wanted & ~offered, 0.0, bias - np.where(np.isfinite(least), least, 0.0))
         synth.set_position_bias(bias, edges, classes)
     report('## Position bias found -- you can copy it to config.')
     report('position_bias = %s' % ({'bias': bias.tolist(), 'edges': [int(e) for e in edges], 'classes': classes},))

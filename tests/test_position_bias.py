@@ -104,3 +104,20 @@ def test_bucket_edges():
         assert len(e) == n - 1 and all(a < b for a, b in zip(e, e[1:])) and set([0, 1, 2]) <= set(e)
     with pytest.raises(ValueError):
         hp.position_bucket_edges(3, 10)
+
+
+@pytest.mark.parametrize('classes', [None, {'a': 0, 'b': 1, 'never': 2}])
+def test_a_bucket_that_no_candidate_offers_stays_where_it_is(classes):
+    """Units lie up to 97 apart here: steps beyond 500 are in no path."""
+    s, lines = StubSynthesiser(), []
+    goals = [0.2, 0.1, 0.3, 0.15, 0.25]
+    res = train_position_bias(s, goals, [0, 1, 2, 500], classes, max_epochs=40, rate=0.8, thresh=1e-2, report=lines.append)
+    n = 3 if classes else 1
+    assert res['bias'].shape == (n, 5) and np.all(res['bias'][:, 4] == 0.0) and np.all(np.isfinite(res['bias'])) and np.abs(res['bias']).max() < 20.0
+    assert np.all(res['bias'][:2, :4].min(axis=1) == 0.0)
+    assert sum('no candidates offer bucket 4' in l for l in lines) == n
+    if classes:                                          # a class on no join: nothing learned
+        assert not res['bias'][2].any()
+    wanted = np.array(goals[:4]) / sum(goals[:4])
+    shares = res['uses'][0] / res['uses'][0].sum()
+    assert np.abs(shares[:4] - wanted).max() <= res['losses'][-1] + 1e-12 and shares[4] == 0.0
