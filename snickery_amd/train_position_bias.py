@@ -14,6 +14,7 @@ Every iteration moves a bias by rate * temperature * log(uses / (n * goal)), a s
 proportion: nothing is to be learned of it, and F would have its bias fall without end.
 
     position_goals = {'edges': [0, 1, 2], 'goals': [0.1, 0.0, 0.7, 0.2], 'classes': {...}}       # goals: a list, or one per class
+    position_goals = {'max_distance': 1000, 'goals': [0.02, 0.03, 0.05, 0.0, 0.6, 0.15, 0.1, 0.05]}   # edges by hostprep.position_bucket_edges
     unit_sampling = {'temperature': 0.5}
 
     python -m snickery_amd.train_position_bias -c voice.cfg
@@ -21,6 +22,16 @@ proportion: nothing is to be learned of it, and F would have its bias fall witho
 from argparse import ArgumentParser
 
 import numpy as np
+
+from . import hostprep as hp
+
+
+def goals_and_edges(settings):
+    """Goals and edges of a position_goals setting: its own edges, or as many buckets as it has goals up to its max_distance."""
+    goals, edges = settings['goals'], settings.get('edges')
+    if (edges is None) == ('max_distance' not in settings):
+        raise ValueError('position_goals: either edges or max_distance')
+    return goals, hp.position_bucket_edges(np.shape(goals)[-1], settings['max_distance']) if edges is None else edges
 
 
 def bias_step(bias, uses, goals, temperature, rate, floor=1e-6):
@@ -63,8 +74,7 @@ def train_position_bias(synth, goals, edges, classes=None, n_tune=10, max_epochs
     per_utt = [synth.join_classes(w, len(c)) for w, c in zip(names, cands)]
     join_class = None if per_utt[0] is None else np.concatenate(per_utt)
     # At a temperature far above every cost all paths weigh the same: what is used there is what the candidates offer.
-    ceiling = 1e6 * max(1.0, float(np.abs(dist[np.isfinite(dist)]).max(initial=0.0)))
-    offered = synth.engine.path_posterior(cand, dist, row_offsets=offs, join_class=join_class, temperature=ceiling)[2] > 0.0
+    offered = synth.engine.path_posterior(cand, dist, row_offsets=offs, join_class=join_class, temperature=1e100)[2] > 0.0
     wanted, goals = goals > 0.0, np.where(offered, goals, 0.0)
     for c, k in zip(*np.nonzero(wanted & ~offered)):
         report('## class %d: no candidates offer bucket %d' % (c, k))
@@ -100,7 +110,8 @@ def main(argv=None):
     synth = Synthesiser(opts.config_fname, device=opts.device)
     try:
         how = synth.config['position_goals']
-        train_position_bias(synth, how['goals'], how['edges'], how.get('classes'))
+        goals, edges = goals_and_edges(how)
+        train_position_bias(synth, goals, edges, how.get('classes'))
     finally:
         synth.close()
 

@@ -121,3 +121,18 @@ def test_a_bucket_that_no_candidate_offers_stays_where_it_is(classes):
     wanted = np.array(goals[:4]) / sum(goals[:4])
     shares = res['uses'][0] / res['uses'][0].sum()
     assert np.abs(shares[:4] - wanted).max() <= res['losses'][-1] + 1e-12 and shares[4] == 0.0
+
+
+def test_edges_of_a_setting():
+    from snickery_amd import hostprep as hp
+    from snickery_amd.train_position_bias import goals_and_edges
+    assert goals_and_edges({'goals': [0.5, 0.5], 'edges': [1]}) == ([0.5, 0.5], [1])
+    for goals in ([0.125] * 8, [[0.125] * 8] * 2):
+        g, edges = goals_and_edges({'goals': goals, 'max_distance': 90})
+        assert g == goals and edges == hp.position_bucket_edges(8, 90) and len(edges) == 7
+    s = StubSynthesiser()
+    res = train_position_bias(s, *goals_and_edges({'goals': [0.1, 0.1, 0.2, 0.3, 0.2, 0.1], 'max_distance': 40}), max_epochs=3, report=lambda line: None)
+    assert res['bias'].shape == (1, 6) and res['edges'] == hp.position_bucket_edges(6, 40)
+    for bad in ({'goals': [0.5, 0.5]}, {'goals': [0.5, 0.5], 'edges': [1], 'max_distance': 9}, {'goals': [0.5] * 3, 'max_distance': 9}):
+        with pytest.raises(ValueError):
+            goals_and_edges(bad)
