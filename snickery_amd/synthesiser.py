@@ -442,6 +442,7 @@ class Synthesiser(object):
         u = np.concatenate([self._random_numbers(n, (1, k)) for n, k in zip(names, lengths)], axis=1)
         if not how.get('joins', True):
             path = self.sample_units(cand, dist, u)
+            self.last_path_cost = None                          # (no joins: not a path's cost)
         else:
             classes = [self.join_classes(w, k) for w, k in zip(unit_names, lengths)]
             join_class = None if classes[0] is None else np.concatenate(classes)
