@@ -419,7 +419,7 @@ class Synthesiser(object):
         """A unit per row, drawn from its target costs alone: unit ids (draws, rows) with -1 where a row has no candidate.
         u (draws, rows)."""
         candidates = np.asarray(candidates, dtype=np.int64)
-        usable = (candidates >= 1) & (candidates < self.join_contexts_unweighted.shape[0] - 2)
+        usable = (candidates >= 1) & (candidates < self.join_contexts_unweighted.shape[0] - 2) & np.isfinite(distances)
         scores = np.where(usable, -np.asarray(distances, dtype=np.float64), -np.inf)
         index, _ = self.engine.sample_rows(scores, np.ascontiguousarray(np.asarray(u).T), **self._sampling_rule())
         units = np.take_along_axis(candidates, np.maximum(index, 0), axis=1)

@@ -41,3 +41,13 @@ def test_the_cost_of_a_path_is_the_last_ones(synth):
     synth.config['unit_sampling']['joins'] = False
     path = synth.draw_paths(['a'], [cand], [dist], [None])[0]
     assert len(path) == 7 and synth.last_path_cost is None
+
+
+def test_candidates_without_a_finite_target_cost_are_not_drawn(synth):
+    """With joins or without: the same candidates take part."""
+    cand = np.array([[3, 4, 5], [6, 7, 8], [0, 9, 59]])
+    dist = np.array([[0.1, -np.inf, np.nan], [np.inf, np.nan, -np.inf], [0.0, 0.2, 0.0]])
+    u = np.random.RandomState(0).rand(4, 3)
+    units = synth.sample_units(cand, dist, u)
+    assert np.array_equal(units, np.repeat([[3, -1, 9]], 4, axis=0))
+    assert np.all(synth.sample_search(cand, dist, u, row_offsets=[0, 1, 2, 3])[0] == units)
