@@ -1039,10 +1039,11 @@ static void launch_rows_split(const T *scores, int64_t stride, int64_t R, int64_
     w.left = (int *)take(R * 4);
     const dim3 grid((unsigned)w.chunks, (unsigned)R), spans((unsigned)w.spans, (unsigned)R);
     hipLaunchKernelGGL((rows_extremes_kernel<T>), spans, dim3(512), 0, s, scores, stride, V, w);
-    const size_t bins_lds = (size_t)w.bins * 16;                // (with the workgroup's own few words beyond 64 KB at the most bins)
+    const size_t bins_lds = (size_t)w.bins * 16;
     static size_t attr_set[32] = {0};
-    lds_attr_ensure(attr_set, bins_lds, [&] {
-        (void)hipFuncSetAttribute(reinterpret_cast<const void *>(&rows_histogram_kernel<T>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bins_lds); });
+    if (w.bins == SNK_BINS_MOST)                                // 64 KB, and the workgroup's own few words
+        lds_attr_ensure(attr_set, bins_lds, [&] {
+            (void)hipFuncSetAttribute(reinterpret_cast<const void *>(&rows_histogram_kernel<T>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bins_lds); });
     hipLaunchKernelGGL((rows_histogram_kernel<T>), spans, dim3(512), bins_lds, s, scores, stride, V, rule, rules, unit, w);
     for (int by_mass = 0; by_mass < 2; ++by_mass) {
         if (!rules && (by_mass ? !(rule.top_p < 1.0) : !(rule.top_k > 0 && rule.top_k < V))) continue;

@@ -197,6 +197,24 @@ def test_rows_of_scores_within_a_hair(engine, V):
         assert np.array_equal(i.cpu().numpy()[0], want)
 
 
+def test_a_row_of_the_most_bins_in_a_graph(engine):
+    """Histograms of more than 64 KB, recorded with the graph's own workspace."""
+    import torch
+    g = torch.Generator(device='cuda').manual_seed(3)
+    x = torch.randn((2, 600001), device='cuda', generator=g)
+    u = torch.rand((2, 3), device='cuda', dtype=torch.float64, generator=g)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = engine.sample_rows(x, u, top_p=0.97)
+    for n in range(3):
+        x.copy_(torch.randn((2, 600001), device='cuda', generator=g))
+        graph.replay()
+        want = engine.sample_rows(x, u, top_p=0.97)
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
 # ---- temperature zero ------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize('tau', [9.9e-251, 1e-300, 5e-324])
 def test_a_temperature_that_counts_as_zero_breaks_ties_like_it(engine, tau):
