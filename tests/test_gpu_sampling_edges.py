@@ -335,3 +335,49 @@ def test_rules_of_rows_refused(engine):
     with pytest.raises(SnkError, match='gradient'):
         engine.sample_rows(x, u, temperature=torch.ones(4, device='cuda', requires_grad=True))
     assert engine.sample_rows(x, u, temperature=[1.0, 0.5, 2.0, 0.0])[0].tolist() == [0, 0, 0, 0]
+
+
+# ---- 80 bits ---------------------------------------------------------------------------------------------------------------------------------
+def posterior_in_80_bits(v, cand, dist, tau):
+    """log Z and posteriors of one utterance in numpy's long double, in logarithms."""
+    L = np.longdouble
+    W, low = v.JC.astype(L) * v.wj.astype(L), np.clip(cand, 1, v.n - 2)
+    usable = (cand >= 1) & (cand < v.n - 1)
+    local = np.where(usable, -dist.astype(L) / L(tau), -np.inf)
+    C = []
+    for t in range(len(cand) - 1):
+        c = np.sqrt(((W[low[t] + 1][:, None, :] - W[low[t + 1]][None, :, :]) ** 2).sum(axis=2))
+        c = c + v.bias[0][o.buckets(cand[t], cand[t + 1], v.edges)].astype(L)
+        c[~usable[t]], c[:, ~usable[t + 1]] = np.inf, np.inf
+        C.append(-c / L(tau))
+
+    def lse(x, axis):
+        m = x.max(axis=axis, keepdims=True)
+        m = np.where(np.isfinite(m), m, L(0))
+        with np.errstate(divide='ignore'):
+            return (m + np.log(np.exp(x - m).sum(axis=axis, keepdims=True))).squeeze(axis)
+    alpha, beta = [local[0]], [np.zeros(cand.shape[1], L)]
+    for t in range(len(C)):
+        alpha.append(local[t + 1] + lse(alpha[-1][:, None] + C[t], 0))
+    for t in range(len(C) - 1, -1, -1):
+        beta.append(lse(C[t] + (local[t + 1] + beta[-1])[None, :], 1))
+    z = lse(alpha[-1], 0)
+    return z, np.exp(np.array(alpha) + np.array(beta[::-1]) - z)
+
+
+@pytest.mark.parametrize('T,K,Dj', [(335, 50, 302), (60, 100, 151)])
+def test_posteriors_against_80_bits(engine, T, K, Dj):
+    """The error that is left when the comparison has none of its own (pytest -s prints it)."""
+    v = Voice(engine, Dj=Dj, n=3000)
+    v.wj = v.wj / np.sqrt(Dj)
+    engine.set_weights(None, v.wj)
+    v.set_bias(1, 8)
+    cand, dist, _ = v.candidates([T], K)
+    z, p = posterior_in_80_bits(v, cand, dist, 0.5)
+    logz, post, _ = engine.path_posterior(cand, dist, temperature=0.5)
+    furthest = np.sqrt((v.wj ** 2 * (v.JC.max(axis=0) - v.JC.min(axis=0)).astype(np.float64) ** 2).sum())
+    # the join costs as in include/snk.h, once a row; a row's products, sums and scalings: K + 16 roundings
+    tol = T * (furthest * (Dj + 4.0) * (2.0 ** -43 + 2.0 ** -47) / 0.5 + (K + 16.0) * 2.0 ** -53)
+    err = np.abs(post - p).max()
+    print('\n%d rows of %d, %d columns: posteriors within %.1e of 80 bits (bound %.1e), log Z %.1f within %.1e' % (T, K, Dj, err, 4.0 * tol, z, abs(logz[0] - z)))
+    assert err <= 4.0 * tol and abs(logz[0] - z) <= tol + 2.0 ** -52 * abs(float(z))
