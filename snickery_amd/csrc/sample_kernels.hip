@@ -36,9 +36,9 @@ __device__ __forceinline__ typename ScoreKey<T>::type score_key(double x)
 }
 
 // ---- rows of up to 64 E scores: a wavefront each ------------------------------------------------------------------------------
-// A row is read once, its sums are data-parallel moves within the wavefront, and a lane has a draw.  One row of 30: 2.8 us, a launch;
-// 600 rows of 100, top_p 0.9: 9 us; 19200 rows of 100, top_k 40, top_p 0.95, min_p 0.02, 8 draws: 51 us, 0.4 TB/s: bound by the search
-// for the cuts (wave_row_keep).  8.4 million float32 scores, top_p 0.9: 128 us in rows of 128, 87 of 256, 83 of 512, 99 of 1024.
+// A row is read once, its sums are data-parallel moves within the wavefront, and a lane has a draw.  One row of 30: 2.9 us, a launch;
+// 600 rows of 100, top_p 0.9: 9 us; 19200 rows of 100, top_k 40, top_p 0.95, min_p 0.02, 8 draws: 50 us, 0.4 TB/s: bound by the search
+// for the cuts (wave_row_keep).  8.4 million float32 scores, top_p 0.9: 130 us in rows of 128, 89 of 256, 85 of 512, 96 of 1024.
 template <typename T, int E>
 __global__ void __launch_bounds__(256)
 sample_rows_wave_kernel(const T *__restrict__ scores, int64_t stride, int64_t R, int V, const double *__restrict__ u, int n_draws,
@@ -86,7 +86,7 @@ sample_rows_wave_kernel(const T *__restrict__ scores, int64_t stride, int64_t R,
 
 // ---- longer rows without a workspace: a workgroup each, the row read once per pass ------------------------------------------------------
 // For rows that the passes below leave over and for captured calls without a workspace.  Bound by what one compute unit reads: a row of
-// 1048576 float32 3.3 ms, 37 rows of 50003 179 us.
+// 1048576 float32 3.2 ms, 37 rows of 50003 178 us.
 #define SNK_SAMPLE_TILES 2048
 #define SNK_SAMPLE_VEC 8
 
@@ -345,9 +345,9 @@ __device__ __forceinline__ int score_bin(double e, double scale, int bins)
 // spilled: with 190 and none the rows of 2048 and 4096 scores took 86 and 115 us instead of 74 and 78.  Bound by the scans' and the
 // radix's barriers, some 30 of them.  float32, top_p 0.9, 8.4 million scores in all:
 //     scores a row     1025   2000   4096   8192 us, one row 8192
-//     this              139     78     78    117              27
+//     this              128     71     74    113              27
 //     passes below      677    370    214    147              50
-// Sixteen scores a thread, rows of 16384: 169 us, the passes below 125.
+// Sixteen scores a thread, rows of 16384: 169 us, the passes below 110.
 #define SNK_HELD_MOST 8192
 template <typename T, int NT, int EACH>
 __global__ void __launch_bounds__(NT, 4)
@@ -555,7 +555,7 @@ sample_rows_held_kernel(const T *__restrict__ scores, int64_t stride, int V, con
 // shows in a result.  A boundary bin of equal scores needs no list; one of more than SNK_LIST different ones (or a workspace that a
 // captured graph would have to share) leaves the row to the kernel above.  us a pass, for 1 row of 1048576 float32, 37 of 50003 float32
 // (top_p 0.95: 7.4 MB, 1.5 us at a copy's rate) and 128 of 131071 bfloat16 (top_k 50 and top_p 0.9: 34 MB, 6.6 us):
-//     extremes 6, 5, 13    histogram 13, 11, 36    boundary 12, 11, 2 x 20    select 10, 11, 2 x 5    masses 8, 11, 17    draw 13, 13, 10
+//     extremes 4, 5, 12    histogram 17, 11, 38    boundary 12, 11, 2 x 21    select 12, 12, 2 x 6    masses 8, 11, 18    draw 13, 13, 10
 // The first two are launches and the latency of a few dependent reads each; the third is bound by the float64 work on every score (weight
 // and bin, tested again for the boundary).
 #define SNK_CHUNK 8192

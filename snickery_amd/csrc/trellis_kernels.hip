@@ -133,17 +133,18 @@ trellis_local_kernel(const TrellisView v, double *__restrict__ local, double *__
 // one unit of the second row, so that the norms are those of the candidates' spread and not of their distance from the origin.  Where
 // the difference is small against the norms -- neighbouring frames -- the product form cancels: a cell below SNK_COST_NEAR of them is taken
 // again in differences.  A unit and its natural successor join at exactly 0.  The others carry a relative error of at most Dj 2^-53 / SNK_COST_NEAR,
-// an absolute one of 2^5 Dj 2^-53 of the norms' root.  (2^-8: 2.20 ms for 9600 rows of 100, half the error of the posteriors; 2^-10: 2.11 and
-// 1.2e-14 at most over 335 rows of 50, where logarithms of float64 err by 2e-13.)
+// an absolute one of 2^5 Dj 2^-53 of the norms' root.  (2^-8 took 4 % longer for 9600 rows of 100 and halved the error of the posteriors, which
+// with 2^-10 is 9e-15 at most over 335 rows of 50, a log Z of 455, against 80-bit arithmetic.)
 // Frames that are not finite: a distance that is infinite or no number joins nothing.  The product form says so only while the unit that both
 // sides are taken relative to is finite; where it is not, or a frame brings an infinity of its own into a product, a cell's value is no
 // number, and every such cell of units that can join counts as near: the differences, which know its own two frames alone, decide.
 // A wavefront owns RM x CM tiles of 16 x 16; DC columns of the two sets of rows go through LDS at a time, weighted and widened on
 // the way, the next ones are in flight meanwhile: 32, a cache line of a row (197 us for 600 rows of 100 candidates and 302 columns, 206
 // with 16, before what follows), or 16 in the larger tiles, whose registers hold no more (2.55 ms for 9600 rows, 2.73 with 32 and
-// spills).  9600 rows of 100 candidates, 302 columns: 2.11 ms, 27 TFLOP/s of a large product's 62 (35 with the cells that pad K to
-// 112); bound by the float64 units, which the products hold 43 % of the time and weighing the cells, staging and padding the most of
-// the rest: neither overlaps with products of another wavefront.  1200 rows of 200, 151 columns: 0.66 ms.
+// spills; what the rest of this kernel took before later steps).  9600 rows of 100 candidates, 302 columns: 2.0 ms, 29 TFLOP/s of a large
+// product's 62 (36 with the cells that pad K to 112); bound by the float64 units, which the products hold 48 % of the time and weighing
+// the cells, staging and padding the most of the rest: neither overlaps with products of another wavefront.  1200 rows of 200, 151
+// columns: 0.64 ms.
 #define SNK_COST_NEAR 0x1p-10
 typedef double f64x4 __attribute__((ext_vector_type(4)));
 
@@ -1016,6 +1017,8 @@ trellis_backward_kernel(const TrellisView v, const double *__restrict__ local, c
 // ---- the flagged utterances in logarithms (SUM false: temperature 0, the largest term of every sum) ----------------------------------
 // Every row of the sums is taken relative to the largest weight of the row before (after) it: a row's differences stay the size of a step's
 // costs over tau, where the whole path's would round to more than the differences themselves once tau is 2^-50 of them.
+// A workgroup has an utterance: chains of T steps of one compute unit.  600 rows of 100 candidates: a draw 6.2 ms (2.8 at temperature 0),
+// a posterior 15.4; sixteen such utterances side by side 11.9, 6.8 and 21.5.
 template <bool SUM>
 __global__ void __launch_bounds__(1024)
 trellis_forward_log_kernel(const TrellisView v, const int *__restrict__ flag, double *__restrict__ alpha, double *__restrict__ logz)
