@@ -217,6 +217,10 @@ class QueryBatch(object):
         batch, a, b = self._of
         return batch.Q[a:b]
 
+    @Q.setter
+    def Q(self, rows):
+        self._rows, self._of, self._pinned = _f64(rows), None, False
+
     def pin(self):
         """Copy the rows to page-locked memory and use them there from now on: uploads of this batch, and of its subsets, are then
         queued on the stream instead of making the host wait for it.  The array that Q was before is not uploaded any more and

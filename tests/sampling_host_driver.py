@@ -82,6 +82,8 @@ other = snickery_amd.QueryBatch(utts)
 part = other.subset(0, 1).pin()                       # a subset takes its batch along
 assert np.shares_memory(part.Q, other.Q) and other._pinned and other.pin().Q is other.Q
 assert snickery_amd.QueryBatch([np.zeros((0, 5))]).pin().Q.shape == (0, 5)
+part.Q = np.full((4, 5), 3.0)                         # rows of its own
+assert np.all(part.Q == 3.0) and not np.any(other.Q == 3.0) and not np.shares_memory(part.pin().Q, other.Q) and np.all(part.Q == 3.0)
 
 e.close()
 print('SAMPLING-HOST-OK')
