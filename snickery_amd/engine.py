@@ -544,13 +544,14 @@ class HipSearchEngine(object):
     # GPU (and returns tensors; the work is queued on torch's current stream).  Results carry no gradient: a tensor that asks for
     # one is refused (path_posterior returns what d logZ is made of).
     def _on_device(self, a, what):
-        import torch
         if not _is_device(a):
             raise SnkError('%s: expected a tensor on the GPU, like the other arguments' % what)
         if a.device.index != self.device:
             raise SnkError('%s is on %s, the engine on device %d' % (what, a.device, self.device))
-        if a.requires_grad and torch.is_grad_enabled():
-            raise SnkError('%s requires a gradient, which does not pass through this call: detach it, or call under torch.no_grad()' % what)
+        if a.requires_grad:
+            import torch
+            if torch.is_grad_enabled():
+                raise SnkError('%s requires a gradient, which does not pass through this call: detach it, or call under torch.no_grad()' % what)
 
     def _tensor(self, a, dtype, shape, what):
         import torch
@@ -576,7 +577,9 @@ class HipSearchEngine(object):
         u (R,) or (R, draws): (index int64, log probability float64), both shaped like u.  temperature, top_k, top_p and min_p
         are numbers, or arrays of R for a rule per row."""
         rules = (temperature, top_k, top_p, min_p)
-        per_row = any(not isinstance(r, (int, float)) and np.ndim(r) > 0 for r in rules)
+        number = (int, float)
+        plain = isinstance(temperature, number) and isinstance(top_k, number) and isinstance(top_p, number) and isinstance(min_p, number)
+        per_row = not plain and any(np.ndim(r) > 0 for r in rules)
         if getattr(scores, 'ndim', 0) != 2 or getattr(u, 'ndim', 0) not in (1, 2) or u.shape[0] != scores.shape[0]:
             raise SnkError('sample_rows: scores (R, V) and random numbers (R,) or (R, draws) expected')
         R, V = int(scores.shape[0]), int(scores.shape[1])
@@ -591,7 +594,7 @@ class HipSearchEngine(object):
                 scores = scores.contiguous()
             u = self._tensor(u, 'float64', u.shape, 'u')
             table = None
-            per_row = per_row or any(_is_device(r) for r in rules)          # (a number there is not fetched)
+            per_row = per_row or not plain and any(_is_device(r) for r in rules)      # (a number there is not fetched)
             if per_row:
                 table = torch.empty((R, 4), dtype=torch.float64, device=scores.device)
                 for k, (r, what) in enumerate(zip(rules, ('temperature', 'top_k', 'top_p', 'min_p'))):
